@@ -166,6 +166,67 @@ int wf_bwd_convert(const float* accum, void* out, float scale, int b, int s, int
 int wf_bwd_noalloc(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dO,
                    void* dq, void* dk, void* dv, int b, int sq, int skv, int h, void* stream);
 
+typedef enum wf_dtype { WF_BF16 = 0, WF_FP32 = 1 } wf_dtype;
+
+/* Options of wf_rope.  Strides of q and k are in elements (the last dim is
+   contiguous; every stride a multiple of 16 bytes); outputs are contiguous. */
+typedef struct wf_rope_cfg {
+  int dtype;            /* wf_dtype of q, k and the outputs                   */
+  int inverse;          /* 1 = turn by the negative angle (the backward)      */
+  int max_pos;          /* rows of the table                                  */
+  int pairs_t, pairs_h; /* dim pairs of time and height; width has the rest   */
+  int reserved;
+  long long q_stride_b, q_stride_s, q_stride_h;
+  long long k_stride_b, k_stride_s, k_stride_h;
+  long long pos_stride_b; /* ints between the positions of batch items (0: shared) */
+} wf_rope_cfg;
+
+/*
+ * Rotary positions with three axes (no reference counterpart; the Wan models
+ * turn q and k right before the attention).  Pair i of a 128-dim head, in
+ * fp32, (x[2i], x[2i+1]) -> (x[2i] c - x[2i+1] s, x[2i] s + x[2i+1] c) with
+ * (c, s) = table[positions[token][axis(i)]][i].
+ *   q (b, s, h, 128), k (b, s, h_kv, 128), strided; q_out, k_out contiguous,
+ *   apart from q and k; table (max_pos, 64, 2) fp32; positions (s, 3) int32.
+ * A token with a negative position passes unchanged.  A position >= max_pos
+ * gives NaN in its token's rows and WF_ERR_INVALID_ARG from wf_device_status.
+ */
+int wf_rope(const void* q, const void* k, void* q_out, void* k_out, const float* table, const int* positions, int b,
+            int s, int h, int h_kv, const wf_rope_cfg* cfg, void* stream);
+
+/* Shape of the paged cache of wf_decode; strides in elements, multiples of 8. */
+typedef struct wf_decode_cfg {
+  int n_pages;            /* pages of the cache                               */
+  int page_size;          /* tokens of a page, >= 1                           */
+  int max_pages;          /* entries of a page-table row                      */
+  int reserved;
+  long long table_stride; /* ints between page-table rows                     */
+  long long k_page_stride, k_slot_stride, k_head_stride;
+  long long v_page_stride, v_slot_stride, v_head_stride;
+} wf_decode_cfg;
+
+/* Bytes of workspace that wf_decode needs on the current device for h q heads
+   and h_kv key-value heads, whatever the batch and the lengths. */
+int wf_decode_workspace(int h, int h_kv, size_t* bytes);
+
+/*
+ * Attention of one new token per sequence over a paged key-value cache (no
+ * reference counterpart): o = softmax(q K^T / sqrt(128)) V over the first
+ * lengths[i] tokens of sequence i, token t in slot t % page_size of page
+ * page_table[i][t / page_size]; lse natural log.
+ *   q, o (b, h, 128) bf16 contiguous; lse (b, h) fp32; q head j reads
+ *   key-value head j / (h / h_kv); page_table (b, max_pages) int32, entries
+ *   past a sequence's last page are not read; lengths (b) int32.
+ * A length of 0 gives o = 0 and lse = -inf.  A length outside
+ * [0, max_pages * page_size], or a page outside [0, n_pages) in use, gives
+ * NaN for that sequence (heads of that key-value head at least) and
+ * WF_ERR_INVALID_ARG from wf_device_status.
+ * Two launches; overlapping calls need workspaces of their own.
+ */
+int wf_decode(const void* q, const void* k_cache, const void* v_cache, const int* page_table, const int* lengths,
+              void* o, float* lse, void* workspace, size_t workspace_bytes, int b, int h, int h_kv,
+              const wf_decode_cfg* cfg, void* stream);
+
 /* Message for the last failed call on this thread (empty if none). */
 int wf_last_error(char* buf, int len);
 

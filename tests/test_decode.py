@@ -1,0 +1,208 @@
+"""Paged decode attention against attention in 64 bits: lengths from nothing to
+several CTAs' runs, page sizes that end inside a tile, grouped heads, strided
+caches, impossible lengths and pages, graphs, and refusals."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tests.attn64 import assert_close, attn64
+from wan_flash import _lib
+from wan_flash.decode import wan_flash_decode
+
+
+def make(lens, h, hk, page, seed=0, extra_width=0):
+    g = torch.Generator().manual_seed(seed)
+    per = [-(-n // page) for n in lens]
+    n_pages = sum(per) + 2
+    q = torch.randn(len(lens), h, 128, generator=g).to("cuda", torch.bfloat16)
+    k = torch.randn(n_pages, page, hk, 128, generator=g).to("cuda", torch.bfloat16)
+    v = torch.randn(n_pages, page, hk, 128, generator=g).to("cuda", torch.bfloat16)
+    order = torch.randperm(n_pages, generator=g).tolist()
+    # entries past a sequence's last page are not read: they point nowhere
+    table = torch.full((len(lens), max(per + [0]) + extra_width), 2**31 - 1, dtype=torch.int32)
+    for i, n in enumerate(per):
+        for j in range(n):
+            table[i, j] = order.pop()
+    return q, k, v, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def check(q, k, v, table, lengths, o, lse):
+    page = k.shape[1]
+    for i, n in enumerate(lengths.tolist()):
+        at = torch.arange(n, device="cuda")
+        pg = table[i].long()[at // page] if n else at
+        r = attn64(q[i:i + 1], k[pg, at % page], v[pg, at % page])
+        assert_close(o[i:i + 1], r["o"], r["o_tol"], f"o[{i}] of {n}")
+        assert_close(lse[i][:, None], r["lse"], r["lse_tol"], f"lse[{i}] of {n}")
+
+
+def test_refusals():
+    q = torch.zeros(2, 4, 128, dtype=torch.bfloat16)
+    c = torch.zeros(3, 8, 2, 128, dtype=torch.bfloat16)
+    t, n = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for bad in (
+        (q, c, c, t, n),                        # CPU tensors
+        (q.float(), c, c, t, n),
+        (q[..., :64], c, c, t, n),
+        (q[:, :3], c, c, t, n),                 # 3 heads over 2
+        (q, c, c[:2], t, n),
+        (q, c, c, t[:1], n),
+        (q, c, c, t.long(), n),
+        (q, c, c, t, n.long()),
+        (q, c, c, t, n[:1]),
+        (q, c[:, :0], c[:, :0], t, n),
+        (q, c.transpose(2, 3).contiguous().transpose(2, 3), c, t, n),  # rows not contiguous
+    ):
+        with pytest.raises(AssertionError):
+            wan_flash_decode(*bad)
+
+
+def test_c_entry_refusals():
+    lib = _lib.lib()
+
+    def call(q=16, h=4, hk=2, b=1, ws=1 << 30, **kw):
+        cfg = _lib.DecodeCfg(3, 8, 3, 0, 3, 2048, 256, 128, 2048, 256, 128)
+        for key, x in kw.items():
+            setattr(cfg, key, x)
+        p = ctypes.c_void_p
+        return lib.wf_decode(p(q) if q else None, p(16), p(16), p(16), p(16), p(16), p(16), p(16), ws, b, h, hk,
+                             ctypes.byref(cfg), None)
+
+    assert call(b=-1) == -1 and call(h=3) == -1 and call(page_size=0) == -1 and call(q=None) == -1
+    assert call(q=24) == -3 and call(k_slot_stride=130) == -3 and call(max_pages=2**30, page_size=2) == -2
+    assert call(b=0) == 0
+    assert lib.wf_decode_workspace(4, 3, ctypes.byref(ctypes.c_size_t())) == -1
+
+
+CASES = [
+    # lengths, h, h_kv, page size
+    ([1], 1, 1, 1),
+    ([0], 2, 1, 16),
+    ([63, 64, 65, 0, 1], 4, 4, 16),
+    ([300], 12, 12, 7),
+    ([17, 1000, 129, 0, 4095], 10, 2, 100),
+    ([2000, 3], 8, 1, 64),
+    ([700, 15], 16, 1, 128),
+    ([513, 40], 24, 1, 32),
+    ([513, 40], 32, 1, 256),
+    ([260, 1], 40, 1, 3),       # two blocks of 20 heads
+    ([5000], 3, 3, 1),
+    ([20000, 100], 5, 1, 500),  # one row over many CTAs
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,h,hk,page", CASES)
+def test_against_64_bits(lens, h, hk, page):
+    x = make(lens, h, hk, page, extra_width=1)
+    o, lse = wan_flash_decode(*x)
+    _lib.check_device()
+    assert o.dtype == torch.bfloat16 and lse.dtype == torch.float32
+    check(*x, o, lse)
+    again, lse2 = wan_flash_decode(*x)
+    assert torch.equal(o, again) and torch.equal(lse, lse2)  # the split has a fixed order
+
+
+@pytest.mark.gpu
+def test_many_short_sequences():
+    lens = [(i * 37) % 90 for i in range(700)]
+    x = make(lens, 2, 1, 16)
+    o, lse = wan_flash_decode(*x)
+    _lib.check_device()
+    check(*x, o, lse)
+
+
+@pytest.mark.gpu
+def test_large_scores_and_garbage_behind_the_end():
+    """Scores of hundreds (the running maximum moves) and NaN / infinities in every slot that is not in use."""
+    q, k, v, table, lengths = make([130, 77, 1], 6, 2, 16)
+    q *= 8
+    k *= 8
+    used = torch.zeros(k.shape[:2], dtype=torch.bool, device="cuda")
+    for i, n in enumerate(lengths.tolist()):
+        at = torch.arange(n, device="cuda")
+        used[table[i].long()[at // 16], at % 16] = True
+    k[~used], v[~used] = float("nan"), float("inf")
+    o, lse = wan_flash_decode(q, k, v, table, lengths)
+    _lib.check_device()
+    check(q, k, v, table, lengths, o, lse)
+
+
+@pytest.mark.gpu
+def test_strided_cache_and_queries():
+    q, k, v, table, lengths = make([100, 5], 4, 2, 8)
+    want = wan_flash_decode(q, k, v, table, lengths)
+    both = torch.stack((k, v), 1)                                   # (pages, 2, page, h_kv, 128)
+    heads_first = k.transpose(1, 2).contiguous().transpose(1, 2)    # (pages, h_kv, page, 128) in memory
+    wide = torch.zeros(2, 4, 256, device="cuda", dtype=torch.bfloat16)
+    wide[..., :128] = q
+    for args in ((q, both[:, 0], both[:, 1]), (q, heads_first, v), (wide[..., :128], k, v)):
+        got = wan_flash_decode(*args, table, lengths)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    tall = torch.zeros(2, 2 * table.shape[1], device="cuda", dtype=torch.int32)
+    tall[:, ::2] = table
+    got = wan_flash_decode(q, k, v, tall[:, ::2], lengths)
+    assert torch.equal(got[0], want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["page", "negative page", "length", "negative length"])
+def test_impossible_pages_and_lengths(what):
+    q, k, v, table, lengths = make([100, 50, 33], 4, 2, 16)
+    if what == "page":
+        table[1, 2] = k.shape[0]
+    elif what == "negative page":
+        table[1, 0] = -5
+    elif what == "length":
+        lengths[1] = table.shape[1] * 16 + 1
+    else:
+        lengths[1] = -1
+    o, lse = wan_flash_decode(q, k, v, table, lengths)
+    with pytest.raises(_lib.WanFlashError):
+        _lib.check_device()
+    assert o[1].isnan().all() and lse[1].isnan().all()
+    rest = [0, 2]  # the others are not touched by it
+    check(q[rest], k, v, table[rest], lengths[rest], o[rest], lse[rest])
+    _lib.check_device()
+
+
+@pytest.mark.gpu
+def test_captured_graphs_side_by_side_with_changing_lengths():
+    xs = [make([90, 300], 4, 2, 16, seed=s) for s in range(2)]
+    want = [wan_flash_decode(*x) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            wan_flash_decode(*x)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(wan_flash_decode(*x))
+        graphs.append((graph, side))
+    for _ in range(5):  # both at once: workspaces of their own
+        for graph, side in graphs:
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (o, lse), (wo, wl) in zip(outs, want):
+        assert torch.equal(o, wo) and torch.equal(lse, wl)
+    xs[0][4].copy_(torch.tensor([1, 299], dtype=torch.int32))
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    _lib.check_device()
+    check(*xs[0], *outs[0])
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    q, k, v, table, lengths = make([4], 4, 2, 16)
+    o, lse = wan_flash_decode(q[:0], k, v, table[:0], lengths[:0])
+    assert o.shape == (0, 4, 128) and lse.shape == (0, 4)
+    # an empty cache with empty sequences
+    o, lse = wan_flash_decode(q, k[:0], v[:0], table[:, :0], lengths * 0)
+    _lib.check_device()
+    assert (o == 0).all() and (lse == float("-inf")).all()

@@ -1,0 +1,187 @@
+"""Rotary positions: the table and the positions, the kernel against the
+complex product in 64 bits, its gradients, strides, padding and refusals."""
+
+import pytest
+import torch
+
+from wan_flash import _lib
+from wan_flash.rope import AXES, rope_positions, rope_table, wan_flash_rope
+
+
+def turned64(x, positions, theta=10000.0, axes=AXES, sign=1.0):
+    """x (..., s, h, 128) times exp(i angle), angles from the definition in fp64."""
+    f = [theta ** (-torch.arange(0, d, 2, dtype=torch.float64, device=x.device) / max(d, 1)) for d in axes]
+    pos = positions.double()
+    angle = torch.cat([pos[..., a:a + 1] * f[a] for a in range(3)], -1)
+    angle = torch.where((positions < 0).any(-1, keepdim=True), 0.0, angle)[..., None, :]
+    z = torch.view_as_complex(x.double().reshape(*x.shape[:-1], 64, 2))
+    return torch.view_as_real(z * torch.polar(torch.ones_like(angle), sign * angle)).flatten(-2)
+
+
+def rope_tol(x, want):
+    """One rounding of the result to x's type, and fp32 products of table entries
+    that are half an fp32 step off: (2 * 2^-24 + 2^-24) of each of the pair's values."""
+    pair = x.double().reshape(*x.shape[:-1], 64, 2).abs().sum(-1, keepdim=True).expand(*x.shape[:-1], 64, 2).flatten(-2)
+    return torch.finfo(x.dtype).eps / 2 * want.abs() * (1 + 2**-7) + 4 * 2.0**-24 * pair
+
+
+def test_table_and_positions():
+    t = rope_table(50, theta=100.0, axes=(64, 0, 64))
+    assert t.shape == (50, 64, 2) and t.dtype == torch.float32
+    for p, i in ((0, 0), (49, 0), (49, 31), (7, 32), (33, 63)):
+        angle = torch.tensor(p * 100.0 ** (-2 * (i % 32) / 64), dtype=torch.float64)
+        assert abs(t[p, i, 0].item() - angle.cos().item()) <= 2**-24
+        assert abs(t[p, i, 1].item() - angle.sin().item()) <= 2**-24
+    pos = rope_positions((2, 3, 4))
+    assert pos.dtype == torch.int32 and pos.tolist() == [[a, b, c] for a in range(2) for b in range(3) for c in range(4)]
+    # a shard, a continued clip, and padding behind the grid
+    assert rope_positions((2, 3, 4), start=22, count=4, first_frame=5).tolist() == [[6, 2, 2], [6, 2, 3], [-1] * 3, [-1] * 3]
+    assert rope_positions((0, 3, 4)).shape == (0, 3)
+    with pytest.raises(AssertionError):
+        rope_table(10, axes=(64, 32, 31))
+    with pytest.raises(AssertionError):
+        rope_positions((1, 2, 3), start=-1)
+
+
+def test_refusals():
+    q, pos, table = torch.zeros(1, 4, 2, 128, dtype=torch.bfloat16), torch.zeros(4, 3, dtype=torch.int32), rope_table(8)
+    for bad in (
+        (q, q, pos, table),                                    # CPU tensors
+        (q.half(), q.half(), pos, table),
+        (q, q.float(), pos, table),
+        (q[..., :64], q[..., :64], pos, table),
+        (q, q[:, :3], pos, table),                             # another number of tokens
+        (q, q, pos[:3], table),
+        (q, q, pos.long(), table),
+        (q, q, pos, table.double()),
+        (q, q, pos, table[:, :32]),
+        (q, q, pos, table[:0]),
+        (q, q, pos, table, (44, 42, 40)),
+    ):
+        with pytest.raises(AssertionError):
+            wan_flash_rope(*bad)
+
+
+def test_c_entry_refusals():
+    import ctypes
+
+    lib = _lib.lib()
+
+    def call(q=16, b=1, s=4, h=2, hk=2, null_cfg=False, **kw):
+        cfg = _lib.RopeCfg(0, 0, 8, 22, 21, 0, 1024, 256, 128, 1024, 256, 128, 0)
+        for k, v in kw.items():
+            setattr(cfg, k, v)
+        p = ctypes.c_void_p
+        return lib.wf_rope(p(q) if q else None, p(32), p(48), p(64), p(80), p(96), b, s, h, hk,
+                           None if null_cfg else ctypes.byref(cfg), None)
+
+    assert call(s=-1) == -1 and call(null_cfg=True) == -1 and call(dtype=7) == -2 and call(max_pos=0) == -1
+    assert call(pairs_t=60) == -1 and call(q=None) == -1 and call(h=70000) == -2
+    assert call(q=24) == -3 and call(q_stride_s=250) == -3
+    assert call(b=0) == 0 and call(s=0) == 0  # nothing to do
+
+
+CASES = [
+    # b, grid, pad, h, hk
+    (1, (1, 1, 1), 0, 1, 1),
+    (2, (3, 5, 7), 2, 3, 1),
+    (1, (2, 30, 52), 0, 12, 12),
+    (3, (1, 9, 11), 5, 40, 8),
+    (1, (1, 3, 3), 0, 0, 2),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("b,grid,pad,h,hk", CASES)
+def test_forward_and_gradients(b, grid, pad, h, hk, dtype):
+    n = grid[0] * grid[1] * grid[2]
+    g = torch.Generator().manual_seed(n)
+    table = rope_table(1024, device="cuda")
+    pos = rope_positions(grid, count=n + pad, first_frame=900, device="cuda")
+    x = [torch.randn(b, n + pad, hh, 128, generator=g).to("cuda", dtype) for hh in (h, hk, h, hk)]
+    q, k = x[0].requires_grad_(), x[1].requires_grad_()
+    yq, yk = wan_flash_rope(q, k, pos, table)
+    gq, gk = torch.autograd.grad((yq, yk), (q, k), (x[2], x[3]))
+    _lib.check_device()
+    for src, got, sign in ((q, yq, 1), (k, yk, 1), (x[2], gq, -1), (x[3], gk, -1)):
+        want = turned64(src.detach(), pos, sign=sign)
+        assert got.dtype == dtype and got.is_contiguous() and got.shape == src.shape
+        assert ((got.detach().double() - want).abs() <= rope_tol(src.detach(), want)).all()
+    if pad:
+        assert torch.equal(yq[:, n:], q[:, n:])  # padding passes bit for bit
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    table, pos = rope_table(64, device="cuda"), rope_positions((2, 2, 3), device="cuda")
+    g = torch.Generator().manual_seed(3)
+    q, k, w, dq = (torch.randn(12, 2, 128, generator=g).cuda() for _ in range(4))
+    q.requires_grad_()
+    loss = (wan_flash_rope(q, k, pos, table)[0] * w).sum()
+    (grad,) = torch.autograd.grad(loss, q)
+    # the map is linear: a central difference is exact but for rounding.  Each term
+    # |w y| is off by a few fp32 steps of (|x0| + |x1|) |w|
+    up = (wan_flash_rope(q.detach() + dq, k, pos, table)[0].double() * w.double()).sum()
+    down = (wan_flash_rope(q.detach() - dq, k, pos, table)[0].double() * w.double()).sum()
+    got, want = (grad.double() * dq.double()).sum().item(), ((up - down) / 2).item()
+    tol = 8 * 2.0**-24 * 4 * ((q.detach().abs() + dq.abs()) * w.abs()).double().sum().item()
+    assert abs(got - want) <= tol
+
+
+@pytest.mark.gpu
+def test_strided_packed_and_per_item_positions():
+    g = torch.Generator().manual_seed(5)
+    table = rope_table(128, device="cuda")
+    qkv = torch.randn(2, 10, 3, 4, 128, generator=g).to("cuda", torch.bfloat16)
+    pos = torch.stack([rope_positions((1, 2, 5), device="cuda"), rope_positions((10, 1, 1), first_frame=7, device="cuda")])
+    q, k = qkv[:, :, 0], qkv[:, :, 1]  # slices of a fused projection, read by their strides
+    yq, yk = wan_flash_rope(q, k, pos, table)
+    for src, got in ((q, yq), (k, yk)):
+        want = turned64(src, pos)
+        assert ((got.double() - want).abs() <= rope_tol(src, want)).all()
+    # one packed sequence is the item without its batch dim; a misaligned or transposed view is copied
+    a, b = wan_flash_rope(q[1], k[1], pos[1], table)
+    assert torch.equal(a, yq[1]) and torch.equal(b, yk[1])
+    flat = torch.zeros(2 * 10 * 4 * 128 + 1, device="cuda", dtype=torch.bfloat16)
+    odd = flat[1:].view(2, 10, 4, 128).copy_(q)
+    assert torch.equal(wan_flash_rope(odd, k, pos, table)[0], yq)
+    swapped = q.transpose(1, 3).contiguous().transpose(1, 3)
+    assert torch.equal(wan_flash_rope(swapped, k, pos, table)[0], yq)
+    # heads broadcast from one
+    one = q[:, :, :1].expand(2, 10, 4, 128)
+    assert torch.equal(wan_flash_rope(one, k, pos, table)[0], yq[:, :, :1].expand(2, 10, 4, 128))
+    _lib.check_device()
+
+
+@pytest.mark.gpu
+def test_far_position_is_an_error_of_its_token_only():
+    table = rope_table(16, device="cuda")
+    pos = torch.tensor([[1, 2, 3], [1, 16, 3], [15, 15, 15]], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 2, 128, device="cuda")
+    y, _ = wan_flash_rope(q, q, pos, table)
+    with pytest.raises(_lib.WanFlashError):
+        _lib.check_device()
+    assert y[1].isnan().all() and y[[0, 2]].isfinite().all()
+    _lib.check_device()  # the read cleared it
+
+
+@pytest.mark.gpu
+def test_graph_replay_and_other_stream():
+    table, pos = rope_table(64, device="cuda"), rope_positions((4, 4, 4), device="cuda")
+    q, k = (torch.randn(64, 3, 128, device="cuda") for _ in range(2))
+    want = wan_flash_rope(q, k, pos, table)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = wan_flash_rope(q, k, pos, table)
+        graph = torch.cuda.CUDAGraph()
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            out = wan_flash_rope(q, k, pos, table)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], -want[0]) and torch.equal(out[1], want[1])

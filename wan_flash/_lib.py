@@ -30,6 +30,7 @@ STATUS_NAMES = {
 EXPORTS = (
     "wf_fwd", "wf_fwd_dual", "wf_bwd_pre", "wf_bwd_main", "wf_bwd_convert", "wf_bwd_noalloc", "wf_last_error",
     "wf_device_status", "wf_set_wait_limit_ns", "wf_selftest_wait_timeout", "wf_num_sms", "wf_version",
+    "wf_rope", "wf_decode", "wf_decode_workspace",
 )
 
 
@@ -41,6 +42,22 @@ class FwdCfg(ctypes.Structure):
 class BwdCfg(ctypes.Structure):
     _fields_ = [("nsplit", ctypes.c_int), ("cluster_n", ctypes.c_int), ("deterministic", ctypes.c_int),
                 ("pdl_off", ctypes.c_int), ("sem", ctypes.c_void_p)]
+
+
+class RopeCfg(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("inverse", ctypes.c_int), ("max_pos", ctypes.c_int),
+                ("pairs_t", ctypes.c_int), ("pairs_h", ctypes.c_int), ("reserved", ctypes.c_int),
+                ("q_stride_b", ctypes.c_longlong), ("q_stride_s", ctypes.c_longlong), ("q_stride_h", ctypes.c_longlong),
+                ("k_stride_b", ctypes.c_longlong), ("k_stride_s", ctypes.c_longlong), ("k_stride_h", ctypes.c_longlong),
+                ("pos_stride_b", ctypes.c_longlong)]
+
+
+class DecodeCfg(ctypes.Structure):
+    _fields_ = [("n_pages", ctypes.c_int), ("page_size", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("reserved", ctypes.c_int), ("table_stride", ctypes.c_longlong),
+                ("k_page_stride", ctypes.c_longlong), ("k_slot_stride", ctypes.c_longlong),
+                ("k_head_stride", ctypes.c_longlong), ("v_page_stride", ctypes.c_longlong),
+                ("v_slot_stride", ctypes.c_longlong), ("v_head_stride", ctypes.c_longlong)]
 
 
 class WanFlashError(RuntimeError):
@@ -62,6 +79,9 @@ def _declare(lib):
     lib.wf_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint)]
     lib.wf_set_wait_limit_ns.argtypes = [ctypes.c_ulonglong]
     lib.wf_selftest_wait_timeout.argtypes = [ctypes.c_ulonglong, ctypes.POINTER(ctypes.c_uint)]
+    lib.wf_rope.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, ctypes.POINTER(RopeCfg), vp]
+    lib.wf_decode_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
+    lib.wf_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, ctypes.POINTER(DecodeCfg), vp]
     for name in EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     del fp

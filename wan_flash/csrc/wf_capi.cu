@@ -90,6 +90,8 @@ int device_setup(int* dev_out) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(bwd smem)");
   e = cudaFuncSetAttribute(wf_bwd2_main_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd2_smem_bytes());
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(bwd pair smem)");
+  e = decode_setup();
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode smem)");
   g_dev_sms[dev] = sms;
   g_dev_ready[dev] = true;
   return WF_OK;

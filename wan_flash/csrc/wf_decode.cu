@@ -1,0 +1,596 @@
+// Attention of one new token per sequence over a paged key-value cache:
+// wf_decode (declared in include/wan_flash.h).
+//
+//     o[b, h] = softmax(q[b, h] K_b^T / sqrt(128)) V_b,   lse[b, h]
+// with K_b, V_b the first lengths[b] tokens of sequence b, token t in slot
+// t % page_size of page page_table[b][t / page_size].
+//
+// Bound: HBM (512 bytes of K and V per token and key-value head against
+// 512 * h / h_kv flops).  The q heads of one key-value head are served by
+// one read of its K and V; tensor cores (mma.sync) do the products so that
+// grouped heads cost no more issue slots than one head: S^T = K q^T has 16
+// tokens as M and 8 q heads as N, O^T = V^T P^T 16 dims as M, so nothing is
+// padded beyond 8 heads.  tcgen05's M of 64-128 rows would leave the tensor
+// pipe as idle and add a trip through tensor memory.
+//
+// Split: the work is cut by tiles of 64 tokens, not by sequences.  The tiles
+// of all (sequence, key-value head[, block of heads]) rows stand one behind
+// the other and every CTA takes an equal run of them, whatever the lengths;
+// a row that spans several CTAs leaves partial results (running maximum,
+// sum, unnormalised O, all fp32) which a second kernel joins in a fixed
+// order, so results do not depend on timing.
+#include "wf_common.cuh"
+#include "wf_kernels.h"
+
+namespace wf {
+
+namespace dec {
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 64;                       // tokens of a CTA's tile: 16 per warp
+constexpr int kStages = 3;                      // per-warp ring of 16-token K and V tiles
+constexpr uint32_t kHalfBytes = 16 * 256;       // 16 tokens of K (or V)
+constexpr uint32_t kStageBytes = 2 * kHalfBytes;
+constexpr uint32_t kRingBytes = kWarps * kStages * kStageBytes;  // 96 KB; the join reuses it
+constexpr int kMaxHeads = 32;                   // q heads of a row (4 n-tiles of 8)
+constexpr uint32_t kOffML = kRingBytes;         // [warp][head] running max, then sum
+constexpr uint32_t kSmemBytes = kRingBytes + 2 * kWarps * kMaxHeads * 4 + 64;
+constexpr int kCtasPerSm = 2;
+constexpr int kOPitch = 132;                    // floats per head in the join buffer (128 + 4 against bank conflicts)
+static_assert(kWarps * kMaxHeads * kOPitch * 4 <= kRingBytes, "the join buffer fits in the ring");
+}  // namespace dec
+
+struct DecodeParams {
+  const __nv_bfloat16* q;    // (b, h, 128)
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  long long page_stride[2], slot_stride[2], head_stride[2];  // K, V, in elements
+  const int* page_table;
+  long long table_stride;
+  const int* lengths;
+  __nv_bfloat16* o;          // (b, h, 128)
+  float* lse;                // (b, h)
+  float* part_o;             // (2 * ctas, heads_per_row, 128) unnormalised O
+  float* part_ml;            // (2 * ctas, heads_per_row, 2) running max (scaled log2 units) and sum
+  int4* join;                // per CTA: row that starts there and ends elsewhere (or -1), last CTA of it
+  int b, h, h_kv, group;     // group = h / h_kv
+  int blocks;                // blocks of heads_per_row q heads per key-value head
+  int heads_per_row;
+  int n_pages, page_size, max_pages;
+  float scale_log2;
+};
+
+namespace {
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  // src-size 0: the 16 bytes become zeros and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A length outside [0, max_pages * page_size] counts as 0 tokens (its rows
+// are written as NaN).
+__device__ __forceinline__ bool decode_length_ok(const DecodeParams& p, int len) {
+  return len >= 0 && (long long)len <= (long long)p.max_pages * p.page_size;
+}
+__device__ __forceinline__ int decode_length(const DecodeParams& p, int seq) {
+  const int len = __ldg(p.lengths + seq);
+  return decode_length_ok(p, len) ? len : 0;
+}
+__device__ __forceinline__ int decode_tiles(int len) { return (len + dec::kTile - 1) / dec::kTile; }
+
+}  // namespace
+
+// kN: n-tiles of 8 q heads that a row has.
+template <int kN>
+__global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kernel(DecodeParams p) {
+  using namespace dec;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ long long s_scan[kWarps + 1];
+  __shared__ long long s_start[2];  // tiles before the first sequence of this CTA's run; that sequence
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t sbase = smem_u32(smem);
+  const int rows_per_seq = p.h_kv * p.blocks;
+  griddep_launch_dependents();
+
+  // ---- this CTA's run [lo, hi) of the tiles of all rows
+  const int per_thread = (p.b + kThreads - 1) / kThreads;
+  const int s0 = min(p.b, (int)threadIdx.x * per_thread), s1 = min(p.b, s0 + per_thread);
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) mine += (long long)decode_tiles(decode_length(p, s)) * rows_per_seq;
+  long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += up;
+  }
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  before += incl - mine;
+  // with fewer tiles than CTAs the first `total` CTAs take one each, so a row's CTAs are neighbours
+  const long long ctas = min((long long)gridDim.x, max(total, 1LL));
+  const long long cta = min((long long)blockIdx.x, ctas);
+  const long long lo = total * cta / ctas, hi = total * min(cta + 1, ctas) / ctas;
+  if (lo < hi && before <= lo && lo < before + mine) {
+    long long at = before;
+    for (int s = s0; s < s1; ++s) {
+      const long long t = (long long)decode_tiles(decode_length(p, s)) * rows_per_seq;
+      if (lo < at + t) {
+        s_start[0] = at;
+        s_start[1] = s;
+        break;
+      }
+      at += t;
+    }
+  }
+  __syncthreads();
+
+  // ---- sequences with nothing cached: o = 0, lse = -inf (NaN where the length is impossible)
+  for (int s = blockIdx.x; s < p.b; s += gridDim.x) {
+    const int len = __ldg(p.lengths + s);
+    if (len > 0 && decode_length_ok(p, len)) continue;
+    const bool bad = !decode_length_ok(p, len);
+    if (bad && threadIdx.x == 0 && atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
+      g_err_info[0] = (unsigned)s;
+      g_err_info[1] = (unsigned)len;
+      g_err_info[2] = kRoleDecode;
+      g_err_info[3] = 1u;
+    }
+    uint4 fill = make_uint4(0u, 0u, 0u, 0u);
+    if (bad) fill = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+    uint4* dst = reinterpret_cast<uint4*>(p.o + (long long)s * p.h * 128);
+    for (int i = threadIdx.x; i < p.h * 16; i += kThreads) dst[i] = fill;
+    for (int i = threadIdx.x; i < p.h; i += kThreads)
+      p.lse[(long long)s * p.h + i] = bad ? __int_as_float(0x7fffffff) : -INFINITY;
+  }
+  if (lo >= hi) {
+    if (threadIdx.x == 0) p.join[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
+
+  const uint32_t ring = sbase + warp * (kStages * kStageBytes);
+  float* const s_m = reinterpret_cast<float*>(smem + kOffML);
+  float* const s_l = s_m + kWarps * kMaxHeads;
+  float* const s_o = reinterpret_cast<float*>(smem);
+  int4 join = make_int4(-1, 0, 0, 0);
+
+  int seq = (int)s_start[1];
+  long long seq_at = s_start[0];  // tiles before this sequence
+  for (long long at = lo; at < hi;) {
+    int len = decode_length(p, seq);
+    int n_tiles = decode_tiles(len);
+    while (at >= seq_at + (long long)n_tiles * rows_per_seq && seq + 1 < p.b) {
+      seq_at += (long long)n_tiles * rows_per_seq;
+      ++seq;
+      len = decode_length(p, seq);
+      n_tiles = decode_tiles(len);
+    }
+    if (at >= seq_at + (long long)n_tiles * rows_per_seq) break;  // lengths changed under the call
+    const int row = (int)((at - seq_at) / n_tiles);        // (key-value head, block of heads) of the sequence
+    const long long row_at = seq_at + (long long)row * n_tiles;
+    const int t0 = (int)(at - row_at);
+    const int t1 = (int)min((long long)n_tiles, hi - row_at);
+    const int kvh = row / p.blocks;
+    const int head0 = kvh * p.group + (row - kvh * p.blocks) * p.heads_per_row;
+    const int n_heads = min(p.heads_per_row, (kvh + 1) * p.group - head0);
+
+    // q as the B operand of S^T = K q^T: lane holds head lane/4, dims 16 ks + 2 (lane%4) + {0, 1, 8, 9}
+    uint32_t qf[kN][8][2];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int hd = n * 8 + (lane >> 2);
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((long long)seq * p.h + head0 + hd) * 128) + (lane & 3);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        qf[n][ks][0] = hd < n_heads ? __ldg(src + ks * 8) : 0u;
+        qf[n][ks][1] = hd < n_heads ? __ldg(src + ks * 8 + 4) : 0u;
+      }
+    }
+
+    // This warp's tokens of tile t: 64 t + 16 warp + [0, 16).  Lane j < 16
+    // finds token j's page; the row's 16 chunks of 16 bytes are copied by 16
+    // lanes, chunk c to place c ^ (row & 7) (ldmatrix without bank conflicts).
+    const int* table = p.page_table + (long long)seq * p.table_stride;
+    bool bad = false;
+    auto slot_of = [&](int t) -> int2 {  // (page, slot) of this lane's token; page -1 behind the end, -2 on a bad entry
+      const int tok = t * kTile + warp * 16 + (lane & 15);
+      if (t >= t1 || tok >= len) return make_int2(-1, 0);
+      const int pg = tok / p.page_size;
+      const int page = __ldg(table + pg);
+      if (page < 0 || page >= p.n_pages) return make_int2(-2, page);
+      return make_int2(page, tok - pg * p.page_size);
+    };
+    auto load = [&](int stage, int2 at_) {
+      if (at_.x == -2) {
+        bad = true;
+        if (atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
+          g_err_info[0] = (unsigned)seq;
+          g_err_info[1] = (unsigned)at_.y;
+          g_err_info[2] = kRoleDecode;
+          g_err_info[3] = 2u;
+        }
+      }
+      const uint32_t dst = ring + stage * kStageBytes;
+      const int c = lane & 15;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 2 * i + (lane >> 4);
+        const int page = __shfl_sync(0xffffffffu, at_.x, r), slot = __shfl_sync(0xffffffffu, at_.y, r);
+        const bool ok = page >= 0;
+        const uint32_t d = dst + r * 256 + ((c ^ (r & 7)) << 4);
+        const __nv_bfloat16* ks = p.k + (ok ? page * p.page_stride[0] + slot * p.slot_stride[0] : 0) + kvh * p.head_stride[0];
+        const __nv_bfloat16* vs = p.v + (ok ? page * p.page_stride[1] + slot * p.slot_stride[1] : 0) + kvh * p.head_stride[1];
+        cp_async16(d, ks + c * 8, ok);
+        cp_async16(d + kHalfBytes, vs + c * 8, ok);
+      }
+      cp_async_commit();
+    };
+
+    float m[kN][2], l[kN][2], acc[kN][8][4];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][d][i] = 0.f;
+    }
+    for (int s = 0; s < kStages - 1; ++s) load(s, slot_of(t0 + s));
+    int2 next = slot_of(t0 + kStages - 1);
+    int stage = 0;
+    for (int t = t0; t < t1; ++t) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      {
+        // refill the stage that the previous step read (every lane is past it)
+        int fill = stage + kStages - 1;
+        if (fill >= kStages) fill -= kStages;
+        load(fill, next);
+        next = slot_of(t + kStages);
+      }
+      const uint32_t sk = ring + stage * kStageBytes, sv = sk + kHalfBytes;
+      if (++stage == kStages) stage = 0;
+      const int tok0 = t * kTile + warp * 16;
+      if (tok0 >= len) continue;  // this warp has no token in the row's last tile
+      // S^T (16 tokens x 8 heads per n-tile)
+      float s[kN][4];
+#pragma unroll
+      for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      {
+        const int r = (lane & 7) + ((lane >> 3) & 1) * 8;  // matrices 0, 2: tokens 0-7; 1, 3: tokens 8-15
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const int c = 2 * ks + (lane >> 4);              // matrices 2, 3: dims 8-15 of the step
+          uint32_t a[4];
+          ldmatrix_x4(sk + r * 256 + ((c ^ (r & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) mma_16816(s[n], a, qf[n][ks][0], qf[n][ks][1]);
+        }
+      }
+      // online softmax over the tokens: rows lane/4 and lane/4 + 8, heads 2 (lane%4) + {0, 1}
+      const bool in0 = tok0 + (lane >> 2) < len, in1 = tok0 + (lane >> 2) + 8 < len;
+      uint32_t pb[kN][2];
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = (i < 2 ? in0 : in1) ? s[n][i] * p.scale_log2 : -INFINITY;
+        float pr[4];
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(s[n][e], s[n][2 + e]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[n][e], mx);
+          const float ref = mn == -INFINITY ? 0.f : mn;
+          f[e] = ex2_approx(m[n][e] - ref);
+          m[n][e] = mn;
+          pr[e] = ex2_approx(s[n][e] - ref);
+          pr[2 + e] = ex2_approx(s[n][2 + e] - ref);
+          l[n][e] = l[n][e] * f[e] + pr[e] + pr[2 + e];
+        }
+        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            acc[n][d][0] *= f[0];
+            acc[n][d][1] *= f[1];
+            acc[n][d][2] *= f[0];
+            acc[n][d][3] *= f[1];
+          }
+        }
+        // P^T (tokens x heads) to the B operand of O^T = V^T P^T: 8x8
+        // transposes within the warp.  P is rounded to bf16 for the tensor
+        // core (relative 2^-9, the rounding that o itself gets); the sum l
+        // keeps the fp32 values.
+        pb[n][0] = movmatrix_trans(pack_bf16(pr[0], pr[1]));
+        pb[n][1] = movmatrix_trans(pack_bf16(pr[2], pr[3]));
+      }
+      // O^T (16 dims x 8 heads) += V^T P^T
+      {
+        const int r = (lane & 7) + (lane >> 4) * 8;        // matrices 0, 1: tokens 0-7; 2, 3: tokens 8-15
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const int c = 2 * d + ((lane >> 3) & 1);         // matrices 1, 3: dims 8-15 of the tile
+          uint32_t a[4];
+          ldmatrix_x4_trans(sv + r * 256 + ((c ^ (r & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) mma_16816(acc[n][d], a, pb[n][0], pb[n][1]);
+        }
+      }
+    }
+    cp_async_wait<0>();
+    bad = __any_sync(0xffffffffu, bad);
+    // ---- join the four warps' results
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[n][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (bad) x = __int_as_float(0x7fffffff);
+        l[n][e] = x;
+        if (lane < 4) {
+          s_m[warp * kMaxHeads + n * 8 + 2 * lane + e] = m[n][e];
+          s_l[warp * kMaxHeads + n * 8 + 2 * lane + e] = x;
+        }
+      }
+    __syncthreads();  // every warp is past its ring: it becomes the join buffer
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int hd = n * 8 + 2 * (lane & 3) + e;
+        float top = s_m[hd];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * kMaxHeads + hd]);
+        f[e] = ex2_approx(m[n][e] - (top == -INFINITY ? 0.f : top));
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int hd = n * 8 + 2 * (lane & 3) + (i & 1);
+          s_o[(warp * (8 * kN) + hd) * kOPitch + d * 16 + (lane >> 2) + (i >> 1) * 8] = acc[n][d][i] * f[i & 1];
+        }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == n_tiles;
+    const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+    // thread = 4 dims of a head; a warp writes one head's 128
+    for (int hd = warp; hd < n_heads; hd += kWarps) {
+      float top = s_m[hd];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * kMaxHeads + hd]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        sum += s_l[w * kMaxHeads + hd] * ex2_approx(s_m[w * kMaxHeads + hd] - ref);
+        const float4 y = *reinterpret_cast<const float4*>(s_o + (w * (8 * kN) + hd) * kOPitch + lane * 4);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      }
+      if (whole) {
+        const float inv = 1.f / sum;  // a row with tokens has a sum >= 1 (or NaN)
+        uint2 w2;
+        w2.x = pack_bf16(x.x * inv, x.y * inv);
+        w2.y = pack_bf16(x.z * inv, x.w * inv);
+        const long long out = (long long)seq * p.h + head0 + hd;
+        *reinterpret_cast<uint2*>(p.o + out * 128 + lane * 4) = w2;
+        if (lane == 0) p.lse[out] = (top + log2f(sum)) * 0.69314718055994531f;
+      } else {
+        const long long out = (long long)slot * p.heads_per_row + hd;
+        *reinterpret_cast<float4*>(p.part_o + out * 128 + lane * 4) = x;
+        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + out * 2) = make_float2(top, sum);
+      }
+    }
+    if (t0 == 0 && t1 < n_tiles) {
+      // the CTA whose run holds tile row_at + n_tiles - 1 ends the row
+      const long long last = row_at + n_tiles - 1;
+      long long e = (last * ctas) / total;
+      while (total * (e + 1) / ctas <= last) ++e;
+      while (total * e / ctas > last) --e;
+      join = make_int4(head0, n_heads, (int)e, seq);
+    }
+    __syncthreads();  // the join buffer is read: the ring may be filled again
+    at = row_at + t1;
+  }
+  if (threadIdx.x == 0) p.join[blockIdx.x] = join;
+}
+
+// Joins the rows that span several CTAs: block (c, head) takes the row that
+// starts in CTA c's run (slot 1 of c, slot 0 of the CTAs behind it); block
+// (c, y) its heads y, y + gridDim.y, ...
+__global__ void __launch_bounds__(256) wf_decode_join_kernel(DecodeParams p) {
+  griddep_wait();
+  const int c = blockIdx.x;
+  const int4 j = p.join[c];
+  if (j.x < 0) return;
+  const int n = j.z - c + 1;
+  __shared__ float s_red[8];
+  __shared__ float4 s_acc[8][32];
+  __shared__ float s_sum[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int hd = blockIdx.y; hd < j.y; hd += gridDim.y) {
+    auto slot = [&](int i) -> long long { return (long long)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.heads_per_row + hd; };
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, p.part_ml[slot(i) * 2]);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (lane == 0) s_red[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_red[w]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < n; i += 8) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
+      const float4 y = *reinterpret_cast<const float4*>(p.part_o + slot(i) * 128 + lane * 4);
+      const float f = ex2_approx(ml.x - ref);
+      sum += ml.y * f;
+      x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+    }
+    s_acc[warp][lane] = x;
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      sum = 0.f;
+      x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float4 y = s_acc[w][lane];
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        sum += s_sum[w];
+      }
+      const float inv = 1.f / sum;
+      uint2 w2;
+      w2.x = pack_bf16(x.x * inv, x.y * inv);
+      w2.y = pack_bf16(x.z * inv, x.w * inv);
+      const long long out = (long long)j.w * p.h + j.x + hd;
+      *reinterpret_cast<uint2*>(p.o + out * 128 + lane * 4) = w2;
+      if (lane == 0) p.lse[out] = (top + log2f(sum)) * 0.69314718055994531f;
+    }
+    __syncthreads();
+  }
+}
+
+namespace {
+
+int decode_rows(int h, int h_kv, int* blocks, int* heads_per_row) {
+  if (h < 1 || h_kv < 1 || h % h_kv) return fail(WF_ERR_INVALID_ARG, "h=%d is not a multiple of h_kv=%d", h, h_kv);
+  const int group = h / h_kv;
+  *blocks = (group + dec::kMaxHeads - 1) / dec::kMaxHeads;
+  *heads_per_row = (group + *blocks - 1) / *blocks;
+  return WF_OK;
+}
+
+template <int kN>
+int decode_launch(const DecodeParams& p, int ctas, cudaStream_t st) {
+  wf_decode_kernel<kN><<<ctas, dec::kThreads, dec::kSmemBytes, st>>>(p);
+  int rc = launch_check("wf_decode launch");
+  if (rc) return rc;
+  cudaError_t e = launch_ex(wf_decode_join_kernel, dim3(ctas, std::min(p.heads_per_row, 8)), dim3(256), 0, st, true, 1u, p);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_decode join launch");
+  return launch_check("wf_decode join launch");
+}
+
+// workspace: join descriptors, then (max, sum) pairs, then O of two partial rows per CTA
+size_t decode_workspace_bytes(int ctas, int heads_per_row) {
+  return (size_t)ctas * 16 + (size_t)2 * ctas * heads_per_row * (8 + 512);
+}
+
+}  // namespace
+
+// One-time per-device set-up (from device_setup, with that device current).
+cudaError_t decode_setup() {
+  cudaError_t e = cudaSuccess;
+  for (auto k : {wf_decode_kernel<1>, wf_decode_kernel<2>, wf_decode_kernel<3>, wf_decode_kernel<4>})
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec::kSmemBytes);
+  return e;
+}
+}  // namespace wf
+
+extern "C" int wf_decode_workspace(int h, int h_kv, size_t* bytes) {
+  using namespace wf;
+  if (!bytes) return fail(WF_ERR_INVALID_ARG, "null pointer");
+  int blocks, heads, dev, rc;
+  if ((rc = decode_rows(h, h_kv, &blocks, &heads))) return rc;
+  if ((rc = device_setup(&dev))) return rc;
+  *bytes = decode_workspace_bytes(g_dev_sms[dev] * dec::kCtasPerSm, heads);
+  return WF_OK;
+}
+
+extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache, const int* page_table,
+                         const int* lengths, void* o, float* lse, void* workspace, size_t workspace_bytes, int b, int h,
+                         int h_kv, const wf_decode_cfg* cfg, void* stream) {
+  using namespace wf;
+  if (b < 0 || h < 0 || h_kv < 0) return fail(WF_ERR_INVALID_ARG, "negative size");
+  if (!cfg) return fail(WF_ERR_INVALID_ARG, "null cfg");
+  if (cfg->n_pages < 0 || cfg->page_size < 1 || cfg->max_pages < 0)
+    return fail(WF_ERR_INVALID_ARG, "n_pages %d, page_size %d, max_pages %d", cfg->n_pages, cfg->page_size, cfg->max_pages);
+  if ((long long)cfg->page_size * cfg->max_pages > 0x7fffffffLL - 1024)
+    return fail(WF_ERR_UNSUPPORTED, "max_pages * page_size = %lld tokens exceed 2^31 - 1025",
+                (long long)cfg->page_size * cfg->max_pages);
+  if (b == 0 || h == 0) return WF_OK;
+  DecodeParams p;
+  int rc, dev;
+  if ((rc = decode_rows(h, h_kv, &p.blocks, &p.heads_per_row))) return rc;
+  if (!q || !lengths || !o || !lse || !workspace || (cfg->max_pages > 0 && !page_table) ||
+      (cfg->n_pages > 0 && (!k_cache || !v_cache)))
+    return fail(WF_ERR_INVALID_ARG, "null pointer");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || !aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(lengths) & 3) ||
+      (reinterpret_cast<uintptr_t>(page_table) & 3) || cfg->k_page_stride % 8 || cfg->k_slot_stride % 8 ||
+      cfg->k_head_stride % 8 || cfg->v_page_stride % 8 || cfg->v_slot_stride % 8 || cfg->v_head_stride % 8)
+    return fail(WF_ERR_MISALIGNED, "q/k_cache/v_cache/o/workspace and the caches' strides must be multiples of 16 bytes");
+  if ((rc = device_setup(&dev))) return rc;
+  const int ctas = g_dev_sms[dev] * dec::kCtasPerSm;
+  const size_t need = decode_workspace_bytes(ctas, p.heads_per_row);
+  if (workspace_bytes < need)
+    return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  p.k = reinterpret_cast<const __nv_bfloat16*>(k_cache);
+  p.v = reinterpret_cast<const __nv_bfloat16*>(v_cache);
+  p.page_stride[0] = cfg->k_page_stride, p.slot_stride[0] = cfg->k_slot_stride, p.head_stride[0] = cfg->k_head_stride;
+  p.page_stride[1] = cfg->v_page_stride, p.slot_stride[1] = cfg->v_slot_stride, p.head_stride[1] = cfg->v_head_stride;
+  p.page_table = page_table;
+  p.table_stride = cfg->table_stride;
+  p.lengths = lengths;
+  p.o = reinterpret_cast<__nv_bfloat16*>(o);
+  p.lse = lse;
+  p.join = reinterpret_cast<int4*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(p.join + ctas);
+  p.part_o = p.part_ml + (size_t)2 * ctas * p.heads_per_row * 2;
+  p.b = b, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
+  p.n_pages = cfg->n_pages, p.page_size = cfg->page_size, p.max_pages = cfg->max_pages;
+  p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch ((p.heads_per_row + 7) / 8) {
+    case 1: return decode_launch<1>(p, ctas, st);
+    case 2: return decode_launch<2>(p, ctas, st);
+    case 3: return decode_launch<3>(p, ctas, st);
+    default: return decode_launch<4>(p, ctas, st);
+  }
+}

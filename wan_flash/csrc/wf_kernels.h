@@ -4,6 +4,7 @@
 
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -60,6 +61,12 @@ __global__ void wf_bwd_pre_kernel(const __nv_bfloat16* __restrict__ o, const __n
                                   int sq_rounded, int h);
 __global__ void wf_convert_kernel(const float* __restrict__ accum, __nv_bfloat16* __restrict__ out, float scale,
                                   int s, int s_rounded, int h);
+
+// per-device kernel attributes of the operators that bring their own entry points
+cudaError_t decode_setup();
+
+// role ids recorded with a device error by the operators without mbarrier roles
+enum : uint32_t { kRoleRope = 21, kRoleDecode = 22 };
 
 size_t fwd_smem_bytes();
 size_t fwd2_smem_bytes();

@@ -8,3 +8,5 @@
 #include "wf_bwd2.cu"
 #include "wf_aux.cu"
 #include "wf_noalloc.cu"
+#include "wf_rope.cu"
+#include "wf_decode.cu"
