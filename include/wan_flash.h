@@ -227,6 +227,26 @@ int wf_decode(const void* q, const void* k_cache, const void* v_cache, const int
               void* o, float* lse, void* workspace, size_t workspace_bytes, int b, int h, int h_kv,
               const wf_decode_cfg* cfg, void* stream);
 
+/* Bytes of workspace of wf_packed_fwd for n sequences in total_q query rows. */
+int wf_packed_fwd_workspace(int n, int total_q, size_t* bytes);
+
+/*
+ * Forward attention over n packed sequences (no reference counterpart): rows
+ * [q_offsets[i], q_offsets[i+1]) of q against rows [k_offsets[i],
+ * k_offsets[i+1]) of k and v.
+ *   q, o (total_q, h, 128), k, v (total_k, h_kv, 128) bf16 contiguous; q head
+ *   j reads key-value head j / (h / h_kv); lse (h, total_q) fp32 natural log;
+ *   offsets (n + 1) int32 in device memory, not falling, within the tensors.
+ * causal = 1: query i of a sequence with lq queries and lk keys sees keys
+ * j <= i + lk - lq.  A row that sees no key, and a row outside every
+ * sequence, gets o = 0 and lse = -inf.  Impossible offsets give NaN
+ * everywhere and WF_ERR_INVALID_ARG from wf_device_status.
+ * Two launches; overlapping calls need workspaces of their own.
+ */
+int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, void* o,
+                  float* lse, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,
+                  int h_kv, int causal, void* stream);
+
 /* Message for the last failed call on this thread (empty if none). */
 int wf_last_error(char* buf, int len);
 

@@ -1,0 +1,215 @@
+"""Packed attention, forward: against attention in 64 bits sequence by
+sequence, with lengths around the tiles, empty sequences and rows, NaN in rows
+outside every sequence, grouped heads, graphs, streams and refusals."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tests.attn64 import assert_close, attn64
+from wan_flash import _lib
+from wan_flash.packed import wan_flash_packed_fwd
+
+
+def offsets(lens, lead=0, device="cuda"):
+    at = [lead]
+    for n in lens:
+        at.append(at[-1] + n)
+    return torch.tensor(at, dtype=torch.int32, device=device)
+
+
+def make(lq, lk, h, hk, lead=0, tail=0, std=1.0, seed=0, device="cuda"):
+    """q, k, v, do and the offsets; lead rows before and tail rows behind the sequences hold NaN."""
+    g = torch.Generator().manual_seed(seed)
+    shapes = ((sum(lq), h), (sum(lk), hk), (sum(lk), hk), (sum(lq), h))
+    out = []
+    for i, (n, hh) in enumerate(shapes):
+        x = torch.randn(n, hh, 128, generator=g) * (std if i < 2 else 1.0)
+        nan = torch.full((1, hh, 128), float("nan"))
+        out.append(torch.cat((nan.expand(lead, -1, -1), x, nan.expand(tail, -1, -1))).to(device, torch.bfloat16))
+    return (*out, offsets(lq, lead, device), offsets(lk, lead, device))
+
+
+def check_fwd(q, k, v, qo, ko, causal, o, lse):
+    qo, ko = qo.tolist(), ko.tolist()
+    for i in range(len(qo) - 1):
+        a, b, c, d = qo[i], qo[i + 1], ko[i], ko[i + 1]
+        if a == b:
+            continue
+        r = attn64(q[a:b], k[c:d], v[c:d], causal)
+        assert_close(o[a:b], r["o"], r["o_tol"], f"o of sequence {i}")
+        assert_close(lse[:, a:b], r["lse"], r["lse_tol"], f"lse of sequence {i}")
+    for rows in (slice(0, qo[0]), slice(qo[-1], None)):
+        assert (o[rows] == 0).all() and (lse[:, rows] == float("-inf")).all()
+
+
+CASES = [
+    # lq, lk (None: the same), h, h_kv, causal
+    ([1], None, 1, 1, True),
+    ([1], None, 1, 1, False),
+    ([128], None, 2, 1, True),
+    ([129, 127, 256, 257, 255], None, 2, 2, True),
+    ([129, 127, 256, 257, 255], None, 2, 2, False),
+    ([64, 1, 0, 300, 0, 2], None, 3, 1, True),
+    ([64, 1, 0, 300, 0, 2], None, 3, 1, False),
+    ([5, 200, 128, 1], [133, 200, 400, 1000], 4, 2, True),     # continued prompts: more keys than queries
+    ([5, 200, 128, 1], [133, 200, 400, 1000], 4, 2, False),
+    ([300, 140, 7], [20, 0, 6], 2, 1, True),                   # fewer keys: rows that see nothing
+    ([300, 140, 7], [20, 0, 6], 2, 1, False),
+    ([0, 0], [10, 0], 2, 2, True),
+    ([1111], None, 8, 1, True),
+    ([700, 513], [130, 900], 12, 4, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,h,hk,causal", CASES)
+@pytest.mark.parametrize("lead,tail", [(0, 0), (3, 150)])
+def test_forward(lq, lk, h, hk, causal, lead, tail):
+    q, k, v, _, qo, ko = make(lq, lk or lq, h, hk, lead, tail)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    _lib.check_device()
+    assert o.shape == q.shape and o.dtype == torch.bfloat16 and lse.shape == (h, q.shape[0])
+    check_fwd(q, k, v, qo, ko, causal, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_large_scores(causal):
+    """N(0, 3^2) q and k: row maxima that keep moving, so O is rescaled."""
+    q, k, v, _, qo, ko = make([700, 90], [700, 90], 4, 2, std=3.0, seed=1)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    _lib.check_device()
+    check_fwd(q, k, v, qo, ko, causal, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_sequences(causal):
+    """More items than CTAs, more sequences than the plan's threads, one and two tiles in turn."""
+    lens = [(i * 53) % 301 for i in range(1500)]
+    q, k, v, _, qo, ko = make(lens, lens, 2, 1, seed=2)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, causal=causal)  # k_offsets defaults to q_offsets
+    _lib.check_device()
+    check_fwd(q, k, v, qo, ko, causal, o, lse)
+
+
+@pytest.mark.gpu
+def test_a_sequence_does_not_see_its_neighbours():
+    """Non-finite values of one sequence stay in it; -inf keys and NaN values behind a causal row's tile too."""
+    q, k, v, _, qo, ko = make([200, 77, 130], [200, 77, 130], 2, 2, seed=3)
+    want, want_lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=True)
+    k[200:277], v[200:277], q[200:277] = float("nan"), float("inf"), float("-inf")
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=True)
+    for rows in (slice(0, 200), slice(277, None)):
+        assert torch.equal(o[rows], want[rows]) and torch.equal(lse[:, rows], want_lse[:, rows])
+    assert o[200:277].isnan().all() and lse[:, 200:277].isnan().all()
+
+
+@pytest.mark.gpu
+def test_matches_the_dense_forward_on_one_sequence():
+    """One full sequence is wan_flash_fwd's problem: same rounding points, so the same to fp32 sums' order."""
+    from wan_flash.interface import wan_flash_fwd
+
+    q, k, v, _, qo, ko = make([640], [640], 2, 2, seed=4)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko)
+    do, dlse = wan_flash_fwd(q[None], k[None], v[None])
+    r = attn64(q, k, v)
+    assert_close(do[0], r["o"], r["o_tol"], "dense o")
+    assert_close(o, r["o"], r["o_tol"], "packed o")
+    assert (lse - dlse[0]).abs().max().item() <= 2 * r["lse_tol"].max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [[0, 60, 50, 100], [-1, 50, 60, 100], [0, 50, 60, 101]])
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_impossible_offsets(bad, which):
+    q, k, v, _, qo, ko = make([50, 10, 40], [50, 10, 40], 2, 1)
+    t = torch.tensor(bad, dtype=torch.int32, device="cuda")
+    o, lse = wan_flash_packed_fwd(q, k, v, t if which == "q" else qo, t if which == "k" else ko, causal=True)
+    with pytest.raises(_lib.WanFlashError):
+        _lib.check_device()
+    assert o.isnan().all() and lse.isnan().all()
+    _lib.check_device()
+
+
+@pytest.mark.gpu
+def test_strided_inputs_other_stream_and_replay_with_other_offsets():
+    g = torch.Generator().manual_seed(6)
+    qkv = torch.randn(400, 3, 2, 128, generator=g).to("cuda", torch.bfloat16)
+    qo = offsets([100, 0, 300])
+    want = wan_flash_packed_fwd(*(qkv[:, i].contiguous() for i in range(3)), qo, causal=True)
+    got = wan_flash_packed_fwd(*(qkv[:, i] for i in range(3)), qo, causal=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q, k, v = (qkv[:, i].contiguous() for i in range(3))
+    graphs, outs = [], []
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            wan_flash_packed_fwd(q, k, v, qo, causal=True)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(wan_flash_packed_fwd(q, k, v, qo, causal=True))
+        graphs.append((graph, side))
+    for _ in range(3):
+        for graph, side in graphs:
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    for o, lse in outs:
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    qo.copy_(torch.tensor([0, 7, 390, 390], dtype=torch.int32))
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    _lib.check_device()
+    check_fwd(q, k, v, qo, qo, True, *outs[0])
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    q, k, v, _, qo, ko = make([0], [5], 2, 1)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko)
+    assert o.shape == (0, 2, 128) and lse.shape == (2, 0)
+    # no sequence at all, and no keys at all
+    q, k, v, _, qo, ko = make([30], [0], 2, 1)
+    for a, b in ((qo, ko), (qo[:1], ko[:1])):
+        o, lse = wan_flash_packed_fwd(q, k, v, a, b, causal=True)
+        _lib.check_device()
+        assert (o == 0).all() and (lse == float("-inf")).all()
+
+
+def test_refusals():
+    q, k, v, do, qo, ko = make([5, 3], [5, 3], 4, 2, device="cpu")
+    for bad in (
+        (q, k, v, qo),                          # CPU tensors
+        (q.float(), k, v, qo),
+        (q[..., :64], k[..., :64], v[..., :64], qo),
+        (q[:, :3], k, v, qo),                   # 3 heads over 2
+        (q, k, v[:4], qo),
+        (q[None], k, v, qo),
+        (q, k, v, qo.long()),
+        (q, k, v, qo, ko[:2]),
+        (q, k, v, qo[:0]),
+        (q, k, v, qo[None]),
+    ):
+        with pytest.raises(AssertionError):
+            wan_flash_packed_fwd(*bad)
+
+
+def test_c_entry_refusals():
+    lib = _lib.lib()
+
+    def call(q=16, n=2, tq=8, tk=8, h=4, hk=2, causal=0, ws=1 << 20):
+        p = ctypes.c_void_p
+        return lib.wf_packed_fwd(p(q) if q else None, p(16), p(16), p(16), p(16), p(16), p(16), p(16), ws, n, tq, tk, h, hk,
+                                 causal, None)
+
+    assert call(n=-1) == -1 and call(h=3) == -1 and call(hk=0) == -1 and call(causal=2) == -1 and call(q=None) == -1
+    assert call(ws=16) == -1 and call(q=24) == -3 and call(tq=2**30 + 1) == -2 and call(n=2**25) == -2
+    assert call(tq=0) == 0 and call(h=0, hk=0) == 0
+    size = ctypes.c_size_t()
+    assert lib.wf_packed_fwd_workspace(3, 1000, ctypes.byref(size)) == 0 and size.value > 0
+    assert lib.wf_packed_fwd_workspace(-1, 1000, ctypes.byref(size)) == -1

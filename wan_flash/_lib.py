@@ -31,6 +31,7 @@ EXPORTS = (
     "wf_fwd", "wf_fwd_dual", "wf_bwd_pre", "wf_bwd_main", "wf_bwd_convert", "wf_bwd_noalloc", "wf_last_error",
     "wf_device_status", "wf_set_wait_limit_ns", "wf_selftest_wait_timeout", "wf_num_sms", "wf_version",
     "wf_rope", "wf_decode", "wf_decode_workspace",
+    "wf_packed_fwd", "wf_packed_fwd_workspace",
 )
 
 
@@ -82,6 +83,8 @@ def _declare(lib):
     lib.wf_rope.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, ctypes.POINTER(RopeCfg), vp]
     lib.wf_decode_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, ctypes.POINTER(DecodeCfg), vp]
+    lib.wf_packed_fwd_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
+    lib.wf_packed_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, i, i, i, vp]
     for name in EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     del fp

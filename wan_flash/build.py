@@ -20,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libwanflash.so"
 SOURCES = ["wf_lib.cu", "wf_capi.cu", "wf_fwd.cu", "wf_fwd2.cu", "wf_bwd.cu", "wf_bwd2.cu", "wf_aux.cu", "wf_noalloc.cu", "wf_rope.cu", "wf_decode.cu",
+           "wf_packed_plan.cu", "wf_packed_fwd.cu", "wf_packed_bwd.cu", "wf_packed_capi.cu",
            "wf_common.cuh", "wf_kernels.h"]
 
 NVCC_FLAGS = [

@@ -92,6 +92,8 @@ int device_setup(int* dev_out) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(bwd pair smem)");
   e = decode_setup();
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode smem)");
+  e = packed_setup();
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed smem)");
   g_dev_sms[dev] = sms;
   g_dev_ready[dev] = true;
   return WF_OK;

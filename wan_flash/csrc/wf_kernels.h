@@ -62,11 +62,52 @@ __global__ void wf_bwd_pre_kernel(const __nv_bfloat16* __restrict__ o, const __n
 __global__ void wf_convert_kernel(const float* __restrict__ accum, __nv_bfloat16* __restrict__ out, float scale,
                                   int s, int s_rounded, int h);
 
+// ---- packed sequences (wf_packed_*.cu) ----
+// Work records that the plan kernel writes and the packed kernels read.
+struct __align__(16) PackedFwdTile {  // up to 256 query rows of one sequence
+  int q0, rows;   // first row in the packed tensor, rows
+  int k0;         // the sequence's first key row
+  int klen;       // keys that the tile's last row sees; 0: nothing to attend, the rows are filled
+  int off;        // causal: keys that row 0 of the tile sees (row r: off + r); may be negative
+  int n_blocks;   // ceil(klen / 128)
+  int pad0, pad1;
+};
+struct __align__(16) PackedKTile {  // up to 128 key rows of one sequence
+  int k0, rows;   // first row in the packed tensor, rows
+  int q0, lq;     // the sequence's query rows
+  int qtile;      // the sequence's first query tile (place in the fp32 workspaces)
+  int m_begin, m_count;  // query tiles of the sequence that see some of these keys
+  int need;       // first query row of the sequence that sees the tile's first key (key r: need + r)
+  int nb, tile;   // place in the sequence; place in the natural order of all key tiles
+  int pad0, pad1;
+};
+struct PackedPlanParams {
+  const int* q_off;
+  const int* k_off;
+  int n, total_q, total_k;
+  int causal, backward, ordered;
+  int cost_shift;           // cost >> cost_shift stays below the number of sort buckets
+  int4* head;               // {tiles, status}: [0] the sorted list, [1] (backward) the query tiles
+  int* base;                // scratch: 3 * (n + 3)
+  PackedFwdTile* fwd_tiles;
+  PackedKTile* k_tiles;
+  int4* q_tiles;            // {first row, rows, 1 inside a sequence, 0}
+};
+struct PackedFwdParams {
+  const int4* head;
+  const PackedFwdTile* tiles;
+  __nv_bfloat16* o;
+  float* lse;               // (h, total_q)
+  int total_q, h, group, causal;
+  float scale_log2, rescale_threshold;
+};
+cudaError_t packed_setup();
+
 // per-device kernel attributes of the operators that bring their own entry points
 cudaError_t decode_setup();
 
 // role ids recorded with a device error by the operators without mbarrier roles
-enum : uint32_t { kRoleRope = 21, kRoleDecode = 22 };
+enum : uint32_t { kRoleRope = 21, kRoleDecode = 22, kRolePackedPlan = 23 };
 
 size_t fwd_smem_bytes();
 size_t fwd2_smem_bytes();

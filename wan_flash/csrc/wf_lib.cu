@@ -10,3 +10,6 @@
 #include "wf_noalloc.cu"
 #include "wf_rope.cu"
 #include "wf_decode.cu"
+#include "wf_packed_plan.cu"
+#include "wf_packed_fwd.cu"
+#include "wf_packed_capi.cu"

@@ -1,0 +1,470 @@
+// Forward attention over packed sequences (sm_100a): sequences of different
+// lengths one behind the other, grouped heads, causal or not.
+//
+//     S = q k^T / sqrt(128), row i of a sequence sees keys j <= i + lk - lq
+//     (causal) or all of them; o = softmax(S) v; lse.
+//
+// Bound: the tensor pipe and, level with it, the MUFU exponentials (a
+// 128 x 128 block of S needs as many cycles of either).  The inner pipeline is
+// that of wf_fwd_kernel: two 128-row query tiles per CTA, S and O in tensor
+// memory, P written over S in two halves, one MMA warp, one TMA warp, one
+// thread per query row.  What differs:
+//
+//   items     A work item is one record of the plan (up to 256 query rows of
+//             one sequence) and one head; the grid is persistent.  The list is
+//             sorted by falling number of key blocks and CTAs take it in
+//             serpentine order, so ragged and causal items end level.  Heads
+//             are innermost: the q heads of one key-value head run side by
+//             side and read its K and V from L2.
+//   walk      Key blocks from the last visible one down: the blocks that need
+//             masks (the ragged end, the causal diagonal) come first, the rest
+//             runs without a compare.  A record of at most 128 rows drives one
+//             of the two tiles only.
+//   masks     A row's visible keys are a count; the block loop compares it
+//             with the block's end and masks by column.  A row whose blocks so
+//             far are all masked keeps -inf as its maximum and exponentiates
+//             against 0; a row that sees nothing ends with l = 0 and is
+//             written as o = 0, lse = -inf.
+//   isolation Tiles are cut at the sequence, TMA boxes are not: rows behind
+//             the end belong to the next sequence or to padding and may hold
+//             NaN.  For K that is harmless (their scores are masked by a
+//             select), for V 0 * NaN is not: the MMA warp zeroes those rows of
+//             the box in shared memory before its product.  Short O tiles are
+//             copied out row by row instead of by tensor store.
+#include "wf_common.cuh"
+#include "wf_kernels.h"
+
+namespace wf {
+
+namespace pfwd {
+constexpr int kThreads = 384;
+constexpr uint32_t kRegsSoftmax = 208;
+constexpr uint32_t kRegsOther = 88;
+constexpr int kKvSlots = 4;
+constexpr uint32_t kBoxBytes = 128 * 128;
+constexpr uint32_t kTileBytes = 2 * kBoxBytes;
+constexpr uint32_t kOffQ = 0;
+constexpr uint32_t kOffKV = 2 * kTileBytes;
+constexpr uint32_t kOffOStage = kOffKV + kKvSlots * kTileBytes;
+constexpr uint32_t kOffBar = kOffOStage + kTileBytes;
+constexpr int kBarQFull = 0;                       // + tile
+constexpr int kBarQEmpty = 2;                      // + tile
+constexpr int kBarKvFull = 4;                      // + slot
+constexpr int kBarKvEmpty = kBarKvFull + kKvSlots;
+constexpr int kBarSFull = kBarKvEmpty + kKvSlots;  // + tile
+constexpr int kBarPFull = kBarSFull + 2;           // + 2 * tile + half
+constexpr int kBarOFull = kBarPFull + 4;           // + tile
+constexpr int kBarDrain = kBarOFull + 2;
+constexpr int kBarOStaged = kBarDrain + 1;
+// A stage use n is freed on barrier n & 1: a warpgroup that waits for use n - 1
+// may not have seen use n - 2 freed, and one barrier's parity could not tell them apart.
+constexpr int kBarOStageFree = kBarOStaged + 1;    // + use & 1
+constexpr int kNumBars = kBarOStageFree + 2;
+constexpr uint32_t kOffTmemHolder = kOffBar + kNumBars * 8;
+constexpr uint32_t kOffAbort = kOffTmemHolder + 4;
+constexpr uint32_t kSmemUsed = kOffAbort + 4;
+constexpr uint32_t kSmemBytes = kSmemUsed + 1024;
+static_assert(kSmemBytes <= 232448, "packed forward shared memory exceeds the per-CTA limit");
+}  // namespace pfwd
+
+// Item k of this CTA: the sorted list in rounds of gridDim.x items, every
+// second round backwards.
+__device__ __forceinline__ int packed_item(int k) {
+  return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
+// Zero rows [first, 128) of a 128-row tile of two 64-column boxes (a
+// converged warp; the swizzle permutes 16-byte chunks inside a row only), and
+// order the stores before the tensor core's reads.
+__device__ __forceinline__ void packed_zero_rows(uint32_t tile, int first) {
+  for (int i = first * 8 + (int)lane_id(); i < 128 * 8; i += 32) {
+    st_shared_v4(tile + i * 16, 0u, 0u, 0u, 0u);
+    st_shared_v4(tile + 128 * 128 + i * 16, 0u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+__global__ void __launch_bounds__(pfwd::kThreads, 1)
+    wf_packed_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+                         PackedFwdParams p) {
+  using namespace pfwd;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + kOffBar;
+  auto bar = [&](int i) -> uint32_t { return bar0 + 8u * (uint32_t)i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOffAbort);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kOffTmemHolder);
+  const int warp = (int)warp_id();
+  const int lane = (int)lane_id();
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar(kBarQFull + t), 1);
+      mbar_init(bar(kBarQEmpty + t), 1);
+      mbar_init(bar(kBarSFull + t), 1);
+      mbar_init(bar(kBarPFull + 2 * t), 4);  // one arrival per softmax warp
+      mbar_init(bar(kBarPFull + 2 * t + 1), 4);
+      mbar_init(bar(kBarOFull + t), 1);
+      mbar_init(bar(kBarOStageFree + t), 1);
+    }
+    for (int s = 0; s < kKvSlots; ++s) {
+      mbar_init(bar(kBarKvFull + s), 1);
+      mbar_init(bar(kBarKvEmpty + s), 1);
+    }
+    mbar_init(bar(kBarDrain), 1);
+    mbar_init(bar(kBarOStaged), 4);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  // a programmatic dependent of the plan kernel: its lists are read from here on
+  griddep_wait();
+  const int n_items = p.head[0].x * p.h;
+  const bool bad = p.head[0].y != 0;
+
+  if (warp == 11) {
+    regs_dec<kRegsOther>();  // idle warp of warpgroup 2
+  } else if (warp == 10) {
+    regs_dec<kRegsOther>();
+    // ------------------------------------------------------------ O store
+    if (lane == 0) tma_prefetch_desc(&tm_o);
+    int n = 0;  // tiles stored
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int item = packed_item(k);
+      if (item >= n_items) break;
+      const PackedFwdTile w = p.tiles[item / p.h];
+      if (w.n_blocks == 0) continue;
+      const int h = item % p.h;
+      for (int t = 0; t * 128 < w.rows; ++t, ++n) {
+        ok = mbar_wait_warp(bar(kBarOStaged), (uint32_t)n & 1, abort_flag, kRoleStore, 50 + t);
+        if (!ok) break;
+        const int rows = w.rows - t * 128;
+        if (rows >= 128) {
+          if (lane == 0) {
+            for (int x = 0; x < 2; ++x)
+              tma_store_4d(&tm_o, sbase + kOffOStage + x * kBoxBytes, x * 64, w.q0 + t * 128, h, 0);
+            bulk_commit_group();
+            bulk_wait_read_all();
+          }
+        } else {
+          // rows behind the sequence's end belong to the next one: copy the
+          // valid ones, two rows of 16 chunks per pass
+          const int c = lane & 15;
+          for (int r = lane >> 4; r < rows; r += 2) {
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + kOffOStage + (c >> 3) * kBoxBytes +
+                                                            sw128_offset((uint32_t)r, (uint32_t)(c & 7)));
+            *reinterpret_cast<uint4*>(p.o + ((size_t)(w.q0 + t * 128 + r) * p.h + h) * 128 + c * 8) = v;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBarOStageFree + (n & 1)));
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  } else if (warp == 9) {
+    regs_dec<kRegsOther>();
+    // ------------------------------------------------------------------ TMA
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      int q_issued[2] = {0, 0};
+      int issued[kKvSlots] = {0, 0, 0, 0};
+      int u = 0;  // K/V units (K and V of a block alternate)
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const int item = packed_item(k);
+        if (item >= n_items) break;
+        const PackedFwdTile w = p.tiles[item / p.h];
+        const int h = item % p.h, kvh = h / p.group;
+        for (int it = 0; it < w.n_blocks && ok; ++it) {
+          const int j = w.n_blocks - 1 - it;
+          for (int kv = 0; kv < 2 && ok; ++kv, ++u) {  // 0 = K, 1 = V
+            const int slot = u % kKvSlots;
+            const int use = u / kKvSlots;
+            if (use > 0) ok = mbar_wait(bar(kBarKvEmpty + slot), (use - 1) & 1, abort_flag, kRoleLoad, 100 + slot);
+            if (!ok) break;
+            mbar_expect_tx(bar(kBarKvFull + slot), kTileBytes);
+            for (int x = 0; x < 2; ++x)
+              tma_load_4d(sbase + kOffKV + slot * kTileBytes + x * kBoxBytes, kv ? &tm_v : &tm_k,
+                          bar(kBarKvFull + slot), x * 64, w.k0 + j * 128, kvh, 0);
+            issued[slot] = use + 1;
+            if (it == 0 && kv == 0) {
+              for (int t = 0; t * 128 < w.rows && ok; ++t) {
+                if (q_issued[t] > 0)
+                  ok = mbar_wait(bar(kBarQEmpty + t), (q_issued[t] - 1) & 1, abort_flag, kRoleLoad, 90 + t);
+                if (!ok) break;
+                mbar_expect_tx(bar(kBarQFull + t), kTileBytes);
+                for (int x = 0; x < 2; ++x)
+                  tma_load_4d(sbase + kOffQ + t * kTileBytes + x * kBoxBytes, &tm_q, bar(kBarQFull + t), x * 64,
+                              w.q0 + t * 128, h, 0);
+                q_issued[t]++;
+              }
+            }
+          }
+        }
+      }
+      if (*abort_flag) {
+        // drain: let every issued copy land before the CTA can exit
+        for (int t = 0; t < 2; ++t)
+          if (q_issued[t] > 0) mbar_wait_drain(bar(kBarQFull + t), (q_issued[t] - 1) & 1);
+        for (int s = 0; s < kKvSlots; ++s)
+          if (issued[s] > 0) mbar_wait_drain(bar(kBarKvFull + s), (issued[s] - 1) & 1);
+      }
+    }
+  } else if (warp == 8) {
+    regs_dec<kRegsOther>();
+    // ------------------------------------------------------------------ MMA
+    // converged warp: all lanes wait and form descriptors, elected lanes issue
+    constexpr uint32_t idesc_qk = idesc_bf16(128, 128, 0, 0);
+    constexpr uint32_t idesc_pv = idesc_bf16(128, 128, 0, 1);
+    const uint32_t sQ = sbase + kOffQ;
+    const uint32_t sKV = sbase + kOffKV;
+    bool ok = true;
+    int pv_phase[2] = {0, 0};
+    int q_phase[2] = {0, 0};
+    auto issue_s = [&](int t, int slot_k) {
+      const uint32_t d = tmem + (uint32_t)(t * 128);
+      const uint64_t a0 = sdesc(sQ + t * kTileBytes, 16, 1024);
+      const uint64_t b0 = sdesc(sKV + slot_k * kTileBytes, 16, 1024);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const uint32_t off = (uint32_t)((ks >> 2) * kBoxBytes + (ks & 3) * 32);
+        mma_ss_e(d, desc_add(a0, off), desc_add(b0, off), idesc_qk, ks > 0);
+      }
+    };
+    auto issue_pv = [&](int t, int slot_v, bool acc) -> bool {
+      const uint32_t d = tmem + 256u + (uint32_t)(t * 128);
+      const uint32_t a = tmem + (uint32_t)(t * 128);
+      const uint64_t b0 = sdesc(sKV + slot_v * kTileBytes, kBoxBytes, 1024);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!mbar_wait_warp(bar(kBarPFull + 2 * t + half), (uint32_t)pv_phase[t] & 1, abort_flag, kRoleMma,
+                            20 + 2 * t + half))
+          return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const int ks = half * 4 + kk;
+          mma_ts_e(d, a + ks * 8, desc_add(b0, (uint32_t)(ks * 2048)), idesc_pv, (acc || ks > 0) ? 1u : 0u);
+        }
+      }
+      pv_phase[t]++;
+      return true;
+    };
+    // One flat pipeline over the blocks of all items: block g issues PV_t(g-1)
+    // before S_t(g) for each tile that the block has.
+    int g = 0;
+    int prev_it = 0, prev_tiles = 0;  // position of block g-1 in its item, query tiles of it
+    int prev_keys = 128;              // keys of block g-1 that exist for its item (128 but for the last block)
+    bool prev_last = false;
+    auto wait_v = [&]() -> bool {  // V of block g-1, its rows behind the last visible key zeroed
+      const int uv = 2 * (g - 1) + 1, slot_v = uv % kKvSlots;
+      if (!mbar_wait_warp(bar(kBarKvFull + slot_v), (uv / kKvSlots) & 1, abort_flag, kRoleMma, 10 + slot_v))
+        return false;
+      if (prev_keys < 128) packed_zero_rows(sKV + slot_v * kTileBytes, prev_keys);
+      return true;
+    };
+    for (int k = 0; ok; ++k) {
+      const int item = packed_item(k);
+      if (item >= n_items) break;
+      const PackedFwdTile w = p.tiles[item / p.h];
+      const int tiles = w.rows > 128 ? 2 : 1;
+      for (int it = 0; it < w.n_blocks && ok; ++it, ++g) {
+        const int uk = 2 * g, slot_k = uk % kKvSlots;
+        ok = mbar_wait_warp(bar(kBarKvFull + slot_k), (uk / kKvSlots) & 1, abort_flag, kRoleMma, 10 + slot_k);
+        if (!ok) break;
+        tc_fence_after();
+        const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;  // of block g-1
+        if (g > 0 && !(ok = wait_v())) break;
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (t < prev_tiles) {
+            if (!(ok = issue_pv(t, slot_v, prev_it > 0))) break;
+            if (prev_last) mma_commit_e(bar(kBarOFull + t));
+          }
+          if (g > 0 && t == 1) mma_commit_e(bar(kBarKvEmpty + slot_v));
+          if (t < tiles) {
+            if (it == 0) {
+              ok = mbar_wait_warp(bar(kBarQFull + t), (uint32_t)q_phase[t] & 1, abort_flag, kRoleMma, t);
+              if (!ok) break;
+              q_phase[t]++;
+              tc_fence_after();
+            }
+            issue_s(t, slot_k);
+            mma_commit_e(bar(kBarSFull + t));
+            if (it == w.n_blocks - 1) mma_commit_e(bar(kBarQEmpty + t));
+          }
+        }
+        if (ok) mma_commit_e(bar(kBarKvEmpty + slot_k));
+        prev_it = it;
+        prev_tiles = tiles;
+        prev_last = (it == w.n_blocks - 1);
+        prev_keys = it == 0 ? w.klen - (w.n_blocks - 1) * 128 : 128;
+      }
+    }
+    if (ok && g > 0) {
+      const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;
+      ok = wait_v();
+      for (int t = 0; t < prev_tiles && ok; ++t) {
+        if (!(ok = issue_pv(t, slot_v, prev_it > 0))) break;
+        mma_commit_e(bar(kBarOFull + t));
+      }
+      if (ok) mma_commit_e(bar(kBarKvEmpty + slot_v));
+    }
+    // drain the tensor pipe before TMEM can be released
+    mma_commit_e(bar(kBarDrain));
+    mbar_wait_drain(bar(kBarDrain), 0);
+  } else {
+    regs_inc<kRegsSoftmax>();
+    // -------------------------------------------------------------- softmax
+    const int t = warp >> 2;  // query tile
+    const int wq = warp & 3;  // TMEM lane quadrant
+    const int r = wq * 32 + lane;
+    const uint32_t role = t ? kRoleSoftmax1 : kRoleSoftmax0;
+    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+    const uint32_t tS = tmem + lane_base + (uint32_t)(t * 128);
+    const uint32_t tO = tmem + lane_base + 256u + (uint32_t)(t * 128);
+    const float sl2 = p.scale_log2;
+    const float thr = p.rescale_threshold;
+    bool ok = true;
+    int s_waits = 0;    // S_t tiles consumed
+    int o_waits = 0;    // items of this tile that had keys
+    int stage_use = 0;  // O tiles of both tiles staged before this item
+    for (int k = 0; ok; ++k) {
+      const int item = packed_item(k);
+      if (item >= n_items) break;
+      const PackedFwdTile w = p.tiles[item / p.h];
+      const int h = item % p.h;
+      const int row = t * 128 + r;  // within the record
+      if (w.n_blocks == 0) {
+        // nothing to attend (or rows outside any sequence): o = 0, lse = -inf;
+        // NaN where the offsets were impossible
+        const uint32_t fill = bad ? 0x7fff7fffu : 0u;
+        for (int i = (int)threadIdx.x; i < w.rows * 16; i += 256)
+          st_global_v4(p.o + ((size_t)(w.q0 + (i >> 4)) * p.h + h) * 128 + (i & 15) * 8, fill, fill, fill, fill);
+        if (row < w.rows) p.lse[(size_t)h * p.total_q + w.q0 + row] = bad ? __int_as_float(0x7fffffff) : -INFINITY;
+        continue;
+      }
+      const int use = stage_use + t;
+      stage_use += w.rows > 128 ? 2 : 1;
+      if (t * 128 >= w.rows) continue;
+      const int seen = p.causal ? min(max(w.off + row, 0), w.klen) : w.klen;  // keys that this row sees
+      float m_s = -INFINITY;  // running reference max, in scaled log2 units
+      float l = 0.f;          // running row sum (relative to m_s)
+      for (int it = 0; it < w.n_blocks; ++it, ++s_waits) {
+        ok = mbar_wait(bar(kBarSFull + t), (uint32_t)s_waits & 1, abort_flag, role, 30 + t);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) reg_fence32(s[c]);
+        const int left = seen - (w.n_blocks - 1 - it) * 128;  // keys of this block that the row sees
+        if (left < 128) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= left) s[c][i] = __float_as_uint(-INFINITY);
+        }
+        __syncwarp();
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            mx[i & 3] = fmax3(mx[i & 3], __uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1]));
+        const float mnew_s = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        if (it == 0) {
+          m_s = mnew_s;
+        } else {
+          // move the reference max only when the row max grew past the rescale
+          // threshold, or was -inf (a row whose blocks were all masked so far:
+          // l and O are 0, the factor 2^-inf = 0)
+          const bool need = mnew_s - m_s > thr;
+          if (__any_sync(0xffffffffu, need)) {
+            const float factor = need ? ex2_approx(m_s - mnew_s) : 1.f;
+            if (need) {
+              l *= factor;
+              m_s = mnew_s;
+            }
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + c * 16, o);
+              tmem_wait_ld();
+              reg_fence16(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+              tmem_st16(tO + c * 16, o);
+            }
+          }
+        }
+        const float ref = m_s == -INFINITY ? 0.f : m_s;
+        const uint64_t sl2x2 = f2_pack(sl2, sl2), negx2 = f2_pack(-ref, -ref);
+        float bsum = fwd_exp_half(s, 0, tS, sl2x2, negx2);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive_warp(bar(kBarPFull + 2 * t));
+        bsum += fwd_exp_half(s, 2, tS, sl2x2, negx2);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive_warp(bar(kBarPFull + 2 * t + 1));
+        l += bsum;
+      }
+      // --------------------------------------------------------- epilogue
+      if (ok) ok = mbar_wait(bar(kBarOFull + t), (uint32_t)o_waits & 1, abort_flag, role, 40 + t);
+      if (!ok) break;
+      ++o_waits;
+      tc_fence_after();
+      const float inv = 1.f / l;
+      if (use > 0)
+        ok = mbar_wait(bar(kBarOStageFree + ((use - 1) & 1)), (uint32_t)((use - 1) >> 1) & 1, abort_flag, role, 45 + t);
+      if (!ok) break;
+      const uint32_t stage = sbase + kOffOStage + (uint32_t)r * 128u;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + c * 32, o);
+        tmem_wait_ld();
+        reg_fence32(o);
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          pk[i] = l == 0.f ? 0u : pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const uint32_t chunk = (uint32_t)((c & 1) * 4 + v);
+          st_shared_v4(stage + (uint32_t)(c >> 1) * kBoxBytes + ((chunk ^ ((uint32_t)r & 7u)) << 4), pk[4 * v],
+                       pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kBarOStaged));
+      if (row < w.rows)
+        p.lse[(size_t)h * p.total_q + w.q0 + row] = l == 0.f ? -INFINITY : (m_s + log2f(l)) * 0.69314718055994531f;
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace wf
