@@ -247,6 +247,30 @@ int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offs
                   float* lse, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,
                   int h_kv, int causal, void* stream);
 
+typedef struct wf_packed_bwd_cfg {
+  int nsplit;        /* >= 1: CTAs per (128-key tile, key-value head); with more
+                        than one, fp32 partial dk/dv are summed in a fixed order */
+  int deterministic; /* 1 = dq's fp32 contributions are added in key order */
+} wf_packed_bwd_cfg;
+
+/* Bytes of workspace of wf_packed_bwd. */
+int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg,
+                            size_t* bytes);
+
+/*
+ * Backward of wf_packed_fwd given its o and lse and dO (total_q, h, 128): dq
+ * like q, dk and dv like k and v, bf16.  dk and dv sum over the q heads that
+ * read the key-value head; they are bitwise reproducible, dq is with
+ * cfg->deterministic.  Rows that see no key, keys that no row sees, and rows
+ * outside every sequence get gradient 0.  Impossible offsets as in
+ * wf_packed_fwd.  total_q and total_k must both be positive (with no queries
+ * or no keys the gradients are zeros that the caller writes).
+ */
+int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dO,
+                  const int* q_offsets, const int* k_offsets, void* dq, void* dk, void* dv, void* workspace,
+                  size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv, int causal,
+                  const wf_packed_bwd_cfg* cfg, void* stream);
+
 /* Message for the last failed call on this thread (empty if none). */
 int wf_last_error(char* buf, int len);
 

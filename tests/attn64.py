@@ -56,3 +56,35 @@ def assert_close(got, want, tol, tag):
     over = torch.where(torch.isfinite(over), over, torch.full_like(over, math.inf))
     assert over.numel() == 0 or over.max().item() <= 0, \
         f"{tag}: off by {over.max().item():.3e} more than allowed, at {int(over.argmax())}"
+
+
+def grads64(q, k, v, do, causal=False):
+    """dq, dk, dv of o = attention(q, k, v) given do, by the formulas in 64 bits, with their bounds.
+
+    Errors of a kernel, entry by entry: P off by e = 4 es relative (its exponent: score and lse) and rounded to bf16
+    (U) before dV = P^T do; dP = do v^T an fp32 sum; D = rowsum(o do) from the o that was rounded (o_tol); dS = P (dP -
+    D) rounded to bf16 (U) before dQ and dK; fp32 sums over rows or keys; one rounding of the result."""
+    r = attn64(q, k, v, causal)
+    g, lq, lk = q.shape[1] // k.shape[1], q.shape[0], k.shape[0]
+    x, y, z, t = (a.double().transpose(0, 1) for a in (q, k, v, do))
+    y, z = y.repeat_interleave(g, 0), z.repeat_interleave(g, 0)
+    p, o, o_tol = r["p"], r["o"].transpose(0, 1), r["o_tol"].transpose(0, 1)
+    e = 4 * r["es"][..., None] + 16 * E32
+    dp = t @ z.transpose(1, 2)
+    delta = (t * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    dp_err = 128 * E32 * (t.abs() @ z.abs().transpose(1, 2))
+    delta_err = (o_tol * t.abs()).sum(-1, keepdim=True) + 128 * E32 * (t * o).abs().sum(-1, keepdim=True)
+    ds_err = (U + (1 + U) * e) * ds.abs() + (1 + U) * p * (dp_err + delta_err)
+    rows = (lq + lk) * E32
+    out = {}
+    p_err = (U + (1 + U) * e) * p
+    out["dv"] = p.transpose(1, 2) @ t, (p_err + rows * p).transpose(1, 2) @ t.abs()
+    out["dq"] = ds @ y * SCALE, (ds_err + rows * ds.abs()) @ y.abs() * SCALE
+    out["dk"] = ds.transpose(1, 2) @ x * SCALE, (ds_err + rows * ds.abs()).transpose(1, 2) @ x.abs() * SCALE
+    for name, (want, tol) in out.items():
+        want, tol = want.transpose(0, 1), tol.transpose(0, 1)
+        if name != "dq":  # the q heads of a group share the key-value head
+            want, tol = (a.unflatten(1, (a.shape[1] // g, g)).sum(2) for a in (want, tol))
+        out[name] = want, tol + U * (want.abs() + tol) + E32 * want.abs()
+    return out

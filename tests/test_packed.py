@@ -169,6 +169,24 @@ def test_strided_inputs_other_stream_and_replay_with_other_offsets():
 
 
 @pytest.mark.gpu
+def test_from_a_thread_without_a_cuda_call_behind_it():
+    import threading
+
+    from wan_flash.interface import wan_flash_fwd
+
+    q, k, v, _, qo, ko = make([100], [100], 2, 2)
+    want, got = wan_flash_packed_fwd(q, k, v, qo, ko), []
+    q4, k4, v4 = q[None], k[None], v[None]
+    dense = wan_flash_fwd(q4, k4, v4)
+    torch.cuda.synchronize()
+    for fn in (lambda: wan_flash_packed_fwd(q, k, v, qo, ko), lambda: wan_flash_fwd(q4, k4, v4)):
+        t = threading.Thread(target=lambda: got.append(fn()))
+        t.start()
+        t.join()
+    assert len(got) == 2 and torch.equal(got[0][0], want[0]) and torch.equal(got[1][0], dense[0])
+
+
+@pytest.mark.gpu
 def test_nothing_to_do():
     q, k, v, _, qo, ko = make([0], [5], 2, 1)
     o, lse = wan_flash_packed_fwd(q, k, v, qo, ko)

@@ -1,0 +1,218 @@
+"""Packed attention, backward: gradients against the formulas in 64 bits and
+against differences, the splits and the ordered mode, NaN outside the
+sequences, graphs, and refusals."""
+
+import pytest
+import torch
+
+from tests.attn64 import assert_close, attn64, grads64
+from tests.test_packed import CASES, make, offsets
+from wan_flash import _lib, features
+from wan_flash.packed import packed_bwd_plan, wan_flash_attn_packed, wan_flash_packed_bwd, wan_flash_packed_fwd
+
+
+@pytest.fixture(autouse=True)
+def _reset_features():
+    yield
+    features.reset()
+
+
+def check_bwd(q, k, v, do, qo, ko, causal, dq, dk, dv):
+    qo, ko = qo.tolist(), ko.tolist()
+    for i in range(len(qo) - 1):
+        a, b, c, d = qo[i], qo[i + 1], ko[i], ko[i + 1]
+        if a == b or c == d:
+            assert (dq[a:b] == 0).all() and (dk[c:d] == 0).all() and (dv[c:d] == 0).all()
+            continue
+        want = grads64(q[a:b], k[c:d], v[c:d], do[a:b], causal)
+        for name, got in (("dq", dq[a:b]), ("dk", dk[c:d]), ("dv", dv[c:d])):
+            assert_close(got, *want[name], f"{name} of sequence {i}")
+    for x, off in ((dq, qo), (dk, ko), (dv, ko)):
+        assert (x[:off[0]] == 0).all() and (x[off[-1]:] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,h,hk,causal", CASES)
+@pytest.mark.parametrize("lead,tail", [(0, 0), (3, 150)])
+def test_backward(lq, lk, h, hk, causal, lead, tail):
+    q, k, v, do, qo, ko = make(lq, lk or lq, h, hk, lead, tail)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+    _lib.check_device()
+    assert all(g.shape == x.shape and g.dtype == x.dtype for g, x in zip(grads, (q, k, v)))
+    check_bwd(q, k, v, do, qo, ko, causal, *grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("nsplit,deterministic", [(1, True), (2, False), (3, True), (7, False), (40, True)])
+def test_splits_and_ordered_mode(nsplit, deterministic, causal):
+    lq, lk = [700, 1, 129, 0], [700, 40, 300, 5]
+    q, k, v, do, qo, ko = make(lq, lk, 6, 2, 1, 9, seed=7)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    features.set_bwd_overrides(nsplit=nsplit, deterministic=deterministic)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+    _lib.check_device()
+    check_bwd(q, k, v, do, qo, ko, causal, *grads)
+    for _ in range(2):
+        again = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+        assert torch.equal(grads[1], again[1]) and torch.equal(grads[2], again[2])
+        if deterministic:
+            assert torch.equal(grads[0], again[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_sequences(causal):
+    lens = [(i * 53) % 301 for i in range(1200)]
+    q, k, v, do, qo, ko = make(lens, lens, 2, 1, seed=2)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, causal=causal)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, causal=causal)
+    _lib.check_device()
+    check_bwd(q, k, v, do, qo, ko, causal, *grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_large_scores(causal):
+    q, k, v, do, qo, ko = make([400, 90], [400, 90], 4, 2, std=3.0, seed=1)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+    _lib.check_device()
+    check_bwd(q, k, v, do, qo, ko, causal, *grads)
+
+
+@pytest.mark.gpu
+def test_a_sequence_does_not_see_its_neighbours():
+    features.set_bwd_overrides(deterministic=True)
+    q, k, v, do, qo, ko = make([200, 77, 130], [200, 77, 130], 2, 2, seed=3)
+
+    def grads():
+        o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=True)
+        return wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=True)
+
+    want = grads()
+    for x in (q, k, v, do):
+        x[200:277] = float("nan")
+    for g, w in zip(grads(), want):
+        assert torch.equal(g[:200], w[:200]) and torch.equal(g[277:], w[277:])
+        assert g[200:277].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_autograd_and_differences(causal):
+    """The gradient along a direction against a central difference of the function in 64 bits."""
+    q, k, v, do, qo, ko = make([150, 37], [170, 37], 4, 2, seed=8)
+    g = torch.Generator().manual_seed(9)
+    move = [torch.randn(x.shape, generator=g).to("cuda").double() for x in (q, k, v)]
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    o = wan_flash_attn_packed(*leaves, qo, ko, causal=causal)
+    grads = torch.autograd.grad(o, leaves, do)
+    _lib.check_device()
+
+    def loss(step):
+        total = 0.0
+        for a, b, c, d in ((0, 150, 0, 170), (150, 187, 170, 207)):
+            x, y, z = ((t.double() + step * m)[s] for t, m, s in zip((q, k, v), move, (slice(a, b), slice(c, d), slice(c, d))))
+            total += (attn64(x, y, z, causal)["o"] * do[a:b].double()).sum().item()
+        return total
+
+    h = 1e-5  # the difference itself is off by h^2 / 6 of the third derivative and 1e-16 / h of the loss: below 1e-6
+    want = (loss(h) - loss(-h)) / (2 * h)
+    got = sum((x.double() * m).sum().item() for x, m in zip(grads, move))
+    tol = 0.0
+    for a, b, c, d in ((0, 150, 0, 170), (150, 187, 170, 207)):
+        w = grads64(q[a:b], k[c:d], v[c:d], do[a:b], causal)
+        tol += sum((w[n][1] * m[s].abs()).sum().item()
+                   for n, m, s in zip(("dq", "dk", "dv"), move, (slice(a, b), slice(c, d), slice(c, d))))
+    assert abs(got - want) <= tol + 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [[0, 60, 50, 100], [-1, 50, 60, 100], [0, 50, 60, 101]])
+def test_impossible_offsets(bad):
+    q, k, v, do, qo, ko = make([50, 10, 40], [50, 10, 40], 2, 1)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko)
+    t = torch.tensor(bad, dtype=torch.int32, device="cuda")
+    for args in ((t, ko), (qo, t)):
+        grads = wan_flash_packed_bwd(q, k, v, o, lse, do, *args)
+        with pytest.raises(_lib.WanFlashError):
+            _lib.check_device()
+        assert all(x.isnan().all() for x in grads)
+    _lib.check_device()
+
+
+@pytest.mark.gpu
+def test_training_step_captured_and_replayed_with_other_offsets():
+    q, k, v, do, qo, ko = make([300, 77], [300, 77], 4, 2, seed=11)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        o = wan_flash_attn_packed(*leaves, qo, causal=True)
+        return o, *torch.autograd.grad(o, leaves, do)
+
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step()
+    for lens in ([300, 77], [1, 376], [377, 0]):
+        qo.copy_(offsets(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        _lib.check_device()
+        check_bwd(q, k, v, do, qo, qo, True, *out[1:])
+
+
+@pytest.mark.gpu
+def test_no_queries_or_no_keys():
+    for lq, lk in (([0], [5]), ([5], [0])):
+        q, k, v, do, qo, ko = make(lq, lk, 2, 1)
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        o = wan_flash_attn_packed(*leaves, qo, ko)
+        for g, x in zip(torch.autograd.grad(o, leaves, do), leaves):
+            assert g.shape == x.shape and (g == 0).all()
+        _lib.check_device()
+
+
+def test_refusals():
+    q, k, v, do, qo, ko = make([5, 3], [5, 3], 4, 2, device="cpu")
+    lse = torch.zeros(4, 8)
+    for bad in (
+        (q, k, v, q, lse, do, qo),                  # CPU tensors
+        (q, k, v, q, lse.double(), do, qo),
+        (q, k, v, q, lse[:, :7], do, qo),
+        (q, k, v, q[:7], lse, do, qo),
+        (q, k, v, q, lse, do.float(), qo),
+    ):
+        with pytest.raises(AssertionError):
+            wan_flash_packed_bwd(*bad)
+
+
+def test_plan_and_c_entry_refusals():
+    import ctypes
+
+    assert packed_bwd_plan(16384, 16384, 4, 12, 12, False, 148) == {"nsplit": 1, "deterministic": False}
+    assert packed_bwd_plan(2048, 2048, 1, 8, 1, True, 148)["nsplit"] > 1     # 16 key tiles on 148 SMs
+    assert packed_bwd_plan(1, 1, 1, 1, 1, True, 148)["nsplit"] == 1
+    features.set_bwd_overrides(nsplit=5, deterministic=True)
+    assert packed_bwd_plan(16384, 16384, 4, 12, 12, False, 148) == {"nsplit": 5, "deterministic": True}
+
+    lib = _lib.lib()
+    size = ctypes.c_size_t()
+    cfg = _lib.PackedBwdCfg(1, 0)
+
+    def call(n=2, tq=8, tk=8, h=4, hk=2, causal=0, nsplit=1, ws=1 << 30, q=16):
+        c = _lib.PackedBwdCfg(nsplit, 0)
+        p = ctypes.c_void_p
+        return lib.wf_packed_bwd(p(q) if q else None, *[p(16)] * 11, ws, n, tq, tk, h, hk, causal, ctypes.byref(c), None)
+
+    assert call(n=-1) == -1 and call(hk=3) == -1 and call(nsplit=0) == -1 and call(causal=3) == -1 and call(q=None) == -1
+    assert call(q=8) == -3 and call(ws=100) == -1 and call(tq=0) == -2 and call(tk=0) == -2
+    assert call(h=0, hk=0) == 0 and call(tq=0, tk=0) == 0
+    assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, ctypes.byref(cfg), ctypes.byref(size)) == 0 and size.value > 0
+    assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, None, ctypes.byref(size)) == -1

@@ -31,7 +31,7 @@ EXPORTS = (
     "wf_fwd", "wf_fwd_dual", "wf_bwd_pre", "wf_bwd_main", "wf_bwd_convert", "wf_bwd_noalloc", "wf_last_error",
     "wf_device_status", "wf_set_wait_limit_ns", "wf_selftest_wait_timeout", "wf_num_sms", "wf_version",
     "wf_rope", "wf_decode", "wf_decode_workspace",
-    "wf_packed_fwd", "wf_packed_fwd_workspace",
+    "wf_packed_fwd", "wf_packed_fwd_workspace", "wf_packed_bwd", "wf_packed_bwd_workspace",
 )
 
 
@@ -61,6 +61,10 @@ class DecodeCfg(ctypes.Structure):
                 ("v_slot_stride", ctypes.c_longlong), ("v_head_stride", ctypes.c_longlong)]
 
 
+class PackedBwdCfg(ctypes.Structure):
+    _fields_ = [("nsplit", ctypes.c_int), ("deterministic", ctypes.c_int)]
+
+
 class WanFlashError(RuntimeError):
     def __init__(self, code: int, message: str):
         self.code = code
@@ -85,6 +89,8 @@ def _declare(lib):
     lib.wf_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, ctypes.POINTER(DecodeCfg), vp]
     lib.wf_packed_fwd_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_packed_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, i, i, i, vp]
+    lib.wf_packed_bwd_workspace.argtypes = [i, i, i, i, i, ctypes.POINTER(PackedBwdCfg), ctypes.POINTER(ctypes.c_size_t)]
+    lib.wf_packed_bwd.argtypes = ([vp] * 12 + [ctypes.c_size_t] + [i] * 6 + [ctypes.POINTER(PackedBwdCfg), vp])
     for name in EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     del fp

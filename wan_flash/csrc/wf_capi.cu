@@ -70,6 +70,11 @@ int device_setup(int* dev_out) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (dev < 0 || dev >= kMaxDevices) return fail(WF_ERR_NO_DEVICE, "device ordinal %d out of range", dev);
   *dev_out = dev;
+  // Make the device's context current in this thread: a thread without a CUDA
+  // call behind it (autograd's) has none, and the tensor-map encoder, a driver
+  // function, refuses then.
+  e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_dev_ready[dev]) return WF_OK;
   int major = 0, minor = 0, sms = 0;

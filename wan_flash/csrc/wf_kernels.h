@@ -78,8 +78,8 @@ struct __align__(16) PackedKTile {  // up to 128 key rows of one sequence
   int qtile;      // the sequence's first query tile (place in the fp32 workspaces)
   int m_begin, m_count;  // query tiles of the sequence that see some of these keys
   int need;       // first query row of the sequence that sees the tile's first key (key r: need + r)
-  int nb, tile;   // place in the sequence; place in the natural order of all key tiles
-  int pad0, pad1;
+  int nb;         // place of the tile in its sequence
+  int pad0, pad1, pad2;
 };
 struct PackedPlanParams {
   const int* q_off;
@@ -100,6 +100,32 @@ struct PackedFwdParams {
   float* lse;               // (h, total_q)
   int total_q, h, group, causal;
   float scale_log2, rescale_threshold;
+};
+struct PackedBwdParams {
+  const int4* head;
+  const PackedKTile* k_tiles;
+  const int4* q_tiles;
+  float* neg_lse_log2;      // (h, q_tile_stride, 128): -lse * log2(e), -inf behind the sequence's end
+  float* dpsum;             // (h, q_tile_stride, 128)
+  float* dq_accum;          // (h, q_tile_stride) tiles of 16384 fp32
+  __nv_bfloat16* dk;        // (total_k, h_kv, 128)
+  __nv_bfloat16* dv;
+  float* dk_part;           // nsplit > 1: (nsplit, h_kv, k_tile_stride) tiles of 16384 fp32
+  float* dv_part;
+  int* sem;                 // ordered: (h, q_tile_stride) key tiles added so far
+  size_t q_tile_stride, k_tile_stride;
+  int total_q, h, h_kv, group, nsplit, ordered, wave;
+  float scale, scale_log2;
+};
+struct PackedConvertParams {
+  const int4* head;
+  const int4* q_tiles;      // or, where null, k_tiles
+  const PackedKTile* k_tiles;
+  const float* accum;
+  size_t tile_stride, part_stride;  // tiles per head; floats between parts
+  int parts, heads;
+  float scale;
+  __nv_bfloat16* out;       // (total, heads, 128)
 };
 cudaError_t packed_setup();
 

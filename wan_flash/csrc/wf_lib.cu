@@ -12,4 +12,5 @@
 #include "wf_decode.cu"
 #include "wf_packed_plan.cu"
 #include "wf_packed_fwd.cu"
+#include "wf_packed_bwd.cu"
 #include "wf_packed_capi.cu"

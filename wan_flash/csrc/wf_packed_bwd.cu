@@ -1,0 +1,586 @@
+// Backward attention over packed sequences (sm_100a): dK/dV-stationary, dQ by
+// fp32 reductions, grouped heads, causal or not.
+//
+// For one tile of 128 keys of one sequence and key-value head the main kernel
+// walks units u = (q head of the group, tile of 128 query rows that sees some
+// of the keys) and forms
+//     S^T  = K Q^T                      P^T = exp2(S^T * scale_log2 - lse * log2(e))
+//     dP^T = V dO^T                     dS^T = P^T * (dP^T - D),  D = rowsum(o * dO)
+//     dV  += P^T dO                     dK  += dS^T Q         dQ_tile += dS K
+// dK and dV of all the q heads of a group stay in tensor memory over the whole
+// walk, so the gradients of shared heads need no reduction and no atomics.
+//
+// Bound: shared-memory traffic of the five products and the dQ staging, as in
+// wf_bwd_main_kernel, whose pipeline, roles and layouts this is (one CTA per
+// key tile; the elementwise warpgroups, the dQ warpgroup, one MMA and one TMA
+// warp).  What differs:
+//
+//   items     The plan's key tiles, sorted by falling number of query tiles
+//             (causal: the first keys of a sequence are seen by all its rows),
+//             heads innermost.  Few long items are split over the units
+//             (nsplit); each split leaves fp32 partial dK/dV of its own, summed
+//             in a fixed order by the convert.
+//   masks     Key r of the tile is seen by query rows >= need + r.  Only units
+//             whose rows start below need + 127 compare.  Masked scores become
+//             -inf before the exponential.
+//   isolation -lse * log2(e) and D come from padded tiles (-inf and 0 behind
+//             the sequence's end), so those columns have P = dS = 0; the rows of
+//             Q, dO and K behind the ends, which belong to a neighbour or to
+//             padding and may be NaN, are zeroed in shared memory before a
+//             product sums over them.
+//   dQ        The fp32 accumulator is tiled by the plan's query tiles, so no
+//             tile holds rows of two sequences.  In ordered mode every tile gets
+//             its contributions key tile by key tile (bitwise reproducible).
+#include "wf_common.cuh"
+#include "wf_kernels.h"
+
+namespace wf {
+
+// Preprocess: D = rowsum(o * dO), -lse * log2(e), and the zeroed dQ
+// accumulator.  Bound: HBM (1036 bytes per row and head).  grid (2 * tiles,
+// h), 256 threads: 64 rows of one tile, 16 threads per row.
+__global__ void __launch_bounds__(256) wf_packed_pre_kernel(PackedBwdParams p, const __nv_bfloat16* __restrict__ o,
+                                                            const __nv_bfloat16* __restrict__ dO,
+                                                            const float* __restrict__ lse) {
+  griddep_launch_dependents();
+  griddep_wait();  // the plan
+  const int tile = blockIdx.x >> 1, half = blockIdx.x & 1, h = blockIdx.y;
+  if (tile >= p.head[1].x) return;
+  const int4 w = p.q_tiles[tile];
+  if (!w.z) return;  // rows outside any sequence
+  const size_t at = (size_t)h * p.q_tile_stride + tile;
+  const int sub = threadIdx.x & 15, rr = threadIdx.x >> 4;
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int r = half * 64 + pass * 16 + rr;
+    float acc = 0.f;
+    if (r < w.y) {
+      const size_t off = ((size_t)(w.x + r) * p.h + h) * 128 + sub * 8;
+      const uint4 a = ldg_u4(o + off);
+      const uint4 c = ldg_u4(dO + off);
+      acc = bf16_dot2(a.x, c.x) + bf16_dot2(a.y, c.y) + bf16_dot2(a.z, c.z) + bf16_dot2(a.w, c.w);
+    }
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
+    if (sub == 0) {
+      float nl2 = -INFINITY;  // pad rows and rows that see nothing: P = 0
+      if (r < w.y) {
+        const float l = lse[(size_t)h * p.total_q + w.x + r];
+        if (l == -INFINITY) acc = 0.f; else nl2 = -(l * 1.4426950408889634f);
+      }
+      p.dpsum[at * 128 + r] = acc;
+      p.neg_lse_log2[at * 128 + r] = nl2;
+    }
+  }
+  float4* run = reinterpret_cast<float4*>(p.dq_accum + at * 16384 + half * 8192);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) run[threadIdx.x + i * 256] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// Unit u of a key tile's walk -> q head within the group, query tile.
+struct PackedUnits {
+  int m_begin, m_count, first, count, reverse;
+  __device__ __forceinline__ void at(int u, int& g, int& m) const {
+    const int i = first + (reverse ? count - 1 - u : u);
+    g = i / m_count;
+    m = m_begin + (i - g * m_count);
+  }
+};
+
+__global__ void __launch_bounds__(bwd::kThreads, 1)
+    wf_packed_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                         PackedBwdParams p) {
+  using namespace bwd;
+  extern __shared__ uint8_t smem_raw[];
+  const uintptr_t raw = reinterpret_cast<uintptr_t>(smem_raw);
+  uint8_t* smem = reinterpret_cast<uint8_t*>((raw + 1023) & ~uintptr_t(1023));
+  griddep_launch_dependents();
+  if ((uint32_t)(reinterpret_cast<uintptr_t>(smem) - raw) + kSmemUsed > dynamic_smem_size()) {
+    // the aligned layout does not fit: report and leave (uniform for the CTA)
+    if (threadIdx.x == 0) atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_SMEM_ALIGN);
+    return;
+  }
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + kOffBar;
+  auto bar = [&](int i) -> uint32_t { return bar0 + 8u * (uint32_t)i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOffAbort);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kOffTmemHolder);
+  const int warp = (int)warp_id();
+  const int lane = (int)lane_id();
+
+  griddep_wait();  // the plan's lists, and what the preprocess wrote
+  const int kvh = blockIdx.x % p.h_kv;
+  const int rest = blockIdx.x / p.h_kv;
+  const int split = rest % p.nsplit;
+  const int tile = rest / p.nsplit;
+  if (tile >= p.head[0].x) return;
+  const PackedKTile w = p.k_tiles[tile];
+  const int units = w.m_count * p.group;
+  const int chunk = (units + p.nsplit - 1) / p.nsplit;
+  PackedUnits walk;
+  walk.m_begin = w.m_begin;
+  walk.m_count = max(w.m_count, 1);
+  walk.first = min(split * chunk, units);
+  walk.count = min(chunk, units - walk.first);
+  // successive waves of CTAs walk in alternating directions and start on the
+  // query tiles that the previous wave touched last (still in L2)
+  walk.reverse = !p.ordered && p.wave > 0 && ((blockIdx.x / (unsigned)p.wave) & 1u);
+  const int cnt = walk.count;
+  // partial dK/dV of this split, in the tiled layout of the dQ accumulator
+  const size_t part = (((size_t)split * p.h_kv + kvh) * p.k_tile_stride + tile) * 16384;
+  if (cnt <= 0) {
+    // no query row sees these keys (or a split without units, or rows outside any sequence)
+    if (p.nsplit > 1) {
+      for (int i = threadIdx.x; i < 4096; i += kThreads) {
+        reinterpret_cast<float4*>(p.dk_part + part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        reinterpret_cast<float4*>(p.dv_part + part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    } else {
+      const uint32_t fill = p.head[0].y ? 0x7fff7fffu : 0u;  // NaN where the offsets were impossible
+      for (int i = threadIdx.x; i < w.rows * 16; i += kThreads) {
+        const size_t off = ((size_t)(w.k0 + (i >> 4)) * p.h_kv + kvh) * 128 + (i & 15) * 8;
+        st_global_v4(p.dk + off, fill, fill, fill, fill);
+        st_global_v4(p.dv + off, fill, fill, fill, fill);
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNumBars; ++i) {
+      const bool ew = (i == kBarPReady || i == kBarDsReady);
+      const uint32_t count = ew ? 256u : (i == kBarDqDrained || i == kBarXchgDone || i == kBarXchgFull) ? 128u : 1u;
+      mbar_init(bar(i), count);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  // first place of q head g of the group, query tile m, in the tiled workspaces
+  auto q_place = [&](int g, int m) -> size_t {
+    return (size_t)(kvh * p.group + g) * p.q_tile_stride + w.qtile + m;
+  };
+
+  if (warp >= 14) {
+    regs_dec<kRegsOther>();  // idle warps of warpgroup 3
+  } else if (warp == 13) {
+    regs_dec<kRegsOther>();
+    // ------------------------------------------------------------------ TMA
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      tma_prefetch_desc(&tm_do);
+      mbar_expect_tx(bar(kBarKvFull), 2 * kTileBytes);
+      for (int x = 0; x < 2; ++x) {
+        tma_load_4d(sbase + kOffK + x * kBoxBytes, &tm_k, bar(kBarKvFull), x * 64, w.k0, kvh, 0);
+        tma_load_4d(sbase + kOffV + x * kBoxBytes, &tm_v, bar(kBarKvFull), x * 64, w.k0, kvh, 0);
+      }
+      int issued0 = 0, issued1 = 0, issued_do = 0;  // completed uses per buffer (for the abort drain)
+      for (int u = 0; u < cnt; ++u) {
+        const int st = u & 1, use = u >> 1;
+        int g, m;
+        walk.at(u, g, m);
+        const int row = w.q0 + m * 128, h = kvh * p.group + g;
+        if (use > 0 && !mbar_wait(bar(kBarQEmpty + st), (use - 1) & 1, abort_flag, kRoleBwdLoad, 3 + st)) break;
+        const uint32_t qfull = bar(kBarQFull + st);
+        mbar_expect_tx(qfull, kTileBytes + 1024);
+        for (int x = 0; x < 2; ++x)
+          tma_load_4d(sbase + kOffQ + st * kTileBytes + x * kBoxBytes, &tm_q, qfull, x * 64, row, h, 0);
+        bulk_load(sbase + kOffLse + st * 512, p.neg_lse_log2 + q_place(g, m) * 128, 512, qfull);
+        bulk_load(sbase + kOffD + st * 512, p.dpsum + q_place(g, m) * 128, 512, qfull);
+        if (st) issued1 = use + 1; else issued0 = use + 1;
+        // dO has one buffer: refill it once dV of the previous unit has read it
+        if (u > 0 && !mbar_wait(bar(kBarDoEmpty), (u - 1) & 1, abort_flag, kRoleBwdLoad, 6)) break;
+        mbar_expect_tx(bar(kBarDoFull), kTileBytes);
+        for (int x = 0; x < 2; ++x)
+          tma_load_4d(sbase + kOffdO + x * kBoxBytes, &tm_do, bar(kBarDoFull), x * 64, row, h, 0);
+        issued_do = u + 1;
+      }
+      if (*abort_flag) {
+        mbar_wait_drain(bar(kBarKvFull), 0);
+        if (issued0 > 0) mbar_wait_drain(bar(kBarQFull + 0), (issued0 - 1) & 1);
+        if (issued1 > 0) mbar_wait_drain(bar(kBarQFull + 1), (issued1 - 1) & 1);
+        if (issued_do > 0) mbar_wait_drain(bar(kBarDoFull), (issued_do - 1) & 1);
+      }
+    }
+  } else if (warp == 12) {
+    regs_dec<kRegsOther>();
+    // ------------------------------------------------------------------ MMA
+    constexpr uint32_t id_kk = idesc_bf16(128, 128, 0, 0);  // A, B K-major
+    constexpr uint32_t id_kb = idesc_bf16(128, 128, 0, 1);  // A K-major (or TMEM), B MN-major
+    constexpr uint32_t id_mm = idesc_bf16(128, 128, 1, 1);  // A, B MN-major
+    const uint32_t tS = tmem, tdP = tmem + 128, tdV = tmem + 256, tdK = tmem + 384;
+    const uint64_t dK_k = sdesc(sbase + kOffK, 16, 1024);
+    const uint64_t dV_k = sdesc(sbase + kOffV, 16, 1024);
+    const uint64_t dK_mn = sdesc(sbase + kOffK, kBoxBytes, 1024);
+    const uint64_t dS_mn = sdesc(sbase + kOffdS, kBoxBytes, 1024);
+    auto koff = [](int ks) -> uint32_t { return (uint32_t)((ks >> 2) * kBoxBytes + (ks & 3) * 32); };
+    auto moff = [](int ks) -> uint32_t { return (uint32_t)(ks * 2048); };
+    // query rows of unit u (128 but for the sequence's last tile)
+    auto unit_rows = [&](int u) -> int {
+      int g, m;
+      walk.at(u, g, m);
+      return min(128, w.lq - m * 128);
+    };
+    auto issue_s = [&](int u) {  // S^T = K Q^T
+      const uint32_t sq = sbase + kOffQ + (u & 1) * kTileBytes;
+      const int rows = unit_rows(u);
+      if (rows < 128) packed_zero_rows(sq, rows);  // dK sums over the query rows
+      const uint64_t q_k = sdesc(sq, 16, 1024);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma_ss_e(tS, desc_add(dK_k, koff(ks)), desc_add(q_k, koff(ks)), id_kk, ks > 0);
+      mma_commit_e(bar(kBarSFull));
+    };
+    const uint64_t do_k = sdesc(sbase + kOffdO, 16, 1024);
+    const uint64_t do_mn = sdesc(sbase + kOffdO, kBoxBytes, 1024);
+    auto issue_dp = [&](int u) {  // dP^T = V dO^T
+      const int rows = unit_rows(u);
+      if (rows < 128) packed_zero_rows(sbase + kOffdO, rows);  // so does dV
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma_ss_e(tdP, desc_add(dV_k, koff(ks)), desc_add(do_k, koff(ks)), id_kk, ks > 0);
+      mma_commit_e(bar(kBarDpFull));
+    };
+    bool ok = mbar_wait_warp(bar(kBarKvFull), 0, abort_flag, kRoleBwdMma, 0) &&
+              mbar_wait_warp(bar(kBarQFull + 0), 0, abort_flag, kRoleBwdMma, 1) &&
+              mbar_wait_warp(bar(kBarDoFull), 0, abort_flag, kRoleBwdMma, 5);
+    if (ok) {
+      tc_fence_after();
+      if (w.rows < 128) packed_zero_rows(sbase + kOffK, w.rows);  // dQ sums over the keys
+      issue_dp(0);
+      issue_s(0);
+    }
+    for (int u = 0; u < cnt && ok; ++u) {
+      const int st = u & 1;
+      // dV += P^T dO   (P^T from TMEM: query 0-63 in columns [0,32), 64-127 in [64,96))
+      if (!(ok = mbar_wait_warp(bar(kBarPReady), u & 1, abort_flag, kRoleBwdMma, 7))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+        mma_ts_e(tdV, tS + (ks >> 2) * 64 + (ks & 3) * 8, desc_add(do_mn, moff(ks)), id_kb, (u > 0 || ks > 0) ? 1u : 0u);
+      mma_commit_e(bar(kBarDoEmpty));  // dO(u) is read by dP(u) and dV(u) only
+      // S^T(u+1): the S columns are free once dV(u) has read P^T(u)
+      if (u + 1 < cnt) {
+        if (!(ok = mbar_wait_warp(bar(kBarQFull + ((u + 1) & 1)), ((u + 1) >> 1) & 1, abort_flag, kRoleBwdMma, 1)))
+          break;
+        tc_fence_after();
+        issue_s(u + 1);
+      }
+      // dK += dS^T Q
+      if (!(ok = mbar_wait_warp(bar(kBarDsReady), u & 1, abort_flag, kRoleBwdMma, 8))) break;
+      tc_fence_after();
+      const uint64_t q_mn = sdesc(sbase + kOffQ + st * kTileBytes, kBoxBytes, 1024);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+        mma_ts_e(tdK, tdP + (ks >> 2) * 64 + (ks & 3) * 8, desc_add(q_mn, moff(ks)), id_kb, (u > 0 || ks > 0) ? 1u : 0u);
+      mma_commit_e(bar(kBarQEmpty + st));
+      // dQ_tile = dS K   (same dS bytes read MN-major) into the dP^T columns
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma_ss_e(tdP, desc_add(dS_mn, moff(ks)), desc_add(dK_mn, moff(ks)), id_mm, ks > 0);
+      mma_commit_e(bar(kBarDqFull));
+      mma_commit_e(bar(kBarDsEmpty));
+      // dP^T(u+1) once dQ(u) has been read out of those columns and dO(u+1) is in
+      if (u + 1 < cnt) {
+        if (!(ok = mbar_wait_warp(bar(kBarDqDrained), u & 1, abort_flag, kRoleBwdMma, 11))) break;
+        if (!(ok = mbar_wait_warp(bar(kBarDoFull), (u + 1) & 1, abort_flag, kRoleBwdMma, 5))) break;
+        tc_fence_after();
+        issue_dp(u + 1);
+      }
+    }
+    if (ok) mma_commit_e(bar(kBarDkvFull));
+    mma_commit_e(bar(kBarDrain));
+    mbar_wait_drain(bar(kBarDrain), 0);
+  } else if (warp < 8) {
+    regs_inc<kRegsEw>();
+    // ---------------------------------------------- elementwise warpgroups
+    const int half = warp >> 2;   // 0: query columns [0,64), 1: [64,128)
+    const int wq = warp & 3;      // TMEM lane quadrant: key rows [32 wq, 32 wq + 32)
+    // 16x256b TMEM reads: thread t holds key rows 32 wq + 16 g + 8 e + t/4 and, in
+    // repetition j, query columns 64 half + 8 j + 2 (t%4) + {0, 1}
+    const int tq = lane & 3;
+    const int tr = lane >> 2;
+    auto kv_row = [&](int g, int e) -> int { return wq * 32 + 16 * g + 8 * e + tr; };
+    bool kv_ok[2][2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) kv_ok[g][e] = kv_row(g, e) < w.rows;
+    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+    constexpr uint32_t kLane16 = 16u << 16;
+    const uint32_t tS = tmem + lane_base + (uint32_t)(half * 64);
+    const uint32_t tdP = tmem + lane_base + 128u + (uint32_t)(half * 64);
+    const float sl2 = p.scale_log2;
+    const uint64_t sl2x2 = f2_pack(sl2, sl2);
+    const uint32_t sdS = sbase + kOffdS + (uint32_t)half * kBoxBytes;
+    bool ok = true;
+    for (int u = 0; u < cnt; ++u) {
+      const int st = u & 1;
+      const float* snl = reinterpret_cast<const float*>(smem + kOffLse + st * 512) + half * 64 + 2 * tq;
+      const float* sD = reinterpret_cast<const float*>(smem + kOffD + st * 512) + half * 64 + 2 * tq;
+      int unit_g, unit_m;
+      walk.at(u, unit_g, unit_m);
+      if (!(ok = mbar_wait(bar(kBarSFull), u & 1, abort_flag, kRoleEw, 5))) break;
+      // -lse*log2(e) / D of this unit arrived with Q (already complete; this
+      // wait makes the bulk-copied bytes visible to these threads)
+      if (!(ok = mbar_wait(bar(kBarQFull + st), (u >> 1) & 1, abort_flag, kRoleEw, 1))) break;
+      tc_fence_after();
+      uint32_t s[2][32];
+      tmem_ld_16x256b_x8(tS, s[0]);
+      tmem_ld_16x256b_x8(tS + kLane16, s[1]);
+      uint64_t nl[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 L = *reinterpret_cast<const float2*>(snl + 8 * j);
+        nl[j] = f2_pack(L.x, L.y);
+      }
+      tmem_wait_ld();
+      reg_fence32(s[0]);
+      reg_fence32(s[1]);
+      // key row r is seen by the unit's columns >= below + r
+      const int below = w.need - unit_m * 128;
+      if (below > -127) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int first = below + kv_row(g, e) - half * 64 - 2 * tq;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (8 * j + i < first) s[g][4 * j + 2 * e + i] = __float_as_uint(-INFINITY);
+          }
+      }
+      // P^T = 2^(S^T * scale_log2 + neg_lse_log2[q]); rounded to bf16 as the
+      // dV product's operand, kept in fp32 for dS.  Rows past the keys' end are zeroed.
+      uint64_t pp[2][16];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[g][4 * j + 2 * e]), __uint_as_float(s[g][4 * j + 2 * e + 1])),
+                                      sl2x2, nl[j]);
+            pp[g][2 * j + e] = exp2_mufu2(x);
+            float p0, p1;
+            f2_unpack(pp[g][2 * j + e], p0, p1);
+            pk[2 * j + e] = kv_ok[g][e] ? pack_bf16(p0, p1) : 0u;
+          }
+        tmem_st_16x128b_x8(tS + (g ? kLane16 : 0u), pk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(bar(kBarPReady));
+      // dS^T = P^T * (dP^T - D[q])
+      if (!(ok = mbar_wait(bar(kBarDpFull), u & 1, abort_flag, kRoleEw, 6))) break;
+      tc_fence_after();
+      uint32_t dp[2][32];
+      tmem_ld_16x256b_x8(tdP, dp[0]);
+      tmem_ld_16x256b_x8(tdP + kLane16, dp[1]);
+      tmem_wait_ld();
+      reg_fence32(dp[0]);
+      reg_fence32(dp[1]);
+      tc_fence_before();  // the dP columns are read; dQ(u) may overwrite them after dS_ready
+      if (u > 0 && !(ok = mbar_wait(bar(kBarDsEmpty), (u - 1) & 1, abort_flag, kRoleEw, 9))) break;
+      const uint64_t m1x2 = f2_pack(-1.f, -1.f);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2 D = *reinterpret_cast<const float2*>(sD + 8 * j);
+          const uint64_t d2 = f2_pack(D.x, D.y);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint64_t dpp = f2_pack(__uint_as_float(dp[g][4 * j + 2 * e]), __uint_as_float(dp[g][4 * j + 2 * e + 1]));
+            float d0, d1;
+            f2_unpack(f2_mul(pp[g][2 * j + e], f2_fma(d2, m1x2, dpp)), d0, d1);
+            pk[2 * j + e] = kv_ok[g][e] ? pack_bf16(d0, d1) : 0u;
+            // row of dS^T in shared memory for the dQ MMA (128B-swizzled
+            // [kv][q] box of this half): 4 bytes of the 16-byte chunk j
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sdS + sw128_offset((uint32_t)kv_row(g, e), (uint32_t)j) +
+                                                          4u * (uint32_t)tq),
+                         "r"(pk[2 * j + e])
+                         : "memory");
+          }
+        }
+        tmem_st_16x128b_x8(tdP + (g ? kLane16 : 0u), pk);
+      }
+      fence_proxy_async_smem();
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(bar(kBarDsReady));
+    }
+    // ----------------------------------------------------------- epilogue
+    // WG A writes dV (unscaled), WG B writes dK (scaled by softmax_scale)
+    const int r = wq * 32 + lane;  // 32x32b reads: thread = one key row
+    if (ok) ok = mbar_wait(bar(kBarDkvFull), 0, abort_flag, kRoleEpi, 12);
+    if (ok) {
+      tc_fence_after();
+      const uint32_t tsrc = tmem + lane_base + (half ? 384u : 256u);
+      const float mul = half ? p.scale : 1.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t a[32];
+        tmem_ld32(tsrc + c * 32, a);
+        tmem_wait_ld();
+        reg_fence32(a);
+        if (p.nsplit == 1) {
+          if (r < w.rows) {
+            __nv_bfloat16* row = (half ? p.dk : p.dv) + ((size_t)(w.k0 + r) * p.h_kv + kvh) * 128;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              st_global_v4(row + c * 32 + v * 8,
+                           pack_bf16(__uint_as_float(a[8 * v + 0]) * mul, __uint_as_float(a[8 * v + 1]) * mul),
+                           pack_bf16(__uint_as_float(a[8 * v + 2]) * mul, __uint_as_float(a[8 * v + 3]) * mul),
+                           pack_bf16(__uint_as_float(a[8 * v + 4]) * mul, __uint_as_float(a[8 * v + 5]) * mul),
+                           pack_bf16(__uint_as_float(a[8 * v + 6]) * mul, __uint_as_float(a[8 * v + 7]) * mul));
+          }
+        } else {
+          float* dst = (half ? p.dk_part : p.dv_part) + part + (size_t)(r >> 6) * 8192 + (size_t)(r & 63) * 4;
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            *reinterpret_cast<float4*>(dst + (size_t)(c * 8 + g) * 256) =
+                make_float4(__uint_as_float(a[4 * g + 0]) * mul, __uint_as_float(a[4 * g + 1]) * mul,
+                            __uint_as_float(a[4 * g + 2]) * mul, __uint_as_float(a[4 * g + 3]) * mul);
+        }
+      }
+    }
+  } else {
+    regs_inc<kRegsDq>();
+    // ------------------------------------------------------- dQ warpgroup
+    // dQ(u) leaves TMEM into registers, goes through a 32 KB staging buffer in
+    // two column halves and is reduced into the accumulator by two bulk
+    // reductions per half
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;  // query row within the tile
+    const uint32_t tQ = tmem + ((uint32_t)(wq * 32) << 16) + 128u;  // dQ lives in the dP^T columns
+    const uint32_t sx = sbase + kOffX;
+    uint8_t* xb = smem + kOffX;
+    const bool leader = (threadIdx.x == 256);
+    for (int u = 0; u < cnt; ++u) {
+      if (!mbar_wait(bar(kBarDqFull), u & 1, abort_flag, kRoleDq, 10)) break;
+      tc_fence_after();
+      uint32_t q[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(tQ + c * 32, q[c]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) reg_fence32(q[c]);
+      tc_fence_before();
+      mbar_arrive(bar(kBarDqDrained));
+      int unit_g, unit_m;
+      walk.at(u, unit_g, unit_m);
+      const size_t place = q_place(unit_g, unit_m);
+      float* dst = p.dq_accum + place * 16384;
+      int* const sem = p.ordered ? p.sem + place : nullptr;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // the staging buffer is free once the previous bulk reduction has read it
+        if (leader) bulk_wait_read_all();
+        mbar_arrive(bar(kBarXchgDone));
+        if (!mbar_wait(bar(kBarXchgDone), (2 * u + half) & 1, abort_flag, kRoleDq, 16)) break;
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            *reinterpret_cast<uint4*>(xb + (((r >> 6) * 16 + cc * 8 + g) * 64 + (r & 63)) * 16) =
+                make_uint4(q[2 * half + cc][4 * g + 0], q[2 * half + cc][4 * g + 1], q[2 * half + cc][4 * g + 2],
+                           q[2 * half + cc][4 * g + 3]);
+        fence_proxy_async_smem();
+        mbar_arrive(bar(kBarXchgFull));
+        if (leader) {
+          if (!mbar_wait(bar(kBarXchgFull), (2 * u + half) & 1, abort_flag, kRoleDq, 15)) break;
+          if (sem != nullptr && half == 0) {
+            // the sequence's key tiles 0..nb-1 add to this query tile first
+            if (!counter_wait_eq(sem, w.nb, abort_flag, kRoleDq, 20)) break;
+            fence_proxy_async_global();
+          }
+          bulk_reduce_add_f32(dst + half * 4096, sx, 16384);
+          bulk_reduce_add_f32(dst + 8192 + half * 4096, sx + 16384, 16384);
+          bulk_commit_group();
+          if (sem != nullptr && half == 1) {
+            bulk_wait_all();  // the reductions have landed in global memory
+            fence_proxy_async_global();
+            st_release_gpu(sem, w.nb + 1);
+          }
+        }
+      }
+      if (*abort_flag) break;
+    }
+    if (leader) bulk_wait_all();
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// fp32 tiles -> bf16 rows, times a scale: the dQ accumulator (parts = 1), or
+// the sum of the splits' partial dK or dV in a fixed order.  Rows outside any
+// sequence become 0 (NaN where the offsets were impossible).  Bound: HBM.
+// grid (4 * tiles, heads), 256 threads: 32 rows x 128 columns.
+__global__ void __launch_bounds__(256) wf_packed_convert_kernel(PackedConvertParams p) {
+  __shared__ float tile[32][132];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int t = blockIdx.x >> 2, row0 = (blockIdx.x & 3) * 32, h = blockIdx.y;
+  const int4 head = *p.head;
+  if (t >= head.x) return;
+  int first, rows;
+  bool inside;
+  if (p.q_tiles) {
+    const int4 w = p.q_tiles[t];
+    first = w.x, rows = w.y, inside = w.z != 0;
+  } else {
+    const PackedKTile w = p.k_tiles[t];
+    first = w.k0, rows = w.rows, inside = w.m_count > 0;
+  }
+  if (row0 >= rows) return;
+  const int half = row0 >> 6, r0 = row0 & 63;
+  if (inside) {
+    const float* src = p.accum + ((size_t)h * p.tile_stride + t) * 16384 + half * 8192;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int idx = threadIdx.x + i * 256;  // 32 groups of 4 columns x 32 rows
+      const int g = idx >> 5, rw = idx & 31;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = 0; s < p.parts; ++s) {
+        const float4 x = *reinterpret_cast<const float4*>(src + s * p.part_stride + (g * 64 + r0 + rw) * 4);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      *reinterpret_cast<float4*>(&tile[rw][4 * g]) = v;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int idx = threadIdx.x + i * 256;  // 32 rows x 16 chunks of 8
+    const int rw = idx >> 4, ch = idx & 15;
+    if (row0 + rw >= rows) continue;
+    const uint32_t fill = head.y ? 0x7fff7fffu : 0u;
+    uint4 w = make_uint4(fill, fill, fill, fill);
+    if (inside) {
+      const float* x = &tile[rw][ch * 8];
+      w.x = pack_bf16(x[0] * p.scale, x[1] * p.scale);
+      w.y = pack_bf16(x[2] * p.scale, x[3] * p.scale);
+      w.z = pack_bf16(x[4] * p.scale, x[5] * p.scale);
+      w.w = pack_bf16(x[6] * p.scale, x[7] * p.scale);
+    }
+    *reinterpret_cast<uint4*>(p.out + ((size_t)(first + row0 + rw) * p.heads + h) * 128 + ch * 8) = w;
+  }
+}
+
+}  // namespace wf

@@ -22,6 +22,33 @@ struct PackedFwdWorkspace {  // byte offsets
   }
 };
 
+struct PackedBwdWorkspace {  // byte offsets
+  size_t head = 0, base, k_tiles, q_tiles, neg_lse_log2, dpsum, dq_accum, dk_part, dv_part, sem, sem_bytes, bytes;
+  size_t q_tile_stride, k_tile_stride;
+  PackedBwdWorkspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg) {
+    q_tile_stride = (size_t)packed_max_tiles(total_q, n, 128);
+    k_tile_stride = (size_t)packed_max_tiles(total_k, n, 128);
+    const size_t q_all = q_tile_stride * h, parts = cfg->nsplit > 1 ? (size_t)cfg->nsplit * h_kv * k_tile_stride : 0;
+    base = 256;
+    k_tiles = align256(base + (size_t)3 * (n + 3) * 4);
+    q_tiles = align256(k_tiles + k_tile_stride * sizeof(PackedKTile));
+    neg_lse_log2 = align256(q_tiles + q_tile_stride * sizeof(int4));
+    dpsum = neg_lse_log2 + q_all * 512;
+    dq_accum = align256(dpsum + q_all * 512);
+    dk_part = dq_accum + q_all * 65536;
+    dv_part = dk_part + parts * 65536;
+    sem = dv_part + parts * 65536;
+    sem_bytes = cfg->deterministic ? q_all * 4 : 0;
+    bytes = sem + sem_bytes;
+  }
+};
+
+int packed_bwd_cfg_check(const wf_packed_bwd_cfg* cfg) {
+  if (!cfg) return fail(WF_ERR_INVALID_ARG, "null cfg");
+  if (cfg->nsplit < 1 || cfg->nsplit > 1024) return fail(WF_ERR_INVALID_ARG, "nsplit=%d outside [1, 1024]", cfg->nsplit);
+  return WF_OK;
+}
+
 int packed_check(int n, int total_q, int total_k, int h, int h_kv, int causal) {
   if (n < 0 || total_q < 0 || total_k < 0 || h < 0 || h_kv < 0) return fail(WF_ERR_INVALID_ARG, "negative size");
   if (causal != 0 && causal != 1) return fail(WF_ERR_INVALID_ARG, "causal %d not in {0, 1}", causal);
@@ -45,7 +72,10 @@ int plan_shift(int total) {
 }  // namespace
 
 cudaError_t packed_setup() {
-  return cudaFuncSetAttribute(wf_packed_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pfwd::kSmemBytes);
+  cudaError_t e =
+      cudaFuncSetAttribute(wf_packed_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pfwd::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(wf_packed_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd::kSmemBytes);
 }
 
 }  // namespace wf
@@ -108,4 +138,110 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
                             mk, mv, mo, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
   return launch_check("wf_packed_fwd launch");
+}
+
+extern "C" int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg,
+                                       size_t* bytes) {
+  if (!bytes) return fail(WF_ERR_INVALID_ARG, "null pointer");
+  int rc;
+  if ((rc = packed_check(n, total_q, total_k, h, h_kv, 0)) || (rc = packed_bwd_cfg_check(cfg))) return rc;
+  *bytes = PackedBwdWorkspace(n, total_q, total_k, h, h_kv, cfg).bytes;
+  return WF_OK;
+}
+
+extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                             const void* dO, const int* q_offsets, const int* k_offsets, void* dq, void* dk, void* dv,
+                             void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv,
+                             int causal, const wf_packed_bwd_cfg* cfg, void* stream) {
+  int rc;
+  if ((rc = packed_check(n, total_q, total_k, h, h_kv, causal)) || (rc = packed_bwd_cfg_check(cfg))) return rc;
+  if (h == 0 || (total_q == 0 && total_k == 0)) return WF_OK;
+  if (total_q == 0 || total_k == 0)
+    return fail(WF_ERR_UNSUPPORTED, "no queries or no keys: the caller must zero the gradients");
+  if (!q || !k || !v || !o || !lse || !dO || !q_offsets || !k_offsets || !dq || !dk || !dv || !workspace)
+    return fail(WF_ERR_INVALID_ARG, "null pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dO) || !aligned16(dq) ||
+      !aligned16(dk) || !aligned16(dv) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) ||
+      (reinterpret_cast<uintptr_t>(q_offsets) & 3) || (reinterpret_cast<uintptr_t>(k_offsets) & 3))
+    return fail(WF_ERR_MISALIGNED, "tensors and workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
+  const PackedBwdWorkspace ws(n, total_q, total_k, h, h_kv, cfg);
+  if (workspace_bytes < ws.bytes)
+    return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
+  const unsigned long long items = (unsigned long long)ws.k_tile_stride * h_kv * cfg->nsplit;
+  if (items > 0x7fffffffULL || ws.q_tile_stride * 4 > 0x7fffffffULL || ws.k_tile_stride * 4 > 0x7fffffffULL)
+    return fail(WF_ERR_UNSUPPORTED, "%llu work items exceed the grid limit", items);
+  int dev;
+  if ((rc = device_setup(&dev))) return rc;
+  CUtensorMap mq, mk, mv, mdo;
+  if ((rc = make_bshd_map(&mq, q, 1, total_q, h)) || (rc = make_bshd_map(&mk, k, 1, total_k, h_kv)) ||
+      (rc = make_bshd_map(&mv, v, 1, total_k, h_kv)) || (rc = make_bshd_map(&mdo, dO, 1, total_q, h)))
+    return rc;
+  uint8_t* const w = reinterpret_cast<uint8_t*>(workspace);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  PackedPlanParams pp = {};
+  pp.q_off = q_offsets, pp.k_off = k_offsets;
+  pp.n = n, pp.total_q = total_q, pp.total_k = total_k, pp.causal = causal;
+  pp.backward = 1;
+  pp.ordered = cfg->deterministic ? 1 : 0;
+  pp.cost_shift = plan_shift(total_q);
+  pp.head = reinterpret_cast<int4*>(w + ws.head);
+  pp.base = reinterpret_cast<int*>(w + ws.base);
+  pp.k_tiles = reinterpret_cast<PackedKTile*>(w + ws.k_tiles);
+  pp.q_tiles = reinterpret_cast<int4*>(w + ws.q_tiles);
+  PackedBwdParams p = {};
+  p.head = pp.head;
+  p.k_tiles = pp.k_tiles;
+  p.q_tiles = pp.q_tiles;
+  p.neg_lse_log2 = reinterpret_cast<float*>(w + ws.neg_lse_log2);
+  p.dpsum = reinterpret_cast<float*>(w + ws.dpsum);
+  p.dq_accum = reinterpret_cast<float*>(w + ws.dq_accum);
+  p.dk = reinterpret_cast<__nv_bfloat16*>(dk);
+  p.dv = reinterpret_cast<__nv_bfloat16*>(dv);
+  p.dk_part = reinterpret_cast<float*>(w + ws.dk_part);
+  p.dv_part = reinterpret_cast<float*>(w + ws.dv_part);
+  p.sem = reinterpret_cast<int*>(w + ws.sem);
+  p.q_tile_stride = ws.q_tile_stride, p.k_tile_stride = ws.k_tile_stride;
+  p.total_q = total_q, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
+  p.nsplit = cfg->nsplit;
+  p.ordered = pp.ordered;
+  p.wave = g_dev_sms[dev];
+  p.scale = (float)(1.0 / std::sqrt(128.0));
+  p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
+  cudaError_t e;
+  if (ws.sem_bytes) {
+    e = cudaMemsetAsync(p.sem, 0, ws.sem_bytes, st);
+    if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd counters");
+  }
+  wf_packed_plan_kernel<<<2, kPlanThreads, 0, st>>>(pp);
+  if ((rc = launch_check("wf_packed plan launch"))) return rc;
+  e = launch_ex(wf_packed_pre_kernel, dim3((unsigned)(2 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, p,
+                reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(dO), lse);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd preprocess launch");
+  e = launch_ex(wf_packed_bwd_kernel, dim3((unsigned)items), dim3(bwd::kThreads), bwd::kSmemBytes, st, true, 1u, mq, mk,
+                mv, mdo, p);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd launch");
+  PackedConvertParams c = {};
+  c.head = pp.head + 1;
+  c.q_tiles = pp.q_tiles;
+  c.accum = p.dq_accum;
+  c.tile_stride = ws.q_tile_stride;
+  c.parts = 1, c.heads = h;
+  c.scale = p.scale;
+  c.out = reinterpret_cast<__nv_bfloat16*>(dq);
+  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, c);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd dq convert launch");
+  for (int i = 0; i < (cfg->nsplit > 1 ? 2 : 0); ++i) {
+    c.head = pp.head;
+    c.q_tiles = nullptr;
+    c.k_tiles = pp.k_tiles;
+    c.accum = i ? p.dv_part : p.dk_part;
+    c.tile_stride = ws.k_tile_stride;
+    c.part_stride = ws.k_tile_stride * h_kv * 16384;
+    c.parts = cfg->nsplit, c.heads = h_kv;
+    c.scale = 1.f;  // dk was scaled where it left the tensor core
+    c.out = reinterpret_cast<__nv_bfloat16*>(i ? dv : dk);
+    e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * ws.k_tile_stride), h_kv), dim3(256), 0, st, true, 1u, c);
+    if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd dk/dv convert launch");
+  }
+  return launch_check("wf_packed_bwd launch");
 }

@@ -137,7 +137,7 @@ __device__ PackedKTile plan_k_tile(const PackedPlanParams& p, bool bad, const in
   w.rows = min(128, lk - n0);
   w.q0 = w.lq = w.m_begin = w.m_count = w.qtile = w.need = 0;
   w.nb = t - kbase[s];
-  w.tile = t;
+  w.pad0 = w.pad1 = w.pad2 = 0;
   if (!bad && s >= 1 && s <= p.n) {
     const int qs = __ldg(p.q_off + s - 1), lq = __ldg(p.q_off + s) - qs;
     w.q0 = qs;

@@ -32,9 +32,9 @@ import ctypes
 
 import torch
 
-from wan_flash import _lib
-from wan_flash.interface import _aligned, _ptr, _stream_ptr
-from wan_flash.shapes import HEAD_DIM
+from wan_flash import _lib, features
+from wan_flash.interface import _aligned, _auto_nsplit, _ptr, _sms, _stream_ptr
+from wan_flash.shapes import HEAD_DIM, TILE_N
 
 
 def _check(q, k, v, q_offsets, k_offsets):
@@ -78,3 +78,68 @@ def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
                              ctypes.c_void_p(_stream_ptr(q.device)))
     _lib.check(rc)
     return o, lse
+
+
+def packed_bwd_plan(total_q: int, total_k: int, n: int, h: int, h_kv: int, causal: bool, sms: int) -> dict:
+    """Split and mode of one backward call (host logic; the lengths themselves
+    are on the device, so the split goes by the mean sequence)."""
+    f = features.get_bwd()
+    tiles = max(1, -(-total_k // TILE_N))
+    # units of a key tile: query tiles of a mean sequence (half of them behind a causal diagonal), per q head of the group
+    units = max(1, -(-total_q // (TILE_N * max(n, 1))) * (h // max(h_kv, 1)) // (2 if causal else 1))
+    nsplit = f.nsplit if f.nsplit > 0 else _auto_nsplit(tiles * h_kv, min(units, 16), sms)
+    return {"nsplit": max(1, min(nsplit, 1024)), "deterministic": bool(f.deterministic)}
+
+
+def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                         do: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor | None = None,
+                         causal: bool = False):
+    """(dq, dk, dv) given the forward's o and lse and the gradient of o.
+
+    dk and dv are bitwise reproducible; dq is accumulated with fp32 reductions
+    unless ``features.set_bwd_overrides(deterministic=True)``.  ``nsplit`` of the
+    backward features applies; its CTA-pair form does not."""
+    q_offsets, k_offsets = _check(q, k, v, q_offsets, k_offsets)
+    total_q, h, _ = q.shape
+    total_k, h_kv, _ = k.shape
+    assert o.dtype == do.dtype == torch.bfloat16 and o.shape == q.shape and do.shape == q.shape
+    assert lse.dtype == torch.float32 and lse.shape == (h, total_q)
+    assert all(t.device == q.device for t in (o, lse, do)), "tensors must be on one CUDA device"
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if dq.numel() == 0 or dk.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    q, k, v, o, do = (_aligned(t) for t in (q, k, v, o, do))
+    lse = lse if lse.is_contiguous() else lse.contiguous()
+    n = q_offsets.numel() - 1
+    plan = packed_bwd_plan(total_q, total_k, n, h, h_kv, causal, _sms(q.device))
+    cfg = _lib.PackedBwdCfg(plan["nsplit"], 1 if plan["deterministic"] else 0)
+    L = _lib.lib()
+    size = _bytes(L.wf_packed_bwd_workspace, n, total_q, total_k, h, h_kv, ctypes.byref(cfg))
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    with torch.cuda.device(q.device):
+        rc = L.wf_packed_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(do), _ptr(q_offsets), _ptr(k_offsets),
+                             _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), size, n, total_q, total_k, h, h_kv,
+                             1 if causal else 0, ctypes.byref(cfg), ctypes.c_void_p(_stream_ptr(q.device)))
+    _lib.check(rc)
+    return dq, dk, dv
+
+
+class _WanFlashAttnPackedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_offsets, k_offsets, causal):
+        o, lse = wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal)
+        ctx.save_for_backward(q, k, v, o, lse, q_offsets, k_offsets)
+        ctx.causal = causal
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse, q_offsets, k_offsets = ctx.saved_tensors
+        dq, dk, dv = wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, ctx.causal)
+        return dq, dk, dv, None, None, None
+
+
+def wan_flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
+                          k_offsets: torch.Tensor | None = None, causal: bool = False):
+    """Differentiable attention over packed sequences -> o (total_q, h, 128) bf16."""
+    return _WanFlashAttnPackedFn.apply(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, bool(causal))
