@@ -248,12 +248,14 @@ int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offs
                   int h_kv, int causal, void* stream);
 
 typedef struct wf_packed_bwd_cfg {
-  int nsplit;        /* >= 1: CTAs per (128-key tile, key-value head); with more
-                        than one, fp32 partial dk/dv are summed in a fixed order */
+  int nsplit;        /* 0 = the device cuts long walks into pieces of about a
+                        quarter of an SM's share; n > 0: pieces of 1/n of the
+                        longest walk.  Pieces leave fp32 partial dk and dv that
+                        are summed in a fixed order */
   int deterministic; /* 1 = dq's fp32 contributions are added in key order */
 } wf_packed_bwd_cfg;
 
-/* Bytes of workspace of wf_packed_bwd. */
+/* Bytes of workspace of wf_packed_bwd on the current device. */
 int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg,
                             size_t* bytes);
 

@@ -8,7 +8,7 @@ import torch
 from tests.attn64 import assert_close, attn64, grads64
 from tests.test_packed import CASES, make, offsets
 from wan_flash import _lib, features
-from wan_flash.packed import packed_bwd_plan, wan_flash_attn_packed, wan_flash_packed_bwd, wan_flash_packed_fwd
+from wan_flash.packed import wan_flash_attn_packed, wan_flash_packed_bwd, wan_flash_packed_fwd
 
 
 @pytest.fixture(autouse=True)
@@ -169,6 +169,27 @@ def test_training_step_captured_and_replayed_with_other_offsets():
 
 
 @pytest.mark.gpu
+def test_c_entry_refuses_a_small_workspace():
+    import ctypes
+
+    lib, cfg, size = _lib.lib(), _lib.PackedBwdCfg(0, 0), ctypes.c_size_t()
+    assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, ctypes.byref(cfg), ctypes.byref(size)) == 0
+    p = ctypes.c_void_p
+    assert lib.wf_packed_bwd(*[p(16)] * 12, size.value - 1, 2, 8, 8, 4, 2, 0, ctypes.byref(cfg), None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_walks_are_cut_into_pieces(causal):
+    """One sequence, one key-value head for 8 q heads: 17 key tiles, cut by the device."""
+    q, k, v, do, qo, ko = make([2100], [2100], 8, 1, seed=12)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+    _lib.check_device()
+    check_bwd(q, k, v, do, qo, ko, causal, *grads)
+
+
+@pytest.mark.gpu
 def test_no_queries_or_no_keys():
     for lq, lk in (([0], [5]), ([5], [0])):
         q, k, v, do, qo, ko = make(lq, lk, 2, 1)
@@ -193,14 +214,8 @@ def test_refusals():
             wan_flash_packed_bwd(*bad)
 
 
-def test_plan_and_c_entry_refusals():
+def test_c_entry_refusals():
     import ctypes
-
-    assert packed_bwd_plan(16384, 16384, 4, 12, 12, False, 148) == {"nsplit": 1, "deterministic": False}
-    assert packed_bwd_plan(2048, 2048, 1, 8, 1, True, 148)["nsplit"] > 1     # 16 key tiles on 148 SMs
-    assert packed_bwd_plan(1, 1, 1, 1, 1, True, 148)["nsplit"] == 1
-    features.set_bwd_overrides(nsplit=5, deterministic=True)
-    assert packed_bwd_plan(16384, 16384, 4, 12, 12, False, 148) == {"nsplit": 5, "deterministic": True}
 
     lib = _lib.lib()
     size = ctypes.c_size_t()
@@ -211,8 +226,8 @@ def test_plan_and_c_entry_refusals():
         p = ctypes.c_void_p
         return lib.wf_packed_bwd(p(q) if q else None, *[p(16)] * 11, ws, n, tq, tk, h, hk, causal, ctypes.byref(c), None)
 
-    assert call(n=-1) == -1 and call(hk=3) == -1 and call(nsplit=0) == -1 and call(causal=3) == -1 and call(q=None) == -1
-    assert call(q=8) == -3 and call(ws=100) == -1 and call(tq=0) == -2 and call(tk=0) == -2
+    assert call(n=-1) == -1 and call(hk=3) == -1 and call(nsplit=-1) == -1 and call(nsplit=2000) == -1 and call(causal=3) == -1 and call(q=None) == -1
+    assert call(q=8) == -3 and call(tq=0) == -2 and call(tk=0) == -2
     assert call(h=0, hk=0) == 0 and call(tq=0, tk=0) == 0
-    assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, ctypes.byref(cfg), ctypes.byref(size)) == 0 and size.value > 0
+    assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 3, ctypes.byref(cfg), ctypes.byref(size)) == -1
     assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, None, ctypes.byref(size)) == -1

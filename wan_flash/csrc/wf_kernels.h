@@ -70,29 +70,37 @@ struct __align__(16) PackedFwdTile {  // up to 256 query rows of one sequence
   int klen;       // keys that the tile's last row sees; 0: nothing to attend, the rows are filled
   int off;        // causal: keys that row 0 of the tile sees (row r: off + r); may be negative
   int n_blocks;   // ceil(klen / 128)
-  int pad0, pad1;
+  int bucket, bucket_items;  // place and number of the items of equal cost
 };
-struct __align__(16) PackedKTile {  // up to 128 key rows of one sequence
+struct __align__(16) PackedBwdItem {  // up to 128 key rows of one sequence, and a piece of their walk
   int k0, rows;   // first row in the packed tensor, rows
   int q0, lq;     // the sequence's query rows
   int qtile;      // the sequence's first query tile (place in the fp32 workspaces)
   int m_begin, m_count;  // query tiles of the sequence that see some of these keys
   int need;       // first query row of the sequence that sees the tile's first key (key r: need + r)
   int nb;         // place of the tile in its sequence
-  int pad0, pad1, pad2;
+  int first, count;      // units (q head of the group, query tile) of this piece
+  int part;       // place of the piece's partial dK and dV; -1: the whole walk, written as the result
+  int bucket, bucket_items;
+  int pad0, pad1;
 };
 struct PackedPlanParams {
   const int* q_off;
   const int* k_off;
   int n, total_q, total_k;
   int causal, backward, ordered;
-  int cost_shift;           // cost >> cost_shift stays below the number of sort buckets
-  int4* head;               // {tiles, status}: [0] the sorted list, [1] (backward) the query tiles
+  int group, h_kv;
+  int nsplit;               // > 0: pieces of the longest walk; 0: by `pieces`
+  int pieces;               // pieces (over all key-value heads) that the whole work is cut into at least
+  int4* head;               // [0] {items, status, split key tiles}, [1] (backward) {query tiles, status}
   int* base;                // scratch: 3 * (n + 3)
   PackedFwdTile* fwd_tiles;
-  PackedKTile* k_tiles;
+  PackedBwdItem* items;
   int4* q_tiles;            // {first row, rows, 1 inside a sequence, 0}
+  int4* split_tiles;        // {first row, rows, first part, parts}
 };
+constexpr int kPackedMinChunk = 4;   // units: below, a piece's own cost exceeds what it evens out
+constexpr int kPackedPiecesPerSm = 4;
 struct PackedFwdParams {
   const int4* head;
   const PackedFwdTile* tiles;
@@ -103,29 +111,28 @@ struct PackedFwdParams {
 };
 struct PackedBwdParams {
   const int4* head;
-  const PackedKTile* k_tiles;
+  const PackedBwdItem* items;
   const int4* q_tiles;
   float* neg_lse_log2;      // (h, q_tile_stride, 128): -lse * log2(e), -inf behind the sequence's end
   float* dpsum;             // (h, q_tile_stride, 128)
   float* dq_accum;          // (h, q_tile_stride) tiles of 16384 fp32
   __nv_bfloat16* dk;        // (total_k, h_kv, 128)
   __nv_bfloat16* dv;
-  float* dk_part;           // nsplit > 1: (nsplit, h_kv, k_tile_stride) tiles of 16384 fp32
+  float* dk_part;           // (parts, h_kv) tiles of 16384 fp32
   float* dv_part;
   int* sem;                 // ordered: (h, q_tile_stride) key tiles added so far
-  size_t q_tile_stride, k_tile_stride;
-  int total_q, h, h_kv, group, nsplit, ordered, wave;
+  size_t q_tile_stride;
+  int total_q, h, h_kv, group, ordered, wave;
   float scale, scale_log2;
 };
 struct PackedConvertParams {
   const int4* head;
-  const int4* q_tiles;      // or, where null, k_tiles
-  const PackedKTile* k_tiles;
-  const float* accum;
-  size_t tile_stride, part_stride;  // tiles per head; floats between parts
-  int parts, heads;
+  const int4* tiles;        // dq: q_tiles; split: split_tiles
+  const float* accum[2];    // the dQ accumulator (h, tile_stride), or partial dK and dV (parts, h_kv)
+  __nv_bfloat16* out[2];    // (total, heads, 128)
+  size_t tile_stride;
+  int split, heads;
   float scale;
-  __nv_bfloat16* out;       // (total, heads, 128)
 };
 cudaError_t packed_setup();
 

@@ -15,11 +15,10 @@
 // key tile; the elementwise warpgroups, the dQ warpgroup, one MMA and one TMA
 // warp).  What differs:
 //
-//   items     The plan's key tiles, sorted by falling number of query tiles
-//             (causal: the first keys of a sequence are seen by all its rows),
-//             heads innermost.  Few long items are split over the units
-//             (nsplit); each split leaves fp32 partial dK/dV of its own, summed
-//             in a fixed order by the convert.
+//   items     The plan's key tiles, sorted by falling number of units (causal:
+//             the first keys of a sequence are seen by all its rows).  A long
+//             walk comes as several pieces; each leaves fp32 partial dK and dV
+//             of its own, summed in a fixed order by the convert.
 //   masks     Key r of the tile is seen by query rows >= need + r.  Only units
 //             whose rows start below need + 127 compare.  Masked scores become
 //             -inf before the exponential.
@@ -77,13 +76,22 @@ __global__ void __launch_bounds__(256) wf_packed_pre_kernel(PackedBwdParams p, c
   for (int i = 0; i < 8; ++i) run[threadIdx.x + i * 256] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
-// Unit u of a key tile's walk -> q head within the group, query tile.
-struct PackedUnits {
-  int m_begin, m_count, first, count, reverse;
-  __device__ __forceinline__ void at(int u, int& g, int& m) const {
-    const int i = first + (reverse ? count - 1 - u : u);
-    g = i / m_count;
-    m = m_begin + (i - g * m_count);
+// The units of an item's walk one by one, forwards or backwards: (q head g of
+// the group, query tile m), m fastest.  Only the start divides.
+struct PackedWalk {
+  int m_begin, m_end, g, m, step;
+  __device__ __forceinline__ PackedWalk(const PackedBwdItem& w, bool reverse) {
+    const int i = w.first + (reverse ? w.count - 1 : 0);
+    m_begin = w.m_begin;
+    m_end = w.m_begin + w.m_count;
+    g = i / w.m_count;
+    m = m_begin + (i - g * w.m_count);
+    step = reverse ? -1 : 1;
+  }
+  __device__ __forceinline__ void next() {
+    m += step;
+    if (m == m_end) m = m_begin, ++g;
+    else if (m < m_begin) m = m_end - 1, --g;
   }
 };
 
@@ -110,39 +118,20 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
   const int lane = (int)lane_id();
 
   griddep_wait();  // the plan's lists, and what the preprocess wrote
-  const int kvh = blockIdx.x % p.h_kv;
-  const int rest = blockIdx.x / p.h_kv;
-  const int split = rest % p.nsplit;
-  const int tile = rest / p.nsplit;
-  if (tile >= p.head[0].x) return;
-  const PackedKTile w = p.k_tiles[tile];
-  const int units = w.m_count * p.group;
-  const int chunk = (units + p.nsplit - 1) / p.nsplit;
-  PackedUnits walk;
-  walk.m_begin = w.m_begin;
-  walk.m_count = max(w.m_count, 1);
-  walk.first = min(split * chunk, units);
-  walk.count = min(chunk, units - walk.first);
+  if ((int)blockIdx.x >= p.head[0].x * p.h_kv) return;
+  int kvh;
+  const PackedBwdItem w = p.items[packed_locate(p.items, (int)blockIdx.x, p.h_kv, kvh)];
   // successive waves of CTAs walk in alternating directions and start on the
   // query tiles that the previous wave touched last (still in L2)
-  walk.reverse = !p.ordered && p.wave > 0 && ((blockIdx.x / (unsigned)p.wave) & 1u);
-  const int cnt = walk.count;
-  // partial dK/dV of this split, in the tiled layout of the dQ accumulator
-  const size_t part = (((size_t)split * p.h_kv + kvh) * p.k_tile_stride + tile) * 16384;
+  const bool reverse = !p.ordered && p.wave > 0 && ((blockIdx.x / (unsigned)p.wave) & 1u);
+  const int cnt = w.count;
   if (cnt <= 0) {
-    // no query row sees these keys (or a split without units, or rows outside any sequence)
-    if (p.nsplit > 1) {
-      for (int i = threadIdx.x; i < 4096; i += kThreads) {
-        reinterpret_cast<float4*>(p.dk_part + part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        reinterpret_cast<float4*>(p.dv_part + part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    } else {
-      const uint32_t fill = p.head[0].y ? 0x7fff7fffu : 0u;  // NaN where the offsets were impossible
-      for (int i = threadIdx.x; i < w.rows * 16; i += kThreads) {
-        const size_t off = ((size_t)(w.k0 + (i >> 4)) * p.h_kv + kvh) * 128 + (i & 15) * 8;
-        st_global_v4(p.dk + off, fill, fill, fill, fill);
-        st_global_v4(p.dv + off, fill, fill, fill, fill);
-      }
+    // no query row sees these keys, or rows outside any sequence
+    const uint32_t fill = p.head[0].y ? 0x7fff7fffu : 0u;  // NaN where the offsets were impossible
+    for (int i = threadIdx.x; i < w.rows * 16; i += kThreads) {
+      const size_t off = ((size_t)(w.k0 + (i >> 4)) * p.h_kv + kvh) * 128 + (i & 15) * 8;
+      st_global_v4(p.dk + off, fill, fill, fill, fill);
+      st_global_v4(p.dv + off, fill, fill, fill, fill);
     }
     return;
   }
@@ -185,10 +174,10 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
         tma_load_4d(sbase + kOffV + x * kBoxBytes, &tm_v, bar(kBarKvFull), x * 64, w.k0, kvh, 0);
       }
       int issued0 = 0, issued1 = 0, issued_do = 0;  // completed uses per buffer (for the abort drain)
-      for (int u = 0; u < cnt; ++u) {
+      PackedWalk at(w, reverse);
+      for (int u = 0; u < cnt; ++u, at.next()) {
         const int st = u & 1, use = u >> 1;
-        int g, m;
-        walk.at(u, g, m);
+        const int g = at.g, m = at.m;
         const int row = w.q0 + m * 128, h = kvh * p.group + g;
         if (use > 0 && !mbar_wait(bar(kBarQEmpty + st), (use - 1) & 1, abort_flag, kRoleBwdLoad, 3 + st)) break;
         const uint32_t qfull = bar(kBarQFull + st);
@@ -225,16 +214,13 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
     const uint64_t dS_mn = sdesc(sbase + kOffdS, kBoxBytes, 1024);
     auto koff = [](int ks) -> uint32_t { return (uint32_t)((ks >> 2) * kBoxBytes + (ks & 3) * 32); };
     auto moff = [](int ks) -> uint32_t { return (uint32_t)(ks * 2048); };
-    // query rows of unit u (128 but for the sequence's last tile)
-    auto unit_rows = [&](int u) -> int {
-      int g, m;
-      walk.at(u, g, m);
-      return min(128, w.lq - m * 128);
-    };
+    PackedWalk at(w, reverse);  // the unit whose S^T is issued next
+    int rows_s = 128, rows_dp = 128;  // query rows of the units of the last S^T and of the next dP^T
     auto issue_s = [&](int u) {  // S^T = K Q^T
       const uint32_t sq = sbase + kOffQ + (u & 1) * kTileBytes;
-      const int rows = unit_rows(u);
-      if (rows < 128) packed_zero_rows(sq, rows);  // dK sums over the query rows
+      rows_s = w.lq - at.m * 128;
+      at.next();
+      if (rows_s < 128) packed_zero_rows(sq, rows_s);  // dK sums over the query rows
       const uint64_t q_k = sdesc(sq, 16, 1024);
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) mma_ss_e(tS, desc_add(dK_k, koff(ks)), desc_add(q_k, koff(ks)), id_kk, ks > 0);
@@ -242,9 +228,8 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
     };
     const uint64_t do_k = sdesc(sbase + kOffdO, 16, 1024);
     const uint64_t do_mn = sdesc(sbase + kOffdO, kBoxBytes, 1024);
-    auto issue_dp = [&](int u) {  // dP^T = V dO^T
-      const int rows = unit_rows(u);
-      if (rows < 128) packed_zero_rows(sbase + kOffdO, rows);  // so does dV
+    auto issue_dp = [&]() {  // dP^T = V dO^T
+      if (rows_dp < 128) packed_zero_rows(sbase + kOffdO, rows_dp);  // dV sums over the query rows too
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) mma_ss_e(tdP, desc_add(dV_k, koff(ks)), desc_add(do_k, koff(ks)), id_kk, ks > 0);
       mma_commit_e(bar(kBarDpFull));
@@ -255,7 +240,8 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
     if (ok) {
       tc_fence_after();
       if (w.rows < 128) packed_zero_rows(sbase + kOffK, w.rows);  // dQ sums over the keys
-      issue_dp(0);
+      rows_dp = w.lq - at.m * 128;
+      issue_dp();
       issue_s(0);
     }
     for (int u = 0; u < cnt && ok; ++u) {
@@ -292,7 +278,8 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
         if (!(ok = mbar_wait_warp(bar(kBarDqDrained), u & 1, abort_flag, kRoleBwdMma, 11))) break;
         if (!(ok = mbar_wait_warp(bar(kBarDoFull), (u + 1) & 1, abort_flag, kRoleBwdMma, 5))) break;
         tc_fence_after();
-        issue_dp(u + 1);
+        rows_dp = rows_s;  // S^T(u+1) has been issued
+        issue_dp();
       }
     }
     if (ok) mma_commit_e(bar(kBarDkvFull));
@@ -321,12 +308,11 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     const uint32_t sdS = sbase + kOffdS + (uint32_t)half * kBoxBytes;
     bool ok = true;
-    for (int u = 0; u < cnt; ++u) {
+    PackedWalk at(w, reverse);
+    for (int u = 0; u < cnt; ++u, at.next()) {
       const int st = u & 1;
       const float* snl = reinterpret_cast<const float*>(smem + kOffLse + st * 512) + half * 64 + 2 * tq;
       const float* sD = reinterpret_cast<const float*>(smem + kOffD + st * 512) + half * 64 + 2 * tq;
-      int unit_g, unit_m;
-      walk.at(u, unit_g, unit_m);
       if (!(ok = mbar_wait(bar(kBarSFull), u & 1, abort_flag, kRoleEw, 5))) break;
       // -lse*log2(e) / D of this unit arrived with Q (already complete; this
       // wait makes the bulk-copied bytes visible to these threads)
@@ -345,7 +331,7 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
       reg_fence32(s[0]);
       reg_fence32(s[1]);
       // key row r is seen by the unit's columns >= below + r
-      const int below = w.need - unit_m * 128;
+      const int below = w.need - at.m * 128;
       if (below > -127) {
 #pragma unroll
         for (int g = 0; g < 2; ++g)
@@ -435,7 +421,7 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
         tmem_ld32(tsrc + c * 32, a);
         tmem_wait_ld();
         reg_fence32(a);
-        if (p.nsplit == 1) {
+        if (w.part < 0) {
           if (r < w.rows) {
             __nv_bfloat16* row = (half ? p.dk : p.dv) + ((size_t)(w.k0 + r) * p.h_kv + kvh) * 128;
 #pragma unroll
@@ -447,7 +433,8 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
                            pack_bf16(__uint_as_float(a[8 * v + 6]) * mul, __uint_as_float(a[8 * v + 7]) * mul));
           }
         } else {
-          float* dst = (half ? p.dk_part : p.dv_part) + part + (size_t)(r >> 6) * 8192 + (size_t)(r & 63) * 4;
+          float* dst = (half ? p.dk_part : p.dv_part) + ((size_t)w.part * p.h_kv + kvh) * 16384 +
+                       (size_t)(r >> 6) * 8192 + (size_t)(r & 63) * 4;
 #pragma unroll
           for (int g = 0; g < 8; ++g)
             *reinterpret_cast<float4*>(dst + (size_t)(c * 8 + g) * 256) =
@@ -468,7 +455,8 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
     const uint32_t sx = sbase + kOffX;
     uint8_t* xb = smem + kOffX;
     const bool leader = (threadIdx.x == 256);
-    for (int u = 0; u < cnt; ++u) {
+    PackedWalk at(w, reverse);
+    for (int u = 0; u < cnt; ++u, at.next()) {
       if (!mbar_wait(bar(kBarDqFull), u & 1, abort_flag, kRoleDq, 10)) break;
       tc_fence_after();
       uint32_t q[4][32];
@@ -479,9 +467,7 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
       for (int c = 0; c < 4; ++c) reg_fence32(q[c]);
       tc_fence_before();
       mbar_arrive(bar(kBarDqDrained));
-      int unit_g, unit_m;
-      walk.at(u, unit_g, unit_m);
-      const size_t place = q_place(unit_g, unit_m);
+      const size_t place = q_place(at.g, at.m);
       float* dst = p.dq_accum + place * 16384;
       int* const sem = p.ordered ? p.sem + place : nullptr;
 #pragma unroll
@@ -528,58 +514,59 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
   if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
-// fp32 tiles -> bf16 rows, times a scale: the dQ accumulator (parts = 1), or
-// the sum of the splits' partial dK or dV in a fixed order.  Rows outside any
-// sequence become 0 (NaN where the offsets were impossible).  Bound: HBM.
-// grid (4 * tiles, heads), 256 threads: 32 rows x 128 columns.
+// fp32 tiles -> bf16 rows, times a scale: the dQ accumulator, or the sums of
+// the pieces' partial dK and dV in a fixed order (blockIdx.z: which).  Rows of
+// dQ outside any sequence become 0 (NaN where the offsets were impossible).
+// Bound: HBM.  grid (4 * tiles, heads[, 2]), 256 threads: 32 rows x 128 columns.
 __global__ void __launch_bounds__(256) wf_packed_convert_kernel(PackedConvertParams p) {
   __shared__ float tile[32][132];
   griddep_launch_dependents();
   griddep_wait();
-  const int t = blockIdx.x >> 2, row0 = (blockIdx.x & 3) * 32, h = blockIdx.y;
+  const int t = blockIdx.x >> 2, row0 = (blockIdx.x & 3) * 32, h = blockIdx.y, which = blockIdx.z;
   const int4 head = *p.head;
-  if (t >= head.x) return;
-  int first, rows;
-  bool inside;
-  if (p.q_tiles) {
-    const int4 w = p.q_tiles[t];
-    first = w.x, rows = w.y, inside = w.z != 0;
-  } else {
-    const PackedKTile w = p.k_tiles[t];
-    first = w.k0, rows = w.rows, inside = w.m_count > 0;
-  }
-  if (row0 >= rows) return;
+  if (t >= (p.split ? head.z : head.x)) return;
+  const int4 w = p.tiles[t];  // first row, rows, dq: inside / split: first part, parts
+  if (row0 >= w.y) return;
   const int half = row0 >> 6, r0 = row0 & 63;
+  const bool inside = p.split || w.z != 0;
   if (inside) {
-    const float* src = p.accum + ((size_t)h * p.tile_stride + t) * 16384 + half * 8192;
+    const int parts = p.split ? w.w : 1;
+    const size_t at = p.split ? (size_t)w.z * p.heads + h : (size_t)h * p.tile_stride + t;
+    const size_t step = (size_t)p.heads * 16384;
+    const float* src = (which ? p.accum[1] : p.accum[0]) + at * 16384 + half * 8192;
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < parts; ++s, src += step) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int idx = threadIdx.x + i * 256;  // 32 groups of 4 columns x 32 rows
+        const float4 x = *reinterpret_cast<const float4*>(src + ((idx >> 5) * 64 + r0 + (idx & 31)) * 4);
+        v[i].x += x.x, v[i].y += x.y, v[i].z += x.z, v[i].w += x.w;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int idx = threadIdx.x + i * 256;  // 32 groups of 4 columns x 32 rows
-      const int g = idx >> 5, rw = idx & 31;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int s = 0; s < p.parts; ++s) {
-        const float4 x = *reinterpret_cast<const float4*>(src + s * p.part_stride + (g * 64 + r0 + rw) * 4);
-        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-      }
-      *reinterpret_cast<float4*>(&tile[rw][4 * g]) = v;
+      const int idx = threadIdx.x + i * 256;
+      *reinterpret_cast<float4*>(&tile[idx & 31][4 * (idx >> 5)]) = v[i];
     }
   }
   __syncthreads();
+  const uint32_t fill = head.y ? 0x7fff7fffu : 0u;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int idx = threadIdx.x + i * 256;  // 32 rows x 16 chunks of 8
     const int rw = idx >> 4, ch = idx & 15;
-    if (row0 + rw >= rows) continue;
-    const uint32_t fill = head.y ? 0x7fff7fffu : 0u;
-    uint4 w = make_uint4(fill, fill, fill, fill);
+    if (row0 + rw >= w.y) continue;
+    uint4 o = make_uint4(fill, fill, fill, fill);
     if (inside) {
       const float* x = &tile[rw][ch * 8];
-      w.x = pack_bf16(x[0] * p.scale, x[1] * p.scale);
-      w.y = pack_bf16(x[2] * p.scale, x[3] * p.scale);
-      w.z = pack_bf16(x[4] * p.scale, x[5] * p.scale);
-      w.w = pack_bf16(x[6] * p.scale, x[7] * p.scale);
+      o.x = pack_bf16(x[0] * p.scale, x[1] * p.scale);
+      o.y = pack_bf16(x[2] * p.scale, x[3] * p.scale);
+      o.z = pack_bf16(x[4] * p.scale, x[5] * p.scale);
+      o.w = pack_bf16(x[6] * p.scale, x[7] * p.scale);
     }
-    *reinterpret_cast<uint4*>(p.out + ((size_t)(first + row0 + rw) * p.heads + h) * 128 + ch * 8) = w;
+    *reinterpret_cast<uint4*>((which ? p.out[1] : p.out[0]) + ((size_t)(w.x + row0 + rw) * p.heads + h) * 128 + ch * 8) = o;
   }
 }
 

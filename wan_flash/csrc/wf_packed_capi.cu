@@ -22,17 +22,36 @@ struct PackedFwdWorkspace {  // byte offsets
   }
 };
 
+// Items, split key tiles and partial tiles (per key-value head) that the plan
+// can make at most.  It cuts walks of more than `chunk` units, and chunk is at
+// least kPackedMinChunk and units * h_kv / pieces: sum ceil(u / chunk) <= tiles +
+// units / chunk, and a cut tile has at most 2 u / chunk parts.
+struct PackedBwdBounds {
+  long long pieces, items, split_tiles, parts;
+  PackedBwdBounds(int n, int total_q, int total_k, int h, int h_kv, int nsplit, int sms) {
+    const long long q_tiles = packed_max_tiles(total_q, n, 128), k_tiles = packed_max_tiles(total_k, n, 128);
+    const long long group = h_kv ? h / h_kv : 0;
+    pieces = (long long)sms * kPackedPiecesPerSm;
+    const long long units = group * q_tiles * k_tiles;
+    const long long cuts = std::min(units / kPackedMinChunk, pieces / std::max(h_kv, 1)) + 1;
+    items = nsplit > 0 ? k_tiles * nsplit : k_tiles + cuts;
+    split_tiles = nsplit > 0 ? k_tiles : std::min(k_tiles, cuts);
+    parts = nsplit > 0 ? (nsplit > 1 ? k_tiles * nsplit : 0) : 2 * cuts;
+  }
+};
+
 struct PackedBwdWorkspace {  // byte offsets
-  size_t head = 0, base, k_tiles, q_tiles, neg_lse_log2, dpsum, dq_accum, dk_part, dv_part, sem, sem_bytes, bytes;
-  size_t q_tile_stride, k_tile_stride;
-  PackedBwdWorkspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg) {
+  size_t head = 0, base, items, q_tiles, split_tiles, neg_lse_log2, dpsum, dq_accum, dk_part, dv_part, sem, sem_bytes, bytes;
+  size_t q_tile_stride;
+  PackedBwdWorkspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg, int sms) {
+    const PackedBwdBounds most(n, total_q, total_k, h, h_kv, cfg->nsplit, sms);
     q_tile_stride = (size_t)packed_max_tiles(total_q, n, 128);
-    k_tile_stride = (size_t)packed_max_tiles(total_k, n, 128);
-    const size_t q_all = q_tile_stride * h, parts = cfg->nsplit > 1 ? (size_t)cfg->nsplit * h_kv * k_tile_stride : 0;
+    const size_t q_all = q_tile_stride * h, parts = (size_t)most.parts * h_kv;
     base = 256;
-    k_tiles = align256(base + (size_t)3 * (n + 3) * 4);
-    q_tiles = align256(k_tiles + k_tile_stride * sizeof(PackedKTile));
-    neg_lse_log2 = align256(q_tiles + q_tile_stride * sizeof(int4));
+    items = align256(base + (size_t)3 * (n + 3) * 4);
+    q_tiles = align256(items + (size_t)most.items * sizeof(PackedBwdItem));
+    split_tiles = align256(q_tiles + q_tile_stride * sizeof(int4));
+    neg_lse_log2 = align256(split_tiles + (size_t)most.split_tiles * sizeof(int4));
     dpsum = neg_lse_log2 + q_all * 512;
     dq_accum = align256(dpsum + q_all * 512);
     dk_part = dq_accum + q_all * 65536;
@@ -45,7 +64,7 @@ struct PackedBwdWorkspace {  // byte offsets
 
 int packed_bwd_cfg_check(const wf_packed_bwd_cfg* cfg) {
   if (!cfg) return fail(WF_ERR_INVALID_ARG, "null cfg");
-  if (cfg->nsplit < 1 || cfg->nsplit > 1024) return fail(WF_ERR_INVALID_ARG, "nsplit=%d outside [1, 1024]", cfg->nsplit);
+  if (cfg->nsplit < 0 || cfg->nsplit > 1024) return fail(WF_ERR_INVALID_ARG, "nsplit=%d outside [0, 1024]", cfg->nsplit);
   return WF_OK;
 }
 
@@ -61,12 +80,6 @@ int packed_check(int n, int total_q, int total_k, int h, int h_kv, int causal) {
   if (packed_max_tiles(total_q, n, 128) * h > 0x7fffffffLL || packed_max_tiles(total_k, n, 128) * h > 0x7fffffffLL)
     return fail(WF_ERR_UNSUPPORTED, "too many (tile, head) items");
   return WF_OK;
-}
-
-int plan_shift(int total) {
-  int shift = 0;
-  while (((total / 128 + 1) >> shift) >= kPlanBuckets) ++shift;
-  return shift;
 }
 
 }  // namespace
@@ -117,7 +130,6 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   PackedPlanParams pp = {};
   pp.q_off = q_offsets, pp.k_off = k_offsets;
   pp.n = n, pp.total_q = total_q, pp.total_k = total_k, pp.causal = causal;
-  pp.cost_shift = plan_shift(total_k);
   pp.head = reinterpret_cast<int4*>(w + ws.head);
   pp.base = reinterpret_cast<int*>(w + ws.base);
   pp.fwd_tiles = reinterpret_cast<PackedFwdTile*>(w + ws.tiles);
@@ -143,9 +155,10 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
 extern "C" int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg,
                                        size_t* bytes) {
   if (!bytes) return fail(WF_ERR_INVALID_ARG, "null pointer");
-  int rc;
+  int rc, dev;
   if ((rc = packed_check(n, total_q, total_k, h, h_kv, 0)) || (rc = packed_bwd_cfg_check(cfg))) return rc;
-  *bytes = PackedBwdWorkspace(n, total_q, total_k, h, h_kv, cfg).bytes;
+  if ((rc = device_setup(&dev))) return rc;
+  *bytes = PackedBwdWorkspace(n, total_q, total_k, h, h_kv, cfg, g_dev_sms[dev]).bytes;
   return WF_OK;
 }
 
@@ -164,14 +177,15 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
       !aligned16(dk) || !aligned16(dv) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) ||
       (reinterpret_cast<uintptr_t>(q_offsets) & 3) || (reinterpret_cast<uintptr_t>(k_offsets) & 3))
     return fail(WF_ERR_MISALIGNED, "tensors and workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
-  const PackedBwdWorkspace ws(n, total_q, total_k, h, h_kv, cfg);
-  if (workspace_bytes < ws.bytes)
-    return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
-  const unsigned long long items = (unsigned long long)ws.k_tile_stride * h_kv * cfg->nsplit;
-  if (items > 0x7fffffffULL || ws.q_tile_stride * 4 > 0x7fffffffULL || ws.k_tile_stride * 4 > 0x7fffffffULL)
-    return fail(WF_ERR_UNSUPPORTED, "%llu work items exceed the grid limit", items);
   int dev;
   if ((rc = device_setup(&dev))) return rc;
+  const int sms = g_dev_sms[dev];
+  const PackedBwdBounds most(n, total_q, total_k, h, h_kv, cfg->nsplit, sms);
+  const PackedBwdWorkspace ws(n, total_q, total_k, h, h_kv, cfg, sms);
+  if (workspace_bytes < ws.bytes)
+    return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
+  if (most.items * h_kv > 0x7fffffffLL || ws.q_tile_stride * 4 > 0x7fffffffULL)
+    return fail(WF_ERR_UNSUPPORTED, "%lld work items exceed the grid limit", most.items * h_kv);
   CUtensorMap mq, mk, mv, mdo;
   if ((rc = make_bshd_map(&mq, q, 1, total_q, h)) || (rc = make_bshd_map(&mk, k, 1, total_k, h_kv)) ||
       (rc = make_bshd_map(&mv, v, 1, total_k, h_kv)) || (rc = make_bshd_map(&mdo, dO, 1, total_q, h)))
@@ -183,14 +197,17 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   pp.n = n, pp.total_q = total_q, pp.total_k = total_k, pp.causal = causal;
   pp.backward = 1;
   pp.ordered = cfg->deterministic ? 1 : 0;
-  pp.cost_shift = plan_shift(total_q);
+  pp.group = h / h_kv, pp.h_kv = h_kv;
+  pp.nsplit = cfg->nsplit;
+  pp.pieces = (int)most.pieces;
   pp.head = reinterpret_cast<int4*>(w + ws.head);
   pp.base = reinterpret_cast<int*>(w + ws.base);
-  pp.k_tiles = reinterpret_cast<PackedKTile*>(w + ws.k_tiles);
+  pp.items = reinterpret_cast<PackedBwdItem*>(w + ws.items);
   pp.q_tiles = reinterpret_cast<int4*>(w + ws.q_tiles);
+  pp.split_tiles = reinterpret_cast<int4*>(w + ws.split_tiles);
   PackedBwdParams p = {};
   p.head = pp.head;
-  p.k_tiles = pp.k_tiles;
+  p.items = pp.items;
   p.q_tiles = pp.q_tiles;
   p.neg_lse_log2 = reinterpret_cast<float*>(w + ws.neg_lse_log2);
   p.dpsum = reinterpret_cast<float*>(w + ws.dpsum);
@@ -200,11 +217,10 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   p.dk_part = reinterpret_cast<float*>(w + ws.dk_part);
   p.dv_part = reinterpret_cast<float*>(w + ws.dv_part);
   p.sem = reinterpret_cast<int*>(w + ws.sem);
-  p.q_tile_stride = ws.q_tile_stride, p.k_tile_stride = ws.k_tile_stride;
+  p.q_tile_stride = ws.q_tile_stride;
   p.total_q = total_q, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
-  p.nsplit = cfg->nsplit;
   p.ordered = pp.ordered;
-  p.wave = g_dev_sms[dev];
+  p.wave = sms;
   p.scale = (float)(1.0 / std::sqrt(128.0));
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
   cudaError_t e;
@@ -217,30 +233,27 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   e = launch_ex(wf_packed_pre_kernel, dim3((unsigned)(2 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, p,
                 reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(dO), lse);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd preprocess launch");
-  e = launch_ex(wf_packed_bwd_kernel, dim3((unsigned)items), dim3(bwd::kThreads), bwd::kSmemBytes, st, true, 1u, mq, mk,
-                mv, mdo, p);
+  e = launch_ex(wf_packed_bwd_kernel, dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true,
+                1u, mq, mk, mv, mdo, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd launch");
   PackedConvertParams c = {};
   c.head = pp.head + 1;
-  c.q_tiles = pp.q_tiles;
-  c.accum = p.dq_accum;
+  c.tiles = pp.q_tiles;
+  c.accum[0] = p.dq_accum;
+  c.out[0] = reinterpret_cast<__nv_bfloat16*>(dq);
   c.tile_stride = ws.q_tile_stride;
-  c.parts = 1, c.heads = h;
+  c.heads = h;
   c.scale = p.scale;
-  c.out = reinterpret_cast<__nv_bfloat16*>(dq);
   e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, c);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd dq convert launch");
-  for (int i = 0; i < (cfg->nsplit > 1 ? 2 : 0); ++i) {
+  if (most.parts > 0) {
     c.head = pp.head;
-    c.q_tiles = nullptr;
-    c.k_tiles = pp.k_tiles;
-    c.accum = i ? p.dv_part : p.dk_part;
-    c.tile_stride = ws.k_tile_stride;
-    c.part_stride = ws.k_tile_stride * h_kv * 16384;
-    c.parts = cfg->nsplit, c.heads = h_kv;
+    c.tiles = pp.split_tiles;
+    c.accum[0] = p.dk_part, c.accum[1] = p.dv_part;
+    c.out[0] = p.dk, c.out[1] = p.dv;
+    c.split = 1, c.heads = h_kv;
     c.scale = 1.f;  // dk was scaled where it left the tensor core
-    c.out = reinterpret_cast<__nv_bfloat16*>(i ? dv : dk);
-    e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * ws.k_tile_stride), h_kv), dim3(256), 0, st, true, 1u, c);
+    e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * most.split_tiles), h_kv, 2), dim3(256), 0, st, true, 1u, c);
     if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd dk/dv convert launch");
   }
   return launch_check("wf_packed_bwd launch");

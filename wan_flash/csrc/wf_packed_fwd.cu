@@ -143,9 +143,9 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     for (int k = 0; ok; ++k) {
       const int item = packed_item(k);
       if (item >= n_items) break;
-      const PackedFwdTile w = p.tiles[item / p.h];
+      int h;
+      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
       if (w.n_blocks == 0) continue;
-      const int h = item % p.h;
       for (int t = 0; t * 128 < w.rows; ++t, ++n) {
         ok = mbar_wait_warp(bar(kBarOStaged), (uint32_t)n & 1, abort_flag, kRoleStore, 50 + t);
         if (!ok) break;
@@ -186,8 +186,9 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       for (int k = 0; ok; ++k) {
         const int item = packed_item(k);
         if (item >= n_items) break;
-        const PackedFwdTile w = p.tiles[item / p.h];
-        const int h = item % p.h, kvh = h / p.group;
+        int h;
+      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
+        const int kvh = h / p.group;
         for (int it = 0; it < w.n_blocks && ok; ++it) {
           const int j = w.n_blocks - 1 - it;
           for (int kv = 0; kv < 2 && ok; ++kv, ++u) {  // 0 = K, 1 = V
@@ -279,7 +280,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     for (int k = 0; ok; ++k) {
       const int item = packed_item(k);
       if (item >= n_items) break;
-      const PackedFwdTile w = p.tiles[item / p.h];
+      int h;
+      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
       const int tiles = w.rows > 128 ? 2 : 1;
       for (int it = 0; it < w.n_blocks && ok; ++it, ++g) {
         const int uk = 2 * g, slot_k = uk % kKvSlots;
@@ -344,8 +346,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     for (int k = 0; ok; ++k) {
       const int item = packed_item(k);
       if (item >= n_items) break;
-      const PackedFwdTile w = p.tiles[item / p.h];
-      const int h = item % p.h;
+      int h;
+      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
       const int row = t * 128 + r;  // within the record
       if (w.n_blocks == 0) {
         // nothing to attend (or rows outside any sequence): o = 0, lse = -inf;

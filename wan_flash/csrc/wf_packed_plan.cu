@@ -5,15 +5,25 @@
 // One CTA per list.  The rows [0, total) fall into n + 2 segments: the rows
 // before the first sequence, the n sequences, the rows behind the last; every
 // segment is cut into tiles of T rows.  A scan over the segments gives each
-// its first tile; each tile finds its segment by binary search.  Lists whose
-// tiles differ in cost (forward query tiles, backward key tiles) are sorted by
-// falling cost, a counting sort on the number of 128-row blocks the tile
-// walks: CTAs that take their items in turn then end together although
-// sequences are ragged and causal tiles grow with their row.
+// its first tile; each tile finds its segment by binary search.
+//
+// Items (forward: query tiles; backward: key tiles, or pieces of one) are
+// sorted by falling cost in a counting sort, so CTAs that take them in turn end
+// together although sequences are ragged and causal tiles grow with their row.
+// Items of equal cost form a bucket, and inside a bucket the kernels run head
+// by head (packed_locate): the tiles of one sequence and head, which read the
+// same keys (backward: queries), run side by side.
+//
+// Backward pieces: a key tile that walks more units (query tile, q head) than
+// `chunk`, a quarter of an SM's even share, is cut into pieces whose partial
+// dK and dV a convert sums.  One long sequence then fills the GPU as evenly as many.
 //
 // Offsets that fall, start below 0 or end behind the tensor set the device
 // error word; the lists then hold only rows outside any sequence, with
 // status 1 (the kernels write NaN there).
+//
+// Bound: latency (a chain of barriers and dependent loads).  Up to 2045
+// sequences the offsets and scans stay in shared memory.
 #include "wf_common.cuh"
 #include "wf_kernels.h"
 
@@ -23,12 +33,16 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBuckets = 1024;
+constexpr int kPlanSmall = 2048;  // n + 3 up to this: offsets and tile bases in shared memory
+static_assert(kPlanBuckets == kPlanThreads, "one bucket per thread in the scan");
 
 struct PlanShared {
   int warp_sum[32];
-  int carry;
-  int bad;
-  int hist[kPlanBuckets];
+  int start[kPlanBuckets + 1];
+  int cursor[kPlanBuckets];
+  unsigned long long units;
+  int most;
+  int q_off[kPlanSmall], k_off[kPlanSmall], base0[kPlanSmall], base1[kPlanSmall];
 };
 
 // Exclusive block scan of one int per thread; returns the prefix, *total the sum.
@@ -42,19 +56,15 @@ __device__ int plan_scan(PlanShared& sh, int x, int* total) {
   }
   if (lane == 31) sh.warp_sum[warp] = incl;
   __syncthreads();
-  if (warp == 0) {
-    int w = sh.warp_sum[lane];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += up;
-    }
-    sh.warp_sum[lane] = w;
+  int before = 0, sum = 0;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i) {
+    const int s = sh.warp_sum[i];
+    if (i < warp) before += s;
+    sum += s;
   }
   __syncthreads();
-  const int before = warp ? sh.warp_sum[warp - 1] : 0;
-  *total = sh.warp_sum[31];
-  __syncthreads();
+  *total = sum;
   return before + incl - x;
 }
 
@@ -65,18 +75,12 @@ __device__ __forceinline__ void plan_segment(const int* off, int n, int total, b
     len = s == 0 ? total : 0;
     return;
   }
-  const int a = s == 0 ? 0 : __ldg(off + s - 1), b = s <= n ? __ldg(off + s) : total;
-  start = a;
-  len = (s == 0 ? __ldg(off) : b) - a;
+  start = s == 0 ? 0 : off[s - 1];
+  len = (s <= n ? off[s] : total) - start;
 }
 
-__device__ bool plan_offsets_bad(const int* off, int n, int total) {
-  bool bad = false;
-  for (int s = threadIdx.x; s <= n; s += kPlanThreads) {
-    const int x = __ldg(off + s);
-    if (x < 0 || x > total || (s > 0 && x < __ldg(off + s - 1))) bad = true;
-  }
-  return __syncthreads_or(bad);
+__device__ __forceinline__ bool plan_bad(const int* off, int s, int total) {
+  return off[s] < 0 || off[s] > total || (s > 0 && off[s] < off[s - 1]);
 }
 
 // base[s] = first tile of segment s (s = 0..n+1), base[n+2] = number of tiles
@@ -106,18 +110,25 @@ __device__ int plan_find(const int* base, int n, int t) {
   return lo;
 }
 
-// Forward tile t: kFwdTileRows query rows.
-__device__ PackedFwdTile plan_fwd_tile(const PackedPlanParams& p, bool bad, const int* base, int t) {
+struct PlanView {
+  const int* q_off;
+  const int* k_off;
+  int n, total_q, total_k;
+  bool bad, causal;
+};
+
+// Forward tile t: up to 256 query rows.
+__device__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int* base, int t) {
   const int s = plan_find(base, p.n, t);
   int qs, lq;
-  plan_segment(p.q_off, p.n, p.total_q, bad, s, qs, lq);
+  plan_segment(p.q_off, p.n, p.total_q, p.bad, s, qs, lq);
   const int m0 = (t - base[s]) * 256;
   PackedFwdTile w;
   w.q0 = qs + m0;
   w.rows = min(256, lq - m0);
-  w.k0 = w.klen = w.off = w.n_blocks = w.pad0 = w.pad1 = 0;
-  if (!bad && s >= 1 && s <= p.n) {
-    const int ks = __ldg(p.k_off + s - 1), lk = __ldg(p.k_off + s) - ks;
+  w.k0 = w.klen = w.off = w.n_blocks = w.bucket = w.bucket_items = 0;
+  if (!p.bad && s >= 1 && s <= p.n) {
+    const int ks = p.k_off[s - 1], lk = p.k_off[s] - ks;
     w.k0 = ks;
     w.off = p.causal ? m0 + lk - lq + 1 : lk;  // keys that the tile's first row sees (causal: may be negative)
     w.klen = p.causal ? max(0, w.off + w.rows - 1) : lk;
@@ -127,19 +138,21 @@ __device__ PackedFwdTile plan_fwd_tile(const PackedPlanParams& p, bool bad, cons
 }
 
 // Backward key tile t: 128 key rows, and the query tiles that see them.
-__device__ PackedKTile plan_k_tile(const PackedPlanParams& p, bool bad, const int* kbase, const int* qbase, int t) {
+__device__ PackedBwdItem plan_k_tile(const PlanView& p, const int* kbase, const int* qbase, int t) {
   const int s = plan_find(kbase, p.n, t);
   int ks, lk;
-  plan_segment(p.k_off, p.n, p.total_k, bad, s, ks, lk);
+  plan_segment(p.k_off, p.n, p.total_k, p.bad, s, ks, lk);
   const int n0 = (t - kbase[s]) * 128;
-  PackedKTile w;
+  PackedBwdItem w;
   w.k0 = ks + n0;
   w.rows = min(128, lk - n0);
-  w.q0 = w.lq = w.m_begin = w.m_count = w.qtile = w.need = 0;
+  w.q0 = w.lq = w.qtile = w.m_begin = w.m_count = w.need = 0;
   w.nb = t - kbase[s];
-  w.pad0 = w.pad1 = w.pad2 = 0;
-  if (!bad && s >= 1 && s <= p.n) {
-    const int qs = __ldg(p.q_off + s - 1), lq = __ldg(p.q_off + s) - qs;
+  w.first = w.count = 0;
+  w.part = -1;
+  w.bucket = w.bucket_items = w.pad0 = w.pad1 = 0;
+  if (!p.bad && s >= 1 && s <= p.n) {
+    const int qs = p.q_off[s - 1], lq = p.q_off[s] - qs;
     w.q0 = qs;
     w.lq = lq;
     w.qtile = qbase[s];
@@ -150,62 +163,152 @@ __device__ PackedKTile plan_k_tile(const PackedPlanParams& p, bool bad, const in
   return w;
 }
 
+// Buckets of falling cost: sizes from count(add), their starts in sh.start.
+template <typename Count>
+__device__ void plan_buckets(PlanShared& sh, int n_tiles, int shift, Count&& count) {
+  for (int i = threadIdx.x; i < kPlanBuckets; i += kPlanThreads) sh.cursor[i] = 0;
+  __syncthreads();
+  for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads)
+    count(t, [&](int cost) { atomicAdd(&sh.cursor[kPlanBuckets - 1 - (cost >> shift)], 1); });
+  __syncthreads();
+  int sum;
+  const int first = plan_scan(sh, sh.cursor[threadIdx.x], &sum);
+  sh.start[threadIdx.x] = sh.cursor[threadIdx.x] = first;
+  if (threadIdx.x == 0) sh.start[kPlanBuckets] = sum;
+  __syncthreads();
+}
+// A place for an item of that cost, and its bucket.
+template <typename Item>
+__device__ int plan_place(PlanShared& sh, int cost, int shift, Item& w) {
+  const int b = kPlanBuckets - 1 - (cost >> shift);
+  w.bucket = sh.start[b];
+  w.bucket_items = sh.start[b + 1] - sh.start[b];
+  return atomicAdd(&sh.cursor[b], 1);
+}
+
 }  // namespace
 
-// grid 1 (forward) or 2 (backward: block 0 the key tiles, block 1 the query tiles)
+// grid 1 (forward) or 2 (backward: block 0 the items, block 1 the query tiles)
 __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlanParams p) {
   __shared__ PlanShared sh;
   griddep_launch_dependents();
-  const bool bad = plan_offsets_bad(p.q_off, p.n, p.total_q) | plan_offsets_bad(p.k_off, p.n, p.total_k);
-  if (bad && threadIdx.x == 0 && atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
+  const bool small = p.n + 3 <= kPlanSmall;
+  if (threadIdx.x == 0) sh.units = 0ull, sh.most = 0;
+  if (small) {
+    for (int s = threadIdx.x; s <= p.n; s += kPlanThreads) {
+      sh.q_off[s] = p.q_off[s];
+      sh.k_off[s] = p.k_off[s];
+    }
+  }
+  __syncthreads();
+  PlanView v;
+  v.q_off = small ? sh.q_off : p.q_off;
+  v.k_off = small ? sh.k_off : p.k_off;
+  v.n = p.n, v.total_q = p.total_q, v.total_k = p.total_k, v.causal = p.causal != 0;
+  bool bad = false;
+  for (int s = threadIdx.x; s <= p.n; s += kPlanThreads)
+    bad |= plan_bad(v.q_off, s, p.total_q) || plan_bad(v.k_off, s, p.total_k);
+  v.bad = __syncthreads_or(bad);
+  if (v.bad && threadIdx.x == 0 && atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
     g_err_info[0] = g_err_info[1] = g_err_info[3] = 0u;
     g_err_info[2] = kRolePackedPlan;
   }
-  const bool q_list = p.backward && blockIdx.x == 1;
-  int* const base = p.base + (q_list ? 2 * (p.n + 3) : 0);
-  const bool k_list = p.backward && !q_list;
-  const int n_tiles = k_list ? plan_bases(sh, p.k_off, p.n, p.total_k, bad, 128, base)
-                             : plan_bases(sh, p.q_off, p.n, p.total_q, bad, p.backward ? 128 : 256, base);
-  if (q_list) {  // in the order of the rows: the index is the tile's place in the fp32 workspaces
+  int* const base0 = small ? sh.base0 : p.base + (blockIdx.x ? 2 * (p.n + 3) : 0);
+  int* const base1 = small ? sh.base1 : p.base + (p.n + 3);  // block 0 of the backward only
+
+  if (!p.backward) {
+    const int n_tiles = plan_bases(sh, v.q_off, p.n, p.total_q, v.bad, 256, base0);
+    int most = 0;
+    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) most = max(most, plan_fwd_tile(v, base0, t).n_blocks);
+    atomicMax(&sh.most, most);
+    __syncthreads();
+    int shift = 0;
+    while ((sh.most >> shift) >= kPlanBuckets) ++shift;
+    plan_buckets(sh, n_tiles, shift, [&](int t, auto add) { add(plan_fwd_tile(v, base0, t).n_blocks); });
     for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
-      const int s = plan_find(base, p.n, t);
-      int qs, lq;
-      plan_segment(p.q_off, p.n, p.total_q, bad, s, qs, lq);
-      const int m0 = (t - base[s]) * 128;
-      p.q_tiles[t] = make_int4(qs + m0, min(128, lq - m0), !bad && s >= 1 && s <= p.n, 0);
+      PackedFwdTile w = plan_fwd_tile(v, base0, t);
+      const int at = plan_place(sh, w.n_blocks, shift, w);
+      p.fwd_tiles[at] = w;
     }
-    if (threadIdx.x == 0) p.head[1] = make_int4(n_tiles, bad, 0, 0);
+    if (threadIdx.x == 0) p.head[0] = make_int4(n_tiles, v.bad, 0, 0);
     return;
   }
-  int* const qbase = p.base + (p.n + 3);
-  if (k_list) plan_bases(sh, p.q_off, p.n, p.total_q, bad, 128, qbase);
-  if (p.ordered) {
-    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) p.k_tiles[t] = plan_k_tile(p, bad, base, qbase, t);
-  } else {
-    for (int i = threadIdx.x; i < kPlanBuckets; i += kPlanThreads) sh.hist[i] = 0;
-    __syncthreads();
-    auto bucket = [&](int cost) { return kPlanBuckets - 1 - min(cost >> p.cost_shift, kPlanBuckets - 1); };
+  if (blockIdx.x == 1) {
+    // query tiles, in the order of the rows: the index is the tile's place in the fp32 workspaces
+    const int n_tiles = plan_bases(sh, v.q_off, p.n, p.total_q, v.bad, 128, base0);
     for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
-      const int cost = k_list ? plan_k_tile(p, bad, base, qbase, t).m_count : plan_fwd_tile(p, bad, base, t).n_blocks;
-      atomicAdd(&sh.hist[bucket(cost)], 1);
+      const int s = plan_find(base0, p.n, t);
+      int qs, lq;
+      plan_segment(v.q_off, p.n, p.total_q, v.bad, s, qs, lq);
+      const int m0 = (t - base0[s]) * 128;
+      p.q_tiles[t] = make_int4(qs + m0, min(128, lq - m0), !v.bad && s >= 1 && s <= p.n, 0);
     }
-    __syncthreads();
-    static_assert(kPlanBuckets == kPlanThreads, "one bucket per thread");
-    int sum;
-    const int first = plan_scan(sh, sh.hist[threadIdx.x], &sum);
-    sh.hist[threadIdx.x] = first;
-    __syncthreads();
-    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
-      if (k_list) {
-        const PackedKTile w = plan_k_tile(p, bad, base, qbase, t);
-        p.k_tiles[atomicAdd(&sh.hist[bucket(w.m_count)], 1)] = w;
-      } else {
-        const PackedFwdTile w = plan_fwd_tile(p, bad, base, t);
-        p.fwd_tiles[atomicAdd(&sh.hist[bucket(w.n_blocks)], 1)] = w;
-      }
-    }
+    if (threadIdx.x == 0) p.head[1] = make_int4(n_tiles, v.bad, 0, 0);
+    return;
   }
-  if (threadIdx.x == 0) p.head[0] = make_int4(n_tiles, bad, 0, 0);
+  const int n_tiles = plan_bases(sh, v.k_off, p.n, p.total_k, v.bad, 128, base0);
+  plan_bases(sh, v.q_off, p.n, p.total_q, v.bad, 128, base1);
+  unsigned long long units = 0;
+  int most = 0;
+  for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
+    const int u = plan_k_tile(v, base0, base1, t).m_count * p.group;
+    units += u;
+    most = max(most, u);
+  }
+  atomicAdd(&sh.units, units);
+  atomicMax(&sh.most, most);
+  __syncthreads();
+  const long long chunk = p.nsplit > 0 ? max(1, (sh.most + p.nsplit - 1) / p.nsplit)
+                                       : max((long long)kPackedMinChunk, (long long)(sh.units * p.h_kv / p.pieces) + 1);
+  auto pieces_of = [&](int u) { return max(1, (int)((u + chunk - 1) / chunk)); };
+  int shift = 0;
+  while ((min((long long)sh.most, chunk) >> shift) >= kPlanBuckets) ++shift;
+  if (!p.ordered)
+    plan_buckets(sh, n_tiles, shift, [&](int t, auto add) {
+      const int u = plan_k_tile(v, base0, base1, t).m_count * p.group, s = pieces_of(u);
+      for (int i = 0; i < s; ++i) add((int)((long long)u * (i + 1) / s) - (int)((long long)u * i / s));
+    });
+  int items = 0, parts = 0, split_tiles = 0;
+  for (int t0 = 0; t0 < n_tiles; t0 += kPlanThreads) {
+    const int t = t0 + threadIdx.x;
+    PackedBwdItem w;
+    int u = 0, s = 0;
+    if (t < n_tiles) {
+      w = plan_k_tile(v, base0, base1, t);
+      u = w.m_count * p.group;
+      s = pieces_of(u);
+    }
+    int n_items, n_parts, n_split;
+    const int at = plan_scan(sh, s, &n_items);
+    const int part = parts + plan_scan(sh, s > 1 ? s : 0, &n_parts);
+    const int split = split_tiles + plan_scan(sh, s > 1 ? 1 : 0, &n_split);
+    if (s > 1) p.split_tiles[split] = make_int4(w.k0, w.rows, part, s);
+    for (int i = 0; i < s; ++i) {
+      w.first = (int)((long long)u * i / s);
+      w.count = (int)((long long)u * (i + 1) / s) - w.first;
+      w.part = s > 1 ? part + i : -1;
+      int place = items + at + i;  // ordered: key tiles as they stand, one after the other
+      w.bucket = place;
+      w.bucket_items = 1;
+      if (!p.ordered) place = plan_place(sh, w.count, shift, w);
+      p.items[place] = w;
+    }
+    items += n_items;
+    parts += n_parts;
+    split_tiles += n_split;
+  }
+  if (threadIdx.x == 0) p.head[0] = make_int4(items, v.bad, split_tiles, 0);
+}
+
+// Work index i (of items * heads) -> item and head: bucket by bucket, inside a
+// bucket head by head.  The item at place i / heads lies in the right bucket.
+template <typename Item>
+__device__ __forceinline__ int packed_locate(const Item* list, int i, int heads, int& head) {
+  const int at = i / heads;
+  const int first = list[at].bucket, n = list[at].bucket_items;
+  const int r = i - first * heads;
+  head = r / n;
+  return first + (r - head * n);
 }
 
 }  // namespace wf

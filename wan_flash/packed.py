@@ -33,8 +33,8 @@ import ctypes
 import torch
 
 from wan_flash import _lib, features
-from wan_flash.interface import _aligned, _auto_nsplit, _ptr, _sms, _stream_ptr
-from wan_flash.shapes import HEAD_DIM, TILE_N
+from wan_flash.interface import _aligned, _ptr, _stream_ptr
+from wan_flash.shapes import HEAD_DIM
 
 
 def _check(q, k, v, q_offsets, k_offsets):
@@ -80,17 +80,6 @@ def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
     return o, lse
 
 
-def packed_bwd_plan(total_q: int, total_k: int, n: int, h: int, h_kv: int, causal: bool, sms: int) -> dict:
-    """Split and mode of one backward call (host logic; the lengths themselves
-    are on the device, so the split goes by the mean sequence)."""
-    f = features.get_bwd()
-    tiles = max(1, -(-total_k // TILE_N))
-    # units of a key tile: query tiles of a mean sequence (half of them behind a causal diagonal), per q head of the group
-    units = max(1, -(-total_q // (TILE_N * max(n, 1))) * (h // max(h_kv, 1)) // (2 if causal else 1))
-    nsplit = f.nsplit if f.nsplit > 0 else _auto_nsplit(tiles * h_kv, min(units, 16), sms)
-    return {"nsplit": max(1, min(nsplit, 1024)), "deterministic": bool(f.deterministic)}
-
-
 def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                          do: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor | None = None,
                          causal: bool = False):
@@ -98,7 +87,8 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
 
     dk and dv are bitwise reproducible; dq is accumulated with fp32 reductions
     unless ``features.set_bwd_overrides(deterministic=True)``.  ``nsplit`` of the
-    backward features applies; its CTA-pair form does not."""
+    backward features cuts the longest key tile's walk into that many pieces (0:
+    the device chooses); the CTA-pair form does not apply."""
     q_offsets, k_offsets = _check(q, k, v, q_offsets, k_offsets)
     total_q, h, _ = q.shape
     total_k, h_kv, _ = k.shape
@@ -111,12 +101,12 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     q, k, v, o, do = (_aligned(t) for t in (q, k, v, o, do))
     lse = lse if lse.is_contiguous() else lse.contiguous()
     n = q_offsets.numel() - 1
-    plan = packed_bwd_plan(total_q, total_k, n, h, h_kv, causal, _sms(q.device))
-    cfg = _lib.PackedBwdCfg(plan["nsplit"], 1 if plan["deterministic"] else 0)
+    f = features.get_bwd()
+    cfg = _lib.PackedBwdCfg(min(int(f.nsplit), 1024), 1 if f.deterministic else 0)
     L = _lib.lib()
-    size = _bytes(L.wf_packed_bwd_workspace, n, total_q, total_k, h, h_kv, ctypes.byref(cfg))
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
     with torch.cuda.device(q.device):
+        size = _bytes(L.wf_packed_bwd_workspace, n, total_q, total_k, h, h_kv, ctypes.byref(cfg))
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
         rc = L.wf_packed_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(do), _ptr(q_offsets), _ptr(k_offsets),
                              _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), size, n, total_q, total_k, h, h_kv,
                              1 if causal else 0, ctypes.byref(cfg), ctypes.c_void_p(_stream_ptr(q.device)))
