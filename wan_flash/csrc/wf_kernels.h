@@ -92,7 +92,7 @@ struct PackedPlanParams {
   int group, h_kv;
   int nsplit;               // > 0: pieces of the longest walk; 0: by `pieces`
   int pieces;               // pieces (over all key-value heads) that the whole work is cut into at least
-  int4* head;               // [0] {items, status, split key tiles}, [1] (backward) {query tiles, status}
+  int4* head;               // [0] {items, status, split key tiles, draw counter}, [1] (backward) {query tiles, status}
   int* base;                // scratch: 3 * (n + 3)
   PackedFwdTile* fwd_tiles;
   PackedBwdItem* items;
@@ -104,6 +104,7 @@ constexpr int kPackedPiecesPerSm = 4;
 struct PackedFwdParams {
   const int4* head;
   const PackedFwdTile* tiles;
+  int* counter;             // items drawn beyond the first of every CTA; the plan sets it to 0
   __nv_bfloat16* o;
   float* lse;               // (h, total_q)
   int total_q, h, group, causal;
@@ -140,7 +141,7 @@ cudaError_t packed_setup();
 cudaError_t decode_setup();
 
 // role ids recorded with a device error by the operators without mbarrier roles
-enum : uint32_t { kRoleRope = 21, kRoleDecode = 22, kRolePackedPlan = 23 };
+enum : uint32_t { kRoleRope = 21, kRoleDecode = 22, kRolePackedPlan = 23, kRoleSchedule = 24 };
 
 size_t fwd_smem_bytes();
 size_t fwd2_smem_bytes();

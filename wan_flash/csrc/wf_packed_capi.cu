@@ -139,6 +139,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   PackedFwdParams p = {};
   p.head = pp.head;
   p.tiles = pp.fwd_tiles;
+  p.counter = &pp.head->w;
   p.o = reinterpret_cast<__nv_bfloat16*>(o);
   p.lse = lse;
   p.total_q = total_q, p.h = h, p.group = h / h_kv, p.causal = causal;

@@ -12,14 +12,17 @@
 //
 //   items     A work item is one record of the plan (up to 256 query rows of
 //             one sequence) and one head; the grid is persistent.  The list is
-//             sorted by falling number of key blocks and CTAs take it in
-//             serpentine order, so ragged and causal items end level.  Heads
-//             are innermost: the q heads of one key-value head run side by
-//             side and read its K and V from L2.
+//             sorted by falling number of key blocks and CTAs draw from it with
+//             a counter, longest first, so ragged and causal items end level.
+//             Warp 11 draws an item when the TMA warp comes to the last block of
+//             the one before (three blocks before the tensor core does) and
+//             hands the record to the other roles through a ring in shared
+//             memory.  Drawing four items ahead cost 16 % on causal 7800.
 //   walk      Key blocks from the last visible one down: the blocks that need
 //             masks (the ragged end, the causal diagonal) come first, the rest
 //             runs without a compare.  A record of at most 128 rows drives one
-//             of the two tiles only.
+//             of the two tiles only, and the first tile starts at its own
+//             diagonal (a block later than the second).
 //   masks     A row's visible keys are a count; the block loop compares it
 //             with the block's end and masks by column.  A row whose blocks so
 //             far are all masked keeps -inf as its maximum and exponentiates
@@ -59,19 +62,28 @@ constexpr int kBarOStaged = kBarDrain + 1;
 // A stage use n is freed on barrier n & 1: a warpgroup that waits for use n - 1
 // may not have seen use n - 2 freed, and one barrier's parity could not tell them apart.
 constexpr int kBarOStageFree = kBarOStaged + 1;    // + use & 1
-constexpr int kNumBars = kBarOStageFree + 2;
-constexpr uint32_t kOffTmemHolder = kOffBar + kNumBars * 8;
+constexpr int kItemSlots = 4;
+constexpr int kBarItemFull = kBarOStageFree + 2;         // + slot
+constexpr int kBarItemEmpty = kBarItemFull + kItemSlots; // + slot; one arrival per reader
+constexpr int kItemReaders = 11;                         // 8 softmax warps, MMA, TMA, store
+constexpr int kBarItemNext = kBarItemEmpty + kItemSlots; // the TMA warp is at its item's last block
+constexpr int kNumBars = kBarItemNext + 1;
+constexpr uint32_t kOffItems = kOffBar + ((kNumBars * 8 + 15) & ~15);
+constexpr uint32_t kOffTmemHolder = kOffItems + kItemSlots * 48;
 constexpr uint32_t kOffAbort = kOffTmemHolder + 4;
 constexpr uint32_t kSmemUsed = kOffAbort + 4;
 constexpr uint32_t kSmemBytes = kSmemUsed + 1024;
 static_assert(kSmemBytes <= 232448, "packed forward shared memory exceeds the per-CTA limit");
 }  // namespace pfwd
 
-// Item k of this CTA: the sorted list in rounds of gridDim.x items, every
-// second round backwards.
-__device__ __forceinline__ int packed_item(int k) {
-  return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-}
+// A drawn item as the roles read it.
+struct __align__(16) PackedFwdItem {
+  PackedFwdTile w;
+  int h;      // q head; -1: no items left
+  int skip0;  // blocks of the walk that no row of tile 0 sees
+  int pad[2];
+};
+static_assert(sizeof(PackedFwdItem) == 48, "three 16-byte words");
 
 // Zero rows [first, 128) of a 128-row tile of two 64-column boxes (a
 // converged warp; the swizzle permutes 16-byte chunks inside a row only), and
@@ -114,6 +126,11 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       mbar_init(bar(kBarKvFull + s), 1);
       mbar_init(bar(kBarKvEmpty + s), 1);
     }
+    for (int s = 0; s < kItemSlots; ++s) {
+      mbar_init(bar(kBarItemFull + s), 1);
+      mbar_init(bar(kBarItemEmpty + s), kItemReaders);
+    }
+    mbar_init(bar(kBarItemNext), 1);
     mbar_init(bar(kBarDrain), 1);
     mbar_init(bar(kBarOStaged), 4);
     *abort_flag = 0;
@@ -129,22 +146,54 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
   const uint32_t tmem = *tmem_holder;
   // a programmatic dependent of the plan kernel: its lists are read from here on
   griddep_wait();
-  const int n_items = p.head[0].x * p.h;
-  const bool bad = p.head[0].y != 0;
+  // The k-th item of this CTA, for a whole warp (or, one = true, for one thread
+  // that alone stands for its warp).  False: no more, or abort.
+  auto get_item = [&](int k, PackedFwdItem& x, uint32_t role, bool one) -> bool {
+    const int slot = k % kItemSlots;
+    const bool ok = one ? mbar_wait(bar(kBarItemFull + slot), (uint32_t)(k / kItemSlots) & 1, abort_flag, role, 60)
+                        : mbar_wait_warp(bar(kBarItemFull + slot), (uint32_t)(k / kItemSlots) & 1, abort_flag, role, 60);
+    if (!ok) return false;
+    x = reinterpret_cast<const PackedFwdItem*>(smem + kOffItems)[slot];
+    if (one) mbar_arrive(bar(kBarItemEmpty + slot));
+    else mbar_arrive_warp(bar(kBarItemEmpty + slot));
+    return x.h >= 0;
+  };
 
   if (warp == 11) {
-    regs_dec<kRegsOther>();  // idle warp of warpgroup 2
+    regs_dec<kRegsOther>();
+    // ------------------------------------------------------ item scheduler
+    if (lane == 0) {
+      const int n_items = p.head->x * p.h;
+      int next = (int)blockIdx.x;
+      for (int k = 0;; ++k) {
+        PackedFwdItem x = {};
+        x.h = -1;
+        if (next < n_items) {
+          x.w = p.tiles[packed_locate(p.tiles, next, p.h, x.h)];
+          const int seen0 = min(x.w.off + 127, x.w.klen);  // keys that the last row of tile 0 sees
+          if (p.causal && x.w.rows > 128 && seen0 > 0) x.skip0 = x.w.n_blocks - (seen0 + 127) / 128;
+        }
+        const int slot = k % kItemSlots;
+        if (k >= kItemSlots && !mbar_wait(bar(kBarItemEmpty + slot), (uint32_t)(k / kItemSlots - 1) & 1, abort_flag,
+                                          kRoleSchedule, 61))
+          break;
+        reinterpret_cast<PackedFwdItem*>(smem + kOffItems)[slot] = x;
+        mbar_arrive(bar(kBarItemFull + slot));
+        if (x.h < 0) break;
+        if (!mbar_wait(bar(kBarItemNext), (uint32_t)k & 1, abort_flag, kRoleSchedule, 62)) break;
+        next = (int)gridDim.x + atomicAdd(p.counter, 1);
+      }
+    }
   } else if (warp == 10) {
     regs_dec<kRegsOther>();
     // ------------------------------------------------------------ O store
     if (lane == 0) tma_prefetch_desc(&tm_o);
     int n = 0;  // tiles stored
     bool ok = true;
-    for (int k = 0; ok; ++k) {
-      const int item = packed_item(k);
-      if (item >= n_items) break;
-      int h;
-      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
+    PackedFwdItem x;
+    for (int k = 0; ok && get_item(k, x, kRoleStore, false); ++k) {
+      const PackedFwdTile& w = x.w;
+      const int h = x.h;
       if (w.n_blocks == 0) continue;
       for (int t = 0; t * 128 < w.rows; ++t, ++n) {
         ok = mbar_wait_warp(bar(kBarOStaged), (uint32_t)n & 1, abort_flag, kRoleStore, 50 + t);
@@ -152,8 +201,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         const int rows = w.rows - t * 128;
         if (rows >= 128) {
           if (lane == 0) {
-            for (int x = 0; x < 2; ++x)
-              tma_store_4d(&tm_o, sbase + kOffOStage + x * kBoxBytes, x * 64, w.q0 + t * 128, h, 0);
+            for (int c = 0; c < 2; ++c)
+              tma_store_4d(&tm_o, sbase + kOffOStage + c * kBoxBytes, c * 64, w.q0 + t * 128, h, 0);
             bulk_commit_group();
             bulk_wait_read_all();
           }
@@ -183,13 +232,13 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       int issued[kKvSlots] = {0, 0, 0, 0};
       int u = 0;  // K/V units (K and V of a block alternate)
       bool ok = true;
-      for (int k = 0; ok; ++k) {
-        const int item = packed_item(k);
-        if (item >= n_items) break;
-        int h;
-      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
-        const int kvh = h / p.group;
+      PackedFwdItem x;
+      for (int k = 0; ok && get_item(k, x, kRoleLoad, true); ++k) {
+        const PackedFwdTile& w = x.w;
+        const int h = x.h, kvh = h / p.group;
+        if (w.n_blocks == 0) mbar_arrive(bar(kBarItemNext));
         for (int it = 0; it < w.n_blocks && ok; ++it) {
+          if (it == w.n_blocks - 1) mbar_arrive(bar(kBarItemNext));
           const int j = w.n_blocks - 1 - it;
           for (int kv = 0; kv < 2 && ok; ++kv, ++u) {  // 0 = K, 1 = V
             const int slot = u % kKvSlots;
@@ -197,9 +246,9 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
             if (use > 0) ok = mbar_wait(bar(kBarKvEmpty + slot), (use - 1) & 1, abort_flag, kRoleLoad, 100 + slot);
             if (!ok) break;
             mbar_expect_tx(bar(kBarKvFull + slot), kTileBytes);
-            for (int x = 0; x < 2; ++x)
-              tma_load_4d(sbase + kOffKV + slot * kTileBytes + x * kBoxBytes, kv ? &tm_v : &tm_k,
-                          bar(kBarKvFull + slot), x * 64, w.k0 + j * 128, kvh, 0);
+            for (int c = 0; c < 2; ++c)
+              tma_load_4d(sbase + kOffKV + slot * kTileBytes + c * kBoxBytes, kv ? &tm_v : &tm_k,
+                          bar(kBarKvFull + slot), c * 64, w.k0 + j * 128, kvh, 0);
             issued[slot] = use + 1;
             if (it == 0 && kv == 0) {
               for (int t = 0; t * 128 < w.rows && ok; ++t) {
@@ -207,8 +256,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
                   ok = mbar_wait(bar(kBarQEmpty + t), (q_issued[t] - 1) & 1, abort_flag, kRoleLoad, 90 + t);
                 if (!ok) break;
                 mbar_expect_tx(bar(kBarQFull + t), kTileBytes);
-                for (int x = 0; x < 2; ++x)
-                  tma_load_4d(sbase + kOffQ + t * kTileBytes + x * kBoxBytes, &tm_q, bar(kBarQFull + t), x * 64,
+                for (int c = 0; c < 2; ++c)
+                  tma_load_4d(sbase + kOffQ + t * kTileBytes + c * kBoxBytes, &tm_q, bar(kBarQFull + t), c * 64,
                               w.q0 + t * 128, h, 0);
                 q_issued[t]++;
               }
@@ -267,8 +316,9 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     // One flat pipeline over the blocks of all items: block g issues PV_t(g-1)
     // before S_t(g) for each tile that the block has.
     int g = 0;
-    int prev_it = 0, prev_tiles = 0;  // position of block g-1 in its item, query tiles of it
-    int prev_keys = 128;              // keys of block g-1 that exist for its item (128 but for the last block)
+    bool prev[2] = {false, false};      // tiles that block g-1 has
+    bool prev_acc[2] = {false, false};  // ... and adds to (not its first block)
+    int prev_keys = 128;                // keys of block g-1 that exist for its item (128 but for the last block)
     bool prev_last = false;
     auto wait_v = [&]() -> bool {  // V of block g-1, its rows behind the last visible key zeroed
       const int uv = 2 * (g - 1) + 1, slot_v = uv % kKvSlots;
@@ -277,12 +327,10 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       if (prev_keys < 128) packed_zero_rows(sKV + slot_v * kTileBytes, prev_keys);
       return true;
     };
-    for (int k = 0; ok; ++k) {
-      const int item = packed_item(k);
-      if (item >= n_items) break;
-      int h;
-      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
-      const int tiles = w.rows > 128 ? 2 : 1;
+    PackedFwdItem x;
+    x.h = 0;
+    for (int k = 0; ok && get_item(k, x, kRoleMma, false); ++k) {
+      const PackedFwdTile& w = x.w;
       for (int it = 0; it < w.n_blocks && ok; ++it, ++g) {
         const int uk = 2 * g, slot_k = uk % kKvSlots;
         ok = mbar_wait_warp(bar(kBarKvFull + slot_k), (uk / kKvSlots) & 1, abort_flag, kRoleMma, 10 + slot_k);
@@ -290,14 +338,19 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         tc_fence_after();
         const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;  // of block g-1
         if (g > 0 && !(ok = wait_v())) break;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (t < prev_tiles) {
-            if (!(ok = issue_pv(t, slot_v, prev_it > 0))) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok) break;
+          if (prev[t]) {
+            if (!(ok = issue_pv(t, slot_v, prev_acc[t]))) break;
             if (prev_last) mma_commit_e(bar(kBarOFull + t));
           }
           if (g > 0 && t == 1) mma_commit_e(bar(kBarKvEmpty + slot_v));
-          if (t < tiles) {
-            if (it == 0) {
+          const int first = t == 0 ? x.skip0 : 0;
+          prev[t] = t * 128 < w.rows && it >= first;
+          prev_acc[t] = it > first;
+          if (prev[t]) {
+            if (it == first) {
               ok = mbar_wait_warp(bar(kBarQFull + t), (uint32_t)q_phase[t] & 1, abort_flag, kRoleMma, t);
               if (!ok) break;
               q_phase[t]++;
@@ -309,17 +362,17 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
           }
         }
         if (ok) mma_commit_e(bar(kBarKvEmpty + slot_k));
-        prev_it = it;
-        prev_tiles = tiles;
         prev_last = (it == w.n_blocks - 1);
         prev_keys = it == 0 ? w.klen - (w.n_blocks - 1) * 128 : 128;
       }
     }
-    if (ok && g > 0) {
+    if (ok && g > 0 && x.h < 0) {  // (an abort leaves another item in x)
       const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;
       ok = wait_v();
-      for (int t = 0; t < prev_tiles && ok; ++t) {
-        if (!(ok = issue_pv(t, slot_v, prev_it > 0))) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || !prev[t]) continue;
+        if (!(ok = issue_pv(t, slot_v, prev_acc[t]))) continue;
         mma_commit_e(bar(kBarOFull + t));
       }
       if (ok) mma_commit_e(bar(kBarKvEmpty + slot_v));
@@ -343,11 +396,11 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     int s_waits = 0;    // S_t tiles consumed
     int o_waits = 0;    // items of this tile that had keys
     int stage_use = 0;  // O tiles of both tiles staged before this item
-    for (int k = 0; ok; ++k) {
-      const int item = packed_item(k);
-      if (item >= n_items) break;
-      int h;
-      const PackedFwdTile w = p.tiles[packed_locate(p.tiles, item, p.h, h)];
+    const bool bad = p.head->y != 0;
+    PackedFwdItem x;
+    for (int k = 0; ok && get_item(k, x, role, false); ++k) {
+      const PackedFwdTile& w = x.w;
+      const int h = x.h;
       const int row = t * 128 + r;  // within the record
       if (w.n_blocks == 0) {
         // nothing to attend (or rows outside any sequence): o = 0, lse = -inf;
@@ -364,7 +417,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       const int seen = p.causal ? min(max(w.off + row, 0), w.klen) : w.klen;  // keys that this row sees
       float m_s = -INFINITY;  // running reference max, in scaled log2 units
       float l = 0.f;          // running row sum (relative to m_s)
-      for (int it = 0; it < w.n_blocks; ++it, ++s_waits) {
+      const int first = t == 0 ? x.skip0 : 0;
+      for (int it = first; it < w.n_blocks; ++it, ++s_waits) {
         ok = mbar_wait(bar(kBarSFull + t), (uint32_t)s_waits & 1, abort_flag, role, 30 + t);
         if (!ok) break;
         tc_fence_after();
@@ -390,7 +444,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
           for (int i = 0; i < 16; ++i)
             mx[i & 3] = fmax3(mx[i & 3], __uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1]));
         const float mnew_s = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-        if (it == 0) {
+        if (it == first) {
           m_s = mnew_s;
         } else {
           // move the reference max only when the row max grew past the rescale
