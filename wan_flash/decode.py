@@ -22,23 +22,21 @@ between replays of a captured CUDA graph; shapes may not.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from wan_flash import _lib
-from wan_flash.interface import _aligned, _ptr, _stream_ptr
+from wan_flash.interface import _aligned, _launch
 from wan_flash.shapes import HEAD_DIM
 
-_WORKSPACE_BYTES: dict = {}  # (device index, h, h_kv) -> bytes
-
-
-def _workspace_bytes(device: torch.device, h: int, h_kv: int) -> int:
-    key = (device.index, h, h_kv)
-    if key not in _WORKSPACE_BYTES:
-        n = ctypes.c_size_t()
-        _lib.check(_lib.lib().wf_decode_workspace(h, h_kv, ctypes.byref(n)))
-        _WORKSPACE_BYTES[key] = n.value
-    return _WORKSPACE_BYTES[key]
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(index: int, h: int, h_kv: int) -> int:
+    """Of device `index`."""
+    size = ctypes.c_size_t()
+    with torch.cuda.device(index):
+        _lib.check(_lib.lib().wf_decode_workspace(h, h_kv, ctypes.byref(size)))
+    return size.value
 
 
 def wan_flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -48,35 +46,35 @@ def wan_flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     A sequence of length 0 gives o = 0 and lse = -inf.  k_cache and v_cache may be
     strided views (of one tensor that holds both, say) as long as rows of 128
     are contiguous and 16-byte aligned."""
-    assert q.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16
+    assert q.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
     assert q.dim() == 3 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape
     b, h, d = q.shape
     n_pages, page_size, h_kv, dk = k_cache.shape
     assert d == HEAD_DIM and dk == HEAD_DIM, "specialized for head_dim=128"
     assert h_kv > 0 and h % h_kv == 0, "q heads are a multiple of key-value heads"
     assert page_size > 0
-    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == b
-    assert lengths.dtype == torch.int32 and lengths.shape == (b,)
-    assert page_table.shape[1] * page_size <= 2**31 - 1025
-    for x in (k_cache, v_cache):
-        assert x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s in x.stride()[:-1]), \
-            "cache rows of 128 must be contiguous and 16-byte aligned"
-    assert q.is_cuda and all(t.device == q.device for t in (k_cache, v_cache, page_table, lengths)), \
-        "tensors must be on one CUDA device"
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(b, h, device=q.device, dtype=torch.float32)
-    if o.numel() == 0:
-        return o, lse
+    assert page_table.dtype is torch.int32 and page_table.dim() == 2 and page_table.shape[0] == b
+    assert lengths.dtype is torch.int32 and lengths.shape == (b,)
+    width = page_table.shape[1]
+    assert width * page_size <= 2**31 - 1025
+    ks, vs = k_cache.stride(), v_cache.stride()
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
+    assert ks[3] == 1 and vs[3] == 1 and (k_ptr | v_ptr) % 16 == 0 and \
+        (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) % 8 == 0, "cache rows of 128 must be contiguous and 16-byte aligned"
+    device = q.device
+    assert q.is_cuda and k_cache.device == device and v_cache.device == device and page_table.device == device and \
+        lengths.device == device, "tensors must be on one CUDA device"
     q = _aligned(q)
-    lengths = lengths if lengths.is_contiguous() else lengths.contiguous()
-    page_table = page_table if page_table.stride(1) == 1 or page_table.shape[1] <= 1 else page_table.contiguous()
-    cfg = _lib.DecodeCfg(n_pages, page_size, page_table.shape[1], 0, page_table.stride(0), *k_cache.stride()[:3],
-                         *v_cache.stride()[:3])
-    with torch.cuda.device(q.device):
-        n = _workspace_bytes(q.device, h, h_kv)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        rc = _lib.lib().wf_decode(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(page_table), _ptr(lengths), _ptr(o),
-                                  _ptr(lse), _ptr(ws), n, b, h, h_kv, ctypes.byref(cfg),
-                                  ctypes.c_void_p(_stream_ptr(q.device)))
-    _lib.check(rc)
+    o = torch.empty_like(q)
+    lse = torch.empty((b, h), device=device, dtype=torch.float32)
+    if b == 0 or h == 0:
+        return o, lse
+    lengths = lengths.contiguous()
+    if width > 1 and page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    cfg = _lib.DecodeCfg(n_pages, page_size, width, 0, page_table.stride(0), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    size = _workspace_bytes(device.index, h, h_kv)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    _launch(_lib.lib().wf_decode, device, q.data_ptr(), k_ptr, v_ptr, page_table.data_ptr(), lengths.data_ptr(),
+            o.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, b, h, h_kv, cfg)
     return o, lse

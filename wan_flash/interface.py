@@ -53,6 +53,20 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _launch(fn, device: torch.device, *args):
+    """fn(*args, stream) with `device` current, on its current stream; raises on a status.
+    The short way for calls whose kernels take a few microseconds: the raw stream handle,
+    and a device switch only where the current device is another one."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != 0:
+        _lib.check(rc)
+
+
 def _ptr(t: torch.Tensor):
     return ctypes.c_void_p(t.data_ptr())
 

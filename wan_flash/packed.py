@@ -29,54 +29,62 @@ can see raise AssertionError before any CUDA call.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from wan_flash import _lib, features
-from wan_flash.interface import _aligned, _ptr, _stream_ptr
+from wan_flash.interface import _aligned, _launch
 from wan_flash.shapes import HEAD_DIM
 
 
 def _check(q, k, v, q_offsets, k_offsets):
-    k_offsets = q_offsets if k_offsets is None else k_offsets
-    assert q.dtype == k.dtype == v.dtype == torch.bfloat16
+    assert q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and v.dtype is torch.bfloat16
     assert q.dim() == 3 and k.dim() == 3 and v.shape == k.shape
-    assert q.shape[2] == HEAD_DIM and k.shape[2] == HEAD_DIM, "specialized for head_dim=128"
-    h, h_kv = q.shape[1], k.shape[1]
+    total_q, h, d = q.shape
+    total_k, h_kv, dk = k.shape
+    assert d == HEAD_DIM and dk == HEAD_DIM, "specialized for head_dim=128"
     assert (h % h_kv == 0) if h_kv else h == 0, "q heads are a multiple of key-value heads"
-    assert q_offsets.dtype == k_offsets.dtype == torch.int32
+    assert q_offsets.dtype is torch.int32 and k_offsets.dtype is torch.int32
     assert q_offsets.dim() == 1 and q_offsets.shape == k_offsets.shape and q_offsets.numel() >= 1
-    assert q.is_cuda and all(t.device == q.device for t in (k, v, q_offsets, k_offsets)), \
-        "tensors must be on one CUDA device"
-    return tuple(t if t.is_contiguous() else t.contiguous() for t in (q_offsets, k_offsets))
+    device = q.device
+    assert q.is_cuda and k.device == device and v.device == device and q_offsets.device == device and \
+        k_offsets.device == device, "tensors must be on one CUDA device"
+    return total_q, total_k, h, h_kv, q_offsets.numel() - 1, device
 
 
-def _bytes(fn, *args) -> int:
-    n = ctypes.c_size_t()
-    _lib.check(fn(*args, ctypes.byref(n)))
-    return n.value
+@functools.lru_cache(maxsize=256)
+def _fwd_bytes(n: int, total_q: int) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.lib().wf_packed_fwd_workspace(n, total_q, ctypes.byref(size)))
+    return size.value
+
+
+@functools.lru_cache(maxsize=256)
+def _bwd_cfg_bytes(index: int, n: int, total_q: int, total_k: int, h: int, h_kv: int, nsplit: int, deterministic: bool):
+    """The C options and the workspace's size on device `index`."""
+    cfg, size = _lib.PackedBwdCfg(min(nsplit, 1024), 1 if deterministic else 0), ctypes.c_size_t()
+    with torch.cuda.device(index):
+        _lib.check(_lib.lib().wf_packed_bwd_workspace(n, total_q, total_k, h, h_kv, ctypes.byref(cfg), ctypes.byref(size)))
+    return cfg, size.value
 
 
 def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                          k_offsets: torch.Tensor | None = None, causal: bool = False):
     """(o, lse) of attention over packed sequences; see the module's text."""
-    q_offsets, k_offsets = _check(q, k, v, q_offsets, k_offsets)
-    q, k, v = (_aligned(t) for t in (q, k, v))
-    total_q, h, _ = q.shape
-    total_k, h_kv, _ = k.shape
-    n = q_offsets.numel() - 1
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(h, total_q, device=q.device, dtype=torch.float32)
-    if o.numel() == 0:
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    total_q, total_k, h, h_kv, n, device = _check(q, k, v, q_offsets, k_offsets)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    q_offsets, k_offsets = q_offsets.contiguous(), k_offsets.contiguous()
+    o = torch.empty_like(q)
+    lse = torch.empty((h, total_q), device=device, dtype=torch.float32)
+    if total_q == 0 or h == 0:
         return o, lse
-    L = _lib.lib()
-    size = _bytes(L.wf_packed_fwd_workspace, n, total_q)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        rc = L.wf_packed_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(q_offsets), _ptr(k_offsets), _ptr(o), _ptr(lse), _ptr(ws),
-                             size, n, total_q, total_k, h, h_kv, 1 if causal else 0,
-                             ctypes.c_void_p(_stream_ptr(q.device)))
-    _lib.check(rc)
+    size = _fwd_bytes(n, total_q)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    _launch(_lib.lib().wf_packed_fwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
+            k_offsets.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, n, total_q, total_k, h, h_kv,
+            1 if causal else 0)
     return o, lse
 
 
@@ -89,28 +97,22 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     unless ``features.set_bwd_overrides(deterministic=True)``.  ``nsplit`` of the
     backward features cuts the longest key tile's walk into that many pieces (0:
     the device chooses); the CTA-pair form does not apply."""
-    q_offsets, k_offsets = _check(q, k, v, q_offsets, k_offsets)
-    total_q, h, _ = q.shape
-    total_k, h_kv, _ = k.shape
-    assert o.dtype == do.dtype == torch.bfloat16 and o.shape == q.shape and do.shape == q.shape
-    assert lse.dtype == torch.float32 and lse.shape == (h, total_q)
-    assert all(t.device == q.device for t in (o, lse, do)), "tensors must be on one CUDA device"
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    if dq.numel() == 0 or dk.numel() == 0:
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    total_q, total_k, h, h_kv, n, device = _check(q, k, v, q_offsets, k_offsets)
+    assert o.dtype is torch.bfloat16 and do.dtype is torch.bfloat16 and o.shape == q.shape and do.shape == q.shape
+    assert lse.dtype is torch.float32 and lse.shape == (h, total_q)
+    assert o.device == device and lse.device == device and do.device == device, "tensors must be on one CUDA device"
+    q, k, v, o, do, lse = _aligned(q), _aligned(k), _aligned(v), _aligned(o), _aligned(do), lse.contiguous()
+    q_offsets, k_offsets = q_offsets.contiguous(), k_offsets.contiguous()
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if total_q == 0 or total_k == 0 or h == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    q, k, v, o, do = (_aligned(t) for t in (q, k, v, o, do))
-    lse = lse if lse.is_contiguous() else lse.contiguous()
-    n = q_offsets.numel() - 1
     f = features.get_bwd()
-    cfg = _lib.PackedBwdCfg(min(int(f.nsplit), 1024), 1 if f.deterministic else 0)
-    L = _lib.lib()
-    with torch.cuda.device(q.device):
-        size = _bytes(L.wf_packed_bwd_workspace, n, total_q, total_k, h, h_kv, ctypes.byref(cfg))
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        rc = L.wf_packed_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(do), _ptr(q_offsets), _ptr(k_offsets),
-                             _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), size, n, total_q, total_k, h, h_kv,
-                             1 if causal else 0, ctypes.byref(cfg), ctypes.c_void_p(_stream_ptr(q.device)))
-    _lib.check(rc)
+    cfg, size = _bwd_cfg_bytes(device.index, n, total_q, total_k, h, h_kv, f.nsplit, f.deterministic)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    _launch(_lib.lib().wf_packed_bwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+            do.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            ws.data_ptr(), size, n, total_q, total_k, h, h_kv, 1 if causal else 0, cfg)
     return dq, dk, dv
 
 

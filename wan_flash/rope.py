@@ -19,12 +19,10 @@ and ``wan_flash._lib.check_device()`` raises.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from wan_flash import _lib
-from wan_flash.interface import _ptr, _stream_ptr
+from wan_flash.interface import _launch
 from wan_flash.shapes import HEAD_DIM
 
 AXES = (44, 42, 42)  # head dims of time, height, width in the Wan models
@@ -58,44 +56,52 @@ def rope_positions(grid, start: int = 0, count: int | None = None, first_frame: 
     return torch.where((i < n)[:, None], pos, -1).to(torch.int32)
 
 
-def _in_place(x: torch.Tensor) -> torch.Tensor:
-    """x itself where the kernel can read it by its strides (16-byte rows), else a contiguous copy."""
-    per16 = 16 // x.element_size()
-    if x.stride(-1) == 1 and all(s % per16 == 0 and s >= 0 for s in x.stride()[:-1]) and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+def _rows(x: torch.Tensor, size: int):
+    """x itself where the kernel can read it by its strides (16-byte rows), else a
+    contiguous copy; and its (batch, token, head) strides."""
+    st = x.stride()
+    batch = st[0] if len(st) == 4 else 0
+    if st[-1] != 1 or (batch | st[-3] | st[-2]) % (16 // size) or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        st = x.stride()
+        batch = st[0] if len(st) == 4 else 0
+    return x, batch, st[-3], st[-2]
 
 
 def _rope_impl(q, k, positions, table, axes, inverse):
-    assert q.dtype == k.dtype and q.dtype in (torch.bfloat16, torch.float32), "q and k are both bf16 or both fp32"
-    assert q.dim() == k.dim() and q.dim() in (3, 4), "(s, h, 128) or (b, s, h, 128)"
-    assert q.shape[:-2] == k.shape[:-2] and q.shape[-1] == k.shape[-1]
-    assert q.shape[-1] == HEAD_DIM, "specialized for head_dim=128"
+    dtype = q.dtype
+    assert k.dtype is dtype and (dtype is torch.bfloat16 or dtype is torch.float32), "q and k are both bf16 or both fp32"
+    dims = q.dim()
+    assert k.dim() == dims and dims in (3, 4), "(s, h, 128) or (b, s, h, 128)"
+    qs, kshape = q.shape, k.shape
+    assert qs[:-2] == kshape[:-2]
+    assert qs[-1] == HEAD_DIM and kshape[-1] == HEAD_DIM, "specialized for head_dim=128"
     assert len(axes) == 3 and sum(axes) == HEAD_DIM and all(d >= 0 and d % 2 == 0 for d in axes), \
         "three even axes that add up to head_dim"
-    s = q.shape[-3]
-    assert positions.dtype == torch.int32 and positions.shape[-1:] == (3,)
-    assert positions.shape in ((s, 3), tuple(q.shape[:-2]) + (3,)), "positions are (s, 3) or one (s, 3) per batch item"
-    assert table.dtype == torch.float32 and table.dim() == 3 and table.shape[1:] == (HEAD_DIM // 2, 2)
+    s, h, h_kv = qs[-3], qs[-2], kshape[-2]
+    b = qs[0] if dims == 4 else 1
+    ps = positions.shape
+    assert positions.dtype is torch.int32 and (ps == (s, 3) or (dims == 4 and ps == (b, s, 3))), \
+        "positions are int32 (s, 3) or one (s, 3) per batch item"
+    assert table.dtype is torch.float32 and table.dim() == 3 and table.shape[1:] == (HEAD_DIM // 2, 2)
     assert table.shape[0] >= 1
-    assert q.is_cuda and all(t.device == q.device for t in (k, positions, table)), "tensors must be on one CUDA device"
-    b = q.shape[0] if q.dim() == 4 else 1
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if oq.numel() + ok.numel() == 0:
+    device = q.device
+    assert q.is_cuda and k.device == device and positions.device == device and table.device == device, \
+        "tensors must be on one CUDA device"
+    oq = torch.empty(qs, dtype=dtype, device=device)
+    ok = torch.empty(kshape, dtype=dtype, device=device)
+    if b == 0 or s == 0 or h + h_kv == 0:
         return oq, ok
-    q, k = _in_place(q), _in_place(k)
-    positions = positions if positions.is_contiguous() else positions.contiguous()
-    table = table if table.is_contiguous() and table.data_ptr() % 8 == 0 else table.clone(
-        memory_format=torch.contiguous_format)
-    st = [x.stride() if x.dim() == 4 else (0, *x.stride()) for x in (q, k)]
-    cfg = _lib.RopeCfg(1 if q.dtype == torch.float32 else 0, 1 if inverse else 0, table.shape[0], axes[0] // 2,
-                       axes[1] // 2, 0, st[0][0], st[0][1], st[0][2], st[1][0], st[1][1], st[1][2],
-                       3 * s if positions.dim() == 3 else 0)
-    with torch.cuda.device(q.device):
-        rc = _lib.lib().wf_rope(_ptr(q), _ptr(k), _ptr(oq), _ptr(ok), _ptr(table), _ptr(positions), b, s, q.shape[-2],
-                                k.shape[-2], ctypes.byref(cfg), ctypes.c_void_p(_stream_ptr(q.device)))
-    _lib.check(rc)
+    size = 2 if dtype is torch.bfloat16 else 4
+    q, q0, q1, q2 = _rows(q, size)
+    k, k0, k1, k2 = _rows(k, size)
+    positions = positions.contiguous()
+    if not table.is_contiguous() or table.data_ptr() % 8:
+        table = table.clone(memory_format=torch.contiguous_format)
+    cfg = _lib.RopeCfg(0 if size == 2 else 1, 1 if inverse else 0, table.shape[0], axes[0] // 2, axes[1] // 2, 0,
+                       q0, q1, q2, k0, k1, k2, 3 * s if len(ps) == 3 else 0)
+    _launch(_lib.lib().wf_rope, device, q.data_ptr(), k.data_ptr(), oq.data_ptr(), ok.data_ptr(), table.data_ptr(),
+            positions.data_ptr(), b, s, h, h_kv, cfg)
     return oq, ok
 
 
@@ -123,4 +129,6 @@ def wan_flash_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     axes: head dims of time, height, width, as given to rope_table.
     q and k may be strided views (slices of a fused qkv projection); heads may
     differ.  Differentiable in q and k (the turn by the negative angle)."""
-    return _WanFlashRopeFn.apply(q, k, positions, table, tuple(int(d) for d in axes))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return _WanFlashRopeFn.apply(q, k, positions, table, axes)
+    return _rope_impl(q, k, positions, table, axes, False)
