@@ -249,7 +249,7 @@ int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offs
 
 typedef struct wf_packed_bwd_cfg {
   int nsplit;        /* 0 = the device cuts long walks into pieces of about a
-                        quarter of an SM's share; n > 0: pieces of 1/n of the
+                        third of an SM's share; n > 0: pieces of 1/n of the
                         longest walk.  Pieces leave fp32 partial dk and dv that
                         are summed in a fixed order */
   int deterministic; /* 1 = dq's fp32 contributions are added in key order */

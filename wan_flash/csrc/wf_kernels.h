@@ -100,7 +100,7 @@ struct PackedPlanParams {
   int4* split_tiles;        // {first row, rows, first part, parts}
 };
 constexpr int kPackedMinChunk = 4;   // units: below, a piece's own cost exceeds what it evens out
-constexpr int kPackedPiecesPerSm = 4;
+constexpr int kPackedPiecesPerSm = 3;
 struct PackedFwdParams {
   const int4* head;
   const PackedFwdTile* tiles;

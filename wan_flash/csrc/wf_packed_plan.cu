@@ -15,15 +15,17 @@
 // same keys (backward: queries), run side by side.
 //
 // Backward pieces: a key tile that walks more units (query tile, q head) than
-// `chunk`, a quarter of an SM's even share, is cut into pieces whose partial
+// `chunk`, a third of an SM's even share, is cut into pieces whose partial
 // dK and dV a convert sums.  One long sequence then fills the GPU as evenly as many.
 //
 // Offsets that fall, start below 0 or end behind the tensor set the device
 // error word; the lists then hold only rows outside any sequence, with
 // status 1 (the kernels write NaN there).
 //
-// Bound: latency (a chain of barriers and dependent loads).  Up to 2045
-// sequences the offsets and scans stay in shared memory.
+// Bound: latency (a chain of barriers, dependent loads and cold code).  Up to
+// 2045 sequences the offsets and scans stay in shared memory; a thread keeps
+// the record of its first tile in registers over the passes; 256 threads
+// because most calls have fewer tiles and barriers cost by the warp.
 #include "wf_common.cuh"
 #include "wf_kernels.h"
 
@@ -31,22 +33,22 @@ namespace wf {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanBuckets = 1024;
+constexpr int kPlanThreads = 256;
+constexpr int kPlanBuckets = 256;
 constexpr int kPlanSmall = 2048;  // n + 3 up to this: offsets and tile bases in shared memory
 static_assert(kPlanBuckets == kPlanThreads, "one bucket per thread in the scan");
 
 struct PlanShared {
-  int warp_sum[32];
+  int warp_sum[kPlanThreads / 32];
   int start[kPlanBuckets + 1];
   int cursor[kPlanBuckets];
   unsigned long long units;
-  int most;
+  int most, parts, split_tiles;
   int q_off[kPlanSmall], k_off[kPlanSmall], base0[kPlanSmall], base1[kPlanSmall];
 };
 
 // Exclusive block scan of one int per thread; returns the prefix, *total the sum.
-__device__ int plan_scan(PlanShared& sh, int x, int* total) {
+__device__ __noinline__ int plan_scan(PlanShared& sh, int x, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int incl = x;
 #pragma unroll
@@ -57,8 +59,8 @@ __device__ int plan_scan(PlanShared& sh, int x, int* total) {
   if (lane == 31) sh.warp_sum[warp] = incl;
   __syncthreads();
   int before = 0, sum = 0;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i) {
+#pragma unroll
+  for (int i = 0; i < kPlanThreads / 32; ++i) {
     const int s = sh.warp_sum[i];
     if (i < warp) before += s;
     sum += s;
@@ -84,7 +86,7 @@ __device__ __forceinline__ bool plan_bad(const int* off, int s, int total) {
 }
 
 // base[s] = first tile of segment s (s = 0..n+1), base[n+2] = number of tiles
-__device__ int plan_bases(PlanShared& sh, const int* off, int n, int total, bool bad, int tile, int* base) {
+__device__ __noinline__ int plan_bases(PlanShared& sh, const int* off, int n, int total, bool bad, int tile, int* base) {
   int carry = 0;
   for (int s0 = 0; s0 < n + 2; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
@@ -118,7 +120,7 @@ struct PlanView {
 };
 
 // Forward tile t: up to 256 query rows.
-__device__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int* base, int t) {
+__device__ __noinline__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int* base, int t) {
   const int s = plan_find(base, p.n, t);
   int qs, lq;
   plan_segment(p.q_off, p.n, p.total_q, p.bad, s, qs, lq);
@@ -138,7 +140,7 @@ __device__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int* base, int t
 }
 
 // Backward key tile t: 128 key rows, and the query tiles that see them.
-__device__ PackedBwdItem plan_k_tile(const PlanView& p, const int* kbase, const int* qbase, int t) {
+__device__ __noinline__ PackedBwdItem plan_k_tile(const PlanView& p, const int* kbase, const int* qbase, int t) {
   const int s = plan_find(kbase, p.n, t);
   int ks, lk;
   plan_segment(p.k_off, p.n, p.total_k, p.bad, s, ks, lk);
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
   __shared__ PlanShared sh;
   griddep_launch_dependents();
   const bool small = p.n + 3 <= kPlanSmall;
-  if (threadIdx.x == 0) sh.units = 0ull, sh.most = 0;
+  if (threadIdx.x == 0) sh.units = 0ull, sh.most = sh.parts = sh.split_tiles = 0;
   if (small) {
     for (int s = threadIdx.x; s <= p.n; s += kPlanThreads) {
       sh.q_off[s] = p.q_off[s];
@@ -218,15 +220,18 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
 
   if (!p.backward) {
     const int n_tiles = plan_bases(sh, v.q_off, p.n, p.total_q, v.bad, 256, base0);
+    PackedFwdTile mine = {};  // this thread's first tile
+    if ((int)threadIdx.x < n_tiles) mine = plan_fwd_tile(v, base0, threadIdx.x);
+    auto tile = [&](int t) { return t < kPlanThreads ? mine : plan_fwd_tile(v, base0, t); };
     int most = 0;
-    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) most = max(most, plan_fwd_tile(v, base0, t).n_blocks);
+    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) most = max(most, tile(t).n_blocks);
     atomicMax(&sh.most, most);
     __syncthreads();
     int shift = 0;
     while ((sh.most >> shift) >= kPlanBuckets) ++shift;
-    plan_buckets(sh, n_tiles, shift, [&](int t, auto add) { add(plan_fwd_tile(v, base0, t).n_blocks); });
+    plan_buckets(sh, n_tiles, shift, [&](int t, auto add) { add(tile(t).n_blocks); });
     for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
-      PackedFwdTile w = plan_fwd_tile(v, base0, t);
+      PackedFwdTile w = tile(t);
       const int at = plan_place(sh, w.n_blocks, shift, w);
       p.fwd_tiles[at] = w;
     }
@@ -248,56 +253,67 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
   }
   const int n_tiles = plan_bases(sh, v.k_off, p.n, p.total_k, v.bad, 128, base0);
   plan_bases(sh, v.q_off, p.n, p.total_q, v.bad, 128, base1);
+  PackedBwdItem mine = {};  // this thread's first key tile
+  if ((int)threadIdx.x < n_tiles) mine = plan_k_tile(v, base0, base1, threadIdx.x);
+  auto tile = [&](int t) { return t < kPlanThreads ? mine : plan_k_tile(v, base0, base1, t); };
   unsigned long long units = 0;
   int most = 0;
   for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
-    const int u = plan_k_tile(v, base0, base1, t).m_count * p.group;
+    const int u = tile(t).m_count * p.group;
     units += u;
     most = max(most, u);
   }
   atomicAdd(&sh.units, units);
   atomicMax(&sh.most, most);
   __syncthreads();
-  const long long chunk = p.nsplit > 0 ? max(1, (sh.most + p.nsplit - 1) / p.nsplit)
-                                       : max((long long)kPackedMinChunk, (long long)(sh.units * p.h_kv / p.pieces) + 1);
-  auto pieces_of = [&](int u) { return max(1, (int)((u + chunk - 1) / chunk)); };
+  most = sh.most;
+  const int chunk =
+      p.nsplit > 0 ? max(1, (int)(((unsigned)most + p.nsplit - 1) / p.nsplit))
+                   : (int)min((unsigned long long)0x7fffffff,
+                              max((unsigned long long)kPackedMinChunk, sh.units * p.h_kv / p.pieces + 1));
+  // a walk of u units in s pieces: the first u % s have one unit more
+  auto pieces_of = [&](int u) { return u > chunk ? (int)(((unsigned)u + (unsigned)chunk - 1u) / (unsigned)chunk) : 1; };
   int shift = 0;
-  while ((min((long long)sh.most, chunk) >> shift) >= kPlanBuckets) ++shift;
+  while ((min(most, chunk) >> shift) >= kPlanBuckets) ++shift;
   if (!p.ordered)
     plan_buckets(sh, n_tiles, shift, [&](int t, auto add) {
-      const int u = plan_k_tile(v, base0, base1, t).m_count * p.group, s = pieces_of(u);
-      for (int i = 0; i < s; ++i) add((int)((long long)u * (i + 1) / s) - (int)((long long)u * i / s));
+      const int u = tile(t).m_count * p.group, s = pieces_of(u), even = u / s, more = u - even * s;
+      for (int i = 0; i < s; ++i) add(even + (i < more ? 1 : 0));
     });
-  int items = 0, parts = 0, split_tiles = 0;
+  int items = 0;
   for (int t0 = 0; t0 < n_tiles; t0 += kPlanThreads) {
     const int t = t0 + threadIdx.x;
     PackedBwdItem w;
-    int u = 0, s = 0;
+    int u = 0, s = 0, at = 0;
     if (t < n_tiles) {
-      w = plan_k_tile(v, base0, base1, t);
+      w = tile(t);
       u = w.m_count * p.group;
       s = pieces_of(u);
     }
-    int n_items, n_parts, n_split;
-    const int at = plan_scan(sh, s, &n_items);
-    const int part = parts + plan_scan(sh, s > 1 ? s : 0, &n_parts);
-    const int split = split_tiles + plan_scan(sh, s > 1 ? 1 : 0, &n_split);
-    if (s > 1) p.split_tiles[split] = make_int4(w.k0, w.rows, part, s);
+    if (p.ordered) {
+      int sum;
+      at = items + plan_scan(sh, s, &sum);
+      items += sum;
+    }
+    int part = -1;
+    if (s > 1) {  // any place will do: the parts of a tile are summed in their order
+      part = atomicAdd(&sh.parts, s);
+      p.split_tiles[atomicAdd(&sh.split_tiles, 1)] = make_int4(w.k0, w.rows, part, s);
+    }
+    const int even = s ? u / s : 0, more = u - even * s;
     for (int i = 0; i < s; ++i) {
-      w.first = (int)((long long)u * i / s);
-      w.count = (int)((long long)u * (i + 1) / s) - w.first;
+      w.first = i * even + min(i, more);
+      w.count = even + (i < more ? 1 : 0);
       w.part = s > 1 ? part + i : -1;
-      int place = items + at + i;  // ordered: key tiles as they stand, one after the other
+      int place = at + i;  // ordered: key tiles as they stand, one after the other
       w.bucket = place;
       w.bucket_items = 1;
       if (!p.ordered) place = plan_place(sh, w.count, shift, w);
       p.items[place] = w;
     }
-    items += n_items;
-    parts += n_parts;
-    split_tiles += n_split;
   }
-  if (threadIdx.x == 0) p.head[0] = make_int4(items, v.bad, split_tiles, 0);
+  __syncthreads();
+  if (threadIdx.x == 0) p.head[0] = make_int4(p.ordered ? items : sh.start[kPlanBuckets], v.bad, sh.split_tiles, 0);
 }
 
 // Work index i (of items * heads) -> item and head: bucket by bucket, inside a
