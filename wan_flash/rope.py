@@ -96,7 +96,7 @@ def _rope_impl(q, k, positions, table, axes, inverse):
     q, q0, q1, q2 = _rows(q, size)
     k, k0, k1, k2 = _rows(k, size)
     positions = positions.contiguous()
-    if not table.is_contiguous() or table.data_ptr() % 8:
+    if not table.is_contiguous() or table.data_ptr() % 16:
         table = table.clone(memory_format=torch.contiguous_format)
     cfg = _lib.RopeCfg(0 if size == 2 else 1, 1 if inverse else 0, table.shape[0], axes[0] // 2, axes[1] // 2, 0,
                        q0, q1, q2, k0, k1, k2, 3 * s if len(ps) == 3 else 0)
