@@ -194,7 +194,8 @@ typedef struct wf_rope_cfg {
 int wf_rope(const void* q, const void* k, void* q_out, void* k_out, const float* table, const int* positions, int b,
             int s, int h, int h_kv, const wf_rope_cfg* cfg, void* stream);
 
-/* Shape of the paged cache of wf_decode; strides in elements, multiples of 8. */
+/* Shape of the paged cache of wf_decode; strides in elements, multiples of 8.
+   K and V may span 2^35 elements (64 GiB) each. */
 typedef struct wf_decode_cfg {
   int n_pages;            /* pages of the cache                               */
   int page_size;          /* tokens of a page, >= 1                           */

@@ -72,6 +72,8 @@ def test_c_entry_refusals():
 
     assert call(b=-1) == -1 and call(h=3) == -1 and call(page_size=0) == -1 and call(q=None) == -1
     assert call(q=24) == -3 and call(k_slot_stride=130) == -3 and call(max_pages=2**30, page_size=2) == -2
+    assert call(v_head_stride=-8) == -2 and call(k_page_stride=2**36) == -2
+    assert call(n_pages=2**20, k_page_stride=2**16) == -2  # 128 GiB
     assert call(b=0) == 0
     assert lib.wf_decode_workspace(4, 3, ctypes.byref(ctypes.c_size_t())) == -1
 

@@ -13,6 +13,14 @@
 // padded beyond 8 heads.  tcgen05's M of 64-128 rows would leave the tensor
 // pipe as idle and add a trip through tensor memory.
 //
+// Loads: 16-byte cp.async into per-warp rings, 16 lanes to a row of 256 bytes.
+// Lane j of a warp finds the page of token j of the next tile and hands its
+// place round as a 32-bit count of 16-byte units, so a row costs a shuffle and
+// a multiply-add.  (64-bit places cost 900 instructions a 16-token tile, which
+// bounded the kernel: eight warps an SM do not hide that many dependent ones.
+// One 256-byte bulk copy per lane cost 512 and no less time: bulk copies take
+// their addresses one lane after the other.)
+//
 // Split: the work is cut by tiles of 64 tokens, not by sequences.  The tiles
 // of all (sequence, key-value head[, block of heads]) rows stand one behind
 // the other and every CTA takes an equal run of them, whatever the lengths;
@@ -29,12 +37,13 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 64;                       // tokens of a CTA's tile: 16 per warp
 constexpr int kStages = 3;                      // per-warp ring of 16-token K and V tiles
-constexpr uint32_t kHalfBytes = 16 * 256;       // 16 tokens of K (or V)
+constexpr uint32_t kRowBytes = 256 + 16;        // a token's 128 dims; 16 bytes more spread ldmatrix over the banks
+constexpr uint32_t kHalfBytes = 16 * kRowBytes; // 16 tokens of K (or V)
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
-constexpr uint32_t kRingBytes = kWarps * kStages * kStageBytes;  // 96 KB; the join reuses it
+constexpr uint32_t kRingBytes = kWarps * kStages * kStageBytes;  // 102 KB; the join reuses it
 constexpr int kMaxHeads = 32;                   // q heads of a row (4 n-tiles of 8)
 constexpr uint32_t kOffML = kRingBytes;         // [warp][head] running max, then sum
-constexpr uint32_t kSmemBytes = kRingBytes + 2 * kWarps * kMaxHeads * 4 + 64;
+constexpr uint32_t kSmemBytes = kOffML + 2 * kWarps * kMaxHeads * 4;
 constexpr int kCtasPerSm = 2;
 constexpr int kOPitch = 132;                    // floats per head in the join buffer (128 + 4 against bank conflicts)
 static_assert(kWarps * kMaxHeads * kOPitch * 4 <= kRingBytes, "the join buffer fits in the ring");
@@ -44,7 +53,7 @@ struct DecodeParams {
   const __nv_bfloat16* q;    // (b, h, 128)
   const __nv_bfloat16* k;
   const __nv_bfloat16* v;
-  long long page_stride[2], slot_stride[2], head_stride[2];  // K, V, in elements
+  unsigned page_stride[2], slot_stride[2], head_stride[2];  // K, V, in units of 16 bytes
   const int* page_table;
   long long table_stride;
   const int* lengths;
@@ -62,9 +71,12 @@ struct DecodeParams {
 
 namespace {
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  // src-size 0: the 16 bytes become zeros and src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  // bytes 0: the 16 bytes become zeros and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -113,7 +125,7 @@ __device__ __forceinline__ int decode_tiles(int len) { return (len + dec::kTile 
 template <int kN>
 __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kernel(DecodeParams p) {
   using namespace dec;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kWarps + 1];
   __shared__ long long s_start[2];  // tiles before the first sequence of this CTA's run; that sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -221,43 +233,59 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
       }
     }
 
-    // This warp's tokens of tile t: 64 t + 16 warp + [0, 16).  Lane j < 16
-    // finds token j's page; the row's 16 chunks of 16 bytes are copied by 16
-    // lanes, chunk c to place c ^ (row & 7) (ldmatrix without bank conflicts).
+    // This warp's tokens of tile t: 64 t + 16 warp + [0, 16).  Lane j (and 16 + j)
+    // steps token j through the pages tile by tile; lanes 0-15 (16-31) copy the
+    // 16-byte chunks of the even (odd) rows.
     const int* table = p.page_table + (long long)seq * p.table_stride;
+    const char* const src_k = reinterpret_cast<const char*>(p.k) + ((long long)kvh * p.head_stride[0] + (lane & 15)) * 16;
+    const char* const src_v = reinterpret_cast<const char*>(p.v) + ((long long)kvh * p.head_stride[1] + (lane & 15)) * 16;
+    const int step_pages = kTile / p.page_size, step_slots = kTile - step_pages * p.page_size;
+    int tok = t0 * kTile + warp * 16 + (lane & 15);  // of the next tile to send for
+    int pg = tok / p.page_size, slot = tok - pg * p.page_size;
+    const int last = min(len, t1 * kTile);           // tokens of this run
+    int page = tok < last ? __ldg(table + pg) : 0;
     bool bad = false;
-    auto slot_of = [&](int t) -> int2 {  // (page, slot) of this lane's token; page -1 behind the end, -2 on a bad entry
-      const int tok = t * kTile + warp * 16 + (lane & 15);
-      if (t >= t1 || tok >= len) return make_int2(-1, 0);
-      const int pg = tok / p.page_size;
-      const int page = __ldg(table + pg);
-      if (page < 0 || page >= p.n_pages) return make_int2(-2, page);
-      return make_int2(page, tok - pg * p.page_size);
-    };
-    auto load = [&](int stage, int2 at_) {
-      if (at_.x == -2) {
+    const uint32_t dst0 = ring + (lane >> 4) * kRowBytes + (lane & 15) * 16;
+    auto load = [&](int stage) {
+      const bool there = tok < last;
+      const bool ok = there && page >= 0 && page < p.n_pages;
+      if (there && !ok) {
         bad = true;
         if (atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
           g_err_info[0] = (unsigned)seq;
-          g_err_info[1] = (unsigned)at_.y;
+          g_err_info[1] = (unsigned)page;
           g_err_info[2] = kRoleDecode;
           g_err_info[3] = 2u;
         }
       }
-      const uint32_t dst = ring + stage * kStageBytes;
-      const int c = lane & 15;
+      const unsigned at_k = (unsigned)page * p.page_stride[0] + (unsigned)slot * p.slot_stride[0];
+      const unsigned at_v = (unsigned)page * p.page_stride[1] + (unsigned)slot * p.slot_stride[1];
+      const unsigned here = __ballot_sync(0xffffffffu, ok);
+      const uint32_t dst = dst0 + stage * kStageBytes;
+      if (here == 0xffffffffu) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 2 * i + (lane >> 4);
-        const int page = __shfl_sync(0xffffffffu, at_.x, r), slot = __shfl_sync(0xffffffffu, at_.y, r);
-        const bool ok = page >= 0;
-        const uint32_t d = dst + r * 256 + ((c ^ (r & 7)) << 4);
-        const __nv_bfloat16* ks = p.k + (ok ? page * p.page_stride[0] + slot * p.slot_stride[0] : 0) + kvh * p.head_stride[0];
-        const __nv_bfloat16* vs = p.v + (ok ? page * p.page_stride[1] + slot * p.slot_stride[1] : 0) + kvh * p.head_stride[1];
-        cp_async16(d, ks + c * 8, ok);
-        cp_async16(d + kHalfBytes, vs + c * 8, ok);
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * i + (lane >> 4);
+          const unsigned ak = __shfl_sync(0xffffffffu, at_k, r), av = __shfl_sync(0xffffffffu, at_v, r);
+          cp_async16(dst + i * 2 * kRowBytes, src_k + (unsigned long long)ak * 16);
+          cp_async16(dst + i * 2 * kRowBytes + kHalfBytes, src_v + (unsigned long long)av * 16);
+        }
+      } else {  // rows behind the end (and of bad pages) become zeros: 0 * NaN would reach the V product
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * i + (lane >> 4);
+          const unsigned ak = __shfl_sync(0xffffffffu, at_k, r), av = __shfl_sync(0xffffffffu, at_v, r);
+          const bool row_ok = (here >> r) & 1;
+          cp_async16(dst + i * 2 * kRowBytes, src_k + (row_ok ? (unsigned long long)ak * 16 : 0), row_ok ? 16 : 0);
+          cp_async16(dst + i * 2 * kRowBytes + kHalfBytes, src_v + (row_ok ? (unsigned long long)av * 16 : 0), row_ok ? 16 : 0);
+        }
       }
       cp_async_commit();
+      tok += kTile;
+      pg += step_pages;
+      slot += step_slots;
+      if (slot >= p.page_size) slot -= p.page_size, ++pg;
+      page = tok < last ? __ldg(table + pg) : 0;
     };
 
     float m[kN][2], l[kN][2], acc[kN][8][4];
@@ -270,21 +298,17 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[n][d][i] = 0.f;
     }
-    for (int s = 0; s < kStages - 1; ++s) load(s, slot_of(t0 + s));
-    int2 next = slot_of(t0 + kStages - 1);
-    int stage = 0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) load(i);
+    int stage = kStages - 1, fill = kStages - 2;
     for (int t = t0; t < t1; ++t) {
       cp_async_wait<kStages - 2>();
       __syncwarp();
-      {
-        // refill the stage that the previous step read (every lane is past it)
-        int fill = stage + kStages - 1;
-        if (fill >= kStages) fill -= kStages;
-        load(fill, next);
-        next = slot_of(t + kStages);
-      }
-      const uint32_t sk = ring + stage * kStageBytes, sv = sk + kHalfBytes;
       if (++stage == kStages) stage = 0;
+      // refill the stage that the previous step read (every lane is past it)
+      if (++fill == kStages) fill = 0;
+      load(fill);
+      const uint32_t sk = ring + stage * kStageBytes, sv = sk + kHalfBytes;
       const int tok0 = t * kTile + warp * 16;
       if (tok0 >= len) continue;  // this warp has no token in the row's last tile
       // S^T (16 tokens x 8 heads per n-tile)
@@ -297,7 +321,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
         for (int ks = 0; ks < 8; ++ks) {
           const int c = 2 * ks + (lane >> 4);              // matrices 2, 3: dims 8-15 of the step
           uint32_t a[4];
-          ldmatrix_x4(sk + r * 256 + ((c ^ (r & 7)) << 4), a);
+          ldmatrix_x4(sk + r * kRowBytes + (c << 4), a);
 #pragma unroll
           for (int n = 0; n < kN; ++n) mma_16816(s[n], a, qf[n][ks][0], qf[n][ks][1]);
         }
@@ -348,7 +372,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
         for (int d = 0; d < 8; ++d) {
           const int c = 2 * d + ((lane >> 3) & 1);         // matrices 1, 3: dims 8-15 of the tile
           uint32_t a[4];
-          ldmatrix_x4_trans(sv + r * 256 + ((c ^ (r & 7)) << 4), a);
+          ldmatrix_x4_trans(sv + r * kRowBytes + (c << 4), a);
 #pragma unroll
           for (int n = 0; n < kN; ++n) mma_16816(acc[n][d], a, pb[n][0], pb[n][1]);
         }
@@ -394,7 +418,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
     }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == n_tiles;
-    const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+    const int part = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
     // thread = 4 dims of a head; a warp writes one head's 128
     for (int hd = warp; hd < n_heads; hd += kWarps) {
       float top = s_m[hd];
@@ -418,7 +442,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
         *reinterpret_cast<uint2*>(p.o + out * 128 + lane * 4) = w2;
         if (lane == 0) p.lse[out] = (top + log2f(sum)) * 0.69314718055994531f;
       } else {
-        const long long out = (long long)slot * p.heads_per_row + hd;
+        const long long out = (long long)part * p.heads_per_row + hd;
         *reinterpret_cast<float4*>(p.part_o + out * 128 + lane * 4) = x;
         if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + out * 2) = make_float2(top, sum);
       }
@@ -553,6 +577,17 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
   if ((long long)cfg->page_size * cfg->max_pages > 0x7fffffffLL - 1024)
     return fail(WF_ERR_UNSUPPORTED, "max_pages * page_size = %lld tokens exceed 2^31 - 1025",
                 (long long)cfg->page_size * cfg->max_pages);
+  for (long long x : {cfg->k_page_stride, cfg->k_slot_stride, cfg->k_head_stride, cfg->v_page_stride, cfg->v_slot_stride,
+                      cfg->v_head_stride})
+    if (x < 0 || x >= (8LL << 32))
+      return fail(WF_ERR_UNSUPPORTED, "cache stride of %lld elements outside [0, 2^35)", x);
+  // places within a cache are 32-bit counts of 16 bytes
+  for (int i = 0; i < 2; ++i) {
+    const double reach = (double)cfg->n_pages * (double)(i ? cfg->v_page_stride : cfg->k_page_stride) +
+                         (double)cfg->page_size * (double)(i ? cfg->v_slot_stride : cfg->k_slot_stride);
+    if (reach >= 8.0 * 4294967296.0)
+      return fail(WF_ERR_UNSUPPORTED, "a cache of %.3g elements exceeds 2^35 (64 GiB)", reach);
+  }
   if (b == 0 || h == 0) return WF_OK;
   DecodeParams p;
   int rc, dev;
@@ -573,8 +608,9 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
   p.k = reinterpret_cast<const __nv_bfloat16*>(k_cache);
   p.v = reinterpret_cast<const __nv_bfloat16*>(v_cache);
-  p.page_stride[0] = cfg->k_page_stride, p.slot_stride[0] = cfg->k_slot_stride, p.head_stride[0] = cfg->k_head_stride;
-  p.page_stride[1] = cfg->v_page_stride, p.slot_stride[1] = cfg->v_slot_stride, p.head_stride[1] = cfg->v_head_stride;
+  p.page_stride[0] = (unsigned)(cfg->k_page_stride / 8), p.page_stride[1] = (unsigned)(cfg->v_page_stride / 8);
+  p.slot_stride[0] = (unsigned)(cfg->k_slot_stride / 8), p.slot_stride[1] = (unsigned)(cfg->v_slot_stride / 8);
+  p.head_stride[0] = (unsigned)(cfg->k_head_stride / 8), p.head_stride[1] = (unsigned)(cfg->v_head_stride / 8);
   p.page_table = page_table;
   p.table_stride = cfg->table_stride;
   p.lengths = lengths;
