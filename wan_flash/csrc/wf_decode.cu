@@ -36,17 +36,29 @@ namespace dec {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 64;                       // tokens of a CTA's tile: 16 per warp
-constexpr int kStages = 3;                      // per-warp ring of 16-token K and V tiles
 constexpr uint32_t kRowBytes = 256 + 16;        // a token's 128 dims; 16 bytes more spread ldmatrix over the banks
 constexpr uint32_t kHalfBytes = 16 * kRowBytes; // 16 tokens of K (or V)
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
-constexpr uint32_t kRingBytes = kWarps * kStages * kStageBytes;  // 102 KB; the join reuses it
 constexpr int kMaxHeads = 32;                   // q heads of a row (4 n-tiles of 8)
-constexpr uint32_t kOffML = kRingBytes;         // [warp][head] running max, then sum
-constexpr uint32_t kSmemBytes = kOffML + 2 * kWarps * kMaxHeads * 4;
-constexpr int kCtasPerSm = 2;
+// Per-warp ring of 16-token K and V tiles, and CTAs per SM, for rows of kN x 8
+// heads.  8 heads: 12 warps with one tile ahead beat 8 with two (48 ragged
+// streams 138 us against 140, 75600-token caches 221 against 228); more heads
+// need more registers than 12 warps have.  From 24 heads on q is read from
+// shared memory tile by tile: its fragments (64 registers at 32 heads) spilled.
+template <int kN>
+struct Shape {
+  static constexpr int kStages = kN == 1 ? 2 : 3;
+  static constexpr int kCtasPerSm = kN == 1 ? 3 : 2;
+  static constexpr bool kQShared = kN >= 3;
+  static constexpr uint32_t kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr uint32_t kOffML = kRingBytes;  // [warp][head] running max, then sum
+  static constexpr uint32_t kOffQ = kOffML + 2 * kWarps * kMaxHeads * 4;
+  static constexpr uint32_t kSmemBytes = kOffQ + (kQShared ? kN * 8 * kRowBytes : 0);
+  static_assert(kCtasPerSm * (kSmemBytes + 2048) <= 233472, "the CTAs of an SM fit in its shared memory");
+};
+constexpr int ctas_per_sm(int heads_per_row) { return heads_per_row <= 8 ? Shape<1>::kCtasPerSm : Shape<2>::kCtasPerSm; }
 constexpr int kOPitch = 132;                    // floats per head in the join buffer (128 + 4 against bank conflicts)
-static_assert(kWarps * kMaxHeads * kOPitch * 4 <= kRingBytes, "the join buffer fits in the ring");
+static_assert(16 * kOPitch * 4 <= kStageBytes, "a round of the join fits in a stage");
 }  // namespace dec
 
 struct DecodeParams {
@@ -119,12 +131,41 @@ __device__ __forceinline__ int decode_length(const DecodeParams& p, int seq) {
 }
 __device__ __forceinline__ int decode_tiles(int len) { return (len + dec::kTile - 1) / dec::kTile; }
 
+// A CTA's run of one row: tiles [t0, t1) of (sequence, key-value head, block of heads).
+struct DecodeRun {
+  int seq, len, n_tiles, row, t0, t1;
+  long long seq_at;  // tiles before the sequence
+  long long row_at;  // tiles before the row
+};
+
+// The run that starts at tile `at` < hi; r holds the run before it, or the
+// sequence to look from.  False where the lengths changed under the call.
+__device__ bool decode_next_run(const DecodeParams& p, int rows_per_seq, long long at, long long hi, DecodeRun& r) {
+  r.len = decode_length(p, r.seq);
+  r.n_tiles = decode_tiles(r.len);
+  while (at >= r.seq_at + (long long)r.n_tiles * rows_per_seq) {
+    if (r.seq + 1 >= p.b) return false;
+    r.seq_at += (long long)r.n_tiles * rows_per_seq;
+    ++r.seq;
+    r.len = decode_length(p, r.seq);
+    r.n_tiles = decode_tiles(r.len);
+  }
+  r.row = (int)((at - r.seq_at) / r.n_tiles);
+  r.row_at = r.seq_at + (long long)r.row * r.n_tiles;
+  r.t0 = (int)(at - r.row_at);
+  r.t1 = (int)min((long long)r.n_tiles, hi - r.row_at);
+  return true;
+}
+
 }  // namespace
 
 // kN: n-tiles of 8 q heads that a row has.
 template <int kN>
-__global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
+    wf_decode_kernel(DecodeParams p) {
   using namespace dec;
+  constexpr int kStages = Shape<kN>::kStages;
+  constexpr bool kQShared = Shape<kN>::kQShared;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kWarps + 1];
   __shared__ long long s_start[2];  // tiles before the first sequence of this CTA's run; that sequence
@@ -195,64 +236,51 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
   }
 
   const uint32_t ring = sbase + warp * (kStages * kStageBytes);
-  float* const s_m = reinterpret_cast<float*>(smem + kOffML);
+  float* const s_m = reinterpret_cast<float*>(smem + Shape<kN>::kOffML);
   float* const s_l = s_m + kWarps * kMaxHeads;
-  float* const s_o = reinterpret_cast<float*>(smem);
   int4 join = make_int4(-1, 0, 0, 0);
 
-  int seq = (int)s_start[1];
-  long long seq_at = s_start[0];  // tiles before this sequence
-  for (long long at = lo; at < hi;) {
-    int len = decode_length(p, seq);
-    int n_tiles = decode_tiles(len);
-    while (at >= seq_at + (long long)n_tiles * rows_per_seq && seq + 1 < p.b) {
-      seq_at += (long long)n_tiles * rows_per_seq;
-      ++seq;
-      len = decode_length(p, seq);
-      n_tiles = decode_tiles(len);
+  // ---- the loader: this warp's tokens of the CTA's tiles one after the other,
+  // two tiles ahead of the products and on into the next rows.  Of tile t a
+  // warp has tokens 64 t + 16 warp + [0, 16); lane j (and 16 + j) steps token j
+  // through the pages; lanes 0-15 (16-31) copy the 16-byte chunks of the even
+  // (odd) rows.
+  DecodeRun ahead;
+  ahead.seq = (int)s_start[1];
+  ahead.seq_at = s_start[0];
+  long long ahead_at = lo;
+  const int* table = nullptr;
+  const char* src_k = nullptr;
+  const char* src_v = nullptr;
+  const int step_pages = kTile / p.page_size, step_slots = kTile - step_pages * p.page_size;
+  int tok = 0, last = 0, pg = 0, slot = 0, page = 0;
+  auto open_run = [&]() {
+    if (!decode_next_run(p, rows_per_seq, ahead_at, hi, ahead)) {
+      ahead_at = hi;
+      last = 0;
+      return;
     }
-    if (at >= seq_at + (long long)n_tiles * rows_per_seq) break;  // lengths changed under the call
-    const int row = (int)((at - seq_at) / n_tiles);        // (key-value head, block of heads) of the sequence
-    const long long row_at = seq_at + (long long)row * n_tiles;
-    const int t0 = (int)(at - row_at);
-    const int t1 = (int)min((long long)n_tiles, hi - row_at);
-    const int kvh = row / p.blocks;
-    const int head0 = kvh * p.group + (row - kvh * p.blocks) * p.heads_per_row;
-    const int n_heads = min(p.heads_per_row, (kvh + 1) * p.group - head0);
-
-    // q as the B operand of S^T = K q^T: lane holds head lane/4, dims 16 ks + 2 (lane%4) + {0, 1, 8, 9}
-    uint32_t qf[kN][8][2];
-#pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const int hd = n * 8 + (lane >> 2);
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((long long)seq * p.h + head0 + hd) * 128) + (lane & 3);
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        qf[n][ks][0] = hd < n_heads ? __ldg(src + ks * 8) : 0u;
-        qf[n][ks][1] = hd < n_heads ? __ldg(src + ks * 8 + 4) : 0u;
-      }
-    }
-
-    // This warp's tokens of tile t: 64 t + 16 warp + [0, 16).  Lane j (and 16 + j)
-    // steps token j through the pages tile by tile; lanes 0-15 (16-31) copy the
-    // 16-byte chunks of the even (odd) rows.
-    const int* table = p.page_table + (long long)seq * p.table_stride;
-    const char* const src_k = reinterpret_cast<const char*>(p.k) + ((long long)kvh * p.head_stride[0] + (lane & 15)) * 16;
-    const char* const src_v = reinterpret_cast<const char*>(p.v) + ((long long)kvh * p.head_stride[1] + (lane & 15)) * 16;
-    const int step_pages = kTile / p.page_size, step_slots = kTile - step_pages * p.page_size;
-    int tok = t0 * kTile + warp * 16 + (lane & 15);  // of the next tile to send for
-    int pg = tok / p.page_size, slot = tok - pg * p.page_size;
-    const int last = min(len, t1 * kTile);           // tokens of this run
-    int page = tok < last ? __ldg(table + pg) : 0;
+    const int kvh = ahead.row / p.blocks;
+    table = p.page_table + (long long)ahead.seq * p.table_stride;
+    src_k = reinterpret_cast<const char*>(p.k) + ((long long)kvh * p.head_stride[0] + (lane & 15)) * 16;
+    src_v = reinterpret_cast<const char*>(p.v) + ((long long)kvh * p.head_stride[1] + (lane & 15)) * 16;
+    tok = ahead.t0 * kTile + warp * 16 + (lane & 15);  // of the next tile to send for
+    last = min(ahead.len, ahead.t1 * kTile);
+    pg = tok / p.page_size;
+    slot = tok - pg * p.page_size;
+    page = tok < last ? __ldg(table + pg) : 0;
+  };
+  open_run();
+  const uint32_t dst0 = ring + (lane >> 4) * kRowBytes + (lane & 15) * 16;
+  auto load = [&](int stage) -> bool {  // whether the tile had a bad page
     bool bad = false;
-    const uint32_t dst0 = ring + (lane >> 4) * kRowBytes + (lane & 15) * 16;
-    auto load = [&](int stage) {
+    if (ahead_at < hi) {
       const bool there = tok < last;
       const bool ok = there && page >= 0 && page < p.n_pages;
       if (there && !ok) {
         bad = true;
         if (atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
-          g_err_info[0] = (unsigned)seq;
+          g_err_info[0] = (unsigned)ahead.seq;
           g_err_info[1] = (unsigned)page;
           g_err_info[2] = kRoleDecode;
           g_err_info[3] = 2u;
@@ -280,14 +308,56 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
           cp_async16(dst + i * 2 * kRowBytes + kHalfBytes, src_v + (row_ok ? (unsigned long long)av * 16 : 0), row_ok ? 16 : 0);
         }
       }
-      cp_async_commit();
-      tok += kTile;
-      pg += step_pages;
-      slot += step_slots;
-      if (slot >= p.page_size) slot -= p.page_size, ++pg;
-      page = tok < last ? __ldg(table + pg) : 0;
-    };
+      if (++ahead_at < ahead.row_at + ahead.t1) {
+        tok += kTile;
+        pg += step_pages;
+        slot += step_slots;
+        if (slot >= p.page_size) slot -= p.page_size, ++pg;
+        page = tok < last ? __ldg(table + pg) : 0;
+      } else if (ahead_at < hi) {
+        open_run();
+      }
+    }
+    cp_async_commit();
+    return bad;
+  };
+  // bad pages of the tiles in flight, one bit a stage
+  unsigned bad_stage = 0;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i)
+    if (load(i)) bad_stage |= 1u << i;
+  int stage = kStages - 1, fill = kStages - 2;
 
+  DecodeRun run;
+  run.seq = (int)s_start[1];
+  run.seq_at = s_start[0];
+  for (long long at = lo; at < hi;) {
+    if (!decode_next_run(p, rows_per_seq, at, hi, run)) break;
+    const int kvh = run.row / p.blocks;
+    const int head0 = kvh * p.group + (run.row - kvh * p.blocks) * p.heads_per_row;
+    const int n_heads = min(p.heads_per_row, (kvh + 1) * p.group - head0);
+
+    // q as the B operand of S^T = K q^T: lane holds head lane/4, dims 16 ks + 2 (lane%4) + {0, 1, 8, 9}
+    uint32_t qf[kQShared ? 1 : kN][8][2];
+    const uint4* const q_rows = reinterpret_cast<const uint4*>(p.q + ((long long)run.seq * p.h + head0) * 128);
+    if constexpr (kQShared) {
+      for (int i = threadIdx.x; i < kN * 8 * 16; i += kThreads) {
+        const uint4 x = i < n_heads * 16 ? __ldg(q_rows + i) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(smem + Shape<kN>::kOffQ + (i >> 4) * kRowBytes + (i & 15) * 16) = x;
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const int hd = n * 8 + (lane >> 2);
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(q_rows + hd * 16) + (lane & 3);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          qf[n][ks][0] = hd < n_heads ? __ldg(src + ks * 8) : 0u;
+          qf[n][ks][1] = hd < n_heads ? __ldg(src + ks * 8 + 4) : 0u;
+        }
+      }
+    }
     float m[kN][2], l[kN][2], acc[kN][8][4];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
@@ -298,41 +368,61 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[n][d][i] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) load(i);
-    int stage = kStages - 1, fill = kStages - 2;
-    for (int t = t0; t < t1; ++t) {
+    bool bad = false;
+    for (int t = run.t0; t < run.t1; ++t) {
       cp_async_wait<kStages - 2>();
       __syncwarp();
       if (++stage == kStages) stage = 0;
+      if (bad_stage >> stage & 1) bad = true;
       // refill the stage that the previous step read (every lane is past it)
       if (++fill == kStages) fill = 0;
-      load(fill);
+      bad_stage &= ~(1u << fill);
+      if (load(fill)) bad_stage |= 1u << fill;
       const uint32_t sk = ring + stage * kStageBytes, sv = sk + kHalfBytes;
       const int tok0 = t * kTile + warp * 16;
-      if (tok0 >= len) continue;  // this warp has no token in the row's last tile
-      // S^T (16 tokens x 8 heads per n-tile)
-      float s[kN][4];
+      if (tok0 >= run.len) continue;  // this warp has no token in the row's last tile
+      // S^T (16 tokens x 8 heads per n-tile); up to 16 heads in two chains of four
+      // products (with more the heads' own chains overlap)
+      float s[kN][4], s2[kN][4];
 #pragma unroll
-      for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
       {
         const int r = (lane & 7) + ((lane >> 3) & 1) * 8;  // matrices 0, 2: tokens 0-7; 1, 3: tokens 8-15
+        const uint32_t row = sk + r * kRowBytes + ((lane >> 4) << 4);  // matrices 2, 3: dims 8-15 of the step
+        if constexpr (kQShared) {
+          const uint32_t sq = sbase + Shape<kN>::kOffQ + (lane & 7) * kRowBytes + ((lane >> 3) << 4);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const int c = 2 * ks + (lane >> 4);              // matrices 2, 3: dims 8-15 of the step
-          uint32_t a[4];
-          ldmatrix_x4(sk + r * kRowBytes + (c << 4), a);
+          for (int ks = 0; ks < 8; ks += 2) {
+            uint32_t a0[4], a1[4];
+            ldmatrix_x4(row + ks * 32, a0);
+            ldmatrix_x4(row + ks * 32 + 32, a1);
 #pragma unroll
-          for (int n = 0; n < kN; ++n) mma_16816(s[n], a, qf[n][ks][0], qf[n][ks][1]);
+            for (int n = 0; n < kN; ++n) {
+              uint32_t b[4];  // the head tile's fragments of steps ks and ks + 1
+              ldmatrix_x4(sq + n * 8 * kRowBytes + ks * 32, b);
+              mma_16816(s[n], a0, b[0], b[1]);
+              mma_16816(s[n], a1, b[2], b[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            uint32_t a[4];
+            ldmatrix_x4(row + ks * 32, a);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma_16816((ks & 1) ? s2[n] : s[n], a, qf[n][ks][0], qf[n][ks][1]);
+          }
         }
       }
       // online softmax over the tokens: rows lane/4 and lane/4 + 8, heads 2 (lane%4) + {0, 1}
-      const bool in0 = tok0 + (lane >> 2) < len, in1 = tok0 + (lane >> 2) + 8 < len;
+      const bool in0 = tok0 + (lane >> 2) < run.len, in1 = tok0 + (lane >> 2) + 8 < run.len;
       uint32_t pb[kN][2];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = (i < 2 ? in0 : in1) ? s[n][i] * p.scale_log2 : -INFINITY;
+        for (int i = 0; i < 4; ++i) s[n][i] = (i < 2 ? in0 : in1) ? (kQShared ? s[n][i] : s[n][i] + s2[n][i]) * p.scale_log2 : -INFINITY;
         float pr[4];
         float f[2];
 #pragma unroll
@@ -360,27 +450,27 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
         }
         // P^T (tokens x heads) to the B operand of O^T = V^T P^T: 8x8
         // transposes within the warp.  P is rounded to bf16 for the tensor
-        // core (relative 2^-9, the rounding that o itself gets); the sum l
-        // keeps the fp32 values.
+        // core (half a step, 2^-8 of the value at most, the rounding that o
+        // itself gets); the sum l keeps the fp32 values.
         pb[n][0] = movmatrix_trans(pack_bf16(pr[0], pr[1]));
         pb[n][1] = movmatrix_trans(pack_bf16(pr[2], pr[3]));
       }
       // O^T (16 dims x 8 heads) += V^T P^T
       {
         const int r = (lane & 7) + (lane >> 4) * 8;        // matrices 0, 1: tokens 0-7; 2, 3: tokens 8-15
+        const uint32_t row = sv + r * kRowBytes + (((lane >> 3) & 1) << 4);  // matrices 1, 3: dims 8-15 of the tile
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          const int c = 2 * d + ((lane >> 3) & 1);         // matrices 1, 3: dims 8-15 of the tile
           uint32_t a[4];
-          ldmatrix_x4_trans(sv + r * kRowBytes + (c << 4), a);
+          ldmatrix_x4_trans(row + d * 32, a);
 #pragma unroll
           for (int n = 0; n < kN; ++n) mma_16816(acc[n][d], a, pb[n][0], pb[n][1]);
         }
       }
     }
-    cp_async_wait<0>();
     bad = __any_sync(0xffffffffu, bad);
-    // ---- join the four warps' results
+    // ---- join the four warps' results.  Each warp's O goes through its ring's
+    // stage that was read last (the others hold the next tiles): 16 heads a round.
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -390,74 +480,78 @@ __global__ void __launch_bounds__(dec::kThreads, dec::kCtasPerSm) wf_decode_kern
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         if (bad) x = __int_as_float(0x7fffffff);
-        l[n][e] = x;
         if (lane < 4) {
           s_m[warp * kMaxHeads + n * 8 + 2 * lane + e] = m[n][e];
           s_l[warp * kMaxHeads + n * 8 + 2 * lane + e] = x;
         }
       }
-    __syncthreads();  // every warp is past its ring: it becomes the join buffer
+    __syncthreads();
+    const bool whole = run.t0 == 0 && run.t1 == run.n_tiles;
+    const int part = 2 * blockIdx.x + (run.t0 == 0 ? 1 : 0);
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      float f[2];
+    for (int n0 = 0; n0 < kN; n0 += 2) {
+      float* const s_o = reinterpret_cast<float*>(smem + stage * kStageBytes);
+      constexpr int kWarpFloats = kStages * kStageBytes / 4;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int hd = n * 8 + 2 * (lane & 3) + e;
+      for (int n = n0; n < (n0 + 2 < kN ? n0 + 2 : kN); ++n) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int hd = n * 8 + 2 * (lane & 3) + e;
+          float top = s_m[hd];
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * kMaxHeads + hd]);
+          f[e] = ex2_approx(m[n][e] - (top == -INFINITY ? 0.f : top));
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s_o[warp * kWarpFloats + ((n - n0) * 8 + 2 * (lane & 3) + (i & 1)) * kOPitch + d * 16 + (lane >> 2) +
+                (i >> 1) * 8] = acc[n][d][i] * f[i & 1];
+      }
+      __syncthreads();
+      // thread = 4 dims of a head; a warp writes one head's 128
+      for (int hd = n0 * 8 + warp; hd < min(n_heads, n0 * 8 + 16); hd += kWarps) {
         float top = s_m[hd];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * kMaxHeads + hd]);
-        f[e] = ex2_approx(m[n][e] - (top == -INFINITY ? 0.f : top));
-      }
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int d = 0; d < 8; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int hd = n * 8 + 2 * (lane & 3) + (i & 1);
-          s_o[(warp * (8 * kN) + hd) * kOPitch + d * 16 + (lane >> 2) + (i >> 1) * 8] = acc[n][d][i] * f[i & 1];
+        for (int w = 0; w < kWarps; ++w) {
+          sum += s_l[w * kMaxHeads + hd] * ex2_approx(s_m[w * kMaxHeads + hd] - ref);
+          const float4 y = *reinterpret_cast<const float4*>(s_o + w * kWarpFloats + (hd - n0 * 8) * kOPitch + lane * 4);
+          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
         }
-    }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == n_tiles;
-    const int part = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
-    // thread = 4 dims of a head; a warp writes one head's 128
-    for (int hd = warp; hd < n_heads; hd += kWarps) {
-      float top = s_m[hd];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * kMaxHeads + hd]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        sum += s_l[w * kMaxHeads + hd] * ex2_approx(s_m[w * kMaxHeads + hd] - ref);
-        const float4 y = *reinterpret_cast<const float4*>(s_o + (w * (8 * kN) + hd) * kOPitch + lane * 4);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        if (whole) {
+          const float inv = 1.f / sum;  // a row with tokens has a sum >= 1 (or NaN)
+          uint2 w2;
+          w2.x = pack_bf16(x.x * inv, x.y * inv);
+          w2.y = pack_bf16(x.z * inv, x.w * inv);
+          const long long out = (long long)run.seq * p.h + head0 + hd;
+          *reinterpret_cast<uint2*>(p.o + out * 128 + lane * 4) = w2;
+          if (lane == 0) p.lse[out] = (top + log2f(sum)) * 0.69314718055994531f;
+        } else {
+          const long long out = (long long)part * p.heads_per_row + hd;
+          *reinterpret_cast<float4*>(p.part_o + out * 128 + lane * 4) = x;
+          if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + out * 2) = make_float2(top, sum);
+        }
       }
-      if (whole) {
-        const float inv = 1.f / sum;  // a row with tokens has a sum >= 1 (or NaN)
-        uint2 w2;
-        w2.x = pack_bf16(x.x * inv, x.y * inv);
-        w2.y = pack_bf16(x.z * inv, x.w * inv);
-        const long long out = (long long)seq * p.h + head0 + hd;
-        *reinterpret_cast<uint2*>(p.o + out * 128 + lane * 4) = w2;
-        if (lane == 0) p.lse[out] = (top + log2f(sum)) * 0.69314718055994531f;
-      } else {
-        const long long out = (long long)part * p.heads_per_row + hd;
-        *reinterpret_cast<float4*>(p.part_o + out * 128 + lane * 4) = x;
-        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + out * 2) = make_float2(top, sum);
-      }
+      __syncthreads();  // the join's stage is read: the next round, or the loader, may write it
     }
-    if (t0 == 0 && t1 < n_tiles) {
-      // the CTA whose run holds tile row_at + n_tiles - 1 ends the row
-      const long long last = row_at + n_tiles - 1;
-      long long e = (last * ctas) / total;
-      while (total * (e + 1) / ctas <= last) ++e;
-      while (total * e / ctas > last) --e;
-      join = make_int4(head0, n_heads, (int)e, seq);
+    if (run.t0 == 0 && run.t1 < run.n_tiles) {
+      // the CTA whose run holds the row's last tile ends it
+      const long long end = run.row_at + run.n_tiles - 1;
+      long long e = (end * ctas) / total;
+      while (total * (e + 1) / ctas <= end) ++e;
+      while (total * e / ctas > end) --e;
+      join = make_int4(head0, n_heads, (int)e, run.seq);
     }
-    __syncthreads();  // the join buffer is read: the ring may be filled again
-    at = row_at + t1;
+    at = run.row_at + run.t1;
   }
+  cp_async_wait<0>();
   if (threadIdx.x == 0) p.join[blockIdx.x] = join;
 }
 
@@ -531,7 +625,8 @@ int decode_rows(int h, int h_kv, int* blocks, int* heads_per_row) {
 
 template <int kN>
 int decode_launch(const DecodeParams& p, int ctas, cudaStream_t st) {
-  wf_decode_kernel<kN><<<ctas, dec::kThreads, dec::kSmemBytes, st>>>(p);
+  using dec::Shape;
+  wf_decode_kernel<kN><<<ctas, dec::kThreads, Shape<kN>::kSmemBytes, st>>>(p);
   int rc = launch_check("wf_decode launch");
   if (rc) return rc;
   cudaError_t e = launch_ex(wf_decode_join_kernel, dim3(ctas, std::min(p.heads_per_row, 8)), dim3(256), 0, st, true, 1u, p);
@@ -548,10 +643,13 @@ size_t decode_workspace_bytes(int ctas, int heads_per_row) {
 
 // One-time per-device set-up (from device_setup, with that device current).
 cudaError_t decode_setup() {
-  cudaError_t e = cudaSuccess;
-  for (auto k : {wf_decode_kernel<1>, wf_decode_kernel<2>, wf_decode_kernel<3>, wf_decode_kernel<4>})
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec::kSmemBytes);
+  auto smem = [](auto* k, uint32_t bytes) {
+    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  };
+  cudaError_t e = smem(wf_decode_kernel<1>, dec::Shape<1>::kSmemBytes);
+  if (e == cudaSuccess) e = smem(wf_decode_kernel<2>, dec::Shape<2>::kSmemBytes);
+  if (e == cudaSuccess) e = smem(wf_decode_kernel<3>, dec::Shape<3>::kSmemBytes);
+  if (e == cudaSuccess) e = smem(wf_decode_kernel<4>, dec::Shape<4>::kSmemBytes);
   return e;
 }
 }  // namespace wf
@@ -562,7 +660,7 @@ extern "C" int wf_decode_workspace(int h, int h_kv, size_t* bytes) {
   int blocks, heads, dev, rc;
   if ((rc = decode_rows(h, h_kv, &blocks, &heads))) return rc;
   if ((rc = device_setup(&dev))) return rc;
-  *bytes = decode_workspace_bytes(g_dev_sms[dev] * dec::kCtasPerSm, heads);
+  *bytes = decode_workspace_bytes(g_dev_sms[dev] * dec::ctas_per_sm(heads), heads);
   return WF_OK;
 }
 
@@ -601,7 +699,7 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
       cfg->k_head_stride % 8 || cfg->v_page_stride % 8 || cfg->v_slot_stride % 8 || cfg->v_head_stride % 8)
     return fail(WF_ERR_MISALIGNED, "q/k_cache/v_cache/o/workspace and the caches' strides must be multiples of 16 bytes");
   if ((rc = device_setup(&dev))) return rc;
-  const int ctas = g_dev_sms[dev] * dec::kCtasPerSm;
+  const int ctas = g_dev_sms[dev] * dec::ctas_per_sm(p.heads_per_row);
   const size_t need = decode_workspace_bytes(ctas, p.heads_per_row);
   if (workspace_bytes < need)
     return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
