@@ -58,17 +58,20 @@ def assert_close(got, want, tol, tag):
         f"{tag}: off by {over.max().item():.3e} more than allowed, at {int(over.argmax())}"
 
 
-def grads64(q, k, v, do, causal=False):
+def grads64(q, k, v, do, causal=False, residual=False):
     """dq, dk, dv of o = attention(q, k, v) given do, by the formulas in 64 bits, with their bounds.
 
     Errors of a kernel, entry by entry: P off by e = 4 es relative (its exponent: score and lse) and rounded to bf16
-    (U) before dV = P^T do; dP = do v^T an fp32 sum; D = rowsum(o do) from the o that was rounded (o_tol); dS = P (dP -
+    (U) before dV = P^T do; dP = do v^T an fp32 sum; D = rowsum(o do) from the o that was rounded
+    (o_tol; with its residual only o's error before that rounding, and its square); dS = P (dP -
     D) rounded to bf16 (U) before dQ and dK; fp32 sums over rows or keys; one rounding of the result."""
     r = attn64(q, k, v, causal)
     g, lq, lk = q.shape[1] // k.shape[1], q.shape[0], k.shape[0]
     x, y, z, t = (a.double().transpose(0, 1) for a in (q, k, v, do))
     y, z = y.repeat_interleave(g, 0), z.repeat_interleave(g, 0)
     p, o, o_tol = r["p"], r["o"].transpose(0, 1), r["o_tol"].transpose(0, 1)
+    if residual:
+        o_tol = o_tol - U * o.abs() + U * U * (o.abs() + o_tol)
     e = 4 * r["es"][..., None] + 16 * E32
     dp = t @ z.transpose(1, 2)
     delta = (t * o).sum(-1, keepdim=True)

@@ -222,7 +222,7 @@ def test_c_entry_refusals():
 
     def call(q=16, n=2, tq=8, tk=8, h=4, hk=2, causal=0, ws=1 << 20):
         p = ctypes.c_void_p
-        return lib.wf_packed_fwd(p(q) if q else None, p(16), p(16), p(16), p(16), p(16), p(16), p(16), ws, n, tq, tk, h, hk,
+        return lib.wf_packed_fwd(p(q) if q else None, *[p(16)] * 8, ws, n, tq, tk, h, hk,
                                  causal, None)
 
     assert call(n=-1) == -1 and call(h=3) == -1 and call(hk=0) == -1 and call(causal=2) == -1 and call(q=None) == -1

@@ -5,7 +5,7 @@ sequences, graphs, and refusals."""
 import pytest
 import torch
 
-from tests.attn64 import assert_close, attn64, grads64
+from tests.attn64 import U, assert_close, attn64, grads64
 from tests.test_packed import CASES, make, offsets
 from wan_flash import _lib, features
 from wan_flash.packed import wan_flash_attn_packed, wan_flash_packed_bwd, wan_flash_packed_fwd
@@ -17,14 +17,14 @@ def _reset_features():
     features.reset()
 
 
-def check_bwd(q, k, v, do, qo, ko, causal, dq, dk, dv):
+def check_bwd(q, k, v, do, qo, ko, causal, dq, dk, dv, residual=False):
     qo, ko = qo.tolist(), ko.tolist()
     for i in range(len(qo) - 1):
         a, b, c, d = qo[i], qo[i + 1], ko[i], ko[i + 1]
         if a == b or c == d:
             assert (dq[a:b] == 0).all() and (dk[c:d] == 0).all() and (dv[c:d] == 0).all()
             continue
-        want = grads64(q[a:b], k[c:d], v[c:d], do[a:b], causal)
+        want = grads64(q[a:b], k[c:d], v[c:d], do[a:b], causal, residual)
         for name, got in (("dq", dq[a:b]), ("dk", dk[c:d]), ("dv", dv[c:d])):
             assert_close(got, *want[name], f"{name} of sequence {i}")
     for x, off in ((dq, qo), (dk, ko), (dv, ko)):
@@ -97,6 +97,28 @@ def test_a_sequence_does_not_see_its_neighbours():
     for g, w in zip(grads(), want):
         assert torch.equal(g[:200], w[:200]) and torch.equal(g[277:], w[277:])
         assert g[200:277].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,h,hk,causal", CASES)
+def test_residual_of_o(lq, lk, h, hk, causal):
+    """o + residual is o to 16 bits, and with it dq and dk do not carry o's rounding through D."""
+    q, k, v, do, qo, ko = make(lq, lk or lq, h, hk, 2, 130)
+    o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal, residual=True)
+    plain, plain_lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    assert torch.equal(o, plain) and torch.equal(lse, plain_lse)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal, o_residual=res)
+    _lib.check_device()
+    check_bwd(q, k, v, do, qo, ko, causal, *grads, residual=True)
+    qo, ko = qo.tolist(), ko.tolist()
+    for i in range(len(qo) - 1):
+        a, b, c, d = qo[i], qo[i + 1], ko[i], ko[i + 1]
+        if a < b:
+            r = attn64(q[a:b], k[c:d], v[c:d], causal)
+            # p's rounding stays; o's own step (2^-8) becomes its square
+            tol = r["o_tol"] - U * r["o"].abs() + U * U * (r["o"].abs() + r["o_tol"])
+            assert_close(o[a:b].double() + res[a:b].double(), r["o"], tol, f"o + residual of sequence {i}")
+    assert (res[:qo[0]] == 0).all() and (res[qo[-1]:] == 0).all()
 
 
 @pytest.mark.gpu
@@ -175,7 +197,7 @@ def test_c_entry_refuses_a_small_workspace():
     lib, cfg, size = _lib.lib(), _lib.PackedBwdCfg(0, 0), ctypes.c_size_t()
     assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, ctypes.byref(cfg), ctypes.byref(size)) == 0
     p = ctypes.c_void_p
-    assert lib.wf_packed_bwd(*[p(16)] * 12, size.value - 1, 2, 8, 8, 4, 2, 0, ctypes.byref(cfg), None) == -1
+    assert lib.wf_packed_bwd(*[p(16)] * 13, size.value - 1, 2, 8, 8, 4, 2, 0, ctypes.byref(cfg), None) == -1
 
 
 @pytest.mark.gpu
@@ -224,7 +246,7 @@ def test_c_entry_refusals():
     def call(n=2, tq=8, tk=8, h=4, hk=2, causal=0, nsplit=1, ws=1 << 30, q=16):
         c = _lib.PackedBwdCfg(nsplit, 0)
         p = ctypes.c_void_p
-        return lib.wf_packed_bwd(p(q) if q else None, *[p(16)] * 11, ws, n, tq, tk, h, hk, causal, ctypes.byref(c), None)
+        return lib.wf_packed_bwd(p(q) if q else None, *[p(16)] * 12, ws, n, tq, tk, h, hk, causal, ctypes.byref(c), None)
 
     assert call(n=-1) == -1 and call(hk=3) == -1 and call(nsplit=-1) == -1 and call(nsplit=2000) == -1 and call(causal=3) == -1 and call(q=None) == -1
     assert call(q=8) == -3 and call(tq=0) == -2 and call(tk=0) == -2

@@ -106,6 +106,7 @@ struct PackedFwdParams {
   const PackedFwdTile* tiles;
   int* counter;             // items drawn beyond the first of every CTA; the plan sets it to 0
   __nv_bfloat16* o;
+  __nv_bfloat16* res;       // what rounding o to bf16 took away, like o; or null
   float* lse;               // (h, total_q)
   int total_q, h, group, causal;
   float scale_log2, rescale_threshold;

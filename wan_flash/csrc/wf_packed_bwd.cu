@@ -35,10 +35,11 @@
 
 namespace wf {
 
-// Preprocess: D = rowsum(o * dO), -lse * log2(e), and the zeroed dQ
+// Preprocess: D = rowsum((o + residual) * dO), -lse * log2(e), and the zeroed dQ
 // accumulator.  Bound: HBM (1036 bytes per row and head).  grid (2 * tiles,
 // h), 256 threads: 64 rows of one tile, 16 threads per row.
 __global__ void __launch_bounds__(256) wf_packed_pre_kernel(PackedBwdParams p, const __nv_bfloat16* __restrict__ o,
+                                                            const __nv_bfloat16* __restrict__ res,
                                                             const __nv_bfloat16* __restrict__ dO,
                                                             const float* __restrict__ lse) {
   griddep_launch_dependents();
@@ -58,6 +59,10 @@ __global__ void __launch_bounds__(256) wf_packed_pre_kernel(PackedBwdParams p, c
       const uint4 a = ldg_u4(o + off);
       const uint4 c = ldg_u4(dO + off);
       acc = bf16_dot2(a.x, c.x) + bf16_dot2(a.y, c.y) + bf16_dot2(a.z, c.z) + bf16_dot2(a.w, c.w);
+      if (res != nullptr) {
+        const uint4 b = ldg_u4(res + off);
+        acc += bf16_dot2(b.x, c.x) + bf16_dot2(b.y, c.y) + bf16_dot2(b.z, c.z) + bf16_dot2(b.w, c.w);
+      }
     }
 #pragma unroll
     for (int m = 8; m >= 1; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);

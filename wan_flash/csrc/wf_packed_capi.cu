@@ -104,25 +104,26 @@ extern "C" int wf_packed_fwd_workspace(int n, int total_q, size_t* bytes) {
 }
 
 extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets,
-                             void* o, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q,
-                             int total_k, int h, int h_kv, int causal, void* stream) {
+                             void* o, void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n,
+                             int total_q, int total_k, int h, int h_kv, int causal, void* stream) {
   int rc = packed_check(n, total_q, total_k, h, h_kv, causal);
   if (rc) return rc;
   if (total_q == 0 || h == 0) return WF_OK;
   if (!q || !o || !lse || !q_offsets || !k_offsets || !workspace || (total_k > 0 && (!k || !v)))
     return fail(WF_ERR_INVALID_ARG, "null pointer");
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(workspace) ||
-      (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(q_offsets) & 3) ||
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_residual) ||
+      !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(q_offsets) & 3) ||
       (reinterpret_cast<uintptr_t>(k_offsets) & 3))
-    return fail(WF_ERR_MISALIGNED, "q/k/v/o/workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
+    return fail(WF_ERR_MISALIGNED, "q/k/v/o/o_residual/workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
   const PackedFwdWorkspace ws(n, total_q);
   if (workspace_bytes < ws.bytes)
     return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
   int dev;
   if ((rc = device_setup(&dev))) return rc;
-  CUtensorMap mq, mk, mv, mo;
+  CUtensorMap mq, mk, mv, mo, mr;
   // with no keys at all nothing is loaded: q stands in for the maps of k and v
   if ((rc = make_bshd_map(&mq, q, 1, total_q, h)) || (rc = make_bshd_map(&mo, o, 1, total_q, h)) ||
+      (rc = make_bshd_map(&mr, o_residual ? o_residual : o, 1, total_q, h)) ||
       (rc = make_bshd_map(&mk, total_k ? k : q, 1, total_k ? total_k : total_q, total_k ? h_kv : h)) ||
       (rc = make_bshd_map(&mv, total_k ? v : q, 1, total_k ? total_k : total_q, total_k ? h_kv : h)))
     return rc;
@@ -141,6 +142,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.tiles = pp.fwd_tiles;
   p.counter = &pp.head->w;
   p.o = reinterpret_cast<__nv_bfloat16*>(o);
+  p.res = reinterpret_cast<__nv_bfloat16*>(o_residual);
   p.lse = lse;
   p.total_q = total_q, p.h = h, p.group = h / h_kv, p.causal = causal;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
@@ -148,7 +150,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   const long long items = packed_max_tiles(total_q, n, 256) * h;
   const int grid = (int)std::min<long long>(items, g_dev_sms[dev]);
   cudaError_t e = launch_ex(wf_packed_fwd_kernel, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
-                            mk, mv, mo, p);
+                            mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
   return launch_check("wf_packed_fwd launch");
 }
@@ -163,8 +165,8 @@ extern "C" int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, i
   return WF_OK;
 }
 
-extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                             const void* dO, const int* q_offsets, const int* k_offsets, void* dq, void* dk, void* dv,
+extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o,
+                             const void* o_residual, const float* lse, const void* dO, const int* q_offsets, const int* k_offsets, void* dq, void* dk, void* dv,
                              void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv,
                              int causal, const wf_packed_bwd_cfg* cfg, void* stream) {
   int rc;
@@ -174,7 +176,7 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
     return fail(WF_ERR_UNSUPPORTED, "no queries or no keys: the caller must zero the gradients");
   if (!q || !k || !v || !o || !lse || !dO || !q_offsets || !k_offsets || !dq || !dk || !dv || !workspace)
     return fail(WF_ERR_INVALID_ARG, "null pointer");
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dO) || !aligned16(dq) ||
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_residual) || !aligned16(dO) || !aligned16(dq) ||
       !aligned16(dk) || !aligned16(dv) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) ||
       (reinterpret_cast<uintptr_t>(q_offsets) & 3) || (reinterpret_cast<uintptr_t>(k_offsets) & 3))
     return fail(WF_ERR_MISALIGNED, "tensors and workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
@@ -232,7 +234,8 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   wf_packed_plan_kernel<<<2, kPlanThreads, 0, st>>>(pp);
   if ((rc = launch_check("wf_packed plan launch"))) return rc;
   e = launch_ex(wf_packed_pre_kernel, dim3((unsigned)(2 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, p,
-                reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(dO), lse);
+                reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(o_residual),
+                reinterpret_cast<const __nv_bfloat16*>(dO), lse);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd preprocess launch");
   e = launch_ex(wf_packed_bwd_kernel, dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true,
                 1u, mq, mk, mv, mdo, p);

@@ -34,6 +34,11 @@
 //             select), for V 0 * NaN is not: the MMA warp zeroes those rows of
 //             the box in shared memory before its product.  Short O tiles are
 //             copied out row by row instead of by tensor store.
+//   residual  For training, what rounding o to bf16 took away is written too
+//             (bf16): the backward's D = rowsum(o * dO) then has 16 bits of o.
+//             In rows with few keys the error of an 8-bit o in D is as large as
+//             dS's own rounding (dq 1.7 times the error of one rounding, 1.4 with
+//             the residual); it costs 256 bytes a row and head each way.
 #include "wf_common.cuh"
 #include "wf_kernels.h"
 
@@ -59,11 +64,13 @@ constexpr int kBarPFull = kBarSFull + 2;           // + 2 * tile + half
 constexpr int kBarOFull = kBarPFull + 4;           // + tile
 constexpr int kBarDrain = kBarOFull + 2;
 constexpr int kBarOStaged = kBarDrain + 1;
-// A stage use n is freed on barrier n & 1: a warpgroup that waits for use n - 1
-// may not have seen use n - 2 freed, and one barrier's parity could not tell them apart.
-constexpr int kBarOStageFree = kBarOStaged + 1;    // + use & 1
+// A stage use n is freed on barrier n & 3: a warpgroup that waits for use n - 1
+// may not have seen the uses before it freed (up to two of the other warpgroup
+// and its own last), and one barrier's parity could not tell them apart.  Its
+// own last use but one is always freed, so four barriers can.
+constexpr int kBarOStageFree = kBarOStaged + 1;    // + use & 3
 constexpr int kItemSlots = 4;
-constexpr int kBarItemFull = kBarOStageFree + 2;         // + slot
+constexpr int kBarItemFull = kBarOStageFree + 4;         // + slot
 constexpr int kBarItemEmpty = kBarItemFull + kItemSlots; // + slot; one arrival per reader
 constexpr int kItemReaders = 11;                         // 8 softmax warps, MMA, TMA, store
 constexpr int kBarItemNext = kBarItemEmpty + kItemSlots; // the TMA warp is at its item's last block
@@ -100,7 +107,7 @@ __device__ __forceinline__ void packed_zero_rows(uint32_t tile, int first) {
 __global__ void __launch_bounds__(pfwd::kThreads, 1)
     wf_packed_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
-                         PackedFwdParams p) {
+                         const __grid_constant__ CUtensorMap tm_res, PackedFwdParams p) {
   using namespace pfwd;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -121,6 +128,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       mbar_init(bar(kBarPFull + 2 * t + 1), 4);
       mbar_init(bar(kBarOFull + t), 1);
       mbar_init(bar(kBarOStageFree + t), 1);
+      mbar_init(bar(kBarOStageFree + 2 + t), 1);
     }
     for (int s = 0; s < kKvSlots; ++s) {
       mbar_init(bar(kBarKvFull + s), 1);
@@ -144,6 +152,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  const int passes = p.res != nullptr ? 2 : 1;  // o, and what its rounding took away
   // a programmatic dependent of the plan kernel: its lists are read from here on
   griddep_wait();
   // The k-th item of this CTA, for a whole warp (or, one = true, for one thread
@@ -195,29 +204,33 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       const PackedFwdTile& w = x.w;
       const int h = x.h;
       if (w.n_blocks == 0) continue;
-      for (int t = 0; t * 128 < w.rows; ++t, ++n) {
+      const int stores = (w.rows > 128 ? 2 : 1) * passes;
+      for (int i = 0; i < stores; ++i, ++n) {
+        const int t = i / passes;
+        const bool res = i - t * passes != 0;
         ok = mbar_wait_warp(bar(kBarOStaged), (uint32_t)n & 1, abort_flag, kRoleStore, 50 + t);
         if (!ok) break;
         const int rows = w.rows - t * 128;
         if (rows >= 128) {
           if (lane == 0) {
             for (int c = 0; c < 2; ++c)
-              tma_store_4d(&tm_o, sbase + kOffOStage + c * kBoxBytes, c * 64, w.q0 + t * 128, h, 0);
+              tma_store_4d(res ? &tm_res : &tm_o, sbase + kOffOStage + c * kBoxBytes, c * 64, w.q0 + t * 128, h, 0);
             bulk_commit_group();
             bulk_wait_read_all();
           }
         } else {
           // rows behind the sequence's end belong to the next one: copy the
           // valid ones, two rows of 16 chunks per pass
+          __nv_bfloat16* const out = res ? p.res : p.o;
           const int c = lane & 15;
           for (int r = lane >> 4; r < rows; r += 2) {
             const uint4 v = *reinterpret_cast<const uint4*>(smem + kOffOStage + (c >> 3) * kBoxBytes +
                                                             sw128_offset((uint32_t)r, (uint32_t)(c & 7)));
-            *reinterpret_cast<uint4*>(p.o + ((size_t)(w.q0 + t * 128 + r) * p.h + h) * 128 + c * 8) = v;
+            *reinterpret_cast<uint4*>(out + ((size_t)(w.q0 + t * 128 + r) * p.h + h) * 128 + c * 8) = v;
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kBarOStageFree + (n & 1)));
+        if (lane == 0) mbar_arrive(bar(kBarOStageFree + (n & 3)));
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -406,13 +419,16 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         // nothing to attend (or rows outside any sequence): o = 0, lse = -inf;
         // NaN where the offsets were impossible
         const uint32_t fill = bad ? 0x7fff7fffu : 0u;
-        for (int i = (int)threadIdx.x; i < w.rows * 16; i += 256)
-          st_global_v4(p.o + ((size_t)(w.q0 + (i >> 4)) * p.h + h) * 128 + (i & 15) * 8, fill, fill, fill, fill);
+        for (int i = (int)threadIdx.x; i < w.rows * 16; i += 256) {
+          const size_t at = ((size_t)(w.q0 + (i >> 4)) * p.h + h) * 128 + (i & 15) * 8;
+          st_global_v4(p.o + at, fill, fill, fill, fill);
+          if (passes == 2) st_global_v4(p.res + at, fill, fill, fill, fill);
+        }
         if (row < w.rows) p.lse[(size_t)h * p.total_q + w.q0 + row] = bad ? __int_as_float(0x7fffffff) : -INFINITY;
         continue;
       }
-      const int use = stage_use + t;
-      stage_use += w.rows > 128 ? 2 : 1;
+      const int use0 = stage_use + t * passes;
+      stage_use += (w.rows > 128 ? 2 : 1) * passes;
       if (t * 128 >= w.rows) continue;
       const int seen = p.causal ? min(max(w.off + row, 0), w.klen) : w.klen;  // keys that this row sees
       float m_s = -INFINITY;  // running reference max, in scaled log2 units
@@ -487,30 +503,39 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       ++o_waits;
       tc_fence_after();
       const float inv = 1.f / l;
-      if (use > 0)
-        ok = mbar_wait(bar(kBarOStageFree + ((use - 1) & 1)), (uint32_t)((use - 1) >> 1) & 1, abort_flag, role, 45 + t);
-      if (!ok) break;
       const uint32_t stage = sbase + kOffOStage + (uint32_t)r * 128u;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + c * 32, o);
-        tmem_wait_ld();
-        reg_fence32(o);
-        uint32_t pk[16];
+      for (int pass = 0; pass < passes; ++pass) {
+        const int use = use0 + pass;
+        if (use > 0)
+          ok = mbar_wait(bar(kBarOStageFree + ((use - 1) & 3)), (uint32_t)((use - 1) >> 2) & 1, abort_flag, role, 45 + t);
+        if (!ok) break;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+          uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          pk[i] = l == 0.f ? 0u : pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          for (int i = 0; i < 16; ++i) {
+            const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
+            uint32_t v = pack_bf16(x, y);
+            if (pass) v = pack_bf16(x - __uint_as_float(v << 16), y - __uint_as_float(v & 0xffff0000u));
+            pk[i] = l == 0.f ? 0u : v;
+          }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const uint32_t chunk = (uint32_t)((c & 1) * 4 + v);
-          st_shared_v4(stage + (uint32_t)(c >> 1) * kBoxBytes + ((chunk ^ ((uint32_t)r & 7u)) << 4), pk[4 * v],
-                       pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+          for (int v = 0; v < 4; ++v) {
+            const uint32_t chunk = (uint32_t)((c & 1) * 4 + v);
+            st_shared_v4(stage + (uint32_t)(c >> 1) * kBoxBytes + ((chunk ^ ((uint32_t)r & 7u)) << 4), pk[4 * v],
+                         pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+          }
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBarOStaged));
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kBarOStaged));
+      if (!ok) break;
       if (row < w.rows)
         p.lse[(size_t)h * p.total_q + w.q0 + row] = l == 0.f ? -INFINITY : (m_s + log2f(l)) * 0.69314718055994531f;
     }

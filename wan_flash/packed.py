@@ -1,8 +1,8 @@
 """Attention over packed sequences of different lengths: grouped heads, causal
 or not, forward and backward.
 
-wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets=None, causal=False) -> (o, lse)
-wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets=None, causal=False) -> (dq, dk, dv)
+wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets=None, causal=False) -> (o, lse[, o_residual])
+wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets=None, causal=False, o_residual=None) -> (dq, dk, dv)
 wan_flash_attn_packed(q, k, v, q_offsets, k_offsets=None, causal=False) -> o   (autograd)
 
   q, o, do, dq  (total_q, h, 128) bf16: the sequences' rows one behind the other
@@ -70,28 +70,35 @@ def _bwd_cfg_bytes(index: int, n: int, total_q: int, total_k: int, h: int, h_kv:
 
 
 def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
-                         k_offsets: torch.Tensor | None = None, causal: bool = False):
-    """(o, lse) of attention over packed sequences; see the module's text."""
+                         k_offsets: torch.Tensor | None = None, causal: bool = False, residual: bool = False):
+    """(o, lse) of attention over packed sequences; see the module's text.
+
+    residual: also return what rounding o to bf16 took away, (o, lse, o_residual), for
+    wan_flash_packed_bwd: its row sums of o * do are then free of that rounding, which
+    shows in the gradients of rows with few keys."""
     k_offsets = q_offsets if k_offsets is None else k_offsets
     total_q, total_k, h, h_kv, n, device = _check(q, k, v, q_offsets, k_offsets)
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     q_offsets, k_offsets = q_offsets.contiguous(), k_offsets.contiguous()
     o = torch.empty_like(q)
+    o_residual = torch.empty_like(q) if residual else None
     lse = torch.empty((h, total_q), device=device, dtype=torch.float32)
+    out = (o, lse, o_residual) if residual else (o, lse)
     if total_q == 0 or h == 0:
-        return o, lse
+        return out
     size = _fwd_bytes(n, total_q)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
     _launch(_lib.lib().wf_packed_fwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
-            k_offsets.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, n, total_q, total_k, h, h_kv,
-            1 if causal else 0)
-    return o, lse
+            k_offsets.data_ptr(), o.data_ptr(), o_residual.data_ptr() if residual else None, lse.data_ptr(),
+            ws.data_ptr(), size, n, total_q, total_k, h, h_kv, 1 if causal else 0)
+    return out
 
 
 def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                          do: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor | None = None,
-                         causal: bool = False):
-    """(dq, dk, dv) given the forward's o and lse and the gradient of o.
+                         causal: bool = False, o_residual: torch.Tensor | None = None):
+    """(dq, dk, dv) given the forward's o and lse (and o_residual, if it made one) and
+    the gradient of o.
 
     dk and dv are bitwise reproducible; dq is accumulated with fp32 reductions
     unless ``features.set_bwd_overrides(deterministic=True)``.  ``nsplit`` of the
@@ -102,6 +109,9 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     assert o.dtype is torch.bfloat16 and do.dtype is torch.bfloat16 and o.shape == q.shape and do.shape == q.shape
     assert lse.dtype is torch.float32 and lse.shape == (h, total_q)
     assert o.device == device and lse.device == device and do.device == device, "tensors must be on one CUDA device"
+    if o_residual is not None:
+        assert o_residual.dtype is torch.bfloat16 and o_residual.shape == q.shape and o_residual.device == device
+        o_residual = _aligned(o_residual)
     q, k, v, o, do, lse = _aligned(q), _aligned(k), _aligned(v), _aligned(o), _aligned(do), lse.contiguous()
     q_offsets, k_offsets = q_offsets.contiguous(), k_offsets.contiguous()
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -110,8 +120,8 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     f = features.get_bwd()
     cfg, size = _bwd_cfg_bytes(device.index, n, total_q, total_k, h, h_kv, f.nsplit, f.deterministic)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
-    _launch(_lib.lib().wf_packed_bwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-            do.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    _launch(_lib.lib().wf_packed_bwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+            None if o_residual is None else o_residual.data_ptr(), lse.data_ptr(), do.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             ws.data_ptr(), size, n, total_q, total_k, h, h_kv, 1 if causal else 0, cfg)
     return dq, dk, dv
 
@@ -119,19 +129,22 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
 class _WanFlashAttnPackedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_offsets, k_offsets, causal):
-        o, lse = wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal)
-        ctx.save_for_backward(q, k, v, o, lse, q_offsets, k_offsets)
+        o, lse, o_residual = wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal, residual=True)
+        ctx.save_for_backward(q, k, v, o, lse, o_residual, q_offsets, k_offsets)
         ctx.causal = causal
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse, q_offsets, k_offsets = ctx.saved_tensors
-        dq, dk, dv = wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, ctx.causal)
+        q, k, v, o, lse, o_residual, q_offsets, k_offsets = ctx.saved_tensors
+        dq, dk, dv = wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, ctx.causal, o_residual)
         return dq, dk, dv, None, None, None
 
 
 def wan_flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                           k_offsets: torch.Tensor | None = None, causal: bool = False):
     """Differentiable attention over packed sequences -> o (total_q, h, 128) bf16."""
-    return _WanFlashAttnPackedFn.apply(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, bool(causal))
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WanFlashAttnPackedFn.apply(q, k, v, q_offsets, k_offsets, bool(causal))
+    return wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal)[0]
