@@ -23,14 +23,26 @@ attention) has the same treatment:
     wan_flash::attn_bwd_dual(q, k0, v0, k1, v1, o0, lse0, o1, lse1, do0, do1)
         -> (dq, dk0, dv0, dk1, dv1)
 
-and ``wan_attention_dual(q, k0, v0, k1, v1) -> o0 + o1``.
+and ``wan_attention_dual(q, k0, v0, k1, v1) -> o0 + o1``.  So have rotary
+positions, packed attention and decode:
+
+    wan_flash::rope(q, k, positions, table, axes, inverse) -> (q_rot, k_rot)
+    wan_flash::packed_fwd(q, k, v, q_offsets, k_offsets, causal) -> (o, lse, o_residual)
+    wan_flash::packed_bwd(q, k, v, o, lse, o_residual, do, q_offsets, k_offsets, causal)
+        -> (dq, dk, dv)
+    wan_flash::decode(q, k_cache, v_cache, page_table, lengths) -> (o, lse)
+
+with ``wan_rope``, ``wan_attention_packed`` (differentiable) and ``wan_decode``.
 """
 
 from __future__ import annotations
 
 import torch
 
+from wan_flash.decode import wan_flash_decode
 from wan_flash.interface import wan_flash_bwd, wan_flash_bwd_dual, wan_flash_fwd, wan_flash_fwd_dual
+from wan_flash.packed import wan_flash_packed_bwd, wan_flash_packed_fwd
+from wan_flash.rope import AXES, _rope_impl
 
 
 @torch.library.custom_op("wan_flash::attn_fwd", mutates_args=())
@@ -136,3 +148,101 @@ def wan_attention_dual(q: torch.Tensor, k0: torch.Tensor, v0: torch.Tensor, k1: 
     """attention(q, k0, v0) + attention(q, k1, v1) through the registered operators (differentiable)."""
     o0, _, o1, _ = attn_fwd_dual(q, k0, v0, k1, v1)
     return o0 + o1
+
+
+@torch.library.custom_op("wan_flash::rope", mutates_args=())
+def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, axes: list[int],
+         inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _rope_impl(q, k, positions, table, axes, inverse)
+
+
+@rope.register_fake
+def _rope_fake(q, k, positions, table, axes, inverse):
+    torch._check(q.shape[-1] == 128, lambda: "specialized for head_dim=128")
+    return _like(q), _like(k)
+
+
+def _setup_context_rope(ctx, inputs, output):
+    _, _, positions, table, axes, inverse = inputs
+    ctx.save_for_backward(positions, table)
+    ctx.axes, ctx.inverse = axes, inverse
+
+
+def _backward_rope(ctx, gq, gk):
+    gq, gk = rope(gq, gk, *ctx.saved_tensors, ctx.axes, not ctx.inverse)
+    return gq, gk, None, None, None, None
+
+
+rope.register_autograd(_backward_rope, setup_context=_setup_context_rope)
+
+
+def wan_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, axes=AXES):
+    """wan_flash_rope through the registered operator (differentiable)."""
+    return rope(q, k, positions, table, list(axes), False)
+
+
+@torch.library.custom_op("wan_flash::packed_fwd", mutates_args=())
+def packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
+               causal: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal, residual=True)
+
+
+@packed_fwd.register_fake
+def _packed_fwd_fake(q, k, v, q_offsets, k_offsets, causal):
+    total_q, h, d = q.shape
+    torch._check(d == 128, lambda: "specialized for head_dim=128")
+    return _like(q), q.new_empty((h, total_q), dtype=torch.float32), _like(q)
+
+
+@torch.library.custom_op("wan_flash::packed_bwd", mutates_args=())
+def packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+               o_residual: torch.Tensor, do: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
+               causal: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, causal, o_residual)
+
+
+@packed_bwd.register_fake
+def _packed_bwd_fake(q, k, v, o, lse, o_residual, do, q_offsets, k_offsets, causal):
+    return _like(q), _like(k), _like(v)
+
+
+def _setup_context_packed(ctx, inputs, output):
+    q, k, v, q_offsets, k_offsets, causal = inputs
+    o, lse, o_residual = output
+    ctx.mark_non_differentiable(lse, o_residual)  # as in the dense op
+    ctx.save_for_backward(q, k, v, o, lse, o_residual, q_offsets, k_offsets)
+    ctx.causal = causal
+
+
+def _backward_packed(ctx, do, dlse, dres):
+    q, k, v, o, lse, o_residual, q_offsets, k_offsets = ctx.saved_tensors
+    grads = packed_bwd(q, k, v, o, lse, o_residual, do.contiguous(), q_offsets, k_offsets, ctx.causal)
+    return *grads, None, None, None
+
+
+packed_fwd.register_autograd(_backward_packed, setup_context=_setup_context_packed)
+
+
+def wan_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
+                         k_offsets: torch.Tensor | None = None, causal: bool = False) -> torch.Tensor:
+    """wan_flash_attn_packed through the registered operator (differentiable)."""
+    return packed_fwd(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, causal)[0]
+
+
+@torch.library.custom_op("wan_flash::decode", mutates_args=())
+def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+           lengths: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return wan_flash_decode(q, k_cache, v_cache, page_table, lengths)
+
+
+@decode.register_fake
+def _decode_fake(q, k_cache, v_cache, page_table, lengths):
+    b, h, d = q.shape
+    torch._check(d == 128, lambda: "specialized for head_dim=128")
+    return _like(q), q.new_empty((b, h), dtype=torch.float32)
+
+
+def wan_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+               lengths: torch.Tensor) -> torch.Tensor:
+    """o of wan_flash_decode through the registered operator."""
+    return decode(q, k_cache, v_cache, page_table, lengths)[0]

@@ -111,10 +111,25 @@ def _default_attn():
     return wan_flash_attn
 
 
-def ulysses_self_attention(q, k, v, group=None, attn_fn: Callable | None = None):
+def _default_rope():
+    from wan_flash.rope import wan_flash_rope
+
+    return wan_flash_rope
+
+
+def ulysses_self_attention(q, k, v, group=None, attn_fn: Callable | None = None, rope=None,
+                           rope_fn: Callable | None = None):
     """Self-attention over sequence-sharded (b, S/P, H, D) q/k/v; returns
-    the sequence-sharded output.  Differentiable."""
+    the sequence-sharded output.  Differentiable.
+
+    rope: (positions, table) of this rank's shard turns q and k by their rotary
+    positions before the exchange, where a rank holds all heads of its tokens:
+    positions of tokens [r S/P, (r + 1) S/P) of the grid, as
+    wan_flash.rope.rope_positions(grid, start=r * (S // P), count=S // P) makes
+    them.  rope_fn defaults to wan_flash_rope (tests inject a CPU reference)."""
     attn_fn = attn_fn or _default_attn()
+    if rope is not None:
+        q, k = (rope_fn or _default_rope())(q, k, *rope)
     qh = _SeqToHead.apply(q, group)
     kh = _SeqToHead.apply(k, group)
     vh = _SeqToHead.apply(v, group)
