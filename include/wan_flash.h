@@ -228,8 +228,8 @@ int wf_decode(const void* q, const void* k_cache, const void* v_cache, const int
               void* o, float* lse, void* workspace, size_t workspace_bytes, int b, int h, int h_kv,
               const wf_decode_cfg* cfg, void* stream);
 
-/* Bytes of workspace of wf_packed_fwd for n sequences in total_q query rows. */
-int wf_packed_fwd_workspace(int n, int total_q, size_t* bytes);
+/* Bytes of workspace of wf_packed_fwd on the current device. */
+int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, size_t* bytes);
 
 /*
  * Forward attention over n packed sequences (no reference counterpart): rows
@@ -244,15 +244,16 @@ int wf_packed_fwd_workspace(int n, int total_q, size_t* bytes);
  * everywhere and WF_ERR_INVALID_ARG from wf_device_status.
  * o_residual (like o; NULL: none) receives what rounding o to bf16 took away,
  * for the backward.
- * Two launches; overlapping calls need workspaces of their own.
+ * Two launches (three where few query rows may have their walks cut into pieces,
+ * added in a fixed order); overlapping calls need workspaces of their own.
  */
 int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, void* o,
                   void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,
                   int h_kv, int causal, void* stream);
 
 typedef struct wf_packed_bwd_cfg {
-  int nsplit;        /* 0 = the device cuts long walks into pieces of about a
-                        third of an SM's share; n > 0: pieces of 1/n of the
+  int nsplit;        /* 0 = the device cuts long walks into pieces (about three
+                        per SM, one where there are few key tiles); n > 0: pieces of 1/n of the
                         longest walk.  Pieces leave fp32 partial dk and dv that
                         are summed in a fixed order */
   int deterministic; /* 1 = dq's fp32 contributions are added in key order */

@@ -107,6 +107,32 @@ def test_a_sequence_does_not_see_its_neighbours():
     assert o[200:277].isnan().all() and lse[:, 200:277].isnan().all()
 
 
+SPLIT = [
+    # few query rows, many keys: walks are cut into pieces
+    ([5], [5000], 2, 1, True),
+    ([5], [5000], 2, 1, False),
+    ([300], [9000], 1, 1, True),                  # two tiles of a record, pieces before and on its diagonal
+    ([129, 0, 1, 40], [3000, 700, 4097, 0], 4, 2, True),
+    ([129, 0, 1, 40], [3000, 700, 4097, 0], 4, 2, False),
+    ([2500], [2500], 2, 2, True),
+    ([200, 60], [1300, 20], 3, 3, True),          # rows that see nothing beside a cut walk
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,h,hk,causal", SPLIT)
+@pytest.mark.parametrize("std", [1.0, 3.0])
+def test_cut_walks(lq, lk, h, hk, causal, std):
+    q, k, v, _, qo, ko = make(lq, lk, h, hk, 0, 7, std=std, seed=13)
+    o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal, residual=True)
+    _lib.check_device()
+    check_fwd(q, k, v, qo, ko, causal, o, lse)
+    # the residual is what one more rounding of the same value takes away
+    assert (res.double().abs() <= 2.0**-8 * o.double().abs()).all()
+    again, lse2 = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    assert torch.equal(o, again) and torch.equal(lse, lse2)
+
+
 @pytest.mark.gpu
 def test_matches_the_dense_forward_on_one_sequence():
     """One full sequence is wan_flash_fwd's problem: same rounding points, so the same to fp32 sums' order."""
@@ -226,8 +252,14 @@ def test_c_entry_refusals():
                                  causal, None)
 
     assert call(n=-1) == -1 and call(h=3) == -1 and call(hk=0) == -1 and call(causal=2) == -1 and call(q=None) == -1
-    assert call(ws=16) == -1 and call(q=24) == -3 and call(tq=2**30 + 1) == -2 and call(n=2**25) == -2
+    assert call(q=24) == -3 and call(tq=2**30 + 1) == -2 and call(n=2**25) == -2
     assert call(tq=0) == 0 and call(h=0, hk=0) == 0
-    size = ctypes.c_size_t()
-    assert lib.wf_packed_fwd_workspace(3, 1000, ctypes.byref(size)) == 0 and size.value > 0
-    assert lib.wf_packed_fwd_workspace(-1, 1000, ctypes.byref(size)) == -1
+    assert lib.wf_packed_fwd_workspace(-1, 1000, 1000, 4, ctypes.byref(ctypes.c_size_t())) == -1
+
+
+@pytest.mark.gpu
+def test_c_entry_refuses_a_small_workspace():
+    lib, size, p = _lib.lib(), ctypes.c_size_t(), ctypes.c_void_p
+    for tq in (8, 100000):
+        assert lib.wf_packed_fwd_workspace(2, tq, 5000, 4, ctypes.byref(size)) == 0
+        assert lib.wf_packed_fwd(*[p(16)] * 9, size.value - 1, 2, tq, 5000, 4, 2, 0, None) == -1

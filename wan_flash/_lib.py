@@ -87,7 +87,7 @@ def _declare(lib):
     lib.wf_rope.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, ctypes.POINTER(RopeCfg), vp]
     lib.wf_decode_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, ctypes.POINTER(DecodeCfg), vp]
-    lib.wf_packed_fwd_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
+    lib.wf_packed_fwd_workspace.argtypes = [i, i, i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_packed_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, i, i, i, vp]
     lib.wf_packed_bwd_workspace.argtypes = [i, i, i, i, i, ctypes.POINTER(PackedBwdCfg), ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_packed_bwd.argtypes = ([vp] * 13 + [ctypes.c_size_t] + [i] * 6 + [ctypes.POINTER(PackedBwdCfg), vp])

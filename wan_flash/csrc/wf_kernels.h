@@ -69,8 +69,11 @@ struct __align__(16) PackedFwdTile {  // up to 256 query rows of one sequence
   int k0;         // the sequence's first key row
   int klen;       // keys that the tile's last row sees; 0: nothing to attend, the rows are filled
   int off;        // causal: keys that row 0 of the tile sees (row r: off + r); may be negative
-  int n_blocks;   // ceil(klen / 128)
+  int n_blocks;   // 128-key blocks of this piece of the walk (the whole walk: ceil(klen / 128))
+  int j_last;     // the piece's last block; the walk goes down from it
+  int part;       // place of the piece's partial result; -1: the whole walk, written as the result
   int bucket, bucket_items;  // place and number of the items of equal cost
+  int pad0, pad1;
 };
 struct __align__(16) PackedBwdItem {  // up to 128 key rows of one sequence, and a piece of their walk
   int k0, rows;   // first row in the packed tensor, rows
@@ -89,7 +92,9 @@ struct PackedPlanParams {
   const int* k_off;
   int n, total_q, total_k;
   int causal, backward, ordered;
-  int group, h_kv;
+  int h, group, h_kv;
+  int sms;
+  int may_split;            // forward: the workspace has room for partial results
   int nsplit;               // > 0: pieces of the longest walk; 0: by `pieces`
   int pieces;               // pieces (over all key-value heads) that the whole work is cut into at least
   int4* head;               // [0] {items, status, split key tiles, draw counter}, [1] (backward) {query tiles, status}
@@ -99,8 +104,18 @@ struct PackedPlanParams {
   int4* q_tiles;            // {first row, rows, 1 inside a sequence, 0}
   int4* split_tiles;        // {first row, rows, first part, parts}
 };
-constexpr int kPackedMinChunk = 4;   // units: below, a piece's own cost exceeds what it evens out
+// Backward pieces: about three per SM's even share, of 8 units at least; or,
+// with few key tiles, as many as make one item per SM, of 2 units at least.  A
+// piece's own cost (prologue, K and V, partial dK and dV) is about two units.
+constexpr int kPackedMinChunk = 2;
+constexpr int kPackedMinChunkFull = 8;
 constexpr int kPackedPiecesPerSm = 3;
+constexpr int kPackedPieceCost = 2;
+// Forward pieces: only where whole walks would leave half the SMs without an
+// item, at most one item per SM, of at least 8 blocks (16 us), and where the
+// longest walk gets shorter by more than the join's cost in blocks.
+constexpr int kPackedFwdMinChunk = 8;
+constexpr int kPackedFwdJoinCost = 4;
 struct PackedFwdParams {
   const int4* head;
   const PackedFwdTile* tiles;
@@ -108,8 +123,20 @@ struct PackedFwdParams {
   __nv_bfloat16* o;
   __nv_bfloat16* res;       // what rounding o to bf16 took away, like o; or null
   float* lse;               // (h, total_q)
+  float4* part_o;           // (parts, h) x [2 tiles][32 groups of 4 columns][128 rows]: unnormalised O
+  float2* part_ml;          // (parts, h, 256): reference max (scaled log2 units) and row sum
   int total_q, h, group, causal;
   float scale_log2, rescale_threshold;
+};
+struct PackedFwdJoinParams {
+  const int4* head;
+  const int4* split_tiles;
+  const float4* part_o;
+  const float2* part_ml;
+  __nv_bfloat16* o;
+  __nv_bfloat16* res;
+  float* lse;
+  int total_q, h;
 };
 struct PackedBwdParams {
   const int4* head;

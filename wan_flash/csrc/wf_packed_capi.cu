@@ -13,19 +13,32 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 // ragged one per sequence, and per run of rows before and behind them.
 long long packed_max_tiles(long long total, long long n, int rows) { return total / rows + n + 2; }
 
+// Whether the plan may cut forward walks: where all the query rows make few
+// tiles (rows outside the sequences make tiles too) and a walk can be long
+// enough to gain from it.  It then makes at most one item per SM.
+bool packed_fwd_may_split(int total_q, int total_k, int h, int sms) {
+  return 2LL * ((total_q + 255) / 256) * h <= sms && total_k > 128 * (kPackedFwdMinChunk + kPackedFwdJoinCost);
+}
+
 struct PackedFwdWorkspace {  // byte offsets
-  size_t head = 0, base, tiles, bytes;
-  PackedFwdWorkspace(int n, int total_q) {
+  size_t head = 0, base, tiles, split_tiles, part_ml, part_o, bytes;
+  bool may_split;
+  PackedFwdWorkspace(int n, int total_q, int total_k, int h, int sms) {
+    may_split = packed_fwd_may_split(total_q, total_k, h, sms);
+    const size_t items = may_split ? (size_t)sms : 0;
     base = 256;
     tiles = align256(base + (size_t)3 * (n + 3) * 4);
-    bytes = tiles + (size_t)packed_max_tiles(total_q, n, 256) * sizeof(PackedFwdTile);
+    split_tiles = align256(tiles + (packed_max_tiles(total_q, n, 256) + items) * sizeof(PackedFwdTile));
+    part_ml = align256(split_tiles + items * sizeof(int4));
+    part_o = part_ml + items * 256 * sizeof(float2);
+    bytes = part_o + items * 8192 * sizeof(float4);
   }
 };
 
 // Items, split key tiles and partial tiles (per key-value head) that the plan
 // can make at most.  It cuts walks of more than `chunk` units, and chunk is at
-// least kPackedMinChunk and units * h_kv / pieces: sum ceil(u / chunk) <= tiles +
-// units / chunk, and a cut tile has at most 2 u / chunk parts.
+// least kPackedMinChunk and, few tiles or many, units * h_kv / pieces: sum ceil(u
+// / chunk) <= tiles + units / chunk, and a cut tile has at most 2 u / chunk parts.
 struct PackedBwdBounds {
   long long pieces, items, split_tiles, parts;
   PackedBwdBounds(int n, int total_q, int total_k, int h, int h_kv, int nsplit, int sms) {
@@ -95,11 +108,12 @@ cudaError_t packed_setup() {
 
 using namespace wf;
 
-extern "C" int wf_packed_fwd_workspace(int n, int total_q, size_t* bytes) {
+extern "C" int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, size_t* bytes) {
   if (!bytes) return fail(WF_ERR_INVALID_ARG, "null pointer");
-  int rc = packed_check(n, total_q, 0, 1, 1, 0);
-  if (rc) return rc;
-  *bytes = PackedFwdWorkspace(n, total_q).bytes;
+  int rc, dev;
+  if ((rc = packed_check(n, total_q, total_k, h, h ? 1 : 0, 0))) return rc;
+  if ((rc = device_setup(&dev))) return rc;
+  *bytes = PackedFwdWorkspace(n, total_q, total_k, h, g_dev_sms[dev]).bytes;
   return WF_OK;
 }
 
@@ -115,11 +129,12 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
       !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(q_offsets) & 3) ||
       (reinterpret_cast<uintptr_t>(k_offsets) & 3))
     return fail(WF_ERR_MISALIGNED, "q/k/v/o/o_residual/workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
-  const PackedFwdWorkspace ws(n, total_q);
-  if (workspace_bytes < ws.bytes)
-    return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
   int dev;
   if ((rc = device_setup(&dev))) return rc;
+  const int sms = g_dev_sms[dev];
+  const PackedFwdWorkspace ws(n, total_q, total_k, h, sms);
+  if (workspace_bytes < ws.bytes)
+    return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
   CUtensorMap mq, mk, mv, mo, mr;
   // with no keys at all nothing is loaded: q stands in for the maps of k and v
   if ((rc = make_bshd_map(&mq, q, 1, total_q, h)) || (rc = make_bshd_map(&mo, o, 1, total_q, h)) ||
@@ -134,6 +149,9 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   pp.head = reinterpret_cast<int4*>(w + ws.head);
   pp.base = reinterpret_cast<int*>(w + ws.base);
   pp.fwd_tiles = reinterpret_cast<PackedFwdTile*>(w + ws.tiles);
+  pp.split_tiles = reinterpret_cast<int4*>(w + ws.split_tiles);
+  pp.h = h, pp.sms = sms;
+  pp.may_split = ws.may_split ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   wf_packed_plan_kernel<<<1, kPlanThreads, 0, st>>>(pp);
   if ((rc = launch_check("wf_packed plan launch"))) return rc;
@@ -147,11 +165,23 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.total_q = total_q, p.h = h, p.group = h / h_kv, p.causal = causal;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
   p.rescale_threshold = 8.0f;
-  const long long items = packed_max_tiles(total_q, n, 256) * h;
-  const int grid = (int)std::min<long long>(items, g_dev_sms[dev]);
+  p.part_o = reinterpret_cast<float4*>(w + ws.part_o);
+  p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
+  const int grid = ws.may_split ? sms : (int)std::min<long long>(packed_max_tiles(total_q, n, 256) * h, sms);
   cudaError_t e = launch_ex(wf_packed_fwd_kernel, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
+  if (ws.may_split) {
+    PackedFwdJoinParams j = {};
+    j.head = pp.head;
+    j.split_tiles = pp.split_tiles;
+    j.part_o = p.part_o, j.part_ml = p.part_ml;
+    j.o = p.o, j.res = p.res, j.lse = lse;
+    j.total_q = total_q, j.h = h;
+    // split tiles * h <= items <= SMs
+    e = launch_ex(wf_packed_fwd_join_kernel, dim3(8 * std::max(1, sms / h), h), dim3(256), 0, st, true, 1u, j);
+    if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd join launch");
+  }
   return launch_check("wf_packed_fwd launch");
 }
 
@@ -200,7 +230,7 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   pp.n = n, pp.total_q = total_q, pp.total_k = total_k, pp.causal = causal;
   pp.backward = 1;
   pp.ordered = cfg->deterministic ? 1 : 0;
-  pp.group = h / h_kv, pp.h_kv = h_kv;
+  pp.h = h, pp.group = h / h_kv, pp.h_kv = h_kv, pp.sms = sms;
   pp.nsplit = cfg->nsplit;
   pp.pieces = (int)most.pieces;
   pp.head = reinterpret_cast<int4*>(w + ws.head);

@@ -23,6 +23,10 @@
 //             runs without a compare.  A record of at most 128 rows drives one
 //             of the two tiles only, and the first tile starts at its own
 //             diagonal (a block later than the second).
+//   pieces    Where few tiles would leave SMs idle (a short query behind a long
+//             prefix), the plan cuts their walks; a piece leaves its unnormalised
+//             O, reference maximum and row sum in fp32, and
+//             wf_packed_fwd_join_kernel adds the pieces in a fixed order.
 //   masks     A row's visible keys are a count; the block loop compares it
 //             with the block's end and masks by column.  A row whose blocks so
 //             far are all masked keeps -inf as its maximum and exponentiates
@@ -76,7 +80,7 @@ constexpr int kItemReaders = 11;                         // 8 softmax warps, MMA
 constexpr int kBarItemNext = kBarItemEmpty + kItemSlots; // the TMA warp is at its item's last block
 constexpr int kNumBars = kBarItemNext + 1;
 constexpr uint32_t kOffItems = kOffBar + ((kNumBars * 8 + 15) & ~15);
-constexpr uint32_t kOffTmemHolder = kOffItems + kItemSlots * 48;
+constexpr uint32_t kOffTmemHolder = kOffItems + kItemSlots * 64;
 constexpr uint32_t kOffAbort = kOffTmemHolder + 4;
 constexpr uint32_t kSmemUsed = kOffAbort + 4;
 constexpr uint32_t kSmemBytes = kSmemUsed + 1024;
@@ -87,10 +91,10 @@ static_assert(kSmemBytes <= 232448, "packed forward shared memory exceeds the pe
 struct __align__(16) PackedFwdItem {
   PackedFwdTile w;
   int h;      // q head; -1: no items left
-  int skip0;  // blocks of the walk that no row of tile 0 sees
+  int skip0;  // blocks of the walk that no row of tile 0 sees (but one block is walked at least)
   int pad[2];
 };
-static_assert(sizeof(PackedFwdItem) == 48, "three 16-byte words");
+static_assert(sizeof(PackedFwdItem) == 64, "four 16-byte words");
 
 // Zero rows [first, 128) of a 128-row tile of two 64-column boxes (a
 // converged warp; the swizzle permutes 16-byte chunks inside a row only), and
@@ -180,7 +184,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         if (next < n_items) {
           x.w = p.tiles[packed_locate(p.tiles, next, p.h, x.h)];
           const int seen0 = min(x.w.off + 127, x.w.klen);  // keys that the last row of tile 0 sees
-          if (p.causal && x.w.rows > 128 && seen0 > 0) x.skip0 = x.w.n_blocks - (seen0 + 127) / 128;
+          if (p.causal && x.w.rows > 128 && seen0 > 0)
+            x.skip0 = max(0, min(x.w.j_last + 1 - (seen0 + 127) / 128, x.w.n_blocks - 1));
         }
         const int slot = k % kItemSlots;
         if (k >= kItemSlots && !mbar_wait(bar(kBarItemEmpty + slot), (uint32_t)(k / kItemSlots - 1) & 1, abort_flag,
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     for (int k = 0; ok && get_item(k, x, kRoleStore, false); ++k) {
       const PackedFwdTile& w = x.w;
       const int h = x.h;
-      if (w.n_blocks == 0) continue;
+      if (w.n_blocks == 0 || w.part >= 0) continue;
       const int stores = (w.rows > 128 ? 2 : 1) * passes;
       for (int i = 0; i < stores; ++i, ++n) {
         const int t = i / passes;
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         if (w.n_blocks == 0) mbar_arrive(bar(kBarItemNext));
         for (int it = 0; it < w.n_blocks && ok; ++it) {
           if (it == w.n_blocks - 1) mbar_arrive(bar(kBarItemNext));
-          const int j = w.n_blocks - 1 - it;
+          const int j = w.j_last - it;
           for (int kv = 0; kv < 2 && ok; ++kv, ++u) {  // 0 = K, 1 = V
             const int slot = u % kKvSlots;
             const int use = u / kKvSlots;
@@ -376,7 +381,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         }
         if (ok) mma_commit_e(bar(kBarKvEmpty + slot_k));
         prev_last = (it == w.n_blocks - 1);
-        prev_keys = it == 0 ? w.klen - (w.n_blocks - 1) * 128 : 128;
+        prev_keys = min(128, w.klen - (w.j_last - it) * 128);
       }
     }
     if (ok && g > 0 && x.h < 0) {  // (an abort leaves another item in x)
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         continue;
       }
       const int use0 = stage_use + t * passes;
-      stage_use += (w.rows > 128 ? 2 : 1) * passes;
+      if (w.part < 0) stage_use += (w.rows > 128 ? 2 : 1) * passes;
       if (t * 128 >= w.rows) continue;
       const int seen = p.causal ? min(max(w.off + row, 0), w.klen) : w.klen;  // keys that this row sees
       float m_s = -INFINITY;  // running reference max, in scaled log2 units
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 4; ++c) reg_fence32(s[c]);
-        const int left = seen - (w.n_blocks - 1 - it) * 128;  // keys of this block that the row sees
+        const int left = seen - (w.j_last - it) * 128;  // keys of this block that the row sees
         if (left < 128) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -502,6 +507,24 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       if (!ok) break;
       ++o_waits;
       tc_fence_after();
+      if (w.part >= 0) {
+        // a piece of the walk: its O as it stands, row by row coalesced
+        const size_t slot = (size_t)w.part * p.h + h;
+        float4* dst = p.part_o + (slot * 2 + t) * 4096 + r;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            dst[(c * 8 + g) * 128] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]),
+                                                 __uint_as_float(o[4 * g + 2]), __uint_as_float(o[4 * g + 3]));
+        }
+        p.part_ml[slot * 256 + row] = make_float2(m_s, l);
+        continue;
+      }
       const float inv = 1.f / l;
       const uint32_t stage = sbase + kOffOStage + (uint32_t)r * 128u;
 #pragma unroll 1
@@ -546,6 +569,66 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+// Joins the pieces of the split tiles: o = sum_i w_i O_i / sum_i w_i l_i with
+// w_i = 2^(m_i - max m).  Bound: L2 (520 bytes a row and piece).  grid (8 *
+// split tiles, h), 256 threads: 32 rows x 128 columns.
+__global__ void __launch_bounds__(256) wf_packed_fwd_join_kernel(PackedFwdJoinParams p) {
+  __shared__ float tile[32][132];
+  griddep_wait();
+  const int t = blockIdx.x >> 3, row0 = (blockIdx.x & 7) * 32, h = blockIdx.y;
+  if (t >= p.head->z) return;
+  const int4 w = p.split_tiles[t];  // first row, rows, first part, parts
+  if (row0 >= w.y) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = row0 + lane;
+  float top = -INFINITY;
+  for (int i = 0; i < w.w; ++i) top = fmaxf(top, p.part_ml[((size_t)(w.z + i) * p.h + h) * 256 + row].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  float4 x[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) x[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < w.w; ++i) {
+    const size_t slot = (size_t)(w.z + i) * p.h + h;
+    const float2 ml = p.part_ml[slot * 256 + row];
+    if (ml.y == 0.f) continue;  // the row sees none of this piece's keys (whose values may be anything)
+    const float f = ex2_approx(ml.x - ref);
+    l += f * ml.y;
+    const float4* src = p.part_o + (slot * 2 + (row >> 7)) * 4096 + (row & 127);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 y = src[(warp * 4 + g) * 128];
+      x[g].x += f * y.x, x[g].y += f * y.y, x[g].z += f * y.z, x[g].w += f * y.w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: 0
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float* d = &tile[lane][(warp * 4 + g) * 4];
+    d[0] = l == 0.f ? 0.f : x[g].x * inv, d[1] = l == 0.f ? 0.f : x[g].y * inv;
+    d[2] = l == 0.f ? 0.f : x[g].z * inv, d[3] = l == 0.f ? 0.f : x[g].w * inv;
+  }
+  if (warp == 0 && row < w.y)
+    p.lse[(size_t)h * p.total_q + w.x + row] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.69314718055994531f;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int idx = threadIdx.x + i * 256;  // 32 rows x 16 chunks of 8
+    const int rw = idx >> 4, ch = idx & 15;
+    if (row0 + rw >= w.y) continue;
+    const float* v = &tile[rw][ch * 8];
+    uint32_t o[4], r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      o[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
+      r[k] = pack_bf16(v[2 * k] - __uint_as_float(o[k] << 16), v[2 * k + 1] - __uint_as_float(o[k] & 0xffff0000u));
+    }
+    const size_t at = ((size_t)(w.x + row0 + rw) * p.h + h) * 128 + ch * 8;
+    st_global_v4(p.o + at, o[0], o[1], o[2], o[3]);
+    if (p.res != nullptr) st_global_v4(p.res + at, r[0], r[1], r[2], r[3]);
+  }
 }
 
 }  // namespace wf

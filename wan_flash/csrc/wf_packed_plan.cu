@@ -14,9 +14,11 @@
 // by head (packed_locate): the tiles of one sequence and head, which read the
 // same keys (backward: queries), run side by side.
 //
-// Backward pieces: a key tile that walks more units (query tile, q head) than
-// `chunk`, a third of an SM's even share, is cut into pieces whose partial
-// dK and dV a convert sums.  One long sequence then fills the GPU as evenly as many.
+// Pieces: a backward key tile with a long walk over (query tile, q head) units is
+// cut into pieces whose partial dK and dV a convert sums, so one long sequence
+// fills the GPU as evenly as many; a forward walk over key blocks is cut where
+// few tiles (a short query behind a long prefix) would leave SMs idle, and a
+// join adds its partial results.
 //
 // Offsets that fall, start below 0 or end behind the tensor set the device
 // error word; the lists then hold only rows outside any sequence, with
@@ -43,7 +45,7 @@ struct PlanShared {
   int start[kPlanBuckets + 1];
   int cursor[kPlanBuckets];
   unsigned long long units;
-  int most, parts, split_tiles;
+  int most, items, parts, split_tiles;
   int q_off[kPlanSmall], k_off[kPlanSmall], base0[kPlanSmall], base1[kPlanSmall];
 };
 
@@ -128,13 +130,15 @@ __device__ __noinline__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int
   PackedFwdTile w;
   w.q0 = qs + m0;
   w.rows = min(256, lq - m0);
-  w.k0 = w.klen = w.off = w.n_blocks = w.bucket = w.bucket_items = 0;
+  w.k0 = w.klen = w.off = w.n_blocks = w.j_last = w.bucket = w.bucket_items = w.pad0 = w.pad1 = 0;
+  w.part = -1;
   if (!p.bad && s >= 1 && s <= p.n) {
     const int ks = p.k_off[s - 1], lk = p.k_off[s] - ks;
     w.k0 = ks;
     w.off = p.causal ? m0 + lk - lq + 1 : lk;  // keys that the tile's first row sees (causal: may be negative)
     w.klen = p.causal ? max(0, w.off + w.rows - 1) : lk;
     w.n_blocks = (w.klen + 127) / 128;
+    w.j_last = w.n_blocks - 1;
   }
   return w;
 }
@@ -165,6 +169,35 @@ __device__ __noinline__ PackedBwdItem plan_k_tile(const PlanView& p, const int* 
   return w;
 }
 
+// Adds to sh.units and raises sh.most by every thread's values (one atomic a warp).
+__device__ __noinline__ void plan_totals(PlanShared& sh, unsigned long long units, int most) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) units += __shfl_xor_sync(0xffffffffu, units, d);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) {
+    atomicAdd(&sh.units, units);
+    atomicMax(&sh.most, most);
+  }
+  __syncthreads();
+}
+
+// The smallest chunk from `from` on with which all walks, cut into pieces of at
+// most chunk, make at most `sms` items over `heads` heads; `most` (whole walks)
+// where none does.
+template <typename Cost>
+__device__ int plan_fit(PlanShared& sh, int n_tiles, int heads, int sms, int most, long long from, Cost&& cost) {
+  int chunk = (int)min(from, (long long)max(most, 1));
+  while (chunk < most) {
+    int mine = 0, items;
+    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads)
+      mine += max(1, (int)(((unsigned)cost(t) + (unsigned)chunk - 1u) / (unsigned)chunk));
+    plan_scan(sh, mine, &items);
+    if ((long long)items * heads <= sms) return chunk;
+    chunk = min((long long)most, (long long)chunk + chunk / 8 + 1);
+  }
+  return max(most, 1);
+}
+
 // Buckets of falling cost: sizes from count(add), their starts in sh.start.
 template <typename Count>
 __device__ void plan_buckets(PlanShared& sh, int n_tiles, int shift, Count&& count) {
@@ -188,6 +221,14 @@ __device__ int plan_place(PlanShared& sh, int cost, int shift, Item& w) {
   return atomicAdd(&sh.cursor[b], 1);
 }
 
+// The next free place, for an item of a list that is not sorted.
+template <typename Item>
+__device__ int plan_next(PlanShared& sh, Item& w) {
+  w.bucket = atomicAdd(&sh.items, 1);
+  w.bucket_items = 1;
+  return w.bucket;
+}
+
 }  // namespace
 
 // grid 1 (forward) or 2 (backward: block 0 the items, block 1 the query tiles)
@@ -195,7 +236,7 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
   __shared__ PlanShared sh;
   griddep_launch_dependents();
   const bool small = p.n + 3 <= kPlanSmall;
-  if (threadIdx.x == 0) sh.units = 0ull, sh.most = sh.parts = sh.split_tiles = 0;
+  if (threadIdx.x == 0) sh.units = 0ull, sh.most = sh.items = sh.parts = sh.split_tiles = 0;
   if (small) {
     for (int s = threadIdx.x; s <= p.n; s += kPlanThreads) {
       sh.q_off[s] = p.q_off[s];
@@ -223,19 +264,58 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
     PackedFwdTile mine = {};  // this thread's first tile
     if ((int)threadIdx.x < n_tiles) mine = plan_fwd_tile(v, base0, threadIdx.x);
     auto tile = [&](int t) { return t < kPlanThreads ? mine : plan_fwd_tile(v, base0, t); };
+    const bool few = (long long)n_tiles * p.h <= p.sms;  // all items run at once: no need to sort
+    if (few && !p.may_split) {
+      for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
+        PackedFwdTile w = tile(t);
+        w.bucket = t;
+        w.bucket_items = 1;
+        p.fwd_tiles[t] = w;
+      }
+      if (threadIdx.x == 0) p.head[0] = make_int4(n_tiles, v.bad, 0, 0);
+      return;
+    }
     int most = 0;
-    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) most = max(most, tile(t).n_blocks);
-    atomicMax(&sh.most, most);
-    __syncthreads();
+    unsigned long long blocks = 0;
+    for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
+      most = max(most, tile(t).n_blocks);
+      blocks += tile(t).n_blocks;
+    }
+    plan_totals(sh, blocks, most);
+    most = sh.most;
+    int chunk = max(most, 1);
+    if (p.may_split && 2LL * n_tiles * p.h <= p.sms && most > kPackedFwdMinChunk) {
+      chunk = plan_fit(sh, n_tiles, p.h, p.sms, most,
+                       max((long long)kPackedFwdMinChunk, (long long)(sh.units * p.h + p.sms - 1) / p.sms),
+                       [&](int t) { return tile(t).n_blocks; });
+      if (chunk + kPackedFwdJoinCost > most) chunk = most;  // the join would take what the cut saves
+    }
     int shift = 0;
-    while ((sh.most >> shift) >= kPlanBuckets) ++shift;
-    plan_buckets(sh, n_tiles, shift, [&](int t, auto add) { add(tile(t).n_blocks); });
+    while ((min(most, chunk) >> shift) >= kPlanBuckets) ++shift;
+    auto pieces_of = [&](int n) { return n > chunk ? (n + chunk - 1) / chunk : 1; };
+    if (!few)
+      plan_buckets(sh, n_tiles, shift, [&](int t, auto add) {
+        const int n = tile(t).n_blocks, s = pieces_of(n), even = n / s, more = n - even * s;
+        for (int i = 0; i < s; ++i) add(even + (i < more ? 1 : 0));
+      });
     for (int t = threadIdx.x; t < n_tiles; t += kPlanThreads) {
       PackedFwdTile w = tile(t);
-      const int at = plan_place(sh, w.n_blocks, shift, w);
-      p.fwd_tiles[at] = w;
+      const int n = w.n_blocks, s = pieces_of(n), even = n / s, more = n - even * s;
+      int part = -1;
+      if (s > 1) {  // any place will do: the parts of a tile are joined in their order
+        part = atomicAdd(&sh.parts, s);
+        p.split_tiles[atomicAdd(&sh.split_tiles, 1)] = make_int4(w.q0, w.rows, part, s);
+      }
+      for (int i = 0; i < s; ++i) {
+        w.n_blocks = even + (i < more ? 1 : 0);
+        w.j_last = (i + 1) * even + min(i + 1, more) - 1;
+        w.part = s > 1 ? part + i : -1;
+        const int at = few ? plan_next(sh, w) : plan_place(sh, w.n_blocks, shift, w);
+        p.fwd_tiles[at] = w;
+      }
     }
-    if (threadIdx.x == 0) p.head[0] = make_int4(n_tiles, v.bad, 0, 0);
+    __syncthreads();
+    if (threadIdx.x == 0) p.head[0] = make_int4(few ? sh.items : sh.start[kPlanBuckets], v.bad, sh.split_tiles, 0);
     return;
   }
   if (blockIdx.x == 1) {
@@ -263,19 +343,32 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
     units += u;
     most = max(most, u);
   }
-  atomicAdd(&sh.units, units);
-  atomicMax(&sh.most, most);
-  __syncthreads();
+  plan_totals(sh, units, most);
   most = sh.most;
-  const int chunk =
-      p.nsplit > 0 ? max(1, (int)(((unsigned)most + p.nsplit - 1) / p.nsplit))
-                   : (int)min((unsigned long long)0x7fffffff,
-                              max((unsigned long long)kPackedMinChunk, sh.units * p.h_kv / p.pieces + 1));
+  int chunk;
+  bool one_round = false;  // all items run at once: no need to sort
+  if (p.nsplit > 0) {
+    chunk = max(1, (int)(((unsigned)most + p.nsplit - 1) / p.nsplit));
+  } else {
+    // pieces of a third of an SM's even share, so their uneven ends even out ...
+    chunk = (int)min((unsigned long long)0x7fffffff,
+                     max((unsigned long long)kPackedMinChunkFull, sh.units * p.h_kv / p.pieces + 1));
+    if ((long long)n_tiles * p.h_kv <= p.sms) {
+      // ... or at most one piece per SM: the longest then is the time.  Each piece costs kPackedPieceCost units too
+      const int share = (int)((sh.units * p.h_kv + p.sms - 1) / p.sms);
+      const int one = plan_fit(sh, n_tiles, p.h_kv, p.sms, most, max(kPackedMinChunk, share),
+                               [&](int t) { return tile(t).m_count * p.group; });
+      if (one + kPackedPieceCost <= share + share / chunk * kPackedPieceCost + kPackedPieceCost + chunk / 2) {
+        chunk = one;
+        one_round = !p.ordered;
+      }
+    }
+  }
   // a walk of u units in s pieces: the first u % s have one unit more
   auto pieces_of = [&](int u) { return u > chunk ? (int)(((unsigned)u + (unsigned)chunk - 1u) / (unsigned)chunk) : 1; };
   int shift = 0;
   while ((min(most, chunk) >> shift) >= kPlanBuckets) ++shift;
-  if (!p.ordered)
+  if (!p.ordered && !one_round)
     plan_buckets(sh, n_tiles, shift, [&](int t, auto add) {
       const int u = tile(t).m_count * p.group, s = pieces_of(u), even = u / s, more = u - even * s;
       for (int i = 0; i < s; ++i) add(even + (i < more ? 1 : 0));
@@ -308,12 +401,13 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
       int place = at + i;  // ordered: key tiles as they stand, one after the other
       w.bucket = place;
       w.bucket_items = 1;
-      if (!p.ordered) place = plan_place(sh, w.count, shift, w);
+      if (one_round) place = plan_next(sh, w);
+      else if (!p.ordered) place = plan_place(sh, w.count, shift, w);
       p.items[place] = w;
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) p.head[0] = make_int4(p.ordered ? items : sh.start[kPlanBuckets], v.bad, sh.split_tiles, 0);
+  if (threadIdx.x == 0) p.head[0] = make_int4(p.ordered ? items : one_round ? sh.items : sh.start[kPlanBuckets], v.bad, sh.split_tiles, 0);
 }
 
 // Work index i (of items * heads) -> item and head: bucket by bucket, inside a

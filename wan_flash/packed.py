@@ -54,9 +54,11 @@ def _check(q, k, v, q_offsets, k_offsets):
 
 
 @functools.lru_cache(maxsize=256)
-def _fwd_bytes(n: int, total_q: int) -> int:
+def _fwd_bytes(index: int, n: int, total_q: int, total_k: int, h: int) -> int:
+    """The workspace's size on device `index`."""
     size = ctypes.c_size_t()
-    _lib.check(_lib.lib().wf_packed_fwd_workspace(n, total_q, ctypes.byref(size)))
+    with torch.cuda.device(index):
+        _lib.check(_lib.lib().wf_packed_fwd_workspace(n, total_q, total_k, h, ctypes.byref(size)))
     return size.value
 
 
@@ -86,7 +88,7 @@ def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
     out = (o, lse, o_residual) if residual else (o, lse)
     if total_q == 0 or h == 0:
         return out
-    size = _fwd_bytes(n, total_q)
+    size = _fwd_bytes(device.index, n, total_q, total_k, h)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
     _launch(_lib.lib().wf_packed_fwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
             k_offsets.data_ptr(), o.data_ptr(), o_residual.data_ptr() if residual else None, lse.data_ptr(),
