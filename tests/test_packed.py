@@ -115,7 +115,8 @@ SPLIT = [
     ([129, 0, 1, 40], [3000, 700, 4097, 0], 4, 2, True),
     ([129, 0, 1, 40], [3000, 700, 4097, 0], 4, 2, False),
     ([2500], [2500], 2, 2, True),
-    ([200, 60], [1300, 20], 3, 3, True),          # rows that see nothing beside a cut walk
+    ([200, 60], [1800, 20], 3, 3, True),          # rows that see nothing beside a cut walk
+    ([6000, 1], [6000, 5], 6, 2, True),           # only the longest walks are cut
 ]
 
 

@@ -111,11 +111,12 @@ constexpr int kPackedMinChunk = 2;
 constexpr int kPackedMinChunkFull = 8;
 constexpr int kPackedPiecesPerSm = 3;
 constexpr int kPackedPieceCost = 2;
-// Forward pieces: only where whole walks would leave half the SMs without an
-// item, at most one item per SM, of at least 8 blocks (16 us), and where the
+// Forward pieces: of at least 8 blocks (16 us), of an SM's even share of all
+// blocks or, with few tiles, as many as make one item per SM; only where the
 // longest walk gets shorter by more than the join's cost in blocks.
 constexpr int kPackedFwdMinChunk = 8;
 constexpr int kPackedFwdJoinCost = 4;
+constexpr int kPackedFwdSplitItems = 4;  // per SM: with more items the longest walk is not the time
 struct PackedFwdParams {
   const int4* head;
   const PackedFwdTile* tiles;

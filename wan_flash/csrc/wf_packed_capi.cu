@@ -13,11 +13,13 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 // ragged one per sequence, and per run of rows before and behind them.
 long long packed_max_tiles(long long total, long long n, int rows) { return total / rows + n + 2; }
 
-// Whether the plan may cut forward walks: where all the query rows make few
-// tiles (rows outside the sequences make tiles too) and a walk can be long
-// enough to gain from it.  It then makes at most one item per SM.
+// Whether the plan may cut forward walks: where the query rows make few items
+// and a walk can be long enough to gain from it.  Its pieces are no shorter than
+// an SM's even share of all blocks (items: one per SM more than whole walks;
+// partial results: two per SM), so the bounds hold whatever the lengths.
 bool packed_fwd_may_split(int total_q, int total_k, int h, int sms) {
-  return 2LL * ((total_q + 255) / 256) * h <= sms && total_k > 128 * (kPackedFwdMinChunk + kPackedFwdJoinCost);
+  return (long long)((total_q + 255) / 256) * h <= (long long)kPackedFwdSplitItems * sms &&
+         total_k > 128 * (kPackedFwdMinChunk + kPackedFwdJoinCost);
 }
 
 struct PackedFwdWorkspace {  // byte offsets
@@ -30,8 +32,8 @@ struct PackedFwdWorkspace {  // byte offsets
     tiles = align256(base + (size_t)3 * (n + 3) * 4);
     split_tiles = align256(tiles + (packed_max_tiles(total_q, n, 256) + items) * sizeof(PackedFwdTile));
     part_ml = align256(split_tiles + items * sizeof(int4));
-    part_o = part_ml + items * 256 * sizeof(float2);
-    bytes = part_o + items * 8192 * sizeof(float4);
+    part_o = part_ml + 2 * items * 256 * sizeof(float2);
+    bytes = part_o + 2 * items * 8192 * sizeof(float4);
   }
 };
 
@@ -178,7 +180,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
     j.part_o = p.part_o, j.part_ml = p.part_ml;
     j.o = p.o, j.res = p.res, j.lse = lse;
     j.total_q = total_q, j.h = h;
-    // split tiles * h <= items <= SMs
+    // split tiles * h <= SMs: every one adds an item to those of whole walks
     e = launch_ex(wf_packed_fwd_join_kernel, dim3(8 * std::max(1, sms / h), h), dim3(256), 0, st, true, 1u, j);
     if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd join launch");
   }

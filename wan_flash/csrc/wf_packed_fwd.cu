@@ -157,7 +157,9 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const int passes = p.res != nullptr ? 2 : 1;  // o, and what its rounding took away
-  // a programmatic dependent of the plan kernel: its lists are read from here on
+  // a programmatic dependent of the plan kernel: its lists are read from here
+  // on.  The join, if one follows, may take its place on SMs as they fall free.
+  griddep_launch_dependents();
   griddep_wait();
   // The k-th item of this CTA, for a whole warp (or, one = true, for one thread
   // that alone stands for its warp).  False: no more, or abort.

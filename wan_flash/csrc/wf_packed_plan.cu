@@ -284,10 +284,14 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
     plan_totals(sh, blocks, most);
     most = sh.most;
     int chunk = max(most, 1);
-    if (p.may_split && 2LL * n_tiles * p.h <= p.sms && most > kPackedFwdMinChunk) {
-      chunk = plan_fit(sh, n_tiles, p.h, p.sms, most,
-                       max((long long)kPackedFwdMinChunk, (long long)(sh.units * p.h + p.sms - 1) / p.sms),
-                       [&](int t) { return tile(t).n_blocks; });
+    if (p.may_split && most > kPackedFwdMinChunk) {
+      // an SM's even share of the blocks; a longer walk alone would be the time
+      const long long share = (long long)(sh.units * p.h + p.sms - 1) / p.sms;
+      if (2LL * n_tiles * p.h <= p.sms)  // at most one piece per SM
+        chunk = plan_fit(sh, n_tiles, p.h, p.sms, most, max((long long)kPackedFwdMinChunk, share),
+                         [&](int t) { return tile(t).n_blocks; });
+      else
+        chunk = (int)min((long long)most, max((long long)kPackedFwdMinChunk, share + share / 8 + 1));
       if (chunk + kPackedFwdJoinCost > most) chunk = most;  // the join would take what the cut saves
     }
     int shift = 0;
