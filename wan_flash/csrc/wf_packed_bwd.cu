@@ -20,7 +20,7 @@
 //             walk comes as several pieces; each leaves fp32 partial dK and dV
 //             of its own, summed in a fixed order by the convert.
 //   masks     Key r of the tile is seen by query rows >= need + r.  Only units
-//             whose rows start below need + 127 compare.  Masked scores become
+//             whose rows start below need + 127 compare; masked scores become
 //             -inf before the exponential.
 //   isolation -lse * log2(e) and D come from padded tiles (-inf and 0 behind
 //             the sequence's end), so those columns have P = dS = 0; the rows of
@@ -100,6 +100,7 @@ struct PackedWalk {
   }
 };
 
+template <bool kCausal>
 __global__ void __launch_bounds__(bwd::kThreads, 1)
     wf_packed_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -335,20 +336,24 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
       tmem_wait_ld();
       reg_fence32(s[0]);
       reg_fence32(s[1]);
-      // key row r is seen by the unit's columns >= below + r
-      const int below = w.need - at.m * 128;
-      if (below > -127) {
+      if constexpr (kCausal) {
+        // key row r is seen by the unit's columns >= below + r (a copy of the
+        // exponentials' loop with the compares in it ran 12 % slower, compares
+        // in a kernel for both kinds cost full attention 5 %)
+        const int below = w.need - at.m * 128;
+        if (below > -127) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int first = below + kv_row(g, e) - half * 64 - 2 * tq;
+            for (int e = 0; e < 2; ++e) {
+              const int first = below + kv_row(g, e) - half * 64 - 2 * tq;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+              for (int j = 0; j < 8; ++j)
 #pragma unroll
-              for (int i = 0; i < 2; ++i)
-                if (8 * j + i < first) s[g][4 * j + 2 * e + i] = __float_as_uint(-INFINITY);
-          }
+                for (int i = 0; i < 2; ++i)
+                  if (8 * j + i < first) s[g][4 * j + 2 * e + i] = __float_as_uint(-INFINITY);
+            }
+        }
       }
       // P^T = 2^(S^T * scale_log2 + neg_lse_log2[q]); rounded to bf16 as the
       // dV product's operand, kept in fp32 for dS.  Rows past the keys' end are zeroed.

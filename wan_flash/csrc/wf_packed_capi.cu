@@ -102,8 +102,9 @@ int packed_check(int n, int total_q, int total_k, int h, int h_kv, int causal) {
 cudaError_t packed_setup() {
   cudaError_t e =
       cudaFuncSetAttribute(wf_packed_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pfwd::kSmemBytes);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(wf_packed_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd::kSmemBytes);
+  for (auto k : {wf_packed_bwd_kernel<false>, wf_packed_bwd_kernel<true>})
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd::kSmemBytes);
+  return e;
 }
 
 }  // namespace wf
@@ -269,7 +270,7 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
                 reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(o_residual),
                 reinterpret_cast<const __nv_bfloat16*>(dO), lse);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd preprocess launch");
-  e = launch_ex(wf_packed_bwd_kernel, dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true,
+  e = launch_ex(causal ? wf_packed_bwd_kernel<true> : wf_packed_bwd_kernel<false>, dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true,
                 1u, mq, mk, mv, mdo, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd launch");
   PackedConvertParams c = {};
