@@ -86,9 +86,11 @@ def test_large_scores(causal):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
-def test_many_sequences(causal):
-    """More items than CTAs, more sequences than the plan's threads, one and two tiles in turn."""
-    lens = [(i * 53) % 301 for i in range(1500)]
+@pytest.mark.parametrize("n", [1500, 2500])
+def test_many_sequences(n, causal):
+    """More items than CTAs, more sequences than the plan's threads, one and two tiles in turn; the plan's
+    scans in shared memory and in the workspace."""
+    lens = [(i * 53) % (301 if n < 2000 else 41) for i in range(n)]
     q, k, v, _, qo, ko = make(lens, lens, 2, 1, seed=2)
     o, lse = wan_flash_packed_fwd(q, k, v, qo, causal=causal)  # k_offsets defaults to q_offsets
     _lib.check_device()

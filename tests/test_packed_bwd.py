@@ -63,8 +63,9 @@ def test_splits_and_ordered_mode(nsplit, deterministic, causal):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
-def test_many_sequences(causal):
-    lens = [(i * 53) % 301 for i in range(1200)]
+@pytest.mark.parametrize("n", [1200, 2500])  # the plan's scans in shared memory, and in the workspace
+def test_many_sequences(n, causal):
+    lens = [(i * 53) % (301 if n < 2000 else 41) for i in range(n)]
     q, k, v, do, qo, ko = make(lens, lens, 2, 1, seed=2)
     o, lse = wan_flash_packed_fwd(q, k, v, qo, causal=causal)
     grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, causal=causal)
@@ -163,6 +164,20 @@ def test_impossible_offsets(bad):
             _lib.check_device()
         assert all(x.isnan().all() for x in grads)
     _lib.check_device()
+
+
+@pytest.mark.gpu
+def test_one_derivative_only_and_expanded_gradients():
+    q, k, v, do, qo, _ = make([100, 40], [100, 40], 2, 1)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    o = wan_flash_attn_packed(*leaves, qo)
+    one = torch.ones((), device="cuda", dtype=torch.bfloat16).expand(o.shape)  # as from o.sum()
+    grads = torch.autograd.grad(o, leaves, one, retain_graph=True)
+    _lib.check_device()
+    check_bwd(q, k, v, one, qo, qo, False, *grads, residual=True)
+    (dq,) = torch.autograd.grad(o, leaves[0], do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dq.sum().backward()
 
 
 @pytest.mark.gpu

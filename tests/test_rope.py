@@ -130,6 +130,19 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.gpu
+def test_second_derivative():
+    """The gradient is a turn itself: turning it on gives the identity's rounding error only."""
+    table, pos = rope_table(64, device="cuda"), rope_positions((2, 2, 3), device="cuda")
+    g = torch.Generator().manual_seed(4)
+    q, k, w, x = (torch.randn(12, 2, 128, generator=g).cuda() for _ in range(4))
+    q.requires_grad_(), w.requires_grad_()
+    (grad,) = torch.autograd.grad((wan_flash_rope(q, k, pos, table)[0] * w).sum(), q, create_graph=True)
+    (back,) = torch.autograd.grad((grad * x).sum(), w)  # d/dw of <turn^-1 w, x> = turn x
+    want = turned64(x, pos)
+    assert ((back.double() - want).abs() <= rope_tol(x, want)).all()
+
+
+@pytest.mark.gpu
 def test_strided_packed_and_per_item_positions():
     g = torch.Generator().manual_seed(5)
     table = rope_table(128, device="cuda")

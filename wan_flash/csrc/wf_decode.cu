@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
       long long e = (end * ctas) / total;
       while (total * (e + 1) / ctas <= end) ++e;
       while (total * e / ctas > end) --e;
-      join = make_int4(head0, n_heads, (int)e, run.seq);
+      join = make_int4(head0, n_heads, (int)min(e, ctas - 1), run.seq);
     }
     at = run.row_at + run.t1;
   }

@@ -32,6 +32,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from wan_flash import _lib, features
 from wan_flash.interface import _aligned, _launch
@@ -137,6 +138,7 @@ class _WanFlashAttnPackedFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, o_residual, q_offsets, k_offsets = ctx.saved_tensors
         dq, dk, dv = wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, ctx.causal, o_residual)
@@ -145,7 +147,7 @@ class _WanFlashAttnPackedFn(torch.autograd.Function):
 
 def wan_flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                           k_offsets: torch.Tensor | None = None, causal: bool = False):
-    """Differentiable attention over packed sequences -> o (total_q, h, 128) bf16."""
+    """Differentiable (once) attention over packed sequences -> o (total_q, h, 128) bf16."""
     k_offsets = q_offsets if k_offsets is None else k_offsets
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WanFlashAttnPackedFn.apply(q, k, v, q_offsets, k_offsets, bool(causal))

@@ -107,16 +107,22 @@ def _rope_impl(q, k, positions, table, axes, inverse):
 
 class _WanFlashRopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, table, axes):
+    def forward(ctx, q, k, positions, table, axes, inverse):
         ctx.save_for_backward(positions, table)
-        ctx.axes = axes
-        return _rope_impl(q, k, positions, table, axes, False)
+        ctx.axes, ctx.inverse = axes, inverse
+        return _rope_impl(q, k, positions, table, axes, inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
         positions, table = ctx.saved_tensors
-        gq, gk = _rope_impl(gq, gk, positions, table, ctx.axes, True)
-        return gq, gk, None, None, None
+        gq, gk = _turned(gq, gk, positions, table, ctx.axes, not ctx.inverse)
+        return gq, gk, None, None, None, None
+
+
+def _turned(q, k, positions, table, axes, inverse):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return _WanFlashRopeFn.apply(q, k, positions, table, axes, inverse)
+    return _rope_impl(q, k, positions, table, axes, inverse)
 
 
 def wan_flash_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, axes=AXES):
@@ -128,7 +134,5 @@ def wan_flash_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     table: rope_table(...), more rows than the largest position.
     axes: head dims of time, height, width, as given to rope_table.
     q and k may be strided views (slices of a fused qkv projection); heads may
-    differ.  Differentiable in q and k (the turn by the negative angle)."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        return _WanFlashRopeFn.apply(q, k, positions, table, axes)
-    return _rope_impl(q, k, positions, table, axes, False)
+    differ.  Differentiable in q and k (the turn by the negative angle), any number of times."""
+    return _turned(q, k, positions, table, axes, False)
