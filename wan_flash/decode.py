@@ -66,7 +66,7 @@ def wan_flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         lengths.device == device, "tensors must be on one CUDA device"
     q = _aligned(q)
     o = torch.empty_like(q)
-    lse = torch.empty((b, h), device=device, dtype=torch.float32)
+    lse = q.new_empty((b, h), dtype=torch.float32)
     if b == 0 or h == 0:
         return o, lse
     lengths = lengths.contiguous()

@@ -53,6 +53,11 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape (empty_like is the shortest call where t is contiguous)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _launch(fn, device: torch.device, *args):
     """fn(*args, stream) with `device` current, on its current stream; raises on a status.
     The short way for calls whose kernels take a few microseconds: the raw stream handle,

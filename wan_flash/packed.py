@@ -85,7 +85,7 @@ def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
     q_offsets, k_offsets = q_offsets.contiguous(), k_offsets.contiguous()
     o = torch.empty_like(q)
     o_residual = torch.empty_like(q) if residual else None
-    lse = torch.empty((h, total_q), device=device, dtype=torch.float32)
+    lse = q.new_empty((h, total_q), dtype=torch.float32)
     out = (o, lse, o_residual) if residual else (o, lse)
     if total_q == 0 or h == 0:
         return out

@@ -22,7 +22,7 @@ from __future__ import annotations
 import torch
 
 from wan_flash import _lib
-from wan_flash.interface import _launch
+from wan_flash.interface import _contiguous_like, _launch
 from wan_flash.shapes import HEAD_DIM
 
 AXES = (44, 42, 42)  # head dims of time, height, width in the Wan models
@@ -68,37 +68,40 @@ def _rows(x: torch.Tensor, size: int):
     return x, batch, st[-3], st[-2]
 
 
+def _axes_ok(axes) -> bool:
+    return len(axes) == 3 and sum(axes) == HEAD_DIM and all(d >= 0 and d % 2 == 0 for d in axes)
+
+
 def _rope_impl(q, k, positions, table, axes, inverse):
     dtype = q.dtype
     assert k.dtype is dtype and (dtype is torch.bfloat16 or dtype is torch.float32), "q and k are both bf16 or both fp32"
-    dims = q.dim()
-    assert k.dim() == dims and dims in (3, 4), "(s, h, 128) or (b, s, h, 128)"
-    qs, kshape = q.shape, k.shape
-    assert qs[:-2] == kshape[:-2]
-    assert qs[-1] == HEAD_DIM and kshape[-1] == HEAD_DIM, "specialized for head_dim=128"
-    assert len(axes) == 3 and sum(axes) == HEAD_DIM and all(d >= 0 and d % 2 == 0 for d in axes), \
-        "three even axes that add up to head_dim"
-    s, h, h_kv = qs[-3], qs[-2], kshape[-2]
+    qs, kshape, ps = q.shape, k.shape, positions.shape
+    dims = len(qs)
+    assert len(kshape) == dims and (dims == 3 or dims == 4), "(s, h, 128) or (b, s, h, 128)"
+    s, h, d = qs[-3:]
+    ks, h_kv, dk = kshape[-3:]
     b = qs[0] if dims == 4 else 1
-    ps = positions.shape
+    assert ks == s and (dims == 3 or kshape[0] == b), "q and k have the same tokens"
+    assert d == HEAD_DIM and dk == HEAD_DIM, "specialized for head_dim=128"
+    assert axes is AXES or _axes_ok(axes), "three even axes that add up to head_dim"
     assert positions.dtype is torch.int32 and (ps == (s, 3) or (dims == 4 and ps == (b, s, 3))), \
         "positions are int32 (s, 3) or one (s, 3) per batch item"
     assert table.dtype is torch.float32 and table.dim() == 3 and table.shape[1:] == (HEAD_DIM // 2, 2)
-    assert table.shape[0] >= 1
+    rows = table.shape[0]
+    assert rows >= 1
     device = q.device
     assert q.is_cuda and k.device == device and positions.device == device and table.device == device, \
         "tensors must be on one CUDA device"
-    oq = torch.empty(qs, dtype=dtype, device=device)
-    ok = torch.empty(kshape, dtype=dtype, device=device)
-    if b == 0 or s == 0 or h + h_kv == 0:
-        return oq, ok
     size = 2 if dtype is torch.bfloat16 else 4
     q, q0, q1, q2 = _rows(q, size)
     k, k0, k1, k2 = _rows(k, size)
+    oq, ok = _contiguous_like(q), _contiguous_like(k)
+    if b == 0 or s == 0 or h + h_kv == 0:
+        return oq, ok
     positions = positions.contiguous()
     if not table.is_contiguous() or table.data_ptr() % 16:
         table = table.clone(memory_format=torch.contiguous_format)
-    cfg = _lib.RopeCfg(0 if size == 2 else 1, 1 if inverse else 0, table.shape[0], axes[0] // 2, axes[1] // 2, 0,
+    cfg = _lib.RopeCfg(0 if size == 2 else 1, 1 if inverse else 0, rows, axes[0] // 2, axes[1] // 2, 0,
                        q0, q1, q2, k0, k1, k2, 3 * s if len(ps) == 3 else 0)
     _launch(_lib.lib().wf_rope, device, q.data_ptr(), k.data_ptr(), oq.data_ptr(), ok.data_ptr(), table.data_ptr(),
             positions.data_ptr(), b, s, h, h_kv, cfg)
