@@ -157,11 +157,17 @@ struct PackedBwdParams {
 };
 struct PackedConvertParams {
   const int4* head;
-  const int4* tiles;        // dq: q_tiles; split: split_tiles
-  const float* accum[2];    // the dQ accumulator (h, tile_stride), or partial dK and dV (parts, h_kv)
-  __nv_bfloat16* out[2];    // (total, heads, 128)
-  size_t tile_stride;
-  int split, heads;
+  const int4* q_tiles;
+  const int4* split_tiles;
+  const float* dq_accum;    // (h, q_tile_stride) tiles
+  const float* dk_part;     // (parts, h_kv) tiles
+  const float* dv_part;
+  __nv_bfloat16* dq;
+  __nv_bfloat16* dk;
+  __nv_bfloat16* dv;
+  size_t q_tile_stride;
+  unsigned dq_blocks, split_blocks;  // 4 * tiles * heads
+  int h, h_kv;
   float scale;
 };
 cudaError_t packed_setup();

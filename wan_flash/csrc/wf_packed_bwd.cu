@@ -123,6 +123,8 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
   const int warp = (int)warp_id();
   const int lane = (int)lane_id();
 
+  // (Setting up barriers and tensor memory before this wait slowed full attention
+  // over 7800 tokens by 4 %: the grid has room for more items than there are.)
   griddep_wait();  // the plan's lists, and what the preprocess wrote
   if ((int)blockIdx.x >= p.head[0].x * p.h_kv) return;
   int kvh;
@@ -524,59 +526,74 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
   if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
-// fp32 tiles -> bf16 rows, times a scale: the dQ accumulator, or the sums of
-// the pieces' partial dK and dV in a fixed order (blockIdx.z: which).  Rows of
-// dQ outside any sequence become 0 (NaN where the offsets were impossible).
-// Bound: HBM.  grid (4 * tiles, heads[, 2]), 256 threads: 32 rows x 128 columns.
+// fp32 tiles -> bf16 rows, times a scale: the dQ accumulator, and the sums of
+// the pieces' partial dK and dV in a fixed order.  Rows of dQ outside any
+// sequence become 0 (NaN where the offsets were impossible).  Bound: HBM, and
+// latency where a tile has many parts (two parts' loads are in flight).  grid
+// dq_blocks + 2 * split_blocks, 256 threads: 32 rows x 128 columns of one head.
 __global__ void __launch_bounds__(256) wf_packed_convert_kernel(PackedConvertParams p) {
   __shared__ float tile[32][132];
   griddep_launch_dependents();
   griddep_wait();
-  const int t = blockIdx.x >> 2, row0 = (blockIdx.x & 3) * 32, h = blockIdx.y, which = blockIdx.z;
-  const int4 head = *p.head;
-  if (t >= (p.split ? head.z : head.x)) return;
-  const int4 w = p.tiles[t];  // first row, rows, dq: inside / split: first part, parts
+  const bool split = blockIdx.x >= p.dq_blocks;
+  unsigned i = split ? blockIdx.x - p.dq_blocks : blockIdx.x;
+  const bool is_dv = split && i >= p.split_blocks;
+  if (is_dv) i -= p.split_blocks;
+  const int row0 = (int)(i & 3) * 32;
+  const int heads = split ? p.h_kv : p.h;
+  const int t = (int)(i >> 2) / heads, h = (int)(i >> 2) - t * heads;
+  if (t >= (split ? p.head[0].z : p.head[1].x)) return;
+  const int4 w = split ? p.split_tiles[t] : p.q_tiles[t];  // first row, rows, first part / inside, parts
   if (row0 >= w.y) return;
   const int half = row0 >> 6, r0 = row0 & 63;
-  const bool inside = p.split || w.z != 0;
+  const bool inside = split || w.z != 0;
   if (inside) {
-    const int parts = p.split ? w.w : 1;
-    const size_t at = p.split ? (size_t)w.z * p.heads + h : (size_t)h * p.tile_stride + t;
-    const size_t step = (size_t)p.heads * 16384;
-    const float* src = (which ? p.accum[1] : p.accum[0]) + at * 16384 + half * 8192;
+    const int parts = split ? w.w : 1;
+    const size_t at = split ? (size_t)w.z * heads + h : (size_t)h * p.q_tile_stride + t;
+    const size_t step = (size_t)heads * 16384;
+    const float* src = (!split ? p.dq_accum : is_dv ? p.dv_part : p.dk_part) + at * 16384 + half * 8192;
     float4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < parts; ++s, src += step) {
+    for (int k = 0; k < 4; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < parts; s += 2) {
+      float4 x[2][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int idx = threadIdx.x + i * 256;  // 32 groups of 4 columns x 32 rows
-        const float4 x = *reinterpret_cast<const float4*>(src + ((idx >> 5) * 64 + r0 + (idx & 31)) * 4);
-        v[i].x += x.x, v[i].y += x.y, v[i].z += x.z, v[i].w += x.w;
-      }
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int idx = threadIdx.x + k * 256;  // 32 groups of 4 columns x 32 rows
+          x[q][k] = s + q < parts ? *reinterpret_cast<const float4*>(src + (s + q) * step + ((idx >> 5) * 64 + r0 + (idx & 31)) * 4)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k].x += x[q][k].x, v[k].y += x[q][k].y, v[k].z += x[q][k].z, v[k].w += x[q][k].w;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int idx = threadIdx.x + i * 256;
-      *reinterpret_cast<float4*>(&tile[idx & 31][4 * (idx >> 5)]) = v[i];
+    for (int k = 0; k < 4; ++k) {
+      const int idx = threadIdx.x + k * 256;
+      *reinterpret_cast<float4*>(&tile[idx & 31][4 * (idx >> 5)]) = v[k];
     }
   }
   __syncthreads();
-  const uint32_t fill = head.y ? 0x7fff7fffu : 0u;
+  const uint32_t fill = p.head[1].y ? 0x7fff7fffu : 0u;
+  const float scale = split ? 1.f : p.scale;  // dk was scaled where it left the tensor core
+  __nv_bfloat16* const out = !split ? p.dq : is_dv ? p.dv : p.dk;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int idx = threadIdx.x + i * 256;  // 32 rows x 16 chunks of 8
+  for (int k = 0; k < 2; ++k) {
+    const int idx = threadIdx.x + k * 256;  // 32 rows x 16 chunks of 8
     const int rw = idx >> 4, ch = idx & 15;
     if (row0 + rw >= w.y) continue;
     uint4 o = make_uint4(fill, fill, fill, fill);
     if (inside) {
       const float* x = &tile[rw][ch * 8];
-      o.x = pack_bf16(x[0] * p.scale, x[1] * p.scale);
-      o.y = pack_bf16(x[2] * p.scale, x[3] * p.scale);
-      o.z = pack_bf16(x[4] * p.scale, x[5] * p.scale);
-      o.w = pack_bf16(x[6] * p.scale, x[7] * p.scale);
+      o.x = pack_bf16(x[0] * scale, x[1] * scale);
+      o.y = pack_bf16(x[2] * scale, x[3] * scale);
+      o.z = pack_bf16(x[4] * scale, x[5] * scale);
+      o.w = pack_bf16(x[6] * scale, x[7] * scale);
     }
-    *reinterpret_cast<uint4*>((which ? p.out[1] : p.out[0]) + ((size_t)(w.x + row0 + rw) * p.heads + h) * 128 + ch * 8) = o;
+    *reinterpret_cast<uint4*>(out + ((size_t)(w.x + row0 + rw) * heads + h) * 128 + ch * 8) = o;
   }
 }
 

@@ -220,7 +220,8 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   const PackedBwdWorkspace ws(n, total_q, total_k, h, h_kv, cfg, sms);
   if (workspace_bytes < ws.bytes)
     return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
-  if (most.items * h_kv > 0x7fffffffLL || ws.q_tile_stride * 4 > 0x7fffffffULL)
+  const long long dq_blocks = 4LL * ws.q_tile_stride * h, split_blocks = most.parts ? 4LL * most.split_tiles * h_kv : 0;
+  if (most.items * h_kv > 0x7fffffffLL || dq_blocks + 2 * split_blocks > 0x7fffffffLL)
     return fail(WF_ERR_UNSUPPORTED, "%lld work items exceed the grid limit", most.items * h_kv);
   CUtensorMap mq, mk, mv, mdo;
   if ((rc = make_bshd_map(&mq, q, 1, total_q, h)) || (rc = make_bshd_map(&mk, k, 1, total_k, h_kv)) ||
@@ -274,24 +275,15 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
                 1u, mq, mk, mv, mdo, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd launch");
   PackedConvertParams c = {};
-  c.head = pp.head + 1;
-  c.tiles = pp.q_tiles;
-  c.accum[0] = p.dq_accum;
-  c.out[0] = reinterpret_cast<__nv_bfloat16*>(dq);
-  c.tile_stride = ws.q_tile_stride;
-  c.heads = h;
+  c.head = pp.head;
+  c.q_tiles = pp.q_tiles, c.split_tiles = pp.split_tiles;
+  c.dq_accum = p.dq_accum, c.dk_part = p.dk_part, c.dv_part = p.dv_part;
+  c.dq = reinterpret_cast<__nv_bfloat16*>(dq), c.dk = p.dk, c.dv = p.dv;
+  c.q_tile_stride = ws.q_tile_stride;
+  c.dq_blocks = (unsigned)dq_blocks, c.split_blocks = (unsigned)split_blocks;
+  c.h = h, c.h_kv = h_kv;
   c.scale = p.scale;
-  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, c);
-  if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd dq convert launch");
-  if (most.parts > 0) {
-    c.head = pp.head;
-    c.tiles = pp.split_tiles;
-    c.accum[0] = p.dk_part, c.accum[1] = p.dv_part;
-    c.out[0] = p.dk, c.out[1] = p.dv;
-    c.split = 1, c.heads = h_kv;
-    c.scale = 1.f;  // dk was scaled where it left the tensor core
-    e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(4 * most.split_tiles), h_kv, 2), dim3(256), 0, st, true, 1u, c);
-    if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd dk/dv convert launch");
-  }
+  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(dq_blocks + 2 * split_blocks)), dim3(256), 0, st, true, 1u, c);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd convert launch");
   return launch_check("wf_packed_bwd launch");
 }
