@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
           const unsigned ak = __shfl_sync(0xffffffffu, at_k, r), av = __shfl_sync(0xffffffffu, at_v, r);
           const bool row_ok = (here >> r) & 1;
           cp_async16(dst + i * 2 * kRowBytes, src_k + (row_ok ? (unsigned long long)ak * 16 : 0), row_ok ? 16 : 0);
-          cp_async16(dst + i * 2 * kRowBytes + kHalfBytes, src_v + (row_ok ? (unsigned long long)av * 16 : 0), row_ok ? 16 : 0);
+          cp_async16(dst + i * 2 * kRowBytes + kHalfBytes, src_v + (row_ok ? (unsigned long long)av * 16 : 0),
+                     row_ok ? 16 : 0);
         }
       }
       if (++ahead_at < ahead.row_at + ahead.t1) {
@@ -422,7 +423,10 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = (i < 2 ? in0 : in1) ? (kQShared ? s[n][i] : s[n][i] + s2[n][i]) * p.scale_log2 : -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+          const float x = kQShared ? s[n][i] : s[n][i] + s2[n][i];
+          s[n][i] = (i < 2 ? in0 : in1) ? x * p.scale_log2 : -INFINITY;
+        }
         float pr[4];
         float f[2];
 #pragma unroll

@@ -562,8 +562,9 @@ __global__ void __launch_bounds__(256) wf_packed_convert_kernel(PackedConvertPar
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int idx = threadIdx.x + k * 256;  // 32 groups of 4 columns x 32 rows
-          x[q][k] = s + q < parts ? *reinterpret_cast<const float4*>(src + (s + q) * step + ((idx >> 5) * 64 + r0 + (idx & 31)) * 4)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[q][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (s + q < parts)
+            x[q][k] = *reinterpret_cast<const float4*>(src + (s + q) * step + ((idx >> 5) * 64 + r0 + (idx & 31)) * 4);
         }
 #pragma unroll
       for (int q = 0; q < 2; ++q)

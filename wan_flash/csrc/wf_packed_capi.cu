@@ -56,7 +56,8 @@ struct PackedBwdBounds {
 };
 
 struct PackedBwdWorkspace {  // byte offsets
-  size_t head = 0, base, items, q_tiles, split_tiles, neg_lse_log2, dpsum, dq_accum, dk_part, dv_part, sem, sem_bytes, bytes;
+  size_t head = 0, base, items, q_tiles, split_tiles, neg_lse_log2, dpsum, dq_accum, dk_part, dv_part, sem,
+      sem_bytes, bytes;
   size_t q_tile_stride;
   PackedBwdWorkspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg, int sms) {
     const PackedBwdBounds most(n, total_q, total_k, h, h_kv, cfg->nsplit, sms);
@@ -79,7 +80,8 @@ struct PackedBwdWorkspace {  // byte offsets
 
 int packed_bwd_cfg_check(const wf_packed_bwd_cfg* cfg) {
   if (!cfg) return fail(WF_ERR_INVALID_ARG, "null cfg");
-  if (cfg->nsplit < 0 || cfg->nsplit > 1024) return fail(WF_ERR_INVALID_ARG, "nsplit=%d outside [0, 1024]", cfg->nsplit);
+  if (cfg->nsplit < 0 || cfg->nsplit > 1024)
+    return fail(WF_ERR_INVALID_ARG, "nsplit=%d outside [0, 1024]", cfg->nsplit);
   return WF_OK;
 }
 
@@ -91,7 +93,8 @@ int packed_check(int n, int total_q, int total_k, int h, int h_kv, int causal) {
   if (h > 65535) return fail(WF_ERR_UNSUPPORTED, "h=%d exceeds 65535", h);
   // tile coordinates and item numbers are 32-bit
   if (n > (1 << 24) || total_q > (1 << 30) || total_k > (1 << 30))
-    return fail(WF_ERR_UNSUPPORTED, "n=%d, total_q=%d, total_k=%d exceed 2^24 sequences of 2^30 rows", n, total_q, total_k);
+    return fail(WF_ERR_UNSUPPORTED, "n=%d, total_q=%d, total_k=%d exceed 2^24 sequences of 2^30 rows", n, total_q,
+                total_k);
   if (packed_max_tiles(total_q, n, 128) * h > 0x7fffffffLL || packed_max_tiles(total_k, n, 128) * h > 0x7fffffffLL)
     return fail(WF_ERR_UNSUPPORTED, "too many (tile, head) items");
   return WF_OK;
@@ -103,7 +106,8 @@ cudaError_t packed_setup() {
   cudaError_t e =
       cudaFuncSetAttribute(wf_packed_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pfwd::kSmemBytes);
   for (auto k : {wf_packed_bwd_kernel<false>, wf_packed_bwd_kernel<true>})
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd::kSmemBytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd::kSmemBytes);
   return e;
 }
 
@@ -131,7 +135,8 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_residual) ||
       !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(q_offsets) & 3) ||
       (reinterpret_cast<uintptr_t>(k_offsets) & 3))
-    return fail(WF_ERR_MISALIGNED, "q/k/v/o/o_residual/workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
+    return fail(WF_ERR_MISALIGNED, "q/k/v/o/o_residual/workspace must be 16-byte aligned, lse and offsets 4-byte"
+                                    " aligned");
   int dev;
   if ((rc = device_setup(&dev))) return rc;
   const int sms = g_dev_sms[dev];
@@ -199,7 +204,8 @@ extern "C" int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, i
 }
 
 extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o,
-                             const void* o_residual, const float* lse, const void* dO, const int* q_offsets, const int* k_offsets, void* dq, void* dk, void* dv,
+                             const void* o_residual, const float* lse, const void* dO, const int* q_offsets,
+                             const int* k_offsets, void* dq, void* dk, void* dv,
                              void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv,
                              int causal, const wf_packed_bwd_cfg* cfg, void* stream) {
   int rc;
@@ -209,10 +215,12 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
     return fail(WF_ERR_UNSUPPORTED, "no queries or no keys: the caller must zero the gradients");
   if (!q || !k || !v || !o || !lse || !dO || !q_offsets || !k_offsets || !dq || !dk || !dv || !workspace)
     return fail(WF_ERR_INVALID_ARG, "null pointer");
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_residual) || !aligned16(dO) || !aligned16(dq) ||
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_residual) ||
+      !aligned16(dO) || !aligned16(dq) ||
       !aligned16(dk) || !aligned16(dv) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) ||
       (reinterpret_cast<uintptr_t>(q_offsets) & 3) || (reinterpret_cast<uintptr_t>(k_offsets) & 3))
-    return fail(WF_ERR_MISALIGNED, "tensors and workspace must be 16-byte aligned, lse and offsets 4-byte aligned");
+    return fail(WF_ERR_MISALIGNED, "tensors and workspace must be 16-byte aligned, lse and offsets 4-byte"
+                                    " aligned");
   int dev;
   if ((rc = device_setup(&dev))) return rc;
   const int sms = g_dev_sms[dev];
@@ -271,8 +279,9 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
                 reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(o_residual),
                 reinterpret_cast<const __nv_bfloat16*>(dO), lse);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd preprocess launch");
-  e = launch_ex(causal ? wf_packed_bwd_kernel<true> : wf_packed_bwd_kernel<false>, dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true,
-                1u, mq, mk, mv, mdo, p);
+  e = launch_ex(causal ? wf_packed_bwd_kernel<true> : wf_packed_bwd_kernel<false>,
+                dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true, 1u, mq, mk, mv, mdo,
+                p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd launch");
   PackedConvertParams c = {};
   c.head = pp.head;
@@ -283,7 +292,8 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   c.dq_blocks = (unsigned)dq_blocks, c.split_blocks = (unsigned)split_blocks;
   c.h = h, c.h_kv = h_kv;
   c.scale = p.scale;
-  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(dq_blocks + 2 * split_blocks)), dim3(256), 0, st, true, 1u, c);
+  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(dq_blocks + 2 * split_blocks)), dim3(256), 0, st, true, 1u,
+                c);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd convert launch");
   return launch_check("wf_packed_bwd launch");
 }

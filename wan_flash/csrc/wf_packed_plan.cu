@@ -411,7 +411,10 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) p.head[0] = make_int4(p.ordered ? items : one_round ? sh.items : sh.start[kPlanBuckets], v.bad, sh.split_tiles, 0);
+  if (threadIdx.x == 0) {
+    const int n_items = p.ordered ? items : one_round ? sh.items : sh.start[kPlanBuckets];
+    p.head[0] = make_int4(n_items, v.bad, sh.split_tiles, 0);
+  }
 }
 
 // Work index i (of items * heads) -> item and head: bucket by bucket, inside a

@@ -68,7 +68,8 @@ def _bwd_cfg_bytes(index: int, n: int, total_q: int, total_k: int, h: int, h_kv:
     """The C options and the workspace's size on device `index`."""
     cfg, size = _lib.PackedBwdCfg(min(nsplit, 1024), 1 if deterministic else 0), ctypes.c_size_t()
     with torch.cuda.device(index):
-        _lib.check(_lib.lib().wf_packed_bwd_workspace(n, total_q, total_k, h, h_kv, ctypes.byref(cfg), ctypes.byref(size)))
+        _lib.check(_lib.lib().wf_packed_bwd_workspace(n, total_q, total_k, h, h_kv, ctypes.byref(cfg),
+                                                      ctypes.byref(size)))
     return cfg, size.value
 
 
@@ -124,7 +125,8 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     cfg, size = _bwd_cfg_bytes(device.index, n, total_q, total_k, h, h_kv, f.nsplit, f.deterministic)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
     _launch(_lib.lib().wf_packed_bwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            None if o_residual is None else o_residual.data_ptr(), lse.data_ptr(), do.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            None if o_residual is None else o_residual.data_ptr(), lse.data_ptr(), do.data_ptr(), q_offsets.data_ptr(),
+            k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             ws.data_ptr(), size, n, total_q, total_k, h, h_kv, 1 if causal else 0, cfg)
     return dq, dk, dv
 
