@@ -252,7 +252,7 @@ int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offs
                   int h_kv, int causal, void* stream);
 
 typedef struct wf_packed_bwd_cfg {
-  int nsplit;        /* 0 = the device cuts long walks into pieces (about three
+  int nsplit;        /* 0 = the device cuts long walks into pieces (about two
                         per SM, one where there are few key tiles); n > 0: pieces of 1/n of the
                         longest walk.  Pieces leave fp32 partial dk and dv that
                         are summed in a fixed order */

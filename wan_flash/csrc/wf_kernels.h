@@ -104,12 +104,12 @@ struct PackedPlanParams {
   int4* q_tiles;            // {first row, rows, 1 inside a sequence, 0}
   int4* split_tiles;        // {first row, rows, first part, parts}
 };
-// Backward pieces: about three per SM's even share, of 8 units at least; or,
+// Backward pieces: about two per SM's even share, of 8 units at least; or,
 // with few key tiles, as many as make one item per SM, of 2 units at least.  A
 // piece's own cost (prologue, K and V, partial dK and dV) is about two units.
 constexpr int kPackedMinChunk = 2;
 constexpr int kPackedMinChunkFull = 8;
-constexpr int kPackedPiecesPerSm = 3;
+constexpr int kPackedPiecesPerSm = 2;
 constexpr int kPackedPieceCost = 2;
 // Forward pieces: of at least 8 blocks (16 us), of an SM's even share of all
 // blocks or, with few tiles, as many as make one item per SM; only where the
@@ -166,7 +166,7 @@ struct PackedConvertParams {
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
   size_t q_tile_stride;
-  unsigned dq_blocks, split_blocks;  // 4 * tiles * heads
+  unsigned dq_blocks, split_blocks;  // 2 * tiles * heads
   int h, h_kv;
   float scale;
 };

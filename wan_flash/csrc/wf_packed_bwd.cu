@@ -528,74 +528,64 @@ __global__ void __launch_bounds__(bwd::kThreads, 1)
 
 // fp32 tiles -> bf16 rows, times a scale: the dQ accumulator, and the sums of
 // the pieces' partial dK and dV in a fixed order.  Rows of dQ outside any
-// sequence become 0 (NaN where the offsets were impossible).  Bound: HBM, and
-// latency where a tile has many parts (two parts' loads are in flight).  grid
-// dq_blocks + 2 * split_blocks, 256 threads: 32 rows x 128 columns of one head.
+// sequence become 0 (NaN where the offsets were impossible).
+// Bound: HBM.  A thread turns two groups of four columns of a row into 16 bytes;
+// a warp has 8 rows x 4 such chunks, so it reads 128-byte runs and writes 64-byte
+// runs without a detour through shared memory, eight loads a thread in flight.
+// grid dq_blocks + 2 * split_blocks, 256 threads: 64 rows x 128 columns of one head.
 __global__ void __launch_bounds__(256) wf_packed_convert_kernel(PackedConvertParams p) {
-  __shared__ float tile[32][132];
   griddep_launch_dependents();
   griddep_wait();
   const bool split = blockIdx.x >= p.dq_blocks;
   unsigned i = split ? blockIdx.x - p.dq_blocks : blockIdx.x;
   const bool is_dv = split && i >= p.split_blocks;
   if (is_dv) i -= p.split_blocks;
-  const int row0 = (int)(i & 3) * 32;
+  const int half = (int)(i & 1);
   const int heads = split ? p.h_kv : p.h;
-  const int t = (int)(i >> 2) / heads, h = (int)(i >> 2) - t * heads;
+  const int t = (int)(i >> 1) / heads, h = (int)(i >> 1) - t * heads;
   if (t >= (split ? p.head[0].z : p.head[1].x)) return;
   const int4 w = split ? p.split_tiles[t] : p.q_tiles[t];  // first row, rows, first part / inside, parts
-  if (row0 >= w.y) return;
-  const int half = row0 >> 6, r0 = row0 & 63;
-  const bool inside = split || w.z != 0;
-  if (inside) {
-    const int parts = split ? w.w : 1;
-    const size_t at = split ? (size_t)w.z * heads + h : (size_t)h * p.q_tile_stride + t;
-    const size_t step = (size_t)heads * 16384;
-    const float* src = (!split ? p.dq_accum : is_dv ? p.dv_part : p.dk_part) + at * 16384 + half * 8192;
-    float4 v[4];
+  const int rows = w.y - half * 64;
+  if (rows <= 0) return;
+  __nv_bfloat16* const out = (!split ? p.dq : is_dv ? p.dv : p.dk) + ((size_t)(w.x + half * 64) * heads + h) * 128;
+  const size_t row_stride = (size_t)heads * 128;
+  // this thread's rows r + 8 k' and chunks c + 4 k'' of the 64 x 16
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = (lane >> 2) + 8 * warp, c = lane & 3;
+  if (!split && w.z == 0) {
+    const uint32_t fill = p.head[1].y ? 0x7fff7fffu : 0u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < parts; s += 2) {
-      float4 x[2][4];
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int idx = threadIdx.x + k * 256;  // 32 groups of 4 columns x 32 rows
-          x[q][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (s + q < parts)
-            x[q][k] = *reinterpret_cast<const float4*>(src + (s + q) * step + ((idx >> 5) * 64 + r0 + (idx & 31)) * 4);
-        }
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k].x += x[q][k].x, v[k].y += x[q][k].y, v[k].z += x[q][k].z, v[k].w += x[q][k].w;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int idx = threadIdx.x + k * 256;
-      *reinterpret_cast<float4*>(&tile[idx & 31][4 * (idx >> 5)]) = v[k];
-    }
+    for (int k = 0; k < 4; ++k)
+      if (r < rows) st_global_v4(out + r * row_stride + (c + 4 * k) * 8, fill, fill, fill, fill);
+    return;
   }
-  __syncthreads();
-  const uint32_t fill = p.head[1].y ? 0x7fff7fffu : 0u;
+  if (r >= rows) return;
+  const int parts = split ? w.w : 1;
+  const size_t at = split ? (size_t)w.z * heads + h : (size_t)h * p.q_tile_stride + t;
+  const float4* src = reinterpret_cast<const float4*>((!split ? p.dq_accum : is_dv ? p.dv_part : p.dk_part) + at * 16384 +
+                                                      half * 8192) + r;
+  const size_t step = (size_t)heads * 4096;
+  float4 v[4][2];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) v[k][g] = src[(2 * (c + 4 * k) + g) * 64];
+  for (int s = 1; s < parts; ++s) {
+    src += step;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 x = src[(2 * (c + 4 * k) + g) * 64];
+        v[k][g].x += x.x, v[k][g].y += x.y, v[k][g].z += x.z, v[k][g].w += x.w;
+      }
+  }
   const float scale = split ? 1.f : p.scale;  // dk was scaled where it left the tensor core
-  __nv_bfloat16* const out = !split ? p.dq : is_dv ? p.dv : p.dk;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int idx = threadIdx.x + k * 256;  // 32 rows x 16 chunks of 8
-    const int rw = idx >> 4, ch = idx & 15;
-    if (row0 + rw >= w.y) continue;
-    uint4 o = make_uint4(fill, fill, fill, fill);
-    if (inside) {
-      const float* x = &tile[rw][ch * 8];
-      o.x = pack_bf16(x[0] * scale, x[1] * scale);
-      o.y = pack_bf16(x[2] * scale, x[3] * scale);
-      o.z = pack_bf16(x[4] * scale, x[5] * scale);
-      o.w = pack_bf16(x[6] * scale, x[7] * scale);
-    }
-    *reinterpret_cast<uint4*>(out + ((size_t)(w.x + row0 + rw) * heads + h) * 128 + ch * 8) = o;
-  }
+  for (int k = 0; k < 4; ++k)
+    st_global_v4(out + r * row_stride + (c + 4 * k) * 8, pack_bf16(v[k][0].x * scale, v[k][0].y * scale),
+                 pack_bf16(v[k][0].z * scale, v[k][0].w * scale), pack_bf16(v[k][1].x * scale, v[k][1].y * scale),
+                 pack_bf16(v[k][1].z * scale, v[k][1].w * scale));
 }
 
 }  // namespace wf

@@ -228,7 +228,7 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   const PackedBwdWorkspace ws(n, total_q, total_k, h, h_kv, cfg, sms);
   if (workspace_bytes < ws.bytes)
     return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
-  const long long dq_blocks = 4LL * ws.q_tile_stride * h, split_blocks = most.parts ? 4LL * most.split_tiles * h_kv : 0;
+  const long long dq_blocks = 2LL * ws.q_tile_stride * h, split_blocks = most.parts ? 2LL * most.split_tiles * h_kv : 0;
   if (most.items * h_kv > 0x7fffffffLL || dq_blocks + 2 * split_blocks > 0x7fffffffLL)
     return fail(WF_ERR_UNSUPPORTED, "%lld work items exceed the grid limit", most.items * h_kv);
   CUtensorMap mq, mk, mv, mdo;

@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
   if (p.nsplit > 0) {
     chunk = max(1, (int)(((unsigned)most + p.nsplit - 1) / p.nsplit));
   } else {
-    // pieces of a third of an SM's even share, so their uneven ends even out ...
+    // pieces of half an SM's even share, so their uneven ends even out ...
     chunk = (int)min((unsigned long long)0x7fffffff,
                      max((unsigned long long)kPackedMinChunkFull, sh.units * p.h_kv / p.pieces + 1));
     if ((long long)n_tiles * p.h_kv <= p.sms) {
