@@ -101,6 +101,25 @@ def test_a_sequence_does_not_see_its_neighbours():
 
 
 @pytest.mark.gpu
+def test_rows_that_see_no_key_reach_no_gradient():
+    features.set_bwd_overrides(deterministic=True)
+    lq, lk = [200, 300, 141], [130, 5, 140]
+    q, k, v, do, qo, ko = make(lq, lk, 4, 2, seed=6)
+
+    def grads():
+        o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, causal=True, residual=True)
+        return o, *wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=True, o_residual=res)
+
+    want = grads()
+    for a, n, m in zip(qo.tolist(), lq, lk):  # the first n - m rows of each
+        assert (want[0][a:a + n - m] == 0).all() and (want[1][a:a + n - m] == 0).all()
+        q[a:a + n - m] = float("nan")
+        do[a:a + n - m] = float("nan")
+    for g, w in zip(grads(), want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq,lk,h,hk,causal", CASES)
 def test_residual_of_o(lq, lk, h, hk, causal):
     """o + residual is o to 16 bits, and with it dq and dk do not carry o's rounding through D."""
@@ -203,6 +222,17 @@ def test_training_step_captured_and_replayed_with_other_offsets():
         torch.cuda.synchronize()
         _lib.check_device()
         check_bwd(q, k, v, do, qo, qo, True, *out[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,h,hk,causal", [([256] * 40, 8, 8, False), ([4000], 12, 12, False), ([900, 2300, 17], 16, 4, True)])
+def test_dk_and_dv_are_reproducible(lens, h, hk, causal):
+    q, k, v, do, qo, ko = make(lens, lens, h, hk)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    _, dk, dv = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+    for _ in range(5):
+        again = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+        assert torch.equal(again[1], dk) and torch.equal(again[2], dv)
 
 
 @pytest.mark.gpu

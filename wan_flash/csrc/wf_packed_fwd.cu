@@ -96,11 +96,12 @@ struct __align__(16) PackedFwdItem {
 };
 static_assert(sizeof(PackedFwdItem) == 64, "four 16-byte words");
 
-// Zero rows [first, 128) of a 128-row tile of two 64-column boxes (a
-// converged warp; the swizzle permutes 16-byte chunks inside a row only), and
-// order the stores before the tensor core's reads.
-__device__ __forceinline__ void packed_zero_rows(uint32_t tile, int first) {
-  for (int i = first * 8 + (int)lane_id(); i < 128 * 8; i += 32) {
+// Zero rows [0, none) and [first, 128) of a 128-row tile of two 64-column boxes
+// (a converged warp; the swizzle permutes 16-byte chunks inside a row only),
+// and order the stores before the tensor core's reads.
+__device__ __forceinline__ void packed_zero_rows(uint32_t tile, int first, int none = 0) {
+  for (int i = (none > 0 ? 0 : first * 8) + (int)lane_id(); i < 128 * 8; i += 32) {
+    if (i >= none * 8 && i < first * 8) continue;
     st_shared_v4(tile + i * 16, 0u, 0u, 0u, 0u);
     st_shared_v4(tile + 128 * 128 + i * 16, 0u, 0u, 0u, 0u);
   }
