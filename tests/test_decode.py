@@ -150,6 +150,36 @@ def test_strided_cache_and_queries():
 
 
 @pytest.mark.gpu
+def test_shared_pages():
+    """Sequences that share a prefix's pages, and one page in two places of a sequence."""
+    q, k, v, table, lengths = make([100, 90, 33], 4, 2, 16)
+    table[1, :3] = table[0, :3]
+    table[2, 1] = table[2, 0]
+    o, lse = wan_flash_decode(q, k, v, table, lengths)
+    _lib.check_device()
+    check(q, k, v, table, lengths, o, lse)
+
+
+@pytest.mark.gpu
+def test_cache_places_past_32_bits():
+    """Pages behind the first 2^31 elements (2^32 bytes) of a cache, by number and by stride."""
+    q, k, v, table, lengths = make([300, 17], 4, 2, 16)
+    want = wan_flash_decode(q, k, v, table, lengths)
+    n, page = k.shape[0], 16 * 2 * 128
+    far = 2**31 // page * 9 // 8
+    big = torch.empty(2, far + n, 16, 2, 128, dtype=torch.bfloat16, device="cuda")
+    big[0, far:], big[1, far:] = k, v
+    used = torch.where(table < n, table + far, table)
+    spread = torch.as_strided(big, (2, n, 16, 2, 128), (big.stride(0), (far + n) * page // n // 8 * 8, 256, 128, 1))
+    for args in ((big[0], big[1], used), (spread[0], spread[1], table)):
+        if args[2] is table:
+            spread[0], spread[1] = k, v
+        got = wan_flash_decode(q, *args, lengths)
+        _lib.check_device()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["page", "negative page", "length", "negative length"])
 def test_impossible_pages_and_lengths(what):
     q, k, v, table, lengths = make([100, 50, 33], 4, 2, 16)

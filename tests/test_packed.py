@@ -75,6 +75,20 @@ def test_forward(lq, lk, h, hk, causal, lead, tail):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,lead,tail,causal", [
+    ([300, 140, 1], None, 0, 40000, False),       # every SM has many tiles of padding behind its last with keys
+    ([300, 140, 1], None, 40000, 0, True),
+    ([300, 40000, 129], [300, 0, 257], 0, 0, False),
+    ([40000, 77], [100, 77], 0, 0, True),         # most rows see no key
+])
+def test_many_tiles_without_keys(lq, lk, lead, tail, causal):
+    q, k, v, _, qo, ko = make(lq, lk or lq, 12, 4, lead, tail)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    _lib.check_device()
+    check_fwd(q, k, v, qo, ko, causal, o, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
 def test_large_scores(causal):
     """N(0, 3^2) q and k: row maxima that keep moving, so O is rescaled."""

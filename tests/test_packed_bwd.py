@@ -225,6 +225,31 @@ def test_training_step_captured_and_replayed_with_other_offsets():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_past_32_bits(causal):
+    """Sequences behind 2^31 elements give what they give at the start, bit for bit
+    (with whole walks: the number of key tiles, padding's too, decides on pieces)."""
+    features.set_bwd_overrides(nsplit=1, deterministic=True)
+    h, lens = 16, [300, 1, 140]
+    q, k, v, do, qo, ko = make(lens, lens, h, h)
+    o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal, residual=True)
+    want = o, lse, *wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal, o_residual=res)
+    lead, n = 2**31 // (h * 128) + 77, sum(lens)
+    big = []
+    for x in (q, k, v, do):
+        big.append(torch.empty(lead + n, h, 128, dtype=torch.bfloat16, device="cuda"))
+        big[-1][lead:] = x
+    at = (qo + lead).int()
+    o, lse, res = wan_flash_packed_fwd(*big[:3], at, causal=causal, residual=True)
+    got = o, lse, *wan_flash_packed_bwd(*big[:3], o, lse, big[3], at, causal=causal, o_residual=res)
+    _lib.check_device()
+    for g, w in zip(got, want):
+        g, w = (g[:, lead:], w) if g is lse else (g[lead:], w)
+        assert torch.equal(g, w)
+    assert not o[:lead].any() and not got[2][:lead].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lens,h,hk,causal", [([256] * 40, 8, 8, False), ([4000], 12, 12, False), ([900, 2300, 17], 16, 4, True)])
 def test_dk_and_dv_are_reproducible(lens, h, hk, causal):
     q, k, v, do, qo, ko = make(lens, lens, h, hk)

@@ -168,6 +168,21 @@ def test_strided_packed_and_per_item_positions():
 
 
 @pytest.mark.gpu
+def test_strides_past_32_bits():
+    table, pos = rope_table(64, device="cuda"), rope_positions((3, 2, 1), device="cuda")
+    q, k = (torch.randn(6, 3, 128, device="cuda").bfloat16() for _ in range(2))
+    want = wan_flash_rope(q, k, pos, table)
+    big = torch.empty(5 * 2**29 + 6 * 128, dtype=torch.bfloat16, device="cuda")  # 5 GiB
+    tokens = torch.as_strided(big, (6, 3, 128), (2**29, 128, 1)).copy_(q)
+    heads = torch.as_strided(big, (6, 3, 128), (128, 2**30, 1), 3 * 128)
+    got = wan_flash_rope(tokens, k, pos, table)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    heads.copy_(k)
+    assert torch.equal(wan_flash_rope(q, heads, pos, table)[1], want[1])
+    _lib.check_device()
+
+
+@pytest.mark.gpu
 def test_far_position_is_an_error_of_its_token_only():
     table = rope_table(16, device="cuda")
     pos = torch.tensor([[1, 2, 3], [1, 16, 3], [15, 15, 15]], dtype=torch.int32, device="cuda")

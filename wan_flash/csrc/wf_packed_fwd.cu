@@ -335,8 +335,11 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       return true;
     };
     // One flat pipeline over the blocks of all items: block g issues PV_t(g-1)
-    // before S_t(g) for each tile that the block has.
+    // before S_t(g) for each tile that the block has.  An item without blocks
+    // issues PV(g-1) too: the softmax warps that wait for it read no item until
+    // then, and with the ring full none with blocks would come.
     int g = 0;
+    bool pending = false;               // PV of block g-1 is not issued yet
     bool prev[2] = {false, false};      // tiles that block g-1 has
     bool prev_acc[2] = {false, false};  // ... and adds to (not its first block)
     int prev_keys = 128;                // keys of block g-1 that exist for its item (128 but for the last block)
@@ -348,25 +351,40 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       if (prev_keys < 128) packed_zero_rows(sKV + slot_v * kTileBytes, prev_keys);
       return true;
     };
+    auto flush = [&]() -> bool {
+      if (!pending) return true;
+      pending = false;
+      const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;
+      if (!wait_v()) return false;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!prev[t]) continue;
+        if (!issue_pv(t, slot_v, prev_acc[t])) return false;
+        if (prev_last) mma_commit_e(bar(kBarOFull + t));
+      }
+      mma_commit_e(bar(kBarKvEmpty + slot_v));
+      return true;
+    };
     PackedFwdItem x;
     x.h = 0;
     for (int k = 0; ok && get_item(k, x, kRoleMma, false); ++k) {
       const PackedFwdTile& w = x.w;
+      if (w.n_blocks == 0) ok = flush();
       for (int it = 0; it < w.n_blocks && ok; ++it, ++g) {
         const int uk = 2 * g, slot_k = uk % kKvSlots;
         ok = mbar_wait_warp(bar(kBarKvFull + slot_k), (uk / kKvSlots) & 1, abort_flag, kRoleMma, 10 + slot_k);
         if (!ok) break;
         tc_fence_after();
         const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;  // of block g-1
-        if (g > 0 && !(ok = wait_v())) break;
+        if (pending && !(ok = wait_v())) break;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (!ok) break;
-          if (prev[t]) {
+          if (pending && prev[t]) {
             if (!(ok = issue_pv(t, slot_v, prev_acc[t]))) break;
             if (prev_last) mma_commit_e(bar(kBarOFull + t));
           }
-          if (g > 0 && t == 1) mma_commit_e(bar(kBarKvEmpty + slot_v));
+          if (pending && t == 1) mma_commit_e(bar(kBarKvEmpty + slot_v));
           const int first = t == 0 ? x.skip0 : 0;
           prev[t] = t * 128 < w.rows && it >= first;
           prev_acc[t] = it > first;
@@ -383,21 +401,12 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
           }
         }
         if (ok) mma_commit_e(bar(kBarKvEmpty + slot_k));
+        pending = true;
         prev_last = (it == w.n_blocks - 1);
         prev_keys = min(128, w.klen - (w.j_last - it) * 128);
       }
     }
-    if (ok && g > 0 && x.h < 0) {  // (an abort leaves another item in x)
-      const int slot_v = (2 * g + kKvSlots - 1) % kKvSlots;
-      ok = wait_v();
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (!ok || !prev[t]) continue;
-        if (!(ok = issue_pv(t, slot_v, prev_acc[t]))) continue;
-        mma_commit_e(bar(kBarOFull + t));
-      }
-      if (ok) mma_commit_e(bar(kBarKvEmpty + slot_v));
-    }
+    if (ok && x.h < 0) ok = flush();  // (an abort leaves another item in x)
     // drain the tensor pipe before TMEM can be released
     mma_commit_e(bar(kBarDrain));
     mbar_wait_drain(bar(kBarDrain), 0);

@@ -12,8 +12,9 @@ its queries see everything cached.  Token t of sequence i is slot
 t % page_size of page page_table[i, t // page_size]; writing it is a plain
 index assignment, ``k_cache[page, slot] = k``.
 
-Contract violations raise AssertionError before any CUDA call.  The caches
-are read by their strides and never copied.  Lengths and page numbers are
+Contract violations raise AssertionError before any CUDA call.  There is no
+backward: serving only, and o never asks for a gradient.  The caches are read
+by their strides and never copied.  Lengths and page numbers are
 device data: an impossible one gives NaN in its sequence's outputs, and
 ``wan_flash._lib.check_device()`` raises.  Lengths and pages may change
 between replays of a captured CUDA graph; shapes may not.
@@ -29,6 +30,7 @@ import torch
 from wan_flash import _lib
 from wan_flash.interface import _aligned, _launch
 from wan_flash.shapes import HEAD_DIM
+
 
 @functools.lru_cache(maxsize=64)
 def _workspace_bytes(index: int, h: int, h_kv: int) -> int:

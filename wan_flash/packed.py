@@ -20,8 +20,10 @@ first offset, behind the last) may hold anything: they reach no sequence's
 result, and their o and gradients are 0, their lse -inf.
 
 The offsets are read on the device only: nothing synchronises, and a captured
-CUDA graph may be replayed with other offsets in the same tensors.  Offsets
-that fall, or leave the tensor, give NaN everywhere, and
+CUDA graph may be replayed with other offsets in the same tensors.  (A training
+step is captured while no autograd graph from outside the capture holds the
+same leaves: their gradient accumulation would wait on that graph's stream.)
+Offsets that fall, or leave the tensor, give NaN everywhere, and
 ``wan_flash._lib.check_device()`` raises.  Contract violations that the host
 can see raise AssertionError before any CUDA call.
 """
