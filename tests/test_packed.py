@@ -212,6 +212,47 @@ def test_strided_inputs_other_stream_and_replay_with_other_offsets():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_behind_a_kernel_of_another_stream(captured):
+    """The first kernel may come up early behind its own stream's last one, never before the stream it waits for."""
+    q, k, v, _, qo, ko = make([300, 77], [300, 77], 3, 1)
+
+    def call(x):
+        return wan_flash_packed_fwd(x, k, v, qo, ko, causal=True)
+
+    want = call(q)
+    late = torch.zeros_like(q)
+    big = torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            late.copy_(q + (big @ big)[0, 0] * 0)  # a millisecond behind
+        other = big[:64] * 2  # a short kernel of this stream
+        here.wait_stream(side)
+        out = call(late)
+        return out, other
+
+    run()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+    for _ in range(3):
+        late.zero_()
+        torch.cuda.synchronize()
+        if captured:
+            graph.replay()
+        else:
+            out = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out[0], want))
+    _lib.check_device()
+
+
+@pytest.mark.gpu
 def test_from_a_thread_without_a_cuda_call_behind_it():
     import threading
 

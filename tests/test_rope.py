@@ -213,3 +213,45 @@ def test_graph_replay_and_other_stream():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0], -want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_behind_a_kernel_of_another_stream(captured):
+    """The first kernel may come up early behind its own stream's last one, never before the stream it waits for."""
+    table, pos = rope_table(64, device="cuda"), rope_positions((4, 4, 4), device="cuda")
+    q, k = (torch.randn(64, 3, 128, device="cuda") for _ in range(2))
+
+    def call(x):
+        return wan_flash_rope(x, k, pos, table)
+
+    want = call(q)
+    late = torch.zeros_like(q)
+    big = torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            late.copy_(q + (big @ big)[0, 0] * 0)  # a millisecond behind
+        other = big[:64] * 2  # a short kernel of this stream
+        here.wait_stream(side)
+        out = call(late)
+        return out, other
+
+    run()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+    for _ in range(3):
+        late.zero_()
+        torch.cuda.synchronize()
+        if captured:
+            graph.replay()
+        else:
+            out = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out[0], want))
+    _lib.check_device()

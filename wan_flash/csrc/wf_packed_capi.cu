@@ -161,8 +161,8 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   pp.h = h, pp.sms = sms;
   pp.may_split = ws.may_split ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  wf_packed_plan_kernel<<<1, kPlanThreads, 0, st>>>(pp);
-  if ((rc = launch_check("wf_packed plan launch"))) return rc;
+  cudaError_t e = launch_ex(wf_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, 1u, pp);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_packed plan launch");
   PackedFwdParams p = {};
   p.head = pp.head;
   p.tiles = pp.fwd_tiles;
@@ -176,7 +176,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.part_o = reinterpret_cast<float4*>(w + ws.part_o);
   p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
   const int grid = ws.may_split ? sms : (int)std::min<long long>(packed_max_tiles(total_q, n, 256) * h, sms);
-  cudaError_t e = launch_ex(wf_packed_fwd_kernel, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
+  e = launch_ex(wf_packed_fwd_kernel, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
   if (ws.may_split) {
@@ -268,13 +268,12 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   p.wave = sms;
   p.scale = (float)(1.0 / std::sqrt(128.0));
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
-  cudaError_t e;
   if (ws.sem_bytes) {
-    e = cudaMemsetAsync(p.sem, 0, ws.sem_bytes, st);
+    const cudaError_t e = cudaMemsetAsync(p.sem, 0, ws.sem_bytes, st);
     if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd counters");
   }
-  wf_packed_plan_kernel<<<2, kPlanThreads, 0, st>>>(pp);
-  if ((rc = launch_check("wf_packed plan launch"))) return rc;
+  cudaError_t e = launch_ex(wf_packed_plan_kernel, dim3(2), dim3(kPlanThreads), 0, st, true, 1u, pp);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_packed plan launch");
   e = launch_ex(wf_packed_pre_kernel, dim3((unsigned)(2 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, p,
                 reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(o_residual),
                 reinterpret_cast<const __nv_bfloat16*>(dO), lse);

@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
 // split tiles, h), 256 threads: 32 rows x 128 columns.
 __global__ void __launch_bounds__(256) wf_packed_fwd_join_kernel(PackedFwdJoinParams p) {
   __shared__ float tile[32][132];
+  griddep_launch_dependents();
   griddep_wait();
   const int t = blockIdx.x >> 3, row0 = (blockIdx.x & 7) * 32, h = blockIdx.y;
   if (t >= p.head->z) return;

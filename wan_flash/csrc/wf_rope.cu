@@ -87,6 +87,10 @@ __global__ void __launch_bounds__(256) wf_rope_kernel(RopeParams p) {
   constexpr int kThreadsPerRow = 64 / kPairs;
   constexpr int kRows = 256 / kThreadsPerRow;
   constexpr int kBatch = kRopeBatch;
+  // a programmatic dependent of whatever ran before: its blocks come up while
+  // that drains (480p forward and gradients 139 -> 135 us, one token 14.8 -> 14.3)
+  griddep_launch_dependents();
+  griddep_wait();
   const int c = threadIdx.x % kThreadsPerRow;
   const int place = threadIdx.x / kThreadsPerRow;
   const int lane = place & (p.lanes - 1);
@@ -201,9 +205,8 @@ extern "C" int wf_rope(const void* q, const void* k, void* q_out, void* k_out, c
   const int tokens_per_block = rows_per_block / lanes;
   const dim3 grid((unsigned)((s + (long long)tokens_per_block - 1) / tokens_per_block), b);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (cfg->dtype == WF_BF16)
-    wf_rope_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  else
-    wf_rope_kernel<float><<<grid, 256, 0, st>>>(p);
+  const cudaError_t e = launch_ex(cfg->dtype == WF_BF16 ? wf_rope_kernel<__nv_bfloat16> : wf_rope_kernel<float>, grid,
+                                  dim3(256), 0, st, true, 1u, p);
+  if (e != cudaSuccess) return cuda_fail(e, "wf_rope launch");
   return launch_check("wf_rope launch");
 }
