@@ -238,3 +238,44 @@ def test_nothing_to_do():
     o, lse = wan_flash_decode(q, k[:0], v[:0], table[:, :0], lengths * 0)
     _lib.check_device()
     assert (o == 0).all() and (lse == float("-inf")).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_behind_a_kernel_of_another_stream(captured):
+    """The first kernel may come up early behind its own stream's last one, never before the stream it waits for."""
+    q, k, v, table, lengths = make([300, 17, 1000], 4, 2, 16)
+
+    def call(x):
+        return wan_flash_decode(x, k, v, table, lengths)
+
+    want = call(q)
+    late = torch.zeros_like(q)
+    big = torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            late.copy_(q + (big @ big)[0, 0] * 0)  # a millisecond behind
+        other = big[:64] * 2  # a short kernel of this stream
+        here.wait_stream(side)
+        out = call(late)
+        return out, other
+
+    run()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+    for _ in range(3):
+        late.zero_()
+        torch.cuda.synchronize()
+        if captured:
+            graph.replay()
+        else:
+            out = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out[0], want))
+    _lib.check_device()

@@ -235,8 +235,7 @@ __device__ int plan_next(PlanShared& sh, Item& w) {
 __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlanParams p) {
   __shared__ PlanShared sh;
   // a programmatic dependent of whatever ran before (19.6 -> 18.9 us for a short
-  // forward; the same for wf_decode, whose SMs take three CTAs each, cost 15 %:
-  // they came up around the last join's and lay unevenly)
+  // forward)
   griddep_launch_dependents();
   griddep_wait();
   const bool small = p.n + 3 <= kPlanSmall;
