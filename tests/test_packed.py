@@ -89,6 +89,28 @@ def test_many_tiles_without_keys(lq, lk, lead, tail, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,h,hk,causal", CASES)
+def test_forward_with_many_heads(lq, lk, h, hk, causal):
+    """More items than SMs, so with a plan (the cases above have one only where they are long)."""
+    more = 160 // h
+    q, k, v, _, qo, ko = make(lq, lk or lq, h * more, hk * more, 3, 150)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    _lib.check_device()
+    check_fwd(q, k, v, qo, ko, causal, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [29, 30, 31, 62, 63, 125, 126, 127, 128])
+def test_sequences_around_the_warp(n):
+    """Without a plan the segments are looked through 32 at a time, up to 126 sequences."""
+    lens = [(i * 5) % 3 for i in range(n - 1)] + [4]
+    q, k, v, _, qo, ko = make(lens, lens, 1, 1, 1, 2)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=True)
+    _lib.check_device()
+    check_fwd(q, k, v, qo, ko, True, o, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
 def test_large_scores(causal):
     """N(0, 3^2) q and k: row maxima that keep moving, so O is rescaled."""
@@ -175,6 +197,19 @@ def test_impossible_offsets(bad, which):
         _lib.check_device()
     assert o.isnan().all() and lse.isnan().all()
     _lib.check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [[0, 60, 50, 100], [-1, 50, 60, 100], [0, 50, 60, 101]])
+def test_impossible_offsets_of_many_heads(bad):
+    q, k, v, _, qo, ko = make([50, 10, 40], [50, 10, 40], 60, 30)  # with a plan
+    t = torch.tensor(bad, dtype=torch.int32, device="cuda")
+    for offs in ((t, ko), (qo, t)):
+        o, lse = wan_flash_packed_fwd(q, k, v, *offs, causal=True)
+        with pytest.raises(_lib.WanFlashError):
+            _lib.check_device()
+        assert o.isnan().all() and lse.isnan().all()
+        _lib.check_device()
 
 
 @pytest.mark.gpu

@@ -116,6 +116,9 @@ constexpr int kPackedPieceCost = 2;
 // longest walk gets shorter by more than the join's cost in blocks.
 constexpr int kPackedFwdMinChunk = 8;
 constexpr int kPackedFwdJoinCost = 4;
+// Forward calls with no more (tile, head) items than SMs and no walk to cut make
+// no plan: every CTA finds its own tile, the segments 32 at a time.
+constexpr int kPackedDirectSeqs = 126;
 constexpr int kPackedFwdSplitItems = 4;  // per SM: with more items the longest walk is not the time
 struct PackedFwdParams {
   const int4* head;
@@ -126,6 +129,9 @@ struct PackedFwdParams {
   float* lse;               // (h, total_q)
   float4* part_o;           // (parts, h) x [2 tiles][32 groups of 4 columns][128 rows]: unnormalised O
   float2* part_ml;          // (parts, h, 256): reference max (scaled log2 units) and row sum
+  const int* q_off;         // without a plan only, like k_off, n and total_k
+  const int* k_off;
+  int n, total_k;
   int total_q, h, group, causal;
   float scale_log2, rescale_threshold;
 };

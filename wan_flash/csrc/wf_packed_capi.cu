@@ -103,8 +103,10 @@ int packed_check(int n, int total_q, int total_k, int h, int h_kv, int causal) {
 }  // namespace
 
 cudaError_t packed_setup() {
-  cudaError_t e =
-      cudaFuncSetAttribute(wf_packed_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pfwd::kSmemBytes);
+  cudaError_t e = cudaSuccess;
+  for (auto k : {wf_packed_fwd_kernel<false>, wf_packed_fwd_kernel<true>})
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pfwd::kSmemBytes);
   for (auto k : {wf_packed_bwd_kernel<false>, wf_packed_bwd_kernel<true>})
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd::kSmemBytes);
@@ -161,7 +163,10 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   pp.h = h, pp.sms = sms;
   pp.may_split = ws.may_split ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_ex(wf_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, 1u, pp);
+  const long long most_items = packed_max_tiles(total_q, n, 256) * h;
+  const bool direct = !ws.may_split && most_items <= sms && n <= kPackedDirectSeqs;
+  cudaError_t e = cudaSuccess;
+  if (!direct) e = launch_ex(wf_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, 1u, pp);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed plan launch");
   PackedFwdParams p = {};
   p.head = pp.head;
@@ -175,8 +180,9 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.rescale_threshold = 8.0f;
   p.part_o = reinterpret_cast<float4*>(w + ws.part_o);
   p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
-  const int grid = ws.may_split ? sms : (int)std::min<long long>(packed_max_tiles(total_q, n, 256) * h, sms);
-  e = launch_ex(wf_packed_fwd_kernel, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
+  p.q_off = q_offsets, p.k_off = k_offsets, p.n = n, p.total_k = total_k;
+  const int grid = ws.may_split ? sms : (int)std::min<long long>(most_items, sms);
+  e = launch_ex(direct ? wf_packed_fwd_kernel<true> : wf_packed_fwd_kernel<false>, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
   if (ws.may_split) {

@@ -92,7 +92,8 @@ struct __align__(16) PackedFwdItem {
   PackedFwdTile w;
   int h;      // q head; -1: no items left
   int skip0;  // blocks of the walk that no row of tile 0 sees (but one block is walked at least)
-  int pad[2];
+  int bad;    // kDirect: the offsets were impossible
+  int pad;
 };
 static_assert(sizeof(PackedFwdItem) == 64, "four 16-byte words");
 
@@ -109,6 +110,10 @@ __device__ __forceinline__ void packed_zero_rows(uint32_t tile, int first, int n
   __syncwarp();
 }
 
+// kDirect: there is no plan, CTA i works on tile i / h, head i % h (465 tokens in
+// five sequences, 12 heads: 16.5 us with a plan, 12.4 without).  A kernel of its
+// own: with both schedulers in one, long calls ran 2 % slower.
+template <bool kDirect>
 __global__ void __launch_bounds__(pfwd::kThreads, 1)
     wf_packed_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -158,8 +163,8 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const int passes = p.res != nullptr ? 2 : 1;  // o, and what its rounding took away
-  // a programmatic dependent of the plan kernel: its lists are read from here
-  // on.  The join, if one follows, may take its place on SMs as they fall free.
+  // a programmatic dependent of the plan kernel, whose lists are read from here
+  // on, or of whatever ran before.  The join, if one follows, may take its place on SMs as they fall free.
   griddep_launch_dependents();
   griddep_wait();
   // The k-th item of this CTA, for a whole warp (or, one = true, for one thread
@@ -178,7 +183,31 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
   if (warp == 11) {
     regs_dec<kRegsOther>();
     // ------------------------------------------------------ item scheduler
-    if (lane == 0) {
+    auto set_skip0 = [&](PackedFwdItem& x) {
+      const int seen0 = min(x.w.off + 127, x.w.klen);  // keys that the last row of tile 0 sees
+      if (p.causal && x.w.rows > 128 && seen0 > 0)
+        x.skip0 = max(0, min(x.w.j_last + 1 - (seen0 + 127) / 128, x.w.n_blocks - 1));
+    };
+    if constexpr (kDirect) {  // the one item of this CTA, and the end
+      auto write_item = [&](int slot, const PackedFwdItem& x) {
+        reinterpret_cast<PackedFwdItem*>(smem + kOffItems)[slot] = x;
+        mbar_arrive(bar(kBarItemFull + slot));
+      };
+      PackedFwdItem x = {};
+      PlanView v = {p.q_off, p.k_off, p.n, p.total_q, p.total_k, false, p.causal != 0};
+      const int t = (int)blockIdx.x / p.h;
+      const bool some = plan_direct_tile(v, t, x.w);
+      if (lane == 0) {
+        x.bad = v.bad;
+        if (some) {
+          x.h = (int)blockIdx.x - t * p.h;
+          set_skip0(x);
+          write_item(0, x);
+        }
+        x.h = -1;
+        write_item(some ? 1 : 0, x);
+      }
+    } else if (lane == 0) {
       const int n_items = p.head->x * p.h;
       int next = (int)blockIdx.x;
       for (int k = 0;; ++k) {
@@ -186,9 +215,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
         x.h = -1;
         if (next < n_items) {
           x.w = p.tiles[packed_locate(p.tiles, next, p.h, x.h)];
-          const int seen0 = min(x.w.off + 127, x.w.klen);  // keys that the last row of tile 0 sees
-          if (p.causal && x.w.rows > 128 && seen0 > 0)
-            x.skip0 = max(0, min(x.w.j_last + 1 - (seen0 + 127) / 128, x.w.n_blocks - 1));
+          set_skip0(x);
         }
         const int slot = k % kItemSlots;
         if (k >= kItemSlots && !mbar_wait(bar(kBarItemEmpty + slot), (uint32_t)(k / kItemSlots - 1) & 1, abort_flag,
@@ -426,7 +453,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
     int s_waits = 0;    // S_t tiles consumed
     int o_waits = 0;    // items of this tile that had keys
     int stage_use = 0;  // O tiles of both tiles staged before this item
-    const bool bad = p.head->y != 0;
+    const bool listed_bad = kDirect ? false : p.head->y != 0;
     PackedFwdItem x;
     for (int k = 0; ok && get_item(k, x, role, false); ++k) {
       const PackedFwdTile& w = x.w;
@@ -435,6 +462,7 @@ __global__ void __launch_bounds__(pfwd::kThreads, 1)
       if (w.n_blocks == 0) {
         // nothing to attend (or rows outside any sequence): o = 0, lse = -inf;
         // NaN where the offsets were impossible
+        const bool bad = kDirect ? x.bad != 0 : listed_bad;
         const uint32_t fill = bad ? 0x7fff7fffu : 0u;
         for (int i = (int)threadIdx.x; i < w.rows * 16; i += 256) {
           const size_t at = ((size_t)(w.q0 + (i >> 4)) * p.h + h) * 128 + (i & 15) * 8;

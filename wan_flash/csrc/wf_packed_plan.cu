@@ -121,12 +121,11 @@ struct PlanView {
   bool bad, causal;
 };
 
-// Forward tile t: up to 256 query rows.
-__device__ __noinline__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int* base, int t) {
-  const int s = plan_find(base, p.n, t);
+// Forward tile i of segment s: up to 256 query rows.
+__device__ __forceinline__ PackedFwdTile plan_fwd_tile_of(const PlanView& p, int s, int i) {
   int qs, lq;
   plan_segment(p.q_off, p.n, p.total_q, p.bad, s, qs, lq);
-  const int m0 = (t - base[s]) * 256;
+  const int m0 = i * 256;
   PackedFwdTile w;
   w.q0 = qs + m0;
   w.rows = min(256, lq - m0);
@@ -141,6 +140,49 @@ __device__ __noinline__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int
     w.j_last = w.n_blocks - 1;
   }
   return w;
+}
+
+__device__ __noinline__ PackedFwdTile plan_fwd_tile(const PlanView& p, const int* base, int t) {
+  const int s = plan_find(base, p.n, t);
+  return plan_fwd_tile_of(p, s, t - base[s]);
+}
+
+__device__ __forceinline__ void plan_report_bad() {
+  if (atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
+    g_err_info[0] = g_err_info[1] = g_err_info[3] = 0u;
+    g_err_info[2] = kRolePackedPlan;
+  }
+}
+
+// Forward tile t without a plan, by one converged warp; bad: impossible offsets.
+// False: there is no such tile.
+__device__ __forceinline__ bool plan_direct_tile(PlanView& p, int t, PackedFwdTile& w) {
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (int s = lane; s <= p.n; s += 32) bad |= plan_bad(p.q_off, s, p.total_q) || plan_bad(p.k_off, s, p.total_k);
+  p.bad = __any_sync(0xffffffffu, bad);
+  if (p.bad && lane == 0) plan_report_bad();
+  int carry = 0;
+  for (int s0 = 0; s0 < p.n + 2; s0 += 32) {
+    int start, len = 0;
+    if (s0 + lane < p.n + 2) plan_segment(p.q_off, p.n, p.total_q, p.bad, s0 + lane, start, len);
+    const int tiles = (len + 255) / 256;
+    int incl = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    const int first = carry + incl - tiles;
+    const unsigned here = __ballot_sync(0xffffffffu, t >= first && t < first + tiles);
+    if (here) {
+      const int src = __ffs(here) - 1;
+      w = plan_fwd_tile_of(p, s0 + src, t - __shfl_sync(0xffffffffu, first, src));
+      return true;
+    }
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
 }
 
 // Backward key tile t: 128 key rows, and the query tiles that see them.
@@ -255,10 +297,7 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
   for (int s = threadIdx.x; s <= p.n; s += kPlanThreads)
     bad |= plan_bad(v.q_off, s, p.total_q) || plan_bad(v.k_off, s, p.total_k);
   v.bad = __syncthreads_or(bad);
-  if (v.bad && threadIdx.x == 0 && atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
-    g_err_info[0] = g_err_info[1] = g_err_info[3] = 0u;
-    g_err_info[2] = kRolePackedPlan;
-  }
+  if (v.bad && threadIdx.x == 0) plan_report_bad();
   int* const base0 = small ? sh.base0 : p.base + (blockIdx.x ? 2 * (p.n + 3) : 0);
   int* const base1 = small ? sh.base1 : p.base + (p.n + 3);  // block 0 of the backward only
 
