@@ -41,6 +41,12 @@ def _workspace_bytes(index: int, h: int, h_kv: int) -> int:
     return size.value
 
 
+@functools.lru_cache(maxsize=256)
+def _cfg(*sizes):
+    """The C options of a cache's shape and strides (1.2 us to make, 0.2 to find)."""
+    return _lib.DecodeCfg(*sizes)
+
+
 def wan_flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                      lengths: torch.Tensor):
     """One new token per sequence over the paged cache -> (o, lse); see the module's text.
@@ -74,7 +80,7 @@ def wan_flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     lengths = lengths.contiguous()
     if width > 1 and page_table.stride(1) != 1:
         page_table = page_table.contiguous()
-    cfg = _lib.DecodeCfg(n_pages, page_size, width, 0, page_table.stride(0), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    cfg = _cfg(n_pages, page_size, width, 0, page_table.stride(0), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
     size = _workspace_bytes(device.index, h, h_kv)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
     _launch(_lib.lib().wf_decode, device, q.data_ptr(), k_ptr, v_ptr, page_table.data_ptr(), lengths.data_ptr(),

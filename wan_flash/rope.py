@@ -19,6 +19,8 @@ and ``wan_flash._lib.check_device()`` raises.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from wan_flash import _lib
@@ -68,6 +70,12 @@ def _rows(x: torch.Tensor, size: int):
     return x, batch, st[-3], st[-2]
 
 
+@functools.lru_cache(maxsize=256)
+def _cfg(*sizes):
+    """The C options of a shape and its strides (1.2 us to make, 0.2 to find)."""
+    return _lib.RopeCfg(*sizes)
+
+
 def _axes_ok(axes) -> bool:
     return len(axes) == 3 and sum(axes) == HEAD_DIM and all(d >= 0 and d % 2 == 0 for d in axes)
 
@@ -101,8 +109,8 @@ def _rope_impl(q, k, positions, table, axes, inverse):
     positions = positions.contiguous()
     if not table.is_contiguous() or table.data_ptr() % 16:
         table = table.clone(memory_format=torch.contiguous_format)
-    cfg = _lib.RopeCfg(0 if size == 2 else 1, 1 if inverse else 0, rows, axes[0] // 2, axes[1] // 2, 0,
-                       q0, q1, q2, k0, k1, k2, 3 * s if len(ps) == 3 else 0)
+    cfg = _cfg(0 if size == 2 else 1, 1 if inverse else 0, rows, axes[0] // 2, axes[1] // 2, 0,
+               q0, q1, q2, k0, k1, k2, 3 * s if len(ps) == 3 else 0)
     _launch(_lib.lib().wf_rope, device, q.data_ptr(), k.data_ptr(), oq.data_ptr(), ok.data_ptr(), table.data_ptr(),
             positions.data_ptr(), b, s, h, h_kv, cfg)
     return oq, ok
