@@ -108,6 +108,20 @@ def test_against_64_bits(lens, h, hk, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("h,hk", [(4, 2), (32, 1), (80, 2)])
+@pytest.mark.parametrize("width", [256, 257, 512, 513])
+def test_short_tables(h, hk, width):
+    """Around the widths up to which a row is one CTA's."""
+    for lens in ([width, 0, 1, 200], [64, 65]):
+        q, k, v, table, lengths = make(lens, h, hk, 1)
+        if table.shape[1] < width:
+            table = torch.nn.functional.pad(table, (0, width - table.shape[1]))
+        o, lse = wan_flash_decode(q, k, v, table, lengths)
+        _lib.check_device()
+        check(q, k, v, table, lengths, o, lse)
+
+
+@pytest.mark.gpu
 def test_many_short_sequences():
     lens = [(i * 37) % 90 for i in range(700)]
     x = make(lens, 2, 1, 16)
@@ -201,8 +215,24 @@ def test_impossible_pages_and_lengths(what):
 
 
 @pytest.mark.gpu
-def test_captured_graphs_side_by_side_with_changing_lengths():
-    xs = [make([90, 300], 4, 2, 16, seed=s) for s in range(2)]
+def test_impossible_pages_and_lengths_of_long_rows():
+    """As above where rows are split over CTAs: sequences 1 (a page) and 3 (the length) are lost, no other."""
+    q, k, v, table, lengths = make([900, 1500, 33, 700], 4, 2, 16)
+    table[1, 60] = k.shape[0]
+    lengths[3] = table.shape[1] * 16 + 1
+    o, lse = wan_flash_decode(q, k, v, table, lengths)
+    with pytest.raises(_lib.WanFlashError):
+        _lib.check_device()
+    assert o[[1, 3]].isnan().all() and lse[[1, 3]].isnan().all()
+    rest = [0, 2]
+    check(q[rest], k, v, table[rest], lengths[rest], o[rest], lse[rest])
+    _lib.check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("long", [300, 3000])  # whole rows, and rows over several CTAs
+def test_captured_graphs_side_by_side_with_changing_lengths(long):
+    xs = [make([90, long], 4, 2, 16, seed=s) for s in range(2)]
     want = [wan_flash_decode(*x) for x in xs]
     graphs, outs = [], []
     for x in xs:
@@ -222,7 +252,7 @@ def test_captured_graphs_side_by_side_with_changing_lengths():
     torch.cuda.synchronize()
     for (o, lse), (wo, wl) in zip(outs, want):
         assert torch.equal(o, wo) and torch.equal(lse, wl)
-    xs[0][4].copy_(torch.tensor([1, 299], dtype=torch.int32))
+    xs[0][4].copy_(torch.tensor([1, long - 1], dtype=torch.int32))
     graphs[0][0].replay()
     torch.cuda.synchronize()
     _lib.check_device()

@@ -26,7 +26,8 @@
 // the other and every CTA takes an equal run of them, whatever the lengths;
 // a row that spans several CTAs leaves partial results (running maximum,
 // sum, unnormalised O, all fp32) which a second kernel joins in a fixed
-// order, so results do not depend on timing.
+// order, so results do not depend on timing.  Where the page table is short and
+// the rows are few, a CTA takes a whole row instead.
 #include "wf_common.cuh"
 #include "wf_kernels.h"
 
@@ -40,6 +41,12 @@ constexpr uint32_t kRowBytes = 256 + 16;        // a token's 128 dims; 16 bytes 
 constexpr uint32_t kHalfBytes = 16 * kRowBytes; // 16 tokens of K (or V)
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
 constexpr int kMaxHeads = 32;                   // q heads of a row (4 n-tiles of 8)
+// Tables of at most so many tokens, with no more rows than CTAs: a CTA takes a
+// whole row and no join follows.  One launch less is 2 us of a call, and on the
+// device 12 rows of 300 tokens take 8.2 us either way, 432 rows of 512 22.5
+// against 26.8; 12 rows of 512 10.3 against 8.7, of 1024 16.4 against 10.3; with 32
+// heads a row 512 tokens 18.5 against 16.4.
+constexpr int whole_tokens(int heads_per_row) { return heads_per_row <= 16 ? 512 : 256; }
 // Per-warp ring of 16-token K and V tiles, and CTAs per SM, for rows of kN x 8
 // heads.  8 heads: 12 warps with one tile ahead beat 8 with two (48 ragged
 // streams 138 us against 140, 75600-token caches 221 against 228); more heads
@@ -78,6 +85,7 @@ struct DecodeParams {
   int blocks;                // blocks of heads_per_row q heads per key-value head
   int heads_per_row;
   int n_pages, page_size, max_pages;
+  int whole;                 // CTA i works on row i, no row is split
   float scale_log2;
 };
 
@@ -179,39 +187,48 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
   griddep_wait();
 
   // ---- this CTA's run [lo, hi) of the tiles of all rows
-  const int per_thread = (p.b + kThreads - 1) / kThreads;
-  const int s0 = min(p.b, (int)threadIdx.x * per_thread), s1 = min(p.b, s0 + per_thread);
-  long long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += (long long)decode_tiles(decode_length(p, s)) * rows_per_seq;
-  long long incl = mine;
+  long long total = 0, ctas = 1, lo, hi;
+  if (p.whole) {  // (counted from the row's sequence on)
+    const int seq = (int)blockIdx.x / rows_per_seq;
+    const int n = decode_tiles(decode_length(p, seq));
+    lo = (long long)((int)blockIdx.x - seq * rows_per_seq) * n;
+    hi = lo + n;
+    if (threadIdx.x == 0) s_start[0] = 0, s_start[1] = seq;
+  } else {
+    const int per_thread = (p.b + kThreads - 1) / kThreads;
+    const int s0 = min(p.b, (int)threadIdx.x * per_thread), s1 = min(p.b, s0 + per_thread);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) mine += (long long)decode_tiles(decode_length(p, s)) * rows_per_seq;
+    long long incl = mine;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += up;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  long long before = 0, total = 0;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    long long before = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
-  before += incl - mine;
-  // with fewer tiles than CTAs the first `total` CTAs take one each, so a row's CTAs are neighbours
-  const long long ctas = min((long long)gridDim.x, max(total, 1LL));
-  const long long cta = min((long long)blockIdx.x, ctas);
-  const long long lo = total * cta / ctas, hi = total * min(cta + 1, ctas) / ctas;
-  if (lo < hi && before <= lo && lo < before + mine) {
-    long long at = before;
-    for (int s = s0; s < s1; ++s) {
-      const long long t = (long long)decode_tiles(decode_length(p, s)) * rows_per_seq;
-      if (lo < at + t) {
-        s_start[0] = at;
-        s_start[1] = s;
-        break;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_scan[w];
+      total += s_scan[w];
+    }
+    before += incl - mine;
+    // with fewer tiles than CTAs the first `total` CTAs take one each, so a row's CTAs are neighbours
+    ctas = min((long long)gridDim.x, max(total, 1LL));
+    const long long cta = min((long long)blockIdx.x, ctas);
+    lo = total * cta / ctas, hi = total * min(cta + 1, ctas) / ctas;
+    if (lo < hi && before <= lo && lo < before + mine) {
+      long long at = before;
+      for (int s = s0; s < s1; ++s) {
+        const long long t = (long long)decode_tiles(decode_length(p, s)) * rows_per_seq;
+        if (lo < at + t) {
+          s_start[0] = at;
+          s_start[1] = s;
+          break;
+        }
+        at += t;
       }
-      at += t;
     }
   }
   __syncthreads();
@@ -235,7 +252,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
       p.lse[(long long)s * p.h + i] = bad ? __int_as_float(0x7fffffff) : -INFINITY;
   }
   if (lo >= hi) {
-    if (threadIdx.x == 0) p.join[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0 && !p.whole) p.join[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
 
@@ -560,7 +577,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
     at = run.row_at + run.t1;
   }
   cp_async_wait<0>();
-  if (threadIdx.x == 0) p.join[blockIdx.x] = join;
+  if (threadIdx.x == 0 && !p.whole) p.join[blockIdx.x] = join;
 }
 
 // Joins the rows that span several CTAs: block (c, head) takes the row that
@@ -633,10 +650,11 @@ int decode_rows(int h, int h_kv, int* blocks, int* heads_per_row) {
 
 template <int kN>
 int decode_launch(const DecodeParams& p, int ctas, cudaStream_t st) {
+  if (p.whole) ctas = p.b * p.h_kv * p.blocks;
   using dec::Shape;
   cudaError_t e = launch_ex(wf_decode_kernel<kN>, dim3(ctas), dim3(dec::kThreads), Shape<kN>::kSmemBytes, st, true, 1u, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_decode launch");
-  e = launch_ex(wf_decode_join_kernel, dim3(ctas, std::min(p.heads_per_row, 8)), dim3(256), 0, st, true, 1u, p);
+  if (!p.whole) e = launch_ex(wf_decode_join_kernel, dim3(ctas, std::min(p.heads_per_row, 8)), dim3(256), 0, st, true, 1u, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_decode join launch");
   return launch_check("wf_decode join launch");
 }
@@ -726,6 +744,8 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
   p.part_o = p.part_ml + (size_t)2 * ctas * p.heads_per_row * 2;
   p.b = b, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
   p.n_pages = cfg->n_pages, p.page_size = cfg->page_size, p.max_pages = cfg->max_pages;
+  const long long rows = (long long)b * h_kv * p.blocks;
+  p.whole = rows <= ctas && (long long)cfg->max_pages * cfg->page_size <= dec::whole_tokens(p.heads_per_row);
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch ((p.heads_per_row + 7) / 8) {
