@@ -122,6 +122,17 @@ def test_short_tables(h, hk, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("h,hk", [(12, 12), (24, 8)])
+@pytest.mark.parametrize("longest", [1024, 1025])
+def test_more_rows_than_sms(h, hk, longest):
+    lens = [(i * 131) % 1000 for i in range(24)] + [longest]
+    x = make(lens, h, hk, 1)
+    o, lse = wan_flash_decode(*x)
+    _lib.check_device()
+    check(*x, o, lse)
+
+
+@pytest.mark.gpu
 def test_many_short_sequences():
     lens = [(i * 37) % 90 for i in range(700)]
     x = make(lens, 2, 1, 16)

@@ -42,11 +42,16 @@ constexpr uint32_t kHalfBytes = 16 * kRowBytes; // 16 tokens of K (or V)
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
 constexpr int kMaxHeads = 32;                   // q heads of a row (4 n-tiles of 8)
 // Tables of at most so many tokens, with no more rows than CTAs: a CTA takes a
-// whole row and no join follows.  One launch less is 2 us of a call, and on the
-// device 12 rows of 300 tokens take 8.2 us either way, 432 rows of 512 22.5
-// against 26.8; 12 rows of 512 10.3 against 8.7, of 1024 16.4 against 10.3; with 32
-// heads a row 512 tokens 18.5 against 16.4.
-constexpr int whole_tokens(int heads_per_row) { return heads_per_row <= 16 ? 512 : 256; }
+// whole row and no join follows.  One launch less is 2 us of a call; on the
+// device 12 rows of 300 tokens take 8.2 us either way, 12 of 512 10.3 against 8.7, of
+// 1024 16.4 against 10.3, ragged ones (up to 512 tokens) in 144 rows 10.3 against
+// 12.3, 432 rows 16.4 against 20.5.  With more rows than SMs ragged rows of up to
+// 1024 tokens still gain (192 rows 20.5 against 18.3, 288 20.6 against 25.2, 432 27.3
+// against 35.9), of up to 2048 not always (192 rows 38 against 29).  With 32 heads a
+// row 512 tokens take 18.5 against 16.4.
+constexpr int whole_tokens(int heads_per_row, bool more_rows_than_sms) {
+  return (heads_per_row <= 16 ? 512 : 256) << more_rows_than_sms;
+}
 // Per-warp ring of 16-token K and V tiles, and CTAs per SM, for rows of kN x 8
 // heads.  8 heads: 12 warps with one tile ahead beat 8 with two (48 ragged
 // streams 138 us against 140, 75600-token caches 221 against 228); more heads
@@ -745,7 +750,7 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
   p.b = b, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
   p.n_pages = cfg->n_pages, p.page_size = cfg->page_size, p.max_pages = cfg->max_pages;
   const long long rows = (long long)b * h_kv * p.blocks;
-  p.whole = rows <= ctas && (long long)cfg->max_pages * cfg->page_size <= dec::whole_tokens(p.heads_per_row);
+  p.whole = rows <= ctas && (long long)cfg->max_pages * cfg->page_size <= dec::whole_tokens(p.heads_per_row, rows > g_dev_sms[dev]);
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch ((p.heads_per_row + 7) / 8) {
