@@ -206,9 +206,9 @@ typedef struct wf_decode_cfg {
   long long v_page_stride, v_slot_stride, v_head_stride;
 } wf_decode_cfg;
 
-/* Bytes of workspace that wf_decode needs on the current device for h q heads
-   and h_kv key-value heads, whatever the batch and the lengths. */
-int wf_decode_workspace(int h, int h_kv, size_t* bytes);
+/* Bytes of workspace that wf_decode needs on the current device for these sizes,
+   whatever the lengths (0: workspace may be NULL). */
+int wf_decode_workspace(int b, int h, int h_kv, int max_pages, int page_size, size_t* bytes);
 
 /*
  * Attention of one new token per sequence over a paged key-value cache (no
@@ -222,13 +222,14 @@ int wf_decode_workspace(int h, int h_kv, size_t* bytes);
  * [0, max_pages * page_size], or a page outside [0, n_pages) in use, gives
  * NaN for that sequence (heads of that key-value head at least) and
  * WF_ERR_INVALID_ARG from wf_device_status.
- * Two launches; overlapping calls need workspaces of their own.
+ * Two launches (one, without workspace, where tables are short and rows few);
+ * overlapping calls need workspaces of their own.
  */
 int wf_decode(const void* q, const void* k_cache, const void* v_cache, const int* page_table, const int* lengths,
               void* o, float* lse, void* workspace, size_t workspace_bytes, int b, int h, int h_kv,
               const wf_decode_cfg* cfg, void* stream);
 
-/* Bytes of workspace of wf_packed_fwd on the current device. */
+/* Bytes of workspace of wf_packed_fwd on the current device (0: workspace may be NULL). */
 int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, size_t* bytes);
 
 /*
@@ -244,8 +245,8 @@ int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, size_t* byte
  * everywhere and WF_ERR_INVALID_ARG from wf_device_status.
  * o_residual (like o; NULL: none) receives what rounding o to bf16 took away,
  * for the backward.
- * Two launches (three where few query rows may have their walks cut into pieces,
- * added in a fixed order); overlapping calls need workspaces of their own.
+ * Two launches (one, without workspace, where all items run at once; three where
+ * few query rows may have their walks cut into pieces, added in a fixed order); overlapping calls need workspaces of their own.
  */
 int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, void* o,
                   void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,

@@ -75,7 +75,18 @@ def test_c_entry_refusals():
     assert call(v_head_stride=-8) == -2 and call(k_page_stride=2**36) == -2
     assert call(n_pages=2**20, k_page_stride=2**16) == -2  # 128 GiB
     assert call(b=0) == 0
-    assert lib.wf_decode_workspace(4, 3, ctypes.byref(ctypes.c_size_t())) == -1
+    assert lib.wf_decode_workspace(1, 4, 3, 8, 16, ctypes.byref(ctypes.c_size_t())) == -1
+    assert lib.wf_decode_workspace(1, 4, 2, 8, 0, ctypes.byref(ctypes.c_size_t())) == -1
+
+
+@pytest.mark.gpu
+def test_c_entry_refuses_a_small_workspace():
+    lib, size, p = _lib.lib(), ctypes.c_size_t(), ctypes.c_void_p
+    for pages, more in ((32, 0), (33, 1)):  # 512 and 528 tokens of table
+        assert lib.wf_decode_workspace(1, 4, 2, pages, 16, ctypes.byref(size)) == 0 and (size.value > 0) == bool(more)
+    cfg = _lib.DecodeCfg(3, 16, 33, 0, 33, 4096, 256, 128, 4096, 256, 128)
+    for ws, n in ((16, size.value - 1), (None, 0)):
+        assert lib.wf_decode(*[p(16)] * 7, p(ws), n, 1, 4, 2, ctypes.byref(cfg), None) == -1
 
 
 CASES = [

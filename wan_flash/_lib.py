@@ -85,7 +85,7 @@ def _declare(lib):
     lib.wf_set_wait_limit_ns.argtypes = [ctypes.c_ulonglong]
     lib.wf_selftest_wait_timeout.argtypes = [ctypes.c_ulonglong, ctypes.POINTER(ctypes.c_uint)]
     lib.wf_rope.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, ctypes.POINTER(RopeCfg), vp]
-    lib.wf_decode_workspace.argtypes = [i, i, ctypes.POINTER(ctypes.c_size_t)]
+    lib.wf_decode_workspace.argtypes = [i, i, i, i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, ctypes.POINTER(DecodeCfg), vp]
     lib.wf_packed_fwd_workspace.argtypes = [i, i, i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_packed_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, i, i, i, vp]

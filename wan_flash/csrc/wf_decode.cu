@@ -664,6 +664,13 @@ int decode_launch(const DecodeParams& p, int ctas, cudaStream_t st) {
   return launch_check("wf_decode join launch");
 }
 
+// Whether every row is one CTA's.
+bool decode_whole(int b, int h_kv, int blocks, int heads_per_row, int max_pages, int page_size, int sms) {
+  const long long rows = (long long)b * h_kv * blocks;
+  return rows <= (long long)sms * dec::ctas_per_sm(heads_per_row) &&
+         (long long)max_pages * page_size <= dec::whole_tokens(heads_per_row, rows > sms);
+}
+
 // workspace: join descriptors, then (max, sum) pairs, then O of two partial rows per CTA
 size_t decode_workspace_bytes(int ctas, int heads_per_row) {
   return (size_t)ctas * 16 + (size_t)2 * ctas * heads_per_row * (8 + 512);
@@ -684,13 +691,17 @@ cudaError_t decode_setup() {
 }
 }  // namespace wf
 
-extern "C" int wf_decode_workspace(int h, int h_kv, size_t* bytes) {
+extern "C" int wf_decode_workspace(int b, int h, int h_kv, int max_pages, int page_size, size_t* bytes) {
   using namespace wf;
   if (!bytes) return fail(WF_ERR_INVALID_ARG, "null pointer");
+  if (b < 0 || max_pages < 0 || page_size < 1)
+    return fail(WF_ERR_INVALID_ARG, "b %d, max_pages %d, page_size %d", b, max_pages, page_size);
   int blocks, heads, dev, rc;
   if ((rc = decode_rows(h, h_kv, &blocks, &heads))) return rc;
   if ((rc = device_setup(&dev))) return rc;
-  *bytes = decode_workspace_bytes(g_dev_sms[dev] * dec::ctas_per_sm(heads), heads);
+  *bytes = decode_whole(b, h_kv, blocks, heads, max_pages, page_size, g_dev_sms[dev])
+               ? 0
+               : decode_workspace_bytes(g_dev_sms[dev] * dec::ctas_per_sm(heads), heads);
   return WF_OK;
 }
 
@@ -720,7 +731,7 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
   DecodeParams p;
   int rc, dev;
   if ((rc = decode_rows(h, h_kv, &p.blocks, &p.heads_per_row))) return rc;
-  if (!q || !lengths || !o || !lse || !workspace || (cfg->max_pages > 0 && !page_table) ||
+  if (!q || !lengths || !o || !lse || (!workspace && workspace_bytes) || (cfg->max_pages > 0 && !page_table) ||
       (cfg->n_pages > 0 && (!k_cache || !v_cache)))
     return fail(WF_ERR_INVALID_ARG, "null pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || !aligned16(workspace) ||
@@ -730,7 +741,8 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
     return fail(WF_ERR_MISALIGNED, "q/k_cache/v_cache/o/workspace and the caches' strides must be multiples of 16 bytes");
   if ((rc = device_setup(&dev))) return rc;
   const int ctas = g_dev_sms[dev] * dec::ctas_per_sm(p.heads_per_row);
-  const size_t need = decode_workspace_bytes(ctas, p.heads_per_row);
+  p.whole = decode_whole(b, h_kv, p.blocks, p.heads_per_row, cfg->max_pages, cfg->page_size, g_dev_sms[dev]);
+  const size_t need = p.whole ? 0 : decode_workspace_bytes(ctas, p.heads_per_row);
   if (workspace_bytes < need)
     return fail(WF_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
@@ -749,8 +761,6 @@ extern "C" int wf_decode(const void* q, const void* k_cache, const void* v_cache
   p.part_o = p.part_ml + (size_t)2 * ctas * p.heads_per_row * 2;
   p.b = b, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
   p.n_pages = cfg->n_pages, p.page_size = cfg->page_size, p.max_pages = cfg->max_pages;
-  const long long rows = (long long)b * h_kv * p.blocks;
-  p.whole = rows <= ctas && (long long)cfg->max_pages * cfg->page_size <= dec::whole_tokens(p.heads_per_row, rows > g_dev_sms[dev]);
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch ((p.heads_per_row + 7) / 8) {

@@ -24,16 +24,17 @@ bool packed_fwd_may_split(int total_q, int total_k, int h, int sms) {
 
 struct PackedFwdWorkspace {  // byte offsets
   size_t head = 0, base, tiles, split_tiles, part_ml, part_o, bytes;
-  bool may_split;
+  bool may_split, direct;  // direct: no plan, and no workspace
   PackedFwdWorkspace(int n, int total_q, int total_k, int h, int sms) {
     may_split = packed_fwd_may_split(total_q, total_k, h, sms);
+    direct = !may_split && packed_max_tiles(total_q, n, 256) * h <= sms && n <= kPackedDirectSeqs;
     const size_t items = may_split ? (size_t)sms : 0;
     base = 256;
     tiles = align256(base + (size_t)3 * (n + 3) * 4);
     split_tiles = align256(tiles + (packed_max_tiles(total_q, n, 256) + items) * sizeof(PackedFwdTile));
     part_ml = align256(split_tiles + items * sizeof(int4));
     part_o = part_ml + 2 * items * 256 * sizeof(float2);
-    bytes = part_o + 2 * items * 8192 * sizeof(float4);
+    bytes = direct ? 0 : part_o + 2 * items * 8192 * sizeof(float4);
   }
 };
 
@@ -132,7 +133,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   int rc = packed_check(n, total_q, total_k, h, h_kv, causal);
   if (rc) return rc;
   if (total_q == 0 || h == 0) return WF_OK;
-  if (!q || !o || !lse || !q_offsets || !k_offsets || !workspace || (total_k > 0 && (!k || !v)))
+  if (!q || !o || !lse || !q_offsets || !k_offsets || (!workspace && workspace_bytes) || (total_k > 0 && (!k || !v)))
     return fail(WF_ERR_INVALID_ARG, "null pointer");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_residual) ||
       !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(q_offsets) & 3) ||
@@ -148,10 +149,11 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   CUtensorMap mq, mk, mv, mo, mr;
   // with no keys at all nothing is loaded: q stands in for the maps of k and v
   if ((rc = make_bshd_map(&mq, q, 1, total_q, h)) || (rc = make_bshd_map(&mo, o, 1, total_q, h)) ||
-      (rc = make_bshd_map(&mr, o_residual ? o_residual : o, 1, total_q, h)) ||
+      (o_residual && (rc = make_bshd_map(&mr, o_residual, 1, total_q, h))) ||
       (rc = make_bshd_map(&mk, total_k ? k : q, 1, total_k ? total_k : total_q, total_k ? h_kv : h)) ||
       (rc = make_bshd_map(&mv, total_k ? v : q, 1, total_k ? total_k : total_q, total_k ? h_kv : h)))
     return rc;
+  if (!o_residual) mr = mo;  // never used
   uint8_t* const w = reinterpret_cast<uint8_t*>(workspace);
   PackedPlanParams pp = {};
   pp.q_off = q_offsets, pp.k_off = k_offsets;
@@ -164,9 +166,8 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   pp.may_split = ws.may_split ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const long long most_items = packed_max_tiles(total_q, n, 256) * h;
-  const bool direct = !ws.may_split && most_items <= sms && n <= kPackedDirectSeqs;
   cudaError_t e = cudaSuccess;
-  if (!direct) e = launch_ex(wf_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, 1u, pp);
+  if (!ws.direct) e = launch_ex(wf_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, 1u, pp);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed plan launch");
   PackedFwdParams p = {};
   p.head = pp.head;
@@ -182,7 +183,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
   p.q_off = q_offsets, p.k_off = k_offsets, p.n = n, p.total_k = total_k;
   const int grid = ws.may_split ? sms : (int)std::min<long long>(most_items, sms);
-  e = launch_ex(direct ? wf_packed_fwd_kernel<true> : wf_packed_fwd_kernel<false>, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
+  e = launch_ex(ws.direct ? wf_packed_fwd_kernel<true> : wf_packed_fwd_kernel<false>, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
   if (ws.may_split) {

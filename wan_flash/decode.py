@@ -32,12 +32,12 @@ from wan_flash.interface import _aligned, _launch
 from wan_flash.shapes import HEAD_DIM
 
 
-@functools.lru_cache(maxsize=64)
-def _workspace_bytes(index: int, h: int, h_kv: int) -> int:
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(index: int, b: int, h: int, h_kv: int, max_pages: int, page_size: int) -> int:
     """Of device `index`."""
     size = ctypes.c_size_t()
     with torch.cuda.device(index):
-        _lib.check(_lib.lib().wf_decode_workspace(h, h_kv, ctypes.byref(size)))
+        _lib.check(_lib.lib().wf_decode_workspace(b, h, h_kv, max_pages, page_size, ctypes.byref(size)))
     return size.value
 
 
@@ -81,8 +81,8 @@ def wan_flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if width > 1 and page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     cfg = _cfg(n_pages, page_size, width, 0, page_table.stride(0), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
-    size = _workspace_bytes(device.index, h, h_kv)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    size = _workspace_bytes(device.index, b, h, h_kv, width, page_size)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _launch(_lib.lib().wf_decode, device, q.data_ptr(), k_ptr, v_ptr, page_table.data_ptr(), lengths.data_ptr(),
-            o.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, b, h, h_kv, cfg)
+            o.data_ptr(), lse.data_ptr(), ws.data_ptr() if size else None, size, b, h, h_kv, cfg)
     return o, lse

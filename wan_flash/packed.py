@@ -93,10 +93,10 @@ def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
     if total_q == 0 or h == 0:
         return out
     size = _fwd_bytes(device.index, n, total_q, total_k, h)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _launch(_lib.lib().wf_packed_fwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
             k_offsets.data_ptr(), o.data_ptr(), o_residual.data_ptr() if residual else None, lse.data_ptr(),
-            ws.data_ptr(), size, n, total_q, total_k, h, h_kv, 1 if causal else 0)
+            ws.data_ptr() if size else None, size, n, total_q, total_k, h, h_kv, 1 if causal else 0)
     return out
 
 
