@@ -225,6 +225,34 @@ def test_training_step_captured_and_replayed_with_other_offsets():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("deterministic", [False, True])
+def test_captured_behind_a_copy(deterministic):
+    """A graph whose nodes before the kernels are copies and (in ordered mode) a memset."""
+    features.set_bwd_overrides(deterministic=deterministic)
+    q, k, v, do, qo, ko = make([300, 77], [300, 77], 4, 2)
+    x = torch.zeros_like(q)
+
+    def run():
+        x.copy_(q)
+        o, lse = wan_flash_packed_fwd(x, k, v, qo, ko, causal=True)
+        return wan_flash_packed_bwd(x, k, v, o, lse, do, qo, ko, causal=True)
+
+    want = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name, g, w in zip(("dq", "dk", "dv"), got, want):
+            if deterministic or name != "dq":
+                assert torch.equal(g, w), name
+        check_bwd(q, k, v, do, qo, ko, True, *got)
+    _lib.check_device()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
 def test_rows_past_32_bits(causal):
     """Sequences behind 2^31 elements give what they give at the start, bit for bit
