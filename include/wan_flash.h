@@ -245,8 +245,7 @@ int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, size_t* byte
  * everywhere and WF_ERR_INVALID_ARG from wf_device_status.
  * o_residual (like o; NULL: none) receives what rounding o to bf16 took away,
  * for the backward.
- * Two launches (one, without workspace, where all items run at once; three where
- * few query rows may have their walks cut into pieces, added in a fixed order); overlapping calls need workspaces of their own.
+ * Two launches (one, without workspace, for small calls; three where few query rows may have their walks cut into pieces, added in a fixed order); overlapping calls need workspaces of their own.
  */
 int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, void* o,
                   void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,

@@ -91,8 +91,8 @@ def test_many_tiles_without_keys(lq, lk, lead, tail, causal):
 @pytest.mark.gpu
 @pytest.mark.parametrize("lq,lk,h,hk,causal", CASES)
 def test_forward_with_many_heads(lq, lk, h, hk, causal):
-    """More items than SMs, so with a plan (the cases above have one only where they are long)."""
-    more = 160 // h
+    """More than three items per SM, so with a plan (the cases above have one only where they are long)."""
+    more = 445 // (h * (sum(lq) // 256 + len(lq) + 2)) + 1
     q, k, v, _, qo, ko = make(lq, lk or lq, h * more, hk * more, 3, 150)
     o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
     _lib.check_device()
@@ -153,7 +153,8 @@ SPLIT = [
     ([129, 0, 1, 40], [3000, 700, 4097, 0], 4, 2, True),
     ([129, 0, 1, 40], [3000, 700, 4097, 0], 4, 2, False),
     ([2500], [2500], 2, 2, True),
-    ([200, 60], [1800, 20], 3, 3, True),          # rows that see nothing beside a cut walk
+    ([200, 60], [1800, 20], 3, 3, True),          # 14 blocks: not cut yet
+    ([200, 60], [4800, 20], 3, 3, True),          # rows that see nothing beside a cut walk
     ([6000, 1], [6000, 5], 6, 2, True),           # only the longest walks are cut
 ]
 
@@ -202,7 +203,7 @@ def test_impossible_offsets(bad, which):
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [[0, 60, 50, 100], [-1, 50, 60, 100], [0, 50, 60, 101]])
 def test_impossible_offsets_of_many_heads(bad):
-    q, k, v, _, qo, ko = make([50, 10, 40], [50, 10, 40], 60, 30)  # with a plan
+    q, k, v, _, qo, ko = make([50, 10, 40], [50, 10, 40], 100, 50)  # with a plan
     t = torch.tensor(bad, dtype=torch.int32, device="cuda")
     for offs in ((t, ko), (qo, t)):
         o, lse = wan_flash_packed_fwd(q, k, v, *offs, causal=True)

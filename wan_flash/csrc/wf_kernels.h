@@ -116,8 +116,13 @@ constexpr int kPackedPieceCost = 2;
 // longest walk gets shorter by more than the join's cost in blocks.
 constexpr int kPackedFwdMinChunk = 8;
 constexpr int kPackedFwdJoinCost = 4;
-// Forward calls with no more (tile, head) items than SMs and no walk to cut make
-// no plan: every CTA finds its own tile, the segments 32 at a time.
+// Forward calls without a plan: every CTA finds its own tile, the segments 32 at
+// a time.  The plan and the join are worth 4 to 8 us; what they would even out is
+// worth less up to 3 items per SM with walks of at most 12 blocks (30 drawn calls
+// each: 20.5 -> 16.8 us in the geometric mean up to 1.3 items per SM, 21.6 -> 17.9 up to
+// 2, 23.4 -> 20.5 up to 3; none up to 5, a loss of 5 % above), and up to 1.5 of 16
+// blocks (1536 to 2048 keys: 33.6 -> 29.5 up to 1 item per SM, one long sequence
+// at worst 36.9 -> 41; of up to 3000 keys that one lost 36 %).
 constexpr int kPackedDirectSeqs = 126;
 constexpr int kPackedFwdSplitItems = 4;  // per SM: with more items the longest walk is not the time
 struct PackedFwdParams {

@@ -13,6 +13,13 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 // ragged one per sequence, and per run of rows before and behind them.
 long long packed_max_tiles(long long total, long long n, int rows) { return total / rows + n + 2; }
 
+// Whether the forward goes without a plan; by the most tiles that there can be.
+bool packed_fwd_direct(int n, int total_q, int total_k, int h, int sms) {
+  const long long items = packed_max_tiles(total_q, n, 256) * h;
+  return n <= kPackedDirectSeqs &&
+         (total_k <= 128 * 12 ? items <= 3LL * sms : total_k <= 128 * 16 && 2 * items <= 3LL * sms);
+}
+
 // Whether the plan may cut forward walks: where the query rows make few items
 // and a walk can be long enough to gain from it.  Its pieces are no shorter than
 // an SM's even share of all blocks (items: one per SM more than whole walks;
@@ -26,8 +33,8 @@ struct PackedFwdWorkspace {  // byte offsets
   size_t head = 0, base, tiles, split_tiles, part_ml, part_o, bytes;
   bool may_split, direct;  // direct: no plan, and no workspace
   PackedFwdWorkspace(int n, int total_q, int total_k, int h, int sms) {
-    may_split = packed_fwd_may_split(total_q, total_k, h, sms);
-    direct = !may_split && packed_max_tiles(total_q, n, 256) * h <= sms && n <= kPackedDirectSeqs;
+    direct = packed_fwd_direct(n, total_q, total_k, h, sms);
+    may_split = !direct && packed_fwd_may_split(total_q, total_k, h, sms);
     const size_t items = may_split ? (size_t)sms : 0;
     base = 256;
     tiles = align256(base + (size_t)3 * (n + 3) * 4);
@@ -182,7 +189,7 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.part_o = reinterpret_cast<float4*>(w + ws.part_o);
   p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
   p.q_off = q_offsets, p.k_off = k_offsets, p.n = n, p.total_k = total_k;
-  const int grid = ws.may_split ? sms : (int)std::min<long long>(most_items, sms);
+  const int grid = ws.may_split ? sms : (int)(ws.direct ? most_items : std::min<long long>(most_items, sms));
   e = launch_ex(ws.direct ? wf_packed_fwd_kernel<true> : wf_packed_fwd_kernel<false>, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
