@@ -245,11 +245,13 @@ int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, size_t* byte
  * everywhere and WF_ERR_INVALID_ARG from wf_device_status.
  * o_residual (like o; NULL: none) receives what rounding o to bf16 took away,
  * for the backward.
- * Two launches (one, without workspace, for small calls; three where few query rows may have their walks cut into pieces, added in a fixed order); overlapping calls need workspaces of their own.
+ * Two launches (one, without workspace, for small calls; three where few query
+ * rows may have their walks cut into pieces, added in a fixed order); overlapping
+ * calls need workspaces of their own.
  */
 int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, void* o,
-                  void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,
-                  int h_kv, int causal, void* stream);
+                  void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q,
+                  int total_k, int h, int h_kv, int causal, void* stream);
 
 typedef struct wf_packed_bwd_cfg {
   int nsplit;        /* 0 = the device cuts long walks into pieces (about two
@@ -268,9 +270,9 @@ int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, int h_kv, co
  * like q, dk and dv like k and v, bf16.  dk and dv sum over the q heads that
  * read the key-value head; they are bitwise reproducible, dq is with
  * cfg->deterministic.  With the forward's o_residual (NULL: none) the row sums of
- * o * dO are free of o's rounding, which shows in rows with few keys.  Rows that see no key, keys that no row sees, and rows
- * outside every sequence get gradient 0.  Impossible offsets as in
- * wf_packed_fwd.  total_q and total_k must both be positive (with no queries
+ * o * dO are free of o's rounding, which shows in rows with few keys.  Rows that
+ * see no key, keys that no row sees, and rows outside every sequence get
+ * gradient 0.  Impossible offsets as in wf_packed_fwd.  total_q and total_k must both be positive (with no queries
  * or no keys the gradients are zeros that the caller writes).
  */
 int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_residual, const float* lse,
