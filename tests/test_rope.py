@@ -255,3 +255,20 @@ def test_behind_a_kernel_of_another_stream(captured):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out[0], want))
     _lib.check_device()
+
+
+@pytest.mark.gpu
+def test_right_behind_writers_of_its_inputs():
+    """Each call reads what the kernels just before it wrote, also in place of older values."""
+    g = torch.Generator().manual_seed(2)
+    table = rope_table(64, device="cuda")
+    src = torch.randn(40, 64, 3, 128, generator=g).to("cuda", torch.bfloat16)
+    grids = [rope_positions((4, 4, 4), first_frame=i, device="cuda") for i in range(40)]
+    x, pos, got = torch.empty_like(src[0]), torch.empty_like(grids[0]), []
+    for i in range(40):
+        torch.mul(src[i], 1, out=x)
+        torch.add(grids[i], 0, out=pos)
+        got.append(wan_flash_rope(x, x, pos, table)[0])
+    for i in range(40):
+        assert torch.equal(got[i], wan_flash_rope(src[i], src[i], grids[i], table)[0])
+    _lib.check_device()

@@ -139,7 +139,7 @@ __device__ __forceinline__ bool decode_length_ok(const DecodeParams& p, int len)
   return len >= 0 && (long long)len <= (long long)p.max_pages * p.page_size;
 }
 __device__ __forceinline__ int decode_length(const DecodeParams& p, int seq) {
-  const int len = __ldg(p.lengths + seq);
+  const int len = p.lengths[seq];
   return decode_length_ok(p, len) ? len : 0;
 }
 __device__ __forceinline__ int decode_tiles(int len) { return (len + dec::kTile - 1) / dec::kTile; }
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
   // A programmatic dependent of whatever ran before: 48 ragged streams 142.2 ->
   // 139.7 us, 75600-token caches 219.0 -> 216.9.  The join leaves the way free only
   // as it ends: with the next call's CTAs up around its blocks those cost 15 % more.
+  // (Plain loads from here on, not read-only ones, which may move above the wait.)
   griddep_launch_dependents();
   griddep_wait();
 
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
 
   // ---- sequences with nothing cached: o = 0, lse = -inf (NaN where the length is impossible)
   for (int s = blockIdx.x; s < p.b; s += gridDim.x) {
-    const int len = __ldg(p.lengths + s);
+    const int len = p.lengths[s];
     if (len > 0 && decode_length_ok(p, len)) continue;
     const bool bad = !decode_length_ok(p, len);
     if (bad && threadIdx.x == 0 && atomicCAS(&g_err_code, 0u, (unsigned)WF_ERR_INVALID_ARG) == 0u) {
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
     last = min(ahead.len, ahead.t1 * kTile);
     pg = tok / p.page_size;
     slot = tok - pg * p.page_size;
-    page = tok < last ? __ldg(table + pg) : 0;
+    page = tok < last ? table[pg] : 0;
   };
   open_run();
   const uint32_t dst0 = ring + (lane >> 4) * kRowBytes + (lane & 15) * 16;
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
         pg += step_pages;
         slot += step_slots;
         if (slot >= p.page_size) slot -= p.page_size, ++pg;
-        page = tok < last ? __ldg(table + pg) : 0;
+        page = tok < last ? table[pg] : 0;
       } else if (ahead_at < hi) {
         open_run();
       }
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
     const uint4* const q_rows = reinterpret_cast<const uint4*>(p.q + ((long long)run.seq * p.h + head0) * 128);
     if constexpr (kQShared) {
       for (int i = threadIdx.x; i < kN * 8 * 16; i += kThreads) {
-        const uint4 x = i < n_heads * 16 ? __ldg(q_rows + i) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 x = i < n_heads * 16 ? q_rows[i] : make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(smem + Shape<kN>::kOffQ + (i >> 4) * kRowBytes + (i & 15) * 16) = x;
       }
       __syncthreads();
@@ -380,8 +381,8 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
         const uint32_t* src = reinterpret_cast<const uint32_t*>(q_rows + hd * 16) + (lane & 3);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          qf[n][ks][0] = hd < n_heads ? __ldg(src + ks * 8) : 0u;
-          qf[n][ks][1] = hd < n_heads ? __ldg(src + ks * 8 + 4) : 0u;
+          qf[n][ks][0] = hd < n_heads ? src[ks * 8] : 0u;
+          qf[n][ks][1] = hd < n_heads ? src[ks * 8 + 4] : 0u;
         }
       }
     }

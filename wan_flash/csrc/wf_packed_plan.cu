@@ -278,8 +278,8 @@ __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlan
   __shared__ PlanShared sh;
   // a programmatic dependent of whatever ran before (19.6 -> 18.9 us for a short
   // forward)
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();  // (only now: the next kernels' read-only loads must not meet that one's writes)
   const bool small = p.n + 3 <= kPlanSmall;
   if (threadIdx.x == 0) sh.units = 0ull, sh.most = sh.items = sh.parts = sh.split_tiles = 0;
   if (small) {

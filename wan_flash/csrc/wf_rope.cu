@@ -69,11 +69,14 @@ struct RopeVec<float> {
   }
 };
 
-__device__ __forceinline__ uint4 ldg_stream_u4(const void* p) {
+// Plain loads throughout, not read-only ones: the kernel before may still be
+// writing what this one reads when its blocks come up.
+__device__ __forceinline__ uint4 ld_stream_u4(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+               : "l"(p)
+               : "memory");
   return v;
 }
 
@@ -108,13 +111,13 @@ __global__ void __launch_bounds__(256) wf_rope_kernel(RopeParams p) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int row = row0 + i * p.lanes;
-      if (row < rows) v[i] = ldg_stream_u4(row < hq ? q + row * p.stride_h[0] : k + (row - hq) * p.stride_h[1]);
+      if (row < rows) v[i] = ld_stream_u4(row < hq ? q + row * p.stride_h[0] : k + (row - hq) * p.stride_h[1]);
     }
   };
   load(lane);
   // this thread's pairs of its token
   const int* const pp = p.positions + bb * p.pos_stride_b + 3 * ss;
-  const int pos0 = __ldg(pp), pos1 = __ldg(pp + 1), pos2 = __ldg(pp + 2);
+  const int pos0 = pp[0], pos1 = pp[1], pos2 = pp[2];
   const bool still = (pos0 | pos1 | pos2) < 0;  // padding: passes bit for bit
   const int most = max(pos0, max(pos1, pos2));
   float cs[kPairs], sn[kPairs];
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(256) wf_rope_kernel(RopeParams p) {
     for (int j = 0; j < kPairs; ++j) {
       const int pair = c * kPairs + j;
       const int pos = pair < p.pair_end0 ? pos0 : pair < p.pair_end1 ? pos1 : pos2;
-      const float2 t = __ldg(p.table + (long long)pos * 64 + pair);
+      const float2 t = p.table[(long long)pos * 64 + pair];
       cs[j] = t.x;
       sn[j] = t.y * p.sign;
     }
