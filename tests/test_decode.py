@@ -331,3 +331,33 @@ def test_behind_a_kernel_of_another_stream(captured):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out[0], want))
     _lib.check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h,hk", [(6, 2), (12, 1), (20, 1), (32, 1)])  # one to four blocks of 8 heads a row
+@pytest.mark.parametrize("extra_width", [0, 300])  # a CTA per row, and runs of tiles with a join
+def test_probabilities_are_not_rounded_to_bf16(h, hk, extra_width):
+    """o is off by its own rounding and by fp32 errors only.
+
+    q is 0 but in its first dim, so a score is one exact product.  What is left, relative to a
+    probability: its exponent (three roundings of at most 2 in log2 units, ln 2 * 3 * 2 * 2^-24)
+    and exp2 (2^-22), together below 2^-20, and 2^-16 from the pair of bf16 that it is multiplied as.  An
+    output adds 16 products of either half a step of 64 tokens, then 4 warps and a few CTAs' runs:
+    an fp32 step of the row's sum of |p v| each at most.  The sum of the row, 300 fp32 additions, is
+    below 2^-15 of o.  A probability rounded to one bf16 would be 2^-8 off."""
+    from tests.attn64 import E32, U
+
+    lens = [300, 40, 130, 17]
+    q, k, v, table, lengths = make(lens, h, hk, 16, seed=21, extra_width=extra_width)
+    q[..., 1:] = 0
+    q.clamp_(-2, 2)
+    o, lse = wan_flash_decode(q, k, v, table, lengths)
+    _lib.check_device()
+    check(q, k, v, table, lengths, o, lse)
+    for i, n in enumerate(lens):
+        at = torch.arange(n, device="cuda")
+        pg = table[i].long()[at // 16]
+        r = attn64(q[i:i + 1], k[pg, at % 16], v[pg, at % 16])
+        spread = (r["p"] @ v[pg, at % 16].double().transpose(0, 1).repeat_interleave(h // hk, 0).abs()).transpose(0, 1)
+        fp32 = (2.0**-16 + 2.0**-20 + (2 * 16 * -(-n // 64) + 16) * E32) * spread + 2.0**-15 * r["o"].abs()
+        assert_close(o[i:i + 1], r["o"], fp32 + U * (r["o"].abs() + fp32), f"o[{i}] of {n}")
