@@ -357,3 +357,49 @@ def test_c_entry_refuses_a_small_workspace():
     for tq in (8, 100000):
         assert lib.wf_packed_fwd_workspace(2, tq, 5000, 4, ctypes.byref(size)) == 0
         assert lib.wf_packed_fwd(*[p(16)] * 9, size.value - 1, 2, tq, 5000, 4, 2, 0, None) == -1
+
+
+@pytest.mark.parametrize("op", [False, True])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_forward_mode_tangent_is_refused(monkeypatch, op, which):
+    """As wan_flash_attn refuses it, and not dropped: a missing tangent counts as a zero derivative."""
+    from torch.autograd import forward_ad
+
+    import wan_flash.packed
+    import wan_flash.torch_op
+
+    def launch(q, k, v, q_offsets, k_offsets=None, causal=False, residual=False):
+        lse = torch.zeros(q.shape[1], q.shape[0])
+        return (torch.zeros_like(q), lse, torch.zeros_like(q)) if residual else (torch.zeros_like(q), lse)
+
+    for module in (wan_flash.packed, wan_flash.torch_op):
+        monkeypatch.setattr(module, "wan_flash_packed_fwd", launch)
+    fn = wan_flash.torch_op.wan_attention_packed if op else wan_flash.packed.wan_flash_attn_packed
+    q, k, v, do, qo, ko = make([5, 3], [5, 3], 4, 2, device="cpu")
+    for grad_mode in (False, True):
+        with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+            x = [q, k, v]
+            x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+            with pytest.raises(NotImplementedError):
+                fn(*x, qo, ko)
+    assert fn(q, k, v, qo, ko).shape == q.shape
+
+
+@pytest.mark.parametrize("op", [False, True])
+def test_a_forward_mode_tangent_of_the_gradient_is_refused(monkeypatch, op):
+    from torch.autograd import forward_ad
+
+    import wan_flash.packed
+    import wan_flash.torch_op
+
+    for module in (wan_flash.packed, wan_flash.torch_op):
+        monkeypatch.setattr(module, "wan_flash_packed_fwd",
+                            lambda q, *a, **kw: (torch.zeros_like(q), torch.zeros(4, 8), torch.zeros_like(q)))
+        monkeypatch.setattr(module, "wan_flash_packed_bwd",
+                            lambda q, k, v, *a: (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)))
+    q, k, v, do, qo, ko = make([5, 3], [5, 3], 4, 2, device="cpu")
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    o = (wan_flash.torch_op.wan_attention_packed if op else wan_flash.packed.wan_flash_attn_packed)(*leaves, qo, ko)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        torch.autograd.grad(o, leaves, forward_ad.make_dual(do, torch.ones_like(do)), retain_graph=True)
+    assert len(torch.autograd.grad(o, leaves, do)) == 3

@@ -272,3 +272,61 @@ def test_right_behind_writers_of_its_inputs():
     for i in range(40):
         assert torch.equal(got[i], wan_flash_rope(src[i], src[i], grids[i], table)[0])
     _lib.check_device()
+
+
+def _check_forward_mode(call, q, k, tq, tk):
+    """The tangent of a turn is the turned tangent, with grad mode on or off, for
+    leaves and plain tensors, for one tensor or both, and through the backward."""
+    from torch.autograd import forward_ad
+
+    want, zero = call(tq, tk), torch.zeros_like(k)
+    for grad_mode in (False, True):
+        for leaf in (False, True):
+            with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+                x, y = (t.clone().requires_grad_(leaf) for t in (q, k))
+                both = call(forward_ad.make_dual(x, tq), forward_ad.make_dual(y, tk))
+                one = call(forward_ad.make_dual(x, tq), y)
+                for out, t in zip((*both, *one), (*want, want[0], zero)):
+                    got = forward_ad.unpack_dual(out).tangent
+                    assert torch.equal(torch.zeros_like(t) if got is None and t is zero else got, t)
+                assert all(torch.equal(a, b) for a, b in zip(both, call(q, k)))
+    with forward_ad.dual_level():
+        x = q.clone().requires_grad_()
+        out, _ = call(x, k)
+        (gq,) = torch.autograd.grad(out, x, forward_ad.make_dual(q, tq))
+        back, _ = call(x, k)
+        (plain,) = torch.autograd.grad(back, x, tq)
+        assert torch.equal(forward_ad.unpack_dual(gq).tangent, plain)
+
+
+@pytest.mark.parametrize("op", [False, True])
+def test_forward_mode_derivative_on_a_stand_in(monkeypatch, op):
+    from torch.autograd import forward_ad
+
+    import wan_flash.rope
+    import wan_flash.torch_op
+
+    def launch(q, k, positions, table, axes, inverse):  # knows no derivative, like the kernel
+        return tuple(turned64(forward_ad.unpack_dual(x.detach()).primal, positions, axes=axes, sign=-1.0 if inverse else 1.0)
+                     for x in (q, k))
+
+    for module in (wan_flash.rope, wan_flash.torch_op):
+        monkeypatch.setattr(module, "_rope_impl", launch)
+    g = torch.Generator().manual_seed(3)
+    q, k, tq, tk = (torch.randn(24, h, 128, dtype=torch.float64, generator=g) for h in (3, 2, 3, 2))
+    pos, table = rope_positions((2, 3, 4)), rope_table(8)
+    fn = wan_flash.torch_op.wan_rope if op else wan_flash_rope
+    _check_forward_mode(lambda a, b: fn(a, b, pos, table), q, k, tq, tk)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_forward_mode_derivative(dtype):
+    from wan_flash.torch_op import wan_rope
+
+    g = torch.Generator().manual_seed(3)
+    q, k, tq, tk = (torch.randn(24, h, 128, generator=g).to("cuda", dtype) for h in (3, 2, 3, 2))
+    pos, table = rope_positions((2, 3, 4), device="cuda"), rope_table(8, device="cuda")
+    for fn in (wan_flash_rope, wan_rope):
+        _check_forward_mode(lambda a, b: fn(a, b, pos, table), q, k, tq, tk)
+    _lib.check_device()

@@ -13,7 +13,8 @@ t % page_size of page page_table[i, t // page_size]; writing it is a plain
 index assignment, ``k_cache[page, slot] = k``.
 
 Contract violations raise AssertionError before any CUDA call.  There is no
-backward: serving only, and o never asks for a gradient.  The caches are read
+backward: serving only, and o never asks for a gradient, nor has it a
+forward-mode tangent.  The caches are read
 by their strides and never copied.  Lengths and page numbers are
 device data: an impossible one gives NaN in its sequence's outputs, and
 ``wan_flash._lib.check_device()`` raises.  Lengths and pages may change

@@ -28,6 +28,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from wan_flash import _lib, features
 from wan_flash.shapes import BWD_TILE_M, TILE_N, sm_count
@@ -70,6 +71,12 @@ def _launch(fn, device: torch.device, *args):
             rc = fn(*args, stream)
     if rc != 0:
         _lib.check(rc)
+
+
+def _has_tangent(*tensors: torch.Tensor) -> bool:
+    """Whether one of the tensors carries a forward-mode derivative (it need not require a
+    gradient, nor grad mode be on).  Outside a dual level the first test is all (0.04 us)."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _ptr(t: torch.Tensor):

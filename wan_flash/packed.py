@@ -37,7 +37,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from wan_flash import _lib, features
-from wan_flash.interface import _aligned, _launch
+from wan_flash.interface import _aligned, _has_tangent, _launch
 from wan_flash.shapes import HEAD_DIM
 
 
@@ -144,6 +144,8 @@ class _WanFlashAttnPackedFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
+        if _has_tangent(do):
+            raise NotImplementedError("packed attention's backward has no forward-mode derivative")
         q, k, v, o, lse, o_residual, q_offsets, k_offsets = ctx.saved_tensors
         dq, dk, dv = wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, ctx.causal, o_residual)
         return dq, dk, dv, None, None, None
@@ -151,8 +153,9 @@ class _WanFlashAttnPackedFn(torch.autograd.Function):
 
 def wan_flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                           k_offsets: torch.Tensor | None = None, causal: bool = False):
-    """Differentiable (once) attention over packed sequences -> o (total_q, h, 128) bf16."""
+    """Differentiable (once, in reverse mode) attention over packed sequences -> o (total_q, h, 128)
+    bf16.  A tensor with a forward-mode tangent raises NotImplementedError, as wan_flash_attn does."""
     k_offsets = q_offsets if k_offsets is None else k_offsets
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _has_tangent(q, k, v):
         return _WanFlashAttnPackedFn.apply(q, k, v, q_offsets, k_offsets, bool(causal))
     return wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal)[0]

@@ -24,7 +24,7 @@ import functools
 import torch
 
 from wan_flash import _lib
-from wan_flash.interface import _contiguous_like, _launch
+from wan_flash.interface import _contiguous_like, _has_tangent, _launch
 from wan_flash.shapes import HEAD_DIM
 
 AXES = (44, 42, 42)  # head dims of time, height, width in the Wan models
@@ -120,6 +120,7 @@ class _WanFlashRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, table, axes, inverse):
         ctx.save_for_backward(positions, table)
+        ctx.save_for_forward(positions, table)
         ctx.axes, ctx.inverse = axes, inverse
         return _rope_impl(q, k, positions, table, axes, inverse)
 
@@ -129,9 +130,13 @@ class _WanFlashRopeFn(torch.autograd.Function):
         gq, gk = _turned(gq, gk, positions, table, ctx.axes, not ctx.inverse)
         return gq, gk, None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return _turned(tq, tk, *ctx.saved_tensors, ctx.axes, ctx.inverse)  # the turn is linear
+
 
 def _turned(q, k, positions, table, axes, inverse):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)) or _has_tangent(q, k):
         return _WanFlashRopeFn.apply(q, k, positions, table, axes, inverse)
     return _rope_impl(q, k, positions, table, axes, inverse)
 
@@ -145,5 +150,6 @@ def wan_flash_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     table: rope_table(...), more rows than the largest position.
     axes: head dims of time, height, width, as given to rope_table.
     q and k may be strided views (slices of a fused qkv projection); heads may
-    differ.  Differentiable in q and k (the turn by the negative angle), any number of times."""
+    differ.  Differentiable in q and k (the turn by the negative angle), any number of times,
+    in reverse and in forward mode."""
     return _turned(q, k, positions, table, axes, False)

@@ -33,6 +33,8 @@ positions, packed attention and decode:
     wan_flash::decode(q, k_cache, v_cache, page_table, lengths) -> (o, lse)
 
 with ``wan_rope``, ``wan_attention_packed`` (differentiable) and ``wan_decode``.
+The operators themselves know no forward mode; ``wan_rope`` and
+``wan_attention_packed`` treat tangents as the functions do.
 """
 
 from __future__ import annotations
@@ -40,9 +42,9 @@ from __future__ import annotations
 import torch
 
 from wan_flash.decode import wan_flash_decode
-from wan_flash.interface import wan_flash_bwd, wan_flash_bwd_dual, wan_flash_fwd, wan_flash_fwd_dual
-from wan_flash.packed import wan_flash_packed_bwd, wan_flash_packed_fwd
-from wan_flash.rope import AXES, _rope_impl
+from wan_flash.interface import _has_tangent, wan_flash_bwd, wan_flash_bwd_dual, wan_flash_fwd, wan_flash_fwd_dual
+from wan_flash.packed import wan_flash_attn_packed, wan_flash_packed_bwd, wan_flash_packed_fwd
+from wan_flash.rope import AXES, _rope_impl, _turned, wan_flash_rope
 
 
 @torch.library.custom_op("wan_flash::attn_fwd", mutates_args=())
@@ -169,7 +171,8 @@ def _setup_context_rope(ctx, inputs, output):
 
 
 def _backward_rope(ctx, gq, gk):
-    gq, gk = rope(gq, gk, *ctx.saved_tensors, ctx.axes, not ctx.inverse)
+    turn = _turned if _has_tangent(gq, gk) else rope
+    gq, gk = turn(gq, gk, *ctx.saved_tensors, ctx.axes, not ctx.inverse)
     return gq, gk, None, None, None, None
 
 
@@ -178,6 +181,8 @@ rope.register_autograd(_backward_rope, setup_context=_setup_context_rope)
 
 def wan_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, axes=AXES):
     """wan_flash_rope through the registered operator (differentiable)."""
+    if _has_tangent(q, k):  # an operator would drop it
+        return wan_flash_rope(q, k, positions, table, axes)
     return rope(q, k, positions, table, list(axes), False)
 
 
@@ -215,6 +220,8 @@ def _setup_context_packed(ctx, inputs, output):
 
 
 def _backward_packed(ctx, do, dlse, dres):
+    if _has_tangent(do):
+        raise NotImplementedError("packed attention's backward has no forward-mode derivative")
     q, k, v, o, lse, o_residual, q_offsets, k_offsets = ctx.saved_tensors
     grads = packed_bwd(q, k, v, o, lse, o_residual, do.contiguous(), q_offsets, k_offsets, ctx.causal)
     return *grads, None, None, None
@@ -226,6 +233,8 @@ packed_fwd.register_autograd(_backward_packed, setup_context=_setup_context_pack
 def wan_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                          k_offsets: torch.Tensor | None = None, causal: bool = False) -> torch.Tensor:
     """wan_flash_attn_packed through the registered operator (differentiable)."""
+    if _has_tangent(q, k, v):  # an operator would drop it; this raises
+        return wan_flash_attn_packed(q, k, v, q_offsets, k_offsets, causal)
     return packed_fwd(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, causal)[0]
 
 
