@@ -261,7 +261,9 @@ typedef struct wf_packed_bwd_cfg {
   int deterministic; /* 1 = dq's fp32 contributions are added in key order */
 } wf_packed_bwd_cfg;
 
-/* Bytes of workspace of wf_packed_bwd on the current device. */
+/* Bytes of workspace of wf_packed_bwd on the current device: 512 h total_q of
+   fp32 dq, 5 KiB h a tile of 128 query rows (a ragged one per sequence with rows),
+   and 128 KiB a piece of a cut walk (about two per SM, or as nsplit makes them). */
 int wf_packed_bwd_workspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg,
                             size_t* bytes);
 

@@ -351,3 +351,44 @@ def test_c_entry_refusals():
     assert call(h=0, hk=0) == 0 and call(tq=0, tk=0) == 0
     assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 3, ctypes.byref(cfg), ctypes.byref(size)) == -1
     assert lib.wf_packed_bwd_workspace(2, 8, 8, 4, 2, None, ctypes.byref(size)) == -1
+
+
+def _workspace(n, total_q, total_k, h, hk, nsplit=0, deterministic=0):
+    import ctypes
+
+    cfg, size = _lib.PackedBwdCfg(nsplit, deterministic), ctypes.c_size_t()
+    _lib.check(_lib.lib().wf_packed_bwd_workspace(n, total_q, total_k, h, hk, ctypes.byref(cfg), ctypes.byref(size)))
+    return size.value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,h,hk", [(50000, 2500, 40, 40), (32768, 2048, 32, 8), (1000, 100000, 16, 16)])
+def test_workspace_grows_with_rows_not_with_sequences(rows, n, h, hk):
+    """512 bytes a row and head of fp32 dq; a head and tile of 128 rows 4 KiB (its rows rounded up to 8) and
+    1 KiB of lse and D; less than 1 KiB of records a tile, 64 bytes a sequence; and what one sequence of these
+    rows needs for pieces."""
+    tiles = min(rows, rows // 128 + n + 2)
+    most = _workspace(1, rows, rows, h, hk) + 5 * 1024 * h * tiles + 1024 * tiles + 64 * n
+    assert _workspace(n, rows, rows, h, hk) <= most
+    assert _workspace(n, rows, rows, h, hk, 1, 1) <= most
+
+
+@pytest.mark.gpu
+def test_workspace_of_a_set_split_is_bounded_by_the_units():
+    """A walk over group * query tiles units makes no more pieces than that."""
+    assert _workspace(1, 100, 100, 4, 2, 1024) == _workspace(1, 100, 100, 4, 2, 4)
+    assert _workspace(3, 100, 3000, 4, 2, 1024) <= _workspace(3, 100, 3000, 4, 2, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("nsplit,deterministic", [(0, False), (5, True)])
+def test_sequence_ends_at_every_place_of_a_tile(causal, nsplit, deterministic):
+    lq = [1, 63, 64, 65, 127, 128, 129, 191, 0, 192, 193, 2, 256, 319, 320, 321, 8, 62]
+    lk = [5, 64, 63, 200, 127, 129, 128, 1, 7, 300, 193, 0, 256, 30, 321, 320, 9, 63]
+    q, k, v, do, qo, ko = make(lq, lk, 4, 2, 5, 70, seed=13)
+    o, lse = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal)
+    features.set_bwd_overrides(nsplit=nsplit, deterministic=deterministic)
+    grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
+    _lib.check_device()
+    check_bwd(q, k, v, do, qo, ko, causal, *grads)

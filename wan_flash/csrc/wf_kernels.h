@@ -78,7 +78,7 @@ struct __align__(16) PackedFwdTile {  // up to 256 query rows of one sequence
 struct __align__(16) PackedBwdItem {  // up to 128 key rows of one sequence, and a piece of their walk
   int k0, rows;   // first row in the packed tensor, rows
   int q0, lq;     // the sequence's query rows
-  int qtile;      // the sequence's first query tile (place in the fp32 workspaces)
+  int qtile;      // the sequence's first query tile (place in lse's and D's padded tiles)
   int m_begin, m_count;  // query tiles of the sequence that see some of these keys
   int need;       // first query row of the sequence that sees the tile's first key (key r: need + r)
   int nb;         // place of the tile in its sequence
@@ -156,13 +156,13 @@ struct PackedBwdParams {
   const int4* q_tiles;
   float* neg_lse_log2;      // (h, q_tile_stride, 128): -lse * log2(e), -inf behind the sequence's end
   float* dpsum;             // (h, q_tile_stride, 128)
-  float* dq_accum;          // (h, q_tile_stride) tiles of 16384 fp32
+  float* dq_accum;          // (h, dq_rows, 128) fp32, by query tiles
   __nv_bfloat16* dk;        // (total_k, h_kv, 128)
   __nv_bfloat16* dv;
   float* dk_part;           // (parts, h_kv) tiles of 16384 fp32
   float* dv_part;
   int* sem;                 // ordered: (h, q_tile_stride) key tiles added so far
-  size_t q_tile_stride;
+  size_t q_tile_stride, dq_rows;
   int total_q, h, h_kv, group, ordered, wave;
   float scale, scale_log2;
 };
@@ -170,13 +170,13 @@ struct PackedConvertParams {
   const int4* head;
   const int4* q_tiles;
   const int4* split_tiles;
-  const float* dq_accum;    // (h, q_tile_stride) tiles
+  const float* dq_accum;
   const float* dk_part;     // (parts, h_kv) tiles
   const float* dv_part;
   __nv_bfloat16* dq;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
-  size_t q_tile_stride;
+  size_t dq_rows;
   unsigned dq_blocks, split_blocks;  // 2 * tiles * heads
   int h, h_kv;
   float scale;

@@ -10,8 +10,9 @@ namespace {
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Tiles of `rows` rows that [0, total) and n sequences can need at most: a
-// ragged one per sequence, and per run of rows before and behind them.
-long long packed_max_tiles(long long total, long long n, int rows) { return total / rows + n + 2; }
+// ragged one per sequence, and per run of rows before and behind them; each has
+// a row, so empty sequences need none.
+long long packed_max_tiles(long long total, long long n, int rows) { return std::min(total, total / rows + n + 2); }
 
 // Whether the forward goes without a plan; by the most tiles that there can be.
 bool packed_fwd_direct(int n, int total_q, int total_k, int h, int sms) {
@@ -57,19 +58,22 @@ struct PackedBwdBounds {
     pieces = (long long)sms * kPackedPiecesPerSm;
     const long long units = group * q_tiles * k_tiles;
     const long long cuts = std::min(units / kPackedMinChunk, pieces / std::max(h_kv, 1)) + 1;
-    items = nsplit > 0 ? k_tiles * nsplit : k_tiles + cuts;
+    // a piece has a unit at least, and a walk those of one sequence
+    const long long set = std::min<long long>(nsplit, std::max(group * ((total_q + 127LL) / 128), 1LL));
+    items = nsplit > 0 ? k_tiles * set : k_tiles + cuts;
     split_tiles = nsplit > 0 ? k_tiles : std::min(k_tiles, cuts);
-    parts = nsplit > 0 ? (nsplit > 1 ? k_tiles * nsplit : 0) : 2 * cuts;
+    parts = nsplit > 0 ? (set > 1 ? k_tiles * set : 0) : 2 * cuts;
   }
 };
 
 struct PackedBwdWorkspace {  // byte offsets
   size_t head = 0, base, items, q_tiles, split_tiles, neg_lse_log2, dpsum, dq_accum, dk_part, dv_part, sem,
       sem_bytes, bytes;
-  size_t q_tile_stride;
+  size_t q_tile_stride, dq_rows;
   PackedBwdWorkspace(int n, int total_q, int total_k, int h, int h_kv, const wf_packed_bwd_cfg* cfg, int sms) {
     const PackedBwdBounds most(n, total_q, total_k, h, h_kv, cfg->nsplit, sms);
     q_tile_stride = (size_t)packed_max_tiles(total_q, n, 128);
+    dq_rows = (size_t)total_q + 8 * q_tile_stride;  // a tile's rows are rounded up to 8
     const size_t q_all = q_tile_stride * h, parts = (size_t)most.parts * h_kv;
     base = 256;
     items = align256(base + (size_t)3 * (n + 3) * 4);
@@ -78,7 +82,7 @@ struct PackedBwdWorkspace {  // byte offsets
     neg_lse_log2 = align256(split_tiles + (size_t)most.split_tiles * sizeof(int4));
     dpsum = neg_lse_log2 + q_all * 512;
     dq_accum = align256(dpsum + q_all * 512);
-    dk_part = dq_accum + q_all * 65536;
+    dk_part = dq_accum + dq_rows * h * 512;
     dv_part = dk_part + parts * 65536;
     sem = dv_part + parts * 65536;
     sem_bytes = cfg->deterministic ? q_all * 4 : 0;
@@ -276,7 +280,7 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   p.dk_part = reinterpret_cast<float*>(w + ws.dk_part);
   p.dv_part = reinterpret_cast<float*>(w + ws.dv_part);
   p.sem = reinterpret_cast<int*>(w + ws.sem);
-  p.q_tile_stride = ws.q_tile_stride;
+  p.q_tile_stride = ws.q_tile_stride, p.dq_rows = ws.dq_rows;
   p.total_q = total_q, p.h = h, p.h_kv = h_kv, p.group = h / h_kv;
   p.ordered = pp.ordered;
   p.wave = sms;
@@ -301,8 +305,8 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   c.q_tiles = pp.q_tiles, c.split_tiles = pp.split_tiles;
   c.dq_accum = p.dq_accum, c.dk_part = p.dk_part, c.dv_part = p.dv_part;
   c.dq = reinterpret_cast<__nv_bfloat16*>(dq), c.dk = p.dk, c.dv = p.dv;
-  c.q_tile_stride = ws.q_tile_stride;
   c.dq_blocks = (unsigned)dq_blocks, c.split_blocks = (unsigned)split_blocks;
+  c.dq_rows = ws.dq_rows;
   c.h = h, c.h_kv = h_kv;
   c.scale = p.scale;
   e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(dq_blocks + 2 * split_blocks)), dim3(256), 0, st, true, 1u,
