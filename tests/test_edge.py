@@ -58,3 +58,44 @@ def test_dual_empty_queries():
     dq, dk0, dv0, dk1, dv1 = wan_flash_bwd_dual(q, k0, k0, k1, k1, o0, lse0, o1, lse1, do)
     _lib.check_device()
     assert all(t.float().abs().sum().item() == 0.0 for t in (dk0, dv0, dk1, dv1))
+
+
+@pytest.mark.gpu
+def test_a_current_context_stays_current():
+    """A C host whose current context is not the device's primary one keeps it over a call: its
+    streams and memory belong to it.  (The call only asks for a size: nothing is launched.)"""
+    import ctypes
+
+    from wan_flash import _lib
+
+    torch.cuda.synchronize()
+    lib, driver = _lib.lib(), ctypes.CDLL("libcuda.so.1")
+    size, before, own, after = ctypes.c_size_t(), ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+    assert lib.wf_packed_fwd_workspace(1, 5000, 5000, 4, ctypes.byref(size)) == 0  # the set-up of the primary context
+    assert driver.cuCtxGetCurrent(ctypes.byref(before)) == 0 and before.value
+    assert driver.cuCtxCreate_v2(ctypes.byref(own), 0, torch.cuda.current_device()) == 0
+    try:
+        assert lib.wf_packed_fwd_workspace(1, 5000, 5000, 4, ctypes.byref(size)) == 0
+        assert driver.cuCtxGetCurrent(ctypes.byref(after)) == 0
+    finally:
+        driver.cuCtxSetCurrent(before)
+        driver.cuCtxDestroy_v2(own)
+    assert after.value == own.value
+
+
+@pytest.mark.gpu
+def test_a_thread_without_a_context():
+    """A call from a thread that made no CUDA call before."""
+    import threading
+
+    from wan_flash.packed import wan_flash_packed_fwd
+
+    x = torch.randn(300, 2, 128, device="cuda").bfloat16()
+    off = torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+    want, got = wan_flash_packed_fwd(x, x, x, off)[0], []
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: got.append(wan_flash_packed_fwd(x, x, x, off)[0]))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want)

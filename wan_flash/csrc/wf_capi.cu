@@ -42,8 +42,11 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+using CtxGetCurrentFn = CUresult (*)(CUcontext*);
+
 std::mutex g_mu;
 EncodeTiledFn g_encode = nullptr;
+CtxGetCurrentFn g_ctx_current = nullptr;
 constexpr int kMaxDevices = 64;
 bool g_dev_ready[kMaxDevices] = {false};
 int g_dev_sms[kMaxDevices] = {0};
@@ -62,6 +65,28 @@ int get_encode(EncodeTiledFn* out) {
   return WF_OK;
 }
 
+// Make the device's context current in a thread that has none (one without a
+// CUDA call behind it, like autograd's): the tensor-map encoder, a driver
+// function, refuses there.  A context that is current stays, also where it is not
+// the device's primary one: the caller's stream and memory belong to it.
+int bind_context(int dev) {
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!g_ctx_current) {
+      void* fn = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      const cudaError_t e = cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &q);
+      if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
+        return fail(WF_ERR_CUDA, "cuCtxGetCurrent entry point unavailable (%s)", cudaGetErrorName(e));
+      g_ctx_current = reinterpret_cast<CtxGetCurrentFn>(fn);
+    }
+  }
+  CUcontext ctx = nullptr;
+  if (g_ctx_current(&ctx) == CUDA_SUCCESS && ctx) return WF_OK;
+  const cudaError_t e = cudaSetDevice(dev);
+  return e == cudaSuccess ? WF_OK : cuda_fail(e, "cudaSetDevice");
+}
+
 // Per-device one-time set-up: verify sm_100, record the SM count, opt the
 // big kernels into their dynamic shared memory.
 int device_setup(int* dev_out) {
@@ -70,11 +95,8 @@ int device_setup(int* dev_out) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (dev < 0 || dev >= kMaxDevices) return fail(WF_ERR_NO_DEVICE, "device ordinal %d out of range", dev);
   *dev_out = dev;
-  // Make the device's context current in this thread: a thread without a CUDA
-  // call behind it (autograd's) has none, and the tensor-map encoder, a driver
-  // function, refuses then.
-  e = cudaSetDevice(dev);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+  int rc;
+  if ((rc = bind_context(dev))) return rc;
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_dev_ready[dev]) return WF_OK;
   int major = 0, minor = 0, sms = 0;
