@@ -253,6 +253,13 @@ int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offs
                   void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q,
                   int total_k, int h, int h_kv, int causal, void* stream);
 
+/* wf_packed_fwd with the dense forward's options: rescale_threshold, and num_sms
+   as the number of CTAs that draw items (small calls, without workspace, have one
+   CTA per item).  scheduler and cluster_m do not apply.  NULL: the defaults. */
+int wf_packed_fwd_with(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, void* o,
+                       void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n, int total_q,
+                       int total_k, int h, int h_kv, int causal, const wf_fwd_cfg* cfg, void* stream);
+
 typedef struct wf_packed_bwd_cfg {
   int nsplit;        /* 0 = the device cuts long walks into pieces (about two
                         per SM, one where there are few key tiles); n > 0: pieces of 1/n of the
@@ -282,6 +289,14 @@ int wf_packed_bwd(const void* q, const void* k, const void* v, const void* o, co
                   const int* q_offsets, const int* k_offsets, void* dq, void* dk, void* dv, void* workspace,
                   size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv, int causal,
                   const wf_packed_bwd_cfg* cfg, void* stream);
+
+/* wf_packed_bwd with the dense backward's options: nsplit and deterministic as in
+   wf_packed_bwd_cfg (whose workspace it needs), pdl_off = 1 launches all four
+   kernels plainly.  cluster_n and sem do not apply. */
+int wf_packed_bwd_with(const void* q, const void* k, const void* v, const void* o, const void* o_residual,
+                       const float* lse, const void* dO, const int* q_offsets, const int* k_offsets, void* dq, void* dk,
+                       void* dv, void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h,
+                       int h_kv, int causal, const wf_bwd_cfg* cfg, void* stream);
 
 /* Message for the last failed call on this thread (empty if none). */
 int wf_last_error(char* buf, int len);

@@ -392,3 +392,71 @@ def test_sequence_ends_at_every_place_of_a_tile(causal, nsplit, deterministic):
     grads = wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal)
     _lib.check_device()
     check_bwd(q, k, v, do, qo, ko, causal, *grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,h,hk", [([3000, 200], 6, 2), ([700], 2, 2), ([2500], 1, 1)])  # whole walks, no plan, cut walks
+def test_feature_switches(lens, h, hk):
+    """rescale_skip_threshold moves the roundings (the row maximum grows by less than 8 log2 units over the
+    blocks), num_sms and pdl move none."""
+    q, k, v, do, qo, ko = make(lens, lens, h, hk, seed=14)
+
+    def run():
+        o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, residual=True)
+        return o, lse, *wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, o_residual=res)
+
+    want = run()
+    for a, b in zip(qo.tolist(), qo.tolist()[1:]):
+        r = attn64(q[a:b], k[a:b], v[a:b])
+        assert_close(want[0][a:b], r["o"], r["o_tol"], "o")
+    features.set_bwd_overrides(pdl=False)
+    for sms in (0, 1, 7, 500):
+        features.set_overrides(num_sms=sms)
+        got = run()
+        for i in (0, 1, 3, 4):
+            assert torch.equal(got[i], want[i])
+        check_bwd(q, k, v, do, qo, ko, False, *got[2:], residual=True)
+    features.set_overrides(num_sms=0, rescale_skip_threshold=0.0)
+    got = run()
+    _lib.check_device()
+    assert not torch.equal(got[0], want[0])
+    for a, b in zip(qo.tolist(), qo.tolist()[1:]):
+        r = attn64(q[a:b], k[a:b], v[a:b])
+        assert_close(got[0][a:b], r["o"], r["o_tol"], "o")
+        assert_close(got[1][:, a:b], r["lse"], r["lse_tol"], "lse")
+
+
+def test_feature_switches_reach_the_c_call(monkeypatch):
+    """What the calls pass on, with a stand-in for the launch."""
+    import wan_flash.packed as packed
+
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a)) or 0
+
+    monkeypatch.setattr(packed._lib, "lib", lambda: Lib())
+    monkeypatch.setattr(packed, "_launch", lambda fn, device, *a: fn(*a))
+    monkeypatch.setattr(packed, "_check", lambda q, k, v, a, b: (8, 8, 4, 2, 2, q.device))
+    monkeypatch.setattr(packed, "_fwd_bytes", lambda *a: 0)
+    sizes = {}
+    monkeypatch.setattr(packed, "_bwd_cfg_bytes", lambda *a: sizes.setdefault("args", a) and (None, 0))
+    q, k, v, do, qo, ko = make([5, 3], [5, 3], 4, 2, device="cpu")
+    features.set_overrides(rescale_skip_threshold=0.0, num_sms=3)
+    features.set_bwd_overrides(pdl=False, nsplit=2, deterministic=True)
+    o, lse = packed.wan_flash_packed_fwd(q, k, v, qo, ko)
+    name, args = calls[-1]
+    assert name == "wf_packed_fwd_with" and (args[-1].rescale_threshold, args[-1].num_sms) == (0.0, 3)
+    packed.wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko)
+    assert calls[-1][0] == "wf_packed_bwd_with" and sizes["args"][-3:] == (2, True, False)
+
+
+def test_c_entries_with_options_refuse():
+    import ctypes
+
+    p, lib = ctypes.c_void_p, _lib.lib()
+    bad = _lib.FwdCfg(8.0, 0, -1, 0)
+    assert lib.wf_packed_fwd_with(*[p(16)] * 9, 1 << 30, 2, 8, 8, 4, 2, 0, ctypes.byref(bad), None) == -1
+    for cfg, want in ((None, -1), (ctypes.byref(_lib.BwdCfg(-1, 1)), -1), (ctypes.byref(_lib.BwdCfg(2000, 1)), -1)):
+        assert lib.wf_packed_bwd_with(*[p(16)] * 13, 1 << 30, 2, 8, 8, 4, 2, 0, cfg, None) == want

@@ -31,7 +31,8 @@ EXPORTS = (
     "wf_fwd", "wf_fwd_dual", "wf_bwd_pre", "wf_bwd_main", "wf_bwd_convert", "wf_bwd_noalloc", "wf_last_error",
     "wf_device_status", "wf_set_wait_limit_ns", "wf_selftest_wait_timeout", "wf_num_sms", "wf_version",
     "wf_rope", "wf_decode", "wf_decode_workspace",
-    "wf_packed_fwd", "wf_packed_fwd_workspace", "wf_packed_bwd", "wf_packed_bwd_workspace",
+    "wf_packed_fwd", "wf_packed_fwd_with", "wf_packed_fwd_workspace",
+    "wf_packed_bwd", "wf_packed_bwd_with", "wf_packed_bwd_workspace",
 )
 
 
@@ -89,8 +90,10 @@ def _declare(lib):
     lib.wf_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, ctypes.POINTER(DecodeCfg), vp]
     lib.wf_packed_fwd_workspace.argtypes = [i, i, i, i, ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_packed_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i, i, i, i, i, i, vp]
+    lib.wf_packed_fwd_with.argtypes = lib.wf_packed_fwd.argtypes[:-1] + [ctypes.POINTER(FwdCfg), vp]
     lib.wf_packed_bwd_workspace.argtypes = [i, i, i, i, i, ctypes.POINTER(PackedBwdCfg), ctypes.POINTER(ctypes.c_size_t)]
     lib.wf_packed_bwd.argtypes = ([vp] * 13 + [ctypes.c_size_t] + [i] * 6 + [ctypes.POINTER(PackedBwdCfg), vp])
+    lib.wf_packed_bwd_with.argtypes = lib.wf_packed_bwd.argtypes[:-2] + [ctypes.POINTER(BwdCfg), vp]
     for name in EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     del fp

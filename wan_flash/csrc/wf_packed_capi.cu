@@ -141,8 +141,17 @@ extern "C" int wf_packed_fwd_workspace(int n, int total_q, int total_k, int h, s
 extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets,
                              void* o, void* o_residual, float* lse, void* workspace, size_t workspace_bytes, int n,
                              int total_q, int total_k, int h, int h_kv, int causal, void* stream) {
+  return wf_packed_fwd_with(q, k, v, q_offsets, k_offsets, o, o_residual, lse, workspace, workspace_bytes, n, total_q,
+                            total_k, h, h_kv, causal, nullptr, stream);
+}
+
+extern "C" int wf_packed_fwd_with(const void* q, const void* k, const void* v, const int* q_offsets,
+                                  const int* k_offsets, void* o, void* o_residual, float* lse, void* workspace,
+                                  size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv, int causal,
+                                  const wf_fwd_cfg* cfg, void* stream) {
   int rc = packed_check(n, total_q, total_k, h, h_kv, causal);
   if (rc) return rc;
+  if (cfg && cfg->num_sms < 0) return fail(WF_ERR_INVALID_ARG, "num_sms %d < 0", cfg->num_sms);
   if (total_q == 0 || h == 0) return WF_OK;
   if (!q || !o || !lse || !q_offsets || !k_offsets || (!workspace && workspace_bytes) || (total_k > 0 && (!k || !v)))
     return fail(WF_ERR_INVALID_ARG, "null pointer");
@@ -189,11 +198,12 @@ extern "C" int wf_packed_fwd(const void* q, const void* k, const void* v, const 
   p.lse = lse;
   p.total_q = total_q, p.h = h, p.group = h / h_kv, p.causal = causal;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
-  p.rescale_threshold = 8.0f;
+  p.rescale_threshold = cfg ? cfg->rescale_threshold : 8.0f;
   p.part_o = reinterpret_cast<float4*>(w + ws.part_o);
   p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
   p.q_off = q_offsets, p.k_off = k_offsets, p.n = n, p.total_k = total_k;
-  const int grid = ws.may_split ? sms : (int)(ws.direct ? most_items : std::min<long long>(most_items, sms));
+  const int ctas = cfg && cfg->num_sms > 0 ? cfg->num_sms : sms;  // draw whatever items the plan makes
+  const int grid = ws.may_split ? ctas : (int)(ws.direct ? most_items : std::min<long long>(most_items, ctas));
   e = launch_ex(ws.direct ? wf_packed_fwd_kernel<true> : wf_packed_fwd_kernel<false>, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
@@ -226,8 +236,23 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
                              const int* k_offsets, void* dq, void* dk, void* dv,
                              void* workspace, size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv,
                              int causal, const wf_packed_bwd_cfg* cfg, void* stream) {
+  wf_bwd_cfg all = {};
+  if (cfg) all.nsplit = cfg->nsplit, all.deterministic = cfg->deterministic;
+  return wf_packed_bwd_with(q, k, v, o, o_residual, lse, dO, q_offsets, k_offsets, dq, dk, dv, workspace,
+                            workspace_bytes, n, total_q, total_k, h, h_kv, causal, cfg ? &all : nullptr, stream);
+}
+
+extern "C" int wf_packed_bwd_with(const void* q, const void* k, const void* v, const void* o,
+                                  const void* o_residual, const float* lse, const void* dO, const int* q_offsets,
+                                  const int* k_offsets, void* dq, void* dk, void* dv, void* workspace,
+                                  size_t workspace_bytes, int n, int total_q, int total_k, int h, int h_kv, int causal,
+                                  const wf_bwd_cfg* all, void* stream) {
   int rc;
-  if ((rc = packed_check(n, total_q, total_k, h, h_kv, causal)) || (rc = packed_bwd_cfg_check(cfg))) return rc;
+  if ((rc = packed_check(n, total_q, total_k, h, h_kv, causal))) return rc;
+  if (!all) return fail(WF_ERR_INVALID_ARG, "null cfg");
+  const wf_packed_bwd_cfg sizes = {all->nsplit, all->deterministic}, *const cfg = &sizes;
+  if ((rc = packed_bwd_cfg_check(cfg))) return rc;
+  const bool pdl = !all->pdl_off;
   if (h == 0 || (total_q == 0 && total_k == 0)) return WF_OK;
   if (total_q == 0 || total_k == 0)
     return fail(WF_ERR_UNSUPPORTED, "no queries or no keys: the caller must zero the gradients");
@@ -290,14 +315,14 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
     const cudaError_t e = cudaMemsetAsync(p.sem, 0, ws.sem_bytes, st);
     if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd counters");
   }
-  cudaError_t e = launch_ex(wf_packed_plan_kernel, dim3(2), dim3(kPlanThreads), 0, st, true, 1u, pp);
+  cudaError_t e = launch_ex(wf_packed_plan_kernel, dim3(2), dim3(kPlanThreads), 0, st, pdl, 1u, pp);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed plan launch");
-  e = launch_ex(wf_packed_pre_kernel, dim3((unsigned)(2 * ws.q_tile_stride), h), dim3(256), 0, st, true, 1u, p,
+  e = launch_ex(wf_packed_pre_kernel, dim3((unsigned)(2 * ws.q_tile_stride), h), dim3(256), 0, st, pdl, 1u, p,
                 reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(o_residual),
                 reinterpret_cast<const __nv_bfloat16*>(dO), lse);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd preprocess launch");
   e = launch_ex(causal ? wf_packed_bwd_kernel<true> : wf_packed_bwd_kernel<false>,
-                dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, true, 1u, mq, mk, mv, mdo,
+                dim3((unsigned)(most.items * h_kv)), dim3(bwd::kThreads), bwd::kSmemBytes, st, pdl, 1u, mq, mk, mv, mdo,
                 p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd launch");
   PackedConvertParams c = {};
@@ -309,7 +334,7 @@ extern "C" int wf_packed_bwd(const void* q, const void* k, const void* v, const 
   c.dq_rows = ws.dq_rows;
   c.h = h, c.h_kv = h_kv;
   c.scale = p.scale;
-  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(dq_blocks + 2 * split_blocks)), dim3(256), 0, st, true, 1u,
+  e = launch_ex(wf_packed_convert_kernel, dim3((unsigned)(dq_blocks + 2 * split_blocks)), dim3(256), 0, st, pdl, 1u,
                 c);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_bwd convert launch");
   return launch_check("wf_packed_bwd launch");

@@ -65,19 +65,29 @@ def _fwd_bytes(index: int, n: int, total_q: int, total_k: int, h: int) -> int:
     return size.value
 
 
+@functools.lru_cache(maxsize=16)
+def _fwd_cfg(rescale_skip_threshold: float, num_sms: int):
+    """The C options of the forward's features that apply."""
+    return _lib.FwdCfg(rescale_skip_threshold, 0, num_sms, 0)
+
+
 @functools.lru_cache(maxsize=256)
-def _bwd_cfg_bytes(index: int, n: int, total_q: int, total_k: int, h: int, h_kv: int, nsplit: int, deterministic: bool):
+def _bwd_cfg_bytes(index: int, n: int, total_q: int, total_k: int, h: int, h_kv: int, nsplit: int, deterministic: bool,
+                   pdl: bool):
     """The C options and the workspace's size on device `index`."""
-    cfg, size = _lib.PackedBwdCfg(min(nsplit, 1024), 1 if deterministic else 0), ctypes.c_size_t()
+    sizes, size = _lib.PackedBwdCfg(min(nsplit, 1024), 1 if deterministic else 0), ctypes.c_size_t()
     with torch.cuda.device(index):
-        _lib.check(_lib.lib().wf_packed_bwd_workspace(n, total_q, total_k, h, h_kv, ctypes.byref(cfg),
+        _lib.check(_lib.lib().wf_packed_bwd_workspace(n, total_q, total_k, h, h_kv, ctypes.byref(sizes),
                                                       ctypes.byref(size)))
-    return cfg, size.value
+    return _lib.BwdCfg(sizes.nsplit, 1, sizes.deterministic, 0 if pdl else 1), size.value
 
 
 def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                          k_offsets: torch.Tensor | None = None, causal: bool = False, residual: bool = False):
     """(o, lse) of attention over packed sequences; see the module's text.
+
+    Of the forward features, ``rescale_skip_threshold`` applies, and ``num_sms`` to all but
+    small calls (those have one CTA per item); ``scheduler`` and ``cluster_mn`` do not.
 
     residual: also return what rounding o to bf16 took away, (o, lse, o_residual), for
     wan_flash_packed_bwd: its row sums of o * do are then free of that rounding, which
@@ -94,9 +104,11 @@ def wan_flash_packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
         return out
     size = _fwd_bytes(device.index, n, total_q, total_k, h)
     ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _launch(_lib.lib().wf_packed_fwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
+    f = features.get()
+    _launch(_lib.lib().wf_packed_fwd_with, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
             k_offsets.data_ptr(), o.data_ptr(), o_residual.data_ptr() if residual else None, lse.data_ptr(),
-            ws.data_ptr() if size else None, size, n, total_q, total_k, h, h_kv, 1 if causal else 0)
+            ws.data_ptr() if size else None, size, n, total_q, total_k, h, h_kv, 1 if causal else 0,
+            _fwd_cfg(f.rescale_skip_threshold, f.num_sms))
     return out
 
 
@@ -109,7 +121,8 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     dk and dv are bitwise reproducible; dq is accumulated with fp32 reductions
     unless ``features.set_bwd_overrides(deterministic=True)``.  ``nsplit`` of the
     backward features cuts the longest key tile's walk into that many pieces (0:
-    the device chooses); the CTA-pair form does not apply."""
+    the device chooses), ``pdl=False`` launches the four kernels plainly; the CTA-pair form does
+    not apply."""
     k_offsets = q_offsets if k_offsets is None else k_offsets
     total_q, total_k, h, h_kv, n, device = _check(q, k, v, q_offsets, k_offsets)
     assert o.dtype is torch.bfloat16 and do.dtype is torch.bfloat16 and o.shape == q.shape and do.shape == q.shape
@@ -124,9 +137,9 @@ def wan_flash_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     if total_q == 0 or total_k == 0 or h == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     f = features.get_bwd()
-    cfg, size = _bwd_cfg_bytes(device.index, n, total_q, total_k, h, h_kv, f.nsplit, f.deterministic)
+    cfg, size = _bwd_cfg_bytes(device.index, n, total_q, total_k, h, h_kv, f.nsplit, f.deterministic, f.pdl)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
-    _launch(_lib.lib().wf_packed_bwd, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+    _launch(_lib.lib().wf_packed_bwd_with, device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
             None if o_residual is None else o_residual.data_ptr(), lse.data_ptr(), do.data_ptr(), q_offsets.data_ptr(),
             k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             ws.data_ptr(), size, n, total_q, total_k, h, h_kv, 1 if causal else 0, cfg)
