@@ -403,3 +403,16 @@ def test_a_forward_mode_tangent_of_the_gradient_is_refused(monkeypatch, op):
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         torch.autograd.grad(o, leaves, forward_ad.make_dual(do, torch.ones_like(do)), retain_graph=True)
     assert len(torch.autograd.grad(o, leaves, do)) == 3
+
+
+@pytest.mark.gpu
+def test_one_long_sequence_keeps_its_plan_where_its_walks_can_be_cut():
+    """1537 to 2048 keys: one sequence with few tiles goes by the plan (a workspace), others without."""
+    def planned(n, total, h):
+        size = ctypes.c_size_t()
+        _lib.check(_lib.lib().wf_packed_fwd_workspace(n, total, total, h, ctypes.byref(size)))
+        return size.value > 0
+
+    assert planned(1, 1992, 5) and planned(1, 2048, 1) and planned(1, 1954, 9)
+    assert not planned(1, 1992, 15) and not planned(3, 1992, 5) and not planned(1, 1536, 5)
+    assert planned(1, 2049, 15)

@@ -120,10 +120,15 @@ constexpr int kPackedFwdJoinCost = 4;
 // a time.  The plan and the join are worth 4 to 8 us; what they would even out is
 // worth less up to 3 items per SM with walks of at most 12 blocks (30 drawn calls
 // each: 20.5 -> 16.8 us in the geometric mean up to 1.3 items per SM, 21.6 -> 17.9 up to
-// 2, 23.4 -> 20.5 up to 3; none up to 5, a loss of 5 % above), and up to 1.5 of 16
-// blocks (1536 to 2048 keys: 33.6 -> 29.5 up to 1 item per SM, one long sequence
-// at worst 36.9 -> 41; of up to 3000 keys that one lost 36 %).
+// 2, 23.4 -> 20.5 up to 3; none up to 5, a loss of 5 % above), and up to half as many
+// items with walks of at most 16 blocks (1537 to 2048 keys, 14 calls each, against the
+// plan: -28 % with ten sequences of about one length, -21 % with three, -3 % with one
+// long sequence among ten, 14 % more at worst).  One sequence alone is one walk, which the plan cuts
+// where its tiles leave half the SMs idle: there 36.5 us with it and 38.5 without,
+// 36.5 and 41.0 at worst; with more tiles 48 and 40.
 constexpr int kPackedDirectSeqs = 126;
+constexpr int kPackedDirectBlocks = 12, kPackedDirectMoreBlocks = 16;
+constexpr int kPackedDirectItems = 3;  // per SM
 constexpr int kPackedFwdSplitItems = 4;  // per SM: with more items the longest walk is not the time
 struct PackedFwdParams {
   const int4* head;

@@ -17,8 +17,10 @@ long long packed_max_tiles(long long total, long long n, int rows) { return std:
 // Whether the forward goes without a plan; by the most tiles that there can be.
 bool packed_fwd_direct(int n, int total_q, int total_k, int h, int sms) {
   const long long items = packed_max_tiles(total_q, n, 256) * h;
-  return n <= kPackedDirectSeqs &&
-         (total_k <= 128 * 12 ? items <= 3LL * sms : total_k <= 128 * 16 && 2 * items <= 3LL * sms);
+  if (n > kPackedDirectSeqs) return false;
+  if (total_k <= 128 * kPackedDirectBlocks) return items <= kPackedDirectItems * sms;
+  return total_k <= 128 * kPackedDirectMoreBlocks && 2 * items <= kPackedDirectItems * sms &&
+         (n > 1 || 2LL * ((total_q + 255) / 256) * h > sms);
 }
 
 // Whether the plan may cut forward walks: where the query rows make few items
