@@ -188,8 +188,9 @@ typedef struct wf_rope_cfg {
  * (c, s) = table[positions[token][axis(i)]][i].
  *   q (b, s, h, 128), k (b, s, h_kv, 128), strided; q_out, k_out contiguous,
  *   apart from q and k; table (max_pos, 64, 2) fp32; positions (s, 3) int32.
- * A token with a negative position passes unchanged.  A position >= max_pos
- * gives NaN in its token's rows and WF_ERR_INVALID_ARG from wf_device_status.
+ * A token with a negative position passes unchanged.  A position >= max_pos (on
+ * an axis that has pairs) gives NaN in its token's rows and WF_ERR_INVALID_ARG
+ * from wf_device_status.
  */
 int wf_rope(const void* q, const void* k, void* q_out, void* k_out, const float* table, const int* positions, int b,
             int s, int h, int h_kv, const wf_rope_cfg* cfg, void* stream);

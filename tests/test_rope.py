@@ -330,3 +330,34 @@ def test_forward_mode_derivative(dtype):
     for fn in (wan_flash_rope, wan_rope):
         _check_forward_mode(lambda a, b: fn(a, b, pos, table), q, k, tq, tk)
     _lib.check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("axes", [AXES, (64, 0, 64), (0, 64, 64), (64, 64, 0), (128, 0, 0), (0, 0, 128), (2, 62, 64)])
+def test_other_splits_of_the_axes(axes, dtype):
+    """Forward and gradients against the definition; a large coordinate on an axis without dims turns
+    nothing, on another it is past the table."""
+    g = torch.Generator().manual_seed(4)
+    q, k, gq, gk = (torch.randn(24, h, 128, generator=g).to("cuda", dtype) for h in (3, 2, 3, 2))
+    table, pos = rope_table(8, axes=axes, device="cuda"), rope_positions((2, 3, 4), first_frame=3, device="cuda")
+    pos[5] = -1
+    for a, d in enumerate(axes):
+        if d == 0:
+            pos[:5, a] = 2**31 - 1
+    leaves = [x.clone().requires_grad_() for x in (q, k)]
+    out = wan_flash_rope(*leaves, pos, table, axes)
+    grads = torch.autograd.grad(out, leaves, (gq, gk))
+    _lib.check_device()
+    for got, x, sign in zip((*out, *grads), (q, k, gq, gk), (1.0, 1.0, -1.0, -1.0)):
+        want = turned64(x, pos, axes=axes, sign=sign)
+        assert ((got.double() - want).abs() <= rope_tol(x, want)).all()
+    for a, d in enumerate(axes):
+        if d > 0:
+            bad = pos.clone()
+            bad[7, a] = 8
+            out = wan_flash_rope(q, k, bad, table, axes)
+            with pytest.raises(_lib.WanFlashError):
+                _lib.check_device()
+            for x in out:
+                assert x[7].isnan().all() and not x[:7].isnan().any() and not x[8:].isnan().any()

@@ -119,7 +119,9 @@ __global__ void __launch_bounds__(256) wf_rope_kernel(RopeParams p) {
   const int* const pp = p.positions + bb * p.pos_stride_b + 3 * ss;
   const int pos0 = pp[0], pos1 = pp[1], pos2 = pp[2];
   const bool still = (pos0 | pos1 | pos2) < 0;  // padding: passes bit for bit
-  const int most = max(pos0, max(pos1, pos2));
+  // (an axis without pairs turns nothing and reads no row)
+  const int most = max(p.pair_end0 > 0 ? pos0 : 0,
+                       max(p.pair_end1 > p.pair_end0 ? pos1 : 0, p.pair_end1 < 64 ? pos2 : 0));
   float cs[kPairs], sn[kPairs];
   if (still || most >= p.max_pos) {
     // outside the table: no value is right; say so in the error word too

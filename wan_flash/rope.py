@@ -13,8 +13,8 @@ wan_flash_rope(q, k, positions, table) -> (q_rot, k_rot)   differentiable
 Make the table once and the positions once per grid and keep them, as the
 model keeps its frequency table.  Contract violations raise AssertionError
 before any CUDA call; the kernel runs on ``torch.cuda.current_stream()``.  A
-position past the table is found on the device: its token's rows become NaN
-and ``wan_flash._lib.check_device()`` raises.
+position past the table, on an axis that has dims, is found on the device: its
+token's rows become NaN and ``wan_flash._lib.check_device()`` raises.
 """
 
 from __future__ import annotations
