@@ -80,3 +80,59 @@ def test_decode_op():
     assert torch.equal(o, want[0]) and torch.equal(lse, want[1]) and torch.equal(op.wan_decode(*args), o)
     # unread page-table entries are out of range on purpose: opcheck clones, which is fine
     torch.library.opcheck(torch.ops.wan_flash.decode.default, args, test_utils=("test_schema", "test_faketensor"))
+
+
+def test_residual_is_made_for_gradients_only(monkeypatch):
+    """wan_attention_packed asks for o's rounding residual only where a gradient will read it, and the
+    operator's backward works without one too."""
+    asked, given = [], []
+
+    def fwd(q, k, v, q_offsets, k_offsets, causal, residual=False):
+        asked.append(residual)
+        lse = torch.zeros(q.shape[1], q.shape[0])
+        return (torch.zeros_like(q), lse, torch.zeros_like(q)) if residual else (torch.zeros_like(q), lse)
+
+    def bwd(q, k, v, o, lse, do, q_offsets, k_offsets, causal, o_residual=None):
+        given.append(o_residual)
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+
+    monkeypatch.setattr(op, "wan_flash_packed_fwd", fwd)
+    monkeypatch.setattr(op, "wan_flash_packed_bwd", bwd)
+    q, k = torch.zeros(8, 4, 128, dtype=torch.bfloat16), torch.zeros(8, 2, 128, dtype=torch.bfloat16)
+    off = torch.tensor([0, 5, 8], dtype=torch.int32)
+    op.wan_attention_packed(q, k, k, off)
+    leaf = k.clone().requires_grad_()
+    with torch.no_grad():
+        op.wan_attention_packed(q, leaf, k, off)
+    assert asked == [False, False]
+    o = op.wan_attention_packed(q, leaf, k, off)
+    torch.autograd.grad(o, leaf, o)
+    assert asked == [False, False, True] and given[0].shape == q.shape
+    o, _, res = torch.ops.wan_flash.packed_fwd(q, leaf, k, off, off, False, False)
+    torch.autograd.grad(o, leaf, o)
+    assert res.numel() == 0 and given[1] is None
+
+
+@pytest.mark.gpu
+def test_ops_without_a_residual():
+    from tests.test_packed import make
+    from wan_flash.packed import wan_flash_packed_bwd, wan_flash_packed_fwd
+
+    q, k, v, do, off, _ = make([100, 37, 160], [100, 37, 160], 4, 2)
+    o, lse = wan_flash_packed_fwd(q, k, v, off, causal=True)
+    assert torch.equal(op.wan_attention_packed(q, k, v, off, causal=True), o)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    got = torch.ops.wan_flash.packed_fwd(*leaves, off, off, True, False)
+    assert torch.equal(got[0], o) and torch.equal(got[1], lse)
+    want = wan_flash_packed_bwd(q, k, v, o, lse, do, off, causal=True)
+    grads = torch.autograd.grad(got[0], leaves, do)
+    assert torch.equal(grads[1], want[1]) and torch.equal(grads[2], want[2])
+    torch.library.opcheck(torch.ops.wan_flash.packed_fwd.default, (q, k, v, off, off, True, False),
+                          test_utils=("test_schema", "test_faketensor"))
+    compiled = torch.compile(lambda *x: op.wan_attention_packed(*x, off, causal=True), backend="aot_eager")
+    with torch.no_grad():
+        assert torch.equal(compiled(q, k, v), o)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(compiled(*leaves), leaves, do)
+    direct = torch.autograd.grad(op.wan_attention_packed(*leaves, off, causal=True), leaves, do)
+    assert torch.equal(grads[1], direct[1]) and torch.equal(grads[2], direct[2])

@@ -27,7 +27,8 @@ and ``wan_attention_dual(q, k0, v0, k1, v1) -> o0 + o1``.  So have rotary
 positions, packed attention and decode:
 
     wan_flash::rope(q, k, positions, table, axes, inverse) -> (q_rot, k_rot)
-    wan_flash::packed_fwd(q, k, v, q_offsets, k_offsets, causal) -> (o, lse, o_residual)
+    wan_flash::packed_fwd(q, k, v, q_offsets, k_offsets, causal, residual=True)
+        -> (o, lse, o_residual)      (o_residual empty without residual)
     wan_flash::packed_bwd(q, k, v, o, lse, o_residual, do, q_offsets, k_offsets, causal)
         -> (dq, dk, dv)
     wan_flash::decode(q, k_cache, v_cache, page_table, lengths) -> (o, lse)
@@ -188,22 +189,24 @@ def wan_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: t
 
 @torch.library.custom_op("wan_flash::packed_fwd", mutates_args=())
 def packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
-               causal: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal, residual=True)
+               causal: bool, residual: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    out = wan_flash_packed_fwd(q, k, v, q_offsets, k_offsets, causal, residual=residual)
+    return out if residual else (*out, q.new_empty(0))
 
 
 @packed_fwd.register_fake
-def _packed_fwd_fake(q, k, v, q_offsets, k_offsets, causal):
+def _packed_fwd_fake(q, k, v, q_offsets, k_offsets, causal, residual=True):
     total_q, h, d = q.shape
     torch._check(d == 128, lambda: "specialized for head_dim=128")
-    return _like(q), q.new_empty((h, total_q), dtype=torch.float32), _like(q)
+    return _like(q), q.new_empty((h, total_q), dtype=torch.float32), _like(q) if residual else q.new_empty(0)
 
 
 @torch.library.custom_op("wan_flash::packed_bwd", mutates_args=())
 def packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                o_residual: torch.Tensor, do: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
                causal: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, causal, o_residual)
+    given = o_residual.dim() == 3  # a forward without residual left an empty one
+    return wan_flash_packed_bwd(q, k, v, o, lse, do, q_offsets, k_offsets, causal, o_residual if given else None)
 
 
 @packed_bwd.register_fake
@@ -212,7 +215,7 @@ def _packed_bwd_fake(q, k, v, o, lse, o_residual, do, q_offsets, k_offsets, caus
 
 
 def _setup_context_packed(ctx, inputs, output):
-    q, k, v, q_offsets, k_offsets, causal = inputs
+    q, k, v, q_offsets, k_offsets, causal, _ = inputs
     o, lse, o_residual = output
     ctx.mark_non_differentiable(lse, o_residual)  # as in the dense op
     ctx.save_for_backward(q, k, v, o, lse, o_residual, q_offsets, k_offsets)
@@ -224,7 +227,7 @@ def _backward_packed(ctx, do, dlse, dres):
         raise NotImplementedError("packed attention's backward has no forward-mode derivative")
     q, k, v, o, lse, o_residual, q_offsets, k_offsets = ctx.saved_tensors
     grads = packed_bwd(q, k, v, o, lse, o_residual, do.contiguous(), q_offsets, k_offsets, ctx.causal)
-    return *grads, None, None, None
+    return *grads, None, None, None, None
 
 
 packed_fwd.register_autograd(_backward_packed, setup_context=_setup_context_packed)
@@ -235,7 +238,8 @@ def wan_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_of
     """wan_flash_attn_packed through the registered operator (differentiable)."""
     if _has_tangent(q, k, v):  # an operator would drop it; this raises
         return wan_flash_attn_packed(q, k, v, q_offsets, k_offsets, causal)
-    return packed_fwd(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, causal)[0]
+    residual = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return packed_fwd(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, causal, residual)[0]
 
 
 @torch.library.custom_op("wan_flash::decode", mutates_args=())
