@@ -460,3 +460,76 @@ def test_c_entries_with_options_refuse():
     assert lib.wf_packed_fwd_with(*[p(16)] * 9, 1 << 30, 2, 8, 8, 4, 2, 0, ctypes.byref(bad), None) == -1
     for cfg, want in ((None, -1), (ctypes.byref(_lib.BwdCfg(-1, 1)), -1), (ctypes.byref(_lib.BwdCfg(2000, 1)), -1)):
         assert lib.wf_packed_bwd_with(*[p(16)] * 13, 1 << 30, 2, 8, 8, 4, 2, 0, cfg, None) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk", [([1500, 1100], [1500, 1100]), ([300, 700], [1500, 700]), ([900, 200], [140, 1300])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_each_gradient_depends_on_the_visible_rows_and_keys_alone(lq, lk, causal):
+    """One key of a long row more or less would pass the bounds of the sums; so another key (or row) is put in place
+    of one: what does not see it stays bit for bit, and the first row (last key) that does see it changes.  (A
+    row that sees one key has p = 1 and dS = p (dP - D) = 0 whatever that key is: no dq, and nothing for dk.)"""
+    features.set_bwd_overrides(nsplit=1, deterministic=True)
+    q, k, v, do, qo, ko = make(lq, lk, 4, 2, seed=15)
+
+    def run(q, k, v, do):
+        o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, causal=causal, residual=True)
+        return o, *wan_flash_packed_bwd(q, k, v, o, lse, do, qo, ko, causal=causal, o_residual=res)
+
+    def differ(a, b):  # per row, whether all heads differ / any head differs
+        d = (a != b).any(-1)
+        return d.all(-1), d.any(-1)
+
+    want = run(q, k, v, do)
+    a0, c0 = 0, 0
+    for a, c in zip(lq, lk):
+        for t in (0, 1, 127, 128, c // 2, c - 1):  # key t is seen by rows >= t - (c - a)
+            k2, v2 = k.clone(), v.clone()
+            k2[c0 + t], v2[c0 + t] = k[c0 + t].flip(-1), v[c0 + t].flip(-1)
+            got = run(q, k2, v2, do)
+            first = max(0, t - (c - a)) if causal else 0
+            for i in (0, 1):  # o, dq
+                every, some = differ(got[i], want[i])
+                assert not some[:a0 + first].any() and not some[a0 + a:].any()
+                alone = causal and first + 1 + c - a == 1
+                assert (alone and i == 1) or every[a0 + first]
+                assert every[a0 + a - 1]
+        for r in (0, 1, 127, 128, a // 2, a - 1):  # row r sees keys < r + 1 + c - a
+            q2, do2 = q.clone(), do.clone()
+            q2[a0 + r], do2[a0 + r] = q[a0 + r].flip(-1), do[a0 + r].flip(-1)
+            got = run(q2, k, v, do2)
+            seen = max(0, min(c, r + 1 + c - a)) if causal else c
+            for i in (2, 3):  # dk, dv
+                every, some = differ(got[i], want[i])
+                assert not some[:c0].any() and not some[c0 + seen:].any()
+                assert seen == 0 or (seen == 1 and i == 2) or (every[c0] and every[c0 + seen - 1])
+        a0, c0 = a0 + a, c0 + c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("deterministic", [False, True])
+def test_two_backwards_side_by_side_on_two_streams(deterministic):
+    features.set_bwd_overrides(deterministic=deterministic)
+    work = []
+    for seed, lens in ((16, [900, 33, 1200]), (17, [1500, 640, 1])):
+        q, k, v, do, qo, ko = make(lens, lens, 8, 2, seed=seed)
+        o, lse, res = wan_flash_packed_fwd(q, k, v, qo, ko, causal=True, residual=True)
+        work.append((q, k, v, o, lse, do, qo, ko, True, res))
+    want = [wan_flash_packed_bwd(*w) for w in work]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [[], []]
+        for _ in range(3):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(wan_flash_packed_bwd(*work[i]))
+        torch.cuda.synchronize()
+        for i in range(2):
+            for g in got[i]:
+                assert torch.equal(g[1], want[i][1]) and torch.equal(g[2], want[i][2])
+                if deterministic:
+                    assert torch.equal(g[0], want[i][0])
+                else:  # sums of the same contributions in another order: an fp32 step of each, then a rounding
+                    check_bwd(*work[i][:3], work[i][5], work[i][6], work[i][7], True, *g, residual=True)
+    _lib.check_device()
