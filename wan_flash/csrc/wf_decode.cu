@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
   int4 join = make_int4(-1, 0, 0, 0);
 
   // ---- the loader: this warp's tokens of the CTA's tiles one after the other,
-  // two tiles ahead of the products and on into the next rows.  Of tile t a
+  // kStages - 1 tiles ahead of the products and on into the next rows.  Of tile t a
   // warp has tokens 64 t + 16 warp + [0, 16); lane j (and 16 + j) steps token j
   // through the pages; lanes 0-15 (16-31) copy the 16-byte chunks of the even
   // (odd) rows.

@@ -96,7 +96,7 @@ struct PackedPlanParams {
   int sms;
   int may_split;            // forward: the workspace has room for partial results
   int nsplit;               // > 0: pieces of the longest walk; 0: by `pieces`
-  int pieces;               // pieces (over all key-value heads) that the whole work is cut into at least
+  int pieces;               // sets the smallest piece: the whole work (over all key-value heads) in so many
   int4* head;               // [0] {items, status, split key tiles, draw counter}, [1] (backward) {query tiles, status}
   int* base;                // scratch: 3 * (n + 3)
   PackedFwdTile* fwd_tiles;

@@ -52,7 +52,7 @@ __device__ __forceinline__ size_t packed_dq_place(size_t dq_rows, int h, int x, 
 }
 
 // Preprocess: D = rowsum((o + residual) * dO), -lse * log2(e), and the zeroed dQ
-// accumulator.  Bound: HBM (1036 bytes per row and head).  grid (2 * tiles,
+// accumulator.  Bound: HBM (1036 bytes per row and head, 1292 with the residual).  grid (2 * tiles,
 // h), 256 threads: 64 rows of one tile, 16 threads per row.
 __global__ void __launch_bounds__(256) wf_packed_pre_kernel(PackedBwdParams p, const __nv_bfloat16* __restrict__ o,
                                                             const __nv_bfloat16* __restrict__ res,

@@ -4,8 +4,10 @@
 //     S = q k^T / sqrt(128), row i of a sequence sees keys j <= i + lk - lq
 //     (causal) or all of them; o = softmax(S) v; lse.
 //
-// Bound: the tensor pipe and, level with it, the MUFU exponentials (a
-// 128 x 128 block of S needs as many cycles of either).  The inner pipeline is
+// Bound: the tensor pipe and, level with it, the MUFU exponentials need as many
+// cycles for a 128 x 128 block of S; each is busy 52 to 56 % of the time, the rest is
+// the chain scores -> probabilities -> product of a tile that the other one does
+// not always cover, and the uneven end of the last round.  The inner pipeline is
 // that of wf_fwd_kernel: two 128-row query tiles per CTA, S and O in tensor
 // memory, P written over S in two halves, one MMA warp, one TMA warp, one
 // thread per query row.  What differs:

@@ -276,8 +276,7 @@ __device__ int plan_next(PlanShared& sh, Item& w) {
 // grid 1 (forward) or 2 (backward: block 0 the items, block 1 the query tiles)
 __global__ void __launch_bounds__(kPlanThreads) wf_packed_plan_kernel(PackedPlanParams p) {
   __shared__ PlanShared sh;
-  // a programmatic dependent of whatever ran before (19.6 -> 18.9 us for a short
-  // forward)
+  // a programmatic dependent of whatever ran before
   griddep_wait();
   griddep_launch_dependents();  // (only now: the next kernels' read-only loads must not meet that one's writes)
   const bool small = p.n + 3 <= kPlanSmall;
