@@ -410,7 +410,7 @@ def test_feature_switches(lens, h, hk):
         r = attn64(q[a:b], k[a:b], v[a:b])
         assert_close(want[0][a:b], r["o"], r["o_tol"], "o")
     features.set_bwd_overrides(pdl=False)
-    for sms in (0, 1, 7, 500):
+    for sms in (0, 1, 7, 500, 2**31 - 1):
         features.set_overrides(num_sms=sms)
         got = run()
         for i in (0, 1, 3, 4):

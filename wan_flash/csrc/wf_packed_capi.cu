@@ -204,8 +204,9 @@ extern "C" int wf_packed_fwd_with(const void* q, const void* k, const void* v, c
   p.part_o = reinterpret_cast<float4*>(w + ws.part_o);
   p.part_ml = reinterpret_cast<float2*>(w + ws.part_ml);
   p.q_off = q_offsets, p.k_off = k_offsets, p.n = n, p.total_k = total_k;
-  const int ctas = cfg && cfg->num_sms > 0 ? cfg->num_sms : sms;  // draw whatever items the plan makes
-  const int grid = ws.may_split ? ctas : (int)(ws.direct ? most_items : std::min<long long>(most_items, ctas));
+  // the CTAs draw whatever items the plan makes: up to one per SM more where it may cut
+  const int ctas = cfg && cfg->num_sms > 0 ? cfg->num_sms : sms;
+  const int grid = (int)(ws.direct ? most_items : std::min<long long>(most_items + (ws.may_split ? sms : 0), ctas));
   e = launch_ex(ws.direct ? wf_packed_fwd_kernel<true> : wf_packed_fwd_kernel<false>, dim3(grid), dim3(pfwd::kThreads), pfwd::kSmemBytes, st, true, 1u, mq,
                             mk, mv, mo, mr, p);
   if (e != cudaSuccess) return cuda_fail(e, "wf_packed_fwd launch");
