@@ -361,3 +361,26 @@ def test_probabilities_are_not_rounded_to_bf16(h, hk, extra_width):
         spread = (r["p"] @ v[pg, at % 16].double().transpose(0, 1).repeat_interleave(h // hk, 0).abs()).transpose(0, 1)
         fp32 = (2.0**-16 + 2.0**-20 + (2 * 16 * -(-n // 64) + 16) * E32) * spread + 2.0**-15 * r["o"].abs()
         assert_close(o[i:i + 1], r["o"], fp32 + U * (r["o"].abs() + fp32), f"o[{i}] of {n}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h,hk", [(6, 2), (32, 1)])
+@pytest.mark.parametrize("extra_width", [0, 300])
+def test_infinite_values_stay_infinite(h, hk, extra_width):
+    """A visible token whose value is infinite in a dim makes o infinite there (every probability is above 0), with its
+    sign; two of opposite signs, or a NaN, make NaN; the other dims are as without."""
+    lens = [300, 1, 17, 130]
+    q, k, v, table, lengths = make(lens, h, hk, 16, seed=22, extra_width=extra_width)
+    want, want_lse = wan_flash_decode(q, k, v, table, lengths)
+    inf = float("inf")
+    for i, n in enumerate(lens):
+        for dim, at, x in ((3, 0, inf), (4, n - 1, -inf), (5, n // 2, inf), (6, 0, inf), (6, n - 1, -inf), (127, n // 3, float("nan"))):
+            v[table[i, at // 16].long(), at % 16, :, dim] = x
+    o, lse = wan_flash_decode(q, k, v, table, lengths)
+    _lib.check_device()
+    assert torch.equal(lse, want_lse)
+    for i, n in enumerate(lens):
+        assert (o[i, :, 3] == inf).all() and (o[i, :, 4] == -inf).all() and (o[i, :, 5] == inf).all()
+        assert (o[i, :, 6].isnan() if n > 1 else o[i, :, 6] == -inf).all() and o[i, :, 127].isnan().all()
+        rest = [d for d in range(128) if d not in (3, 4, 5, 6, 127)]
+        assert torch.equal(o[i][:, rest], want[i][:, rest])

@@ -480,33 +480,40 @@ __global__ void __launch_bounds__(dec::kThreads, dec::Shape<kN>::kCtasPerSm)
           }
         }
         // P^T (tokens x heads) to the B operand of O^T = V^T P^T: 8x8
-        // transposes within the warp.  P goes as a pair of bf16, its rounding
-        // and what that took away (2^-16 of the value is lost; a single bf16
-        // loses as much as o's own rounding, and 75600-token caches take 219.5 us
-        // against 218.6, 32 heads a row 81.3 against 79.6); the sum l keeps the fp32 values.
+        // transposes within the warp.  P goes as a pair of bf16, its upper half
+        // cut off and the rest (2^-16 of the value is lost; a single bf16
+        // loses as much as o's own rounding, and 75600-token caches take 219.2 us
+        // against 218.2, 32 heads a row 82.5 against 79.2); the sum l keeps the fp32 values.
+        // The rest is never negative, nor 0 (P's last bit is set, an fp32 step): an
+        // infinite V times either would make NaN of the infinity that P V is.
+        auto rest = [](float x) {
+          return __uint_as_float(__float_as_uint(x) | 1u) - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+        };
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t hi = pack_bf16(pr[2 * i], pr[2 * i + 1]);
-          pb[n][i] = movmatrix_trans(hi);
-          pl[n][i] = movmatrix_trans(
-              pack_bf16(pr[2 * i] - __uint_as_float(hi << 16), pr[2 * i + 1] - __uint_as_float(hi & 0xffff0000u)));
+          const float x = pr[2 * i], y = pr[2 * i + 1];
+          pb[n][i] = movmatrix_trans((__float_as_uint(x) >> 16) | (__float_as_uint(y) & 0xffff0000u));
+          pl[n][i] = pack_bf16(rest(x), rest(y));
+          if constexpr (kN > 2) pl[n][i] = movmatrix_trans(pl[n][i]);  // else behind the first products
         }
       }
-      // O^T (16 dims x 8 heads) += V^T P^T
+      // O^T (16 dims x 8 heads) += V^T P^T, up to 8 independent products in a row
       {
+        constexpr int kDims = kN == 1 ? 8 : kN == 2 ? 4 : 2;
         const int r = (lane & 7) + (lane >> 4) * 8;        // matrices 0, 1: tokens 0-7; 2, 3: tokens 8-15
         const uint32_t row = sv + r * kRowBytes + (((lane >> 3) & 1) << 4);  // matrices 1, 3: dims 8-15 of the tile
 #pragma unroll
-        for (int d = 0; d < 8; d += 2) {
-          uint32_t a0[4], a1[4];
-          ldmatrix_x4_trans(row + d * 32, a0);
-          ldmatrix_x4_trans(row + d * 32 + 32, a1);
+        for (int d0 = 0; d0 < 8; d0 += kDims) {
+          uint32_t a[kDims][4];
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) ldmatrix_x4_trans(row + (d0 + d) * 32, a[d]);
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
-            mma_16816(acc[n][d], a0, pb[n][0], pb[n][1]);
-            mma_16816(acc[n][d + 1], a1, pb[n][0], pb[n][1]);
-            mma_16816(acc[n][d], a0, pl[n][0], pl[n][1]);
-            mma_16816(acc[n][d + 1], a1, pl[n][0], pl[n][1]);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) mma_16816(acc[n][d0 + d], a[d], pb[n][0], pb[n][1]);
+            if (kN <= 2 && d0 == 0) pl[n][0] = movmatrix_trans(pl[n][0]), pl[n][1] = movmatrix_trans(pl[n][1]);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) mma_16816(acc[n][d0 + d], a[d], pl[n][0], pl[n][1]);
           }
         }
       }
